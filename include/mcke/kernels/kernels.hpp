@@ -162,6 +162,20 @@ struct GemmKernelAttrs {
                                                m, n, k, alpha, beta, &t, stream));
 }
 
+// y = act(alpha * A B + bias[col]) + residual on 16-bit operands in one launch; bias and
+// residual may be null, residual may be y (mcke_launch_gemm_lp_bias_act).
+[[nodiscard]] inline Status launch_gemm_lp_bias_act(const void* a, const void* b, const void* bias,
+                                                   const void* residual, void* y, DType ab,
+                                                   DType yd, DType bias_dtype, std::int64_t m,
+                                                   std::int64_t n, std::int64_t k, float alpha,
+                                                   Activation act, GemmTile tile,
+                                                   rt::StreamHandle stream) {
+  const mcke_gemm_tile t = detail::to_c(tile);
+  return detail::status_of(mcke_launch_gemm_lp_bias_act(
+      a, b, bias, residual, y, static_cast<int>(ab), static_cast<int>(yd),
+      static_cast<int>(bias_dtype), m, n, k, alpha, static_cast<int>(act), &t, stream));
+}
+
 // The 16-bit GEMM tile this build picks for a shape.
 [[nodiscard]] inline GemmTile lp_default_tile(std::int64_t m, std::int64_t n, std::int64_t k) {
   mcke_gemm_tile t{};
@@ -174,6 +188,60 @@ struct GemmKernelAttrs {
 [[nodiscard]] constexpr bool gemm_lp_tile_is_supported(const GemmTile& t) {
   return t.bk == 64 && t.bm == t.bn && (t.bm == 256 || t.bm == 128 || t.bm == 64) &&
          t.tm == t.bm / 16 && t.tn == t.bn / 16;
+}
+
+// ---------------------------------------------------------------------------
+// Layer norm and token log probabilities.  No reference counterparts; formulas,
+// optional (null) operands and special rows are those of mcke_amd.h.
+// ---------------------------------------------------------------------------
+[[nodiscard]] inline Status launch_layer_norm(const void* x, const void* weight, const void* bias,
+                                             void* y, float* mean, float* rstd, DType dtype,
+                                             DType param_dtype, std::int64_t rows,
+                                             std::int64_t cols, float eps,
+                                             rt::StreamHandle stream) {
+  return detail::status_of(mcke_launch_layer_norm(x, weight, bias, y, mean, rstd,
+                                                  static_cast<int>(dtype),
+                                                  static_cast<int>(param_dtype), rows, cols, eps,
+                                                  stream));
+}
+
+[[nodiscard]] inline std::size_t layer_norm_backward_workspace_bytes(std::int64_t rows,
+                                                                    std::int64_t cols) noexcept {
+  return mcke_layer_norm_backward_workspace_bytes(rows, cols);
+}
+
+[[nodiscard]] inline Status launch_layer_norm_backward(
+    const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
+    void* dx, void* dweight, void* dbias, DType dtype, DType param_dtype, std::int64_t rows,
+    std::int64_t cols, void* workspace, std::size_t workspace_bytes, rt::StreamHandle stream) {
+  return detail::status_of(mcke_launch_layer_norm_backward(
+      dy, x, weight, mean, rstd, dx, dweight, dbias, static_cast<int>(dtype),
+      static_cast<int>(param_dtype), rows, cols, workspace, workspace_bytes, stream));
+}
+
+[[nodiscard]] inline std::size_t token_logprobs_workspace_bytes(std::int64_t rows,
+                                                               std::int64_t vocab,
+                                                               int top_k) noexcept {
+  return mcke_token_logprobs_workspace_bytes(rows, vocab, top_k);
+}
+
+[[nodiscard]] inline Status launch_token_logprobs(
+    const void* logits, const std::int64_t* tokens, float* logprobs, float* entropy, float* lse,
+    float* top_logprobs, std::int64_t* top_ids, DType dtype, std::int64_t rows,
+    std::int64_t vocab, std::int64_t row_stride, float scale, int top_k, void* workspace,
+    std::size_t workspace_bytes, rt::StreamHandle stream) {
+  return detail::status_of(mcke_launch_token_logprobs(
+      logits, tokens, logprobs, entropy, lse, top_logprobs, top_ids, static_cast<int>(dtype), rows,
+      vocab, row_stride, scale, top_k, workspace, workspace_bytes, stream));
+}
+
+[[nodiscard]] inline Status launch_token_logprobs_backward(
+    const void* logits, const std::int64_t* tokens, const float* lse, const float* entropy,
+    const float* dlogprobs, const float* dentropy, void* dlogits, DType dtype, std::int64_t rows,
+    std::int64_t vocab, std::int64_t row_stride, float scale, rt::StreamHandle stream) {
+  return detail::status_of(mcke_launch_token_logprobs_backward(
+      logits, tokens, lse, entropy, dlogprobs, dentropy, dlogits, static_cast<int>(dtype), rows,
+      vocab, row_stride, scale, stream));
 }
 
 }  // namespace mcke::kernels

@@ -246,6 +246,100 @@ int mcke_launch_gemm_lp_vendor(const void* a, const void* b, void* c, int ab_dty
                                int c_dtype, int64_t m, int64_t n, int64_t k, float alpha,
                                float beta, void* stream);
 
+/* No reference counterpart: the 16-bit product with its bias, activation and residual in the
+ * epilogue, as the layers of a transformer chain them,
+ *   y[i,j] = act(alpha * (A B)[i,j] + bias[j]) + residual[i,j],
+ * computed in fp32 from the fp32 sums and rounded once.  y and residual (m x n, row-major)
+ * are of y_dtype: MCKE_DTYPE_F32 or ab_dtype.  bias (n values of bias_dtype, MCKE_DTYPE_F32 or
+ * ab_dtype) and residual may be null.  residual may be y itself (the residual stream updated
+ * in place); apart from that y overlaps no operand.  activation is an mcke_activation value,
+ * with the meaning it has in mcke_launch_bias_act_f32 (a NaN becomes 0 under ReLU).  m == 0
+ * or n == 0 is a no-op; k == 0 gives act(bias) + residual.  Other validation, tiles, and the
+ * choice of kernel by shape and alignment as mcke_launch_gemm_lp.  Forward only, as every
+ * product here. */
+int mcke_launch_gemm_lp_bias_act(const void* a, const void* b, const void* bias,
+                                 const void* residual, void* y, int ab_dtype, int y_dtype,
+                                 int bias_dtype, int64_t m, int64_t n, int64_t k, float alpha,
+                                 int activation, const mcke_gemm_tile* tile, void* stream);
+
+/* ---- layer norm ------------------------------------------------------------
+ * No reference counterpart; a row operator beside mcke_launch_row_softmax_f32, for the
+ * activations around the 16-bit products.  x, y, dy and dx (rows x cols, row-major, any
+ * alignment of their type) are of dtype; weight, bias (cols values) and their gradients of
+ * param_dtype, MCKE_DTYPE_F32 or dtype; mean and rstd (rows values) fp32.  Arithmetic is fp32,
+ * each output rounded once, and nothing is added atomically: the same input gives the same
+ * bits on every run. */
+
+/* y = (x - mean) * rstd * weight + bias over each row, mean and rstd = 1 / sqrt(var + eps) the
+ * row's own, var over all cols values.  weight null is ones, bias null zeros; mean and rstd
+ * may be null (a backward pass needs them).  eps finite and >= 0.  No output overlaps an
+ * operand.  rows == 0 or cols == 0 is a no-op. */
+int mcke_launch_layer_norm(const void* x, const void* weight, const void* bias, void* y,
+                           float* mean, float* rstd, int dtype, int param_dtype, int64_t rows,
+                           int64_t cols, float eps, void* stream);
+
+/* Bytes of workspace that dweight and dbias need (0 for rows == 0); its contents on entry do not
+ * matter, and two launches that may run at the same time need one each. */
+size_t mcke_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+
+/* The gradients, from dy and what the forward pass had and gave (x, weight, mean, rstd):
+ *   g = dy * weight, xhat = (x - mean) * rstd
+ *   dx = rstd * (g - sum(g) / cols - xhat * sum(g * xhat) / cols)
+ *   dweight = sum over rows of dy * xhat, dbias = sum over rows of dy
+ * Any of dx, dweight, dbias may be null, not all; they are overwritten, not added to.  With
+ * dweight or dbias a 16-byte aligned workspace is needed (see above).  weight null is ones.
+ * rows == 0 gives dweight and dbias of zeros; cols == 0 is a no-op. */
+int mcke_launch_layer_norm_backward(const void* dy, const void* x, const void* weight,
+                                    const float* mean, const float* rstd, void* dx, void* dweight,
+                                    void* dbias, int dtype, int param_dtype, int64_t rows,
+                                    int64_t cols, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+
+/* ---- token log probabilities -------------------------------------------------
+ * No reference counterpart; what the last product's logits are for, beside the row softmax:
+ * the log probability of each row's given token, the row's entropy and its most likely
+ * tokens, in one pass over the logits and without writing the probabilities.  logits are
+ * rows x vocab values of dtype (MCKE_DTYPE_F32, F16 or BF16; any alignment of their type), row r
+ * at r * row_stride, row_stride >= vocab: what lies between is not read.  scale > 0 multiplies
+ * the logits (1 / temperature).  With z = scale * logits[r]:
+ *   lse = log sum exp z, logprob = z[tokens[r]] - lse, entropy = -sum p log p, p = exp(z - lse)
+ *   top_ids, top_logprobs (rows x top_k): the top_k largest logits, ties to the lowest index,
+ *   and their z - lse
+ * Arithmetic is fp32 and the same input gives the same bits on every run.
+ *
+ * Every output may be null, not all; logprobs need tokens.  top_k is 0 .. 64 and at most
+ * vocab.  A row with tokens[r] < 0 (padding) is not read: its logprob, entropy, lse and
+ * top_logprobs are 0, its top_ids -1.  tokens null computes every row.  tokens[r] >= vocab gives
+ * a NaN logprob.  Logits of -inf are masked: they have probability 0; a row of nothing else
+ * has logprob, lse and top_logprobs -inf and entropy 0.  A NaN or +inf logit makes the row's
+ * fp32 results NaN; NaN logits are never among the top_ids, and where fewer than top_k others
+ * are left the rest are -1.
+ * rows == 0 or vocab == 0 is a no-op. */
+
+/* Bytes of workspace that few rows need, which several workgroups share (0 for many rows); its
+ * contents on entry do not matter, and two launches that may run at the same time need one
+ * each. */
+size_t mcke_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k);
+
+int mcke_launch_token_logprobs(const void* logits, const int64_t* tokens, float* logprobs,
+                               float* entropy, float* lse, float* top_logprobs, int64_t* top_ids,
+                               int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                               float scale, int top_k, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* The gradient in the logits, from what the forward pass had and gave:
+ *   dlogits[r, j] = scale * (dlogprobs[r] * ([j == tokens[r]] - p_j)
+ *                            - dentropy[r] * p_j * (log p_j + entropy[r]))
+ * dlogits has the layout and type of logits and does not overlap them; columns from vocab on
+ * are left as they were.  dlogprobs or dentropy may be null, not both; dentropy needs entropy,
+ * dlogprobs need tokens.  A row with tokens[r] < 0, or with every logit masked, has gradient 0
+ * (the former is not read); one with tokens[r] >= vocab, NaN. */
+int mcke_launch_token_logprobs_backward(const void* logits, const int64_t* tokens,
+                                        const float* lse, const float* entropy,
+                                        const float* dlogprobs, const float* dentropy,
+                                        void* dlogits, int dtype, int64_t rows, int64_t vocab,
+                                        int64_t row_stride, float scale, void* stream);
+
 /* ---- runtime: rt::Stream / rt::Event / raw device memory ------------------
  * reference include/mcke/runtime/stream.hpp:82-306, src/core/device.cpp:56-168,
  * src/memory/allocator.cpp:44-73, src/tensor/tensor.cpp:108-138. */

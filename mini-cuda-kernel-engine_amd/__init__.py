@@ -196,6 +196,22 @@ def lib() -> C.CDLL:
         "mcke_gemm_lp_default_tile": (C.c_int, [_I64, _I64, _I64, C.POINTER(GemmTile)]),
         "mcke_launch_gemm_lp_vendor": (C.c_int, [_VP, _VP, _VP, C.c_int, C.c_int, _I64, _I64,
                                                  _I64, C.c_float, C.c_float, _VP]),
+        "mcke_launch_gemm_lp_bias_act": (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_int, C.c_int,
+                                                   C.c_int, _I64, _I64, _I64, C.c_float, C.c_int,
+                                                   C.POINTER(GemmTile), _VP]),
+        "mcke_launch_layer_norm": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, C.c_int, C.c_int,
+                                             _I64, _I64, C.c_float, _VP]),
+        "mcke_layer_norm_backward_workspace_bytes": (C.c_size_t, [_I64, _I64]),
+        "mcke_launch_layer_norm_backward": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
+                                                      C.c_int, C.c_int, _I64, _I64, _VP,
+                                                      C.c_size_t, _VP]),
+        "mcke_token_logprobs_workspace_bytes": (C.c_size_t, [_I64, _I64, C.c_int]),
+        "mcke_launch_token_logprobs": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, C.c_int, _I64,
+                                                 _I64, _I64, C.c_float, C.c_int, _VP, C.c_size_t,
+                                                 _VP]),
+        "mcke_launch_token_logprobs_backward": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP,
+                                                          C.c_int, _I64, _I64, _I64, C.c_float,
+                                                          _VP]),
         "mcke_rt_get_device_count": (C.c_int, [C.POINTER(C.c_int)]),
         "mcke_rt_set_device": (C.c_int, [C.c_int]),
         "mcke_rt_get_device": (C.c_int, [C.POINTER(C.c_int)]),
@@ -566,6 +582,73 @@ def gemm_lp_default_tile(m: int, n: int, k: int) -> GemmTile:
     t = GemmTile()
     _check(lib().mcke_gemm_lp_default_tile(m, n, k, C.byref(t)))
     return t
+
+
+def launch_gemm_lp_bias_act(a, b, bias, residual, y, ab_dtype, y_dtype, bias_dtype, m: int, n: int,
+                            k: int, alpha: float, act, tile: GemmTile | None = None,
+                            stream=None) -> Status:
+    """y = act(alpha * A B + bias[col]) + residual on 16-bit operands in one launch, fp32
+    until the one rounding of y.  bias and residual may be None; residual may be y.  No
+    reference counterpart."""
+    tile = gemm_lp_default_tile(m, n, k) if tile is None else tile
+    return _st(lib().mcke_launch_gemm_lp_bias_act(
+        _ptr(a), _ptr(b), _ptr(bias), _ptr(residual), _ptr(y), int(ab_dtype), int(y_dtype),
+        int(bias_dtype), m, n, k, alpha, int(act), C.byref(tile), _sh(stream)))
+
+
+# ---------------------------------------------------------------------------
+# Layer norm and token log probabilities (no reference counterparts; the conventions
+# are those of the launchers above, see include/mcke_amd.h)
+# ---------------------------------------------------------------------------
+def launch_layer_norm(x, weight, bias, y, mean, rstd, dtype, param_dtype, rows: int, cols: int,
+                      eps: float, stream=None) -> Status:
+    """y = (x - mean) * rstd * weight + bias over each row; weight, bias, mean and rstd may be
+    None."""
+    return _st(lib().mcke_launch_layer_norm(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean),
+                                            _ptr(rstd), int(dtype), int(param_dtype), rows, cols,
+                                            eps, _sh(stream)))
+
+
+def layer_norm_backward_workspace_bytes(rows: int, cols: int) -> int:
+    return int(lib().mcke_layer_norm_backward_workspace_bytes(rows, cols))
+
+
+def launch_layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight, dbias, dtype, param_dtype,
+                               rows: int, cols: int, workspace=None, workspace_bytes: int = 0,
+                               stream=None) -> Status:
+    """The gradients of launch_layer_norm; any of dx, dweight and dbias may be None, and the
+    workspace is for the latter two."""
+    return _st(lib().mcke_launch_layer_norm_backward(
+        _ptr(dy), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight),
+        _ptr(dbias), int(dtype), int(param_dtype), rows, cols, _ptr(workspace), workspace_bytes,
+        _sh(stream)))
+
+
+def token_logprobs_workspace_bytes(rows: int, vocab: int, top_k: int) -> int:
+    return int(lib().mcke_token_logprobs_workspace_bytes(rows, vocab, top_k))
+
+
+def launch_token_logprobs(logits, tokens, logprobs, entropy, lse, top_logprobs, top_ids, dtype,
+                          rows: int, vocab: int, row_stride: int, scale: float = 1.0,
+                          top_k: int = 0, workspace=None, workspace_bytes: int = 0,
+                          stream=None) -> Status:
+    """Each row's log probability of its token, entropy, log of the sum of exponentials and
+    top_k most likely tokens; outputs that are not wanted are None.  A negative token marks a
+    row to leave out."""
+    return _st(lib().mcke_launch_token_logprobs(
+        _ptr(logits), _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(lse), _ptr(top_logprobs),
+        _ptr(top_ids), int(dtype), rows, vocab, row_stride, scale, top_k, _ptr(workspace),
+        workspace_bytes, _sh(stream)))
+
+
+def launch_token_logprobs_backward(logits, tokens, lse, entropy, dlogprobs, dentropy, dlogits,
+                                   dtype, rows: int, vocab: int, row_stride: int,
+                                   scale: float = 1.0, stream=None) -> Status:
+    """The gradient of the log probabilities and entropies in the logits; dlogprobs or dentropy
+    may be None."""
+    return _st(lib().mcke_launch_token_logprobs_backward(
+        _ptr(logits), _ptr(tokens), _ptr(lse), _ptr(entropy), _ptr(dlogprobs), _ptr(dentropy),
+        _ptr(dlogits), int(dtype), rows, vocab, row_stride, scale, _sh(stream)))
 
 
 # ---------------------------------------------------------------------------

@@ -47,6 +47,7 @@
 #include <cstdint>
 #include <utility>
 
+#include "gemm_lp_epilogue.hpp"
 #include "gemm_mfma.hpp"
 
 namespace mcke_amd {
@@ -62,6 +63,10 @@ typedef unsigned u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int kLpBK = 64;            // K depth of one LDS stage (elements)
 constexpr int kLpRowBytes = 128;     // one LDS row: 64 16-bit values
+
+// The output's pointer: a fused residual may lie in the output itself.
+template <typename OutT, class E>
+using OutPtr = std::conditional_t<E::kFused, OutT*, OutT* __restrict__>;
 
 // Input element type -> its MFMA.
 template <typename T> struct LpMfma;
@@ -284,10 +289,10 @@ __device__ __forceinline__ void lp_store_c(const f32x16 (&acc)[BM / 64][BN / 64]
 // 14 bytes per clock and CU at 128 x 128); each operand is read half as often as by 64 x 64
 // tiles, which is what it gains on the split-K kernel: 4095 x 4095 x 1023, fp16 to fp32, 136
 // -> 65.6 us (524 TFLOP/s).
-template <typename T, typename OutT, int BM, int BN, bool VEC, bool WHOLE>
+template <typename T, typename OutT, int BM, int BN, bool VEC, bool WHOLE, class E = NoEpilogue>
 __global__ __launch_bounds__(kMfmaThreads, 1) void gemm_lp_kernel(
-    const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, OutT* __restrict__ C,
-    int M, int N, int K, float alpha, float beta, int tiles_m, int tiles_n) {
+    const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, OutPtr<OutT, E> C,
+    int M, int N, int K, float alpha, float beta, int tiles_m, int tiles_n, E ep) {
   constexpr int WM = BM / 2, WN = BN / 2;
   constexpr int MT = WM / 32, NT = WN / 32;
   static_assert(MT >= 1 && (NT == 1 || NT == 2 || NT == 4), "unsupported wave tile");
@@ -414,7 +419,34 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void gemm_lp_kernel(
     __syncthreads();
   }
 
-  lp_store_c<OutT, BM, BN, VEC, WHOLE>(acc, C, M, N, m0, n0, n_first, wm, wn, h, c, alpha, beta);
+  if constexpr (E::kFused) {
+    // The loop's last barrier is behind every read of the stages.  Each pass takes IP of the
+    // wave's MT block rows, as many as the stages' LDS holds.
+    constexpr int IP = BM * BN * 4 <= 2 * S::kBytes ? MT : MT / 2;
+    constexpr int TR = BM * IP / MT;
+    static_assert(TR * BN * 4 <= 2 * S::kBytes, "a pass must fit the stages");
+    float* sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int pass = 0; pass < MT / IP; ++pass) {
+      if (pass > 0) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < IP; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = wm * (IP * 32) + i * 32 + 8 * (r / 4) + 4 * h + (r % 4);
+          const int col = wn * WN + NT * c;
+          float* p = sums + sum_at<BN>(row, col / 4) + col % 4;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) p[j] = acc[pass * IP + i][j][r];
+        }
+      __syncthreads();
+      store_fused<OutT, TR, BN, kMfmaThreads>(sums, C, M, N, m0, n0, n_first, alpha, ep, [&](int r) {
+        return (r / (IP * 32)) * WM + pass * (IP * 32) + r % (IP * 32);
+      });
+    }
+  } else {
+    lp_store_c<OutT, BM, BN, VEC, WHOLE>(acc, C, M, N, m0, n0, n_first, wm, wn, h, c, alpha, beta);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1054,16 +1086,16 @@ __device__ __forceinline__ float acc_get(float a) {
 //   * the K % 64 remainder is the first pair of steps, not the last: its columns are
 //     loaded through registers with bounds checks, zero past them in both operands, and
 //     the whole pairs follow.
-template <typename T, typename OutT, int BM, int BN, bool EDGE = false>
+template <typename T, typename OutT, int BM, int BN, bool EDGE = false, class E = NoEpilogue>
 __global__ __launch_bounds__(kMfmaThreads, 1) void gemm_lp_dma16_kernel(
-    const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, OutT* __restrict__ C,
-    int M, int N, int K, float alpha, float beta, int tiles_m, int tiles_n) {
+    const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, OutPtr<OutT, E> C,
+    int M, int N, int K, float alpha, float beta, int tiles_m, int tiles_n, E ep) {
   using S = Lp16Shape<BM, BN>;
   constexpr int BK = S::BK;
   constexpr int WM = BM / 2, WN = BN / 2;
   constexpr int MT = S::MT, NT = S::NT, NA = S::NA;
   constexpr int L = S::L;
-  constexpr bool TRANS = sizeof(OutT) == 2;
+  constexpr bool TRANS = sizeof(OutT) == 2 || E::kFused;
 
   __shared__ __attribute__((aligned(1024))) char smem[S::kLdsBytes];
 
@@ -1285,6 +1317,38 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void gemm_lp_dma16_kernel(
   // MFMA's results are ready well before these 16 cycles are over.
   asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
 
+  if constexpr (E::kFused) {
+    // Transposed blocks, a quad of a row per lane and block (see below); each pass takes IP of
+    // the wave's MT block rows, as many as LDS holds in fp32.
+    constexpr int IP = BM * BN * 4 <= S::kLdsBytes ? MT : MT / 2;
+    constexpr int TR = BM * IP / MT;
+    static_assert(TR * BN * 4 <= S::kLdsBytes, "a pass must fit LDS");
+    float* sums = reinterpret_cast<float*>(smem);
+    [&]<int... PASS>(std::integer_sequence<int, PASS...>) {
+      ([&] {
+        __syncthreads();   // the stage buffers, or the pass before, have been read
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < IP; ++i) {
+          const int row = wm * (IP * 16) + 16 * i + r16;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc_get(acc[PASS * IP + i][j][e]);
+            *reinterpret_cast<f32x4*>(sums + sum_at<BN>(row, (wn * WN + 16 * j) / 4 + g)) = v;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+        store_fused<OutT, TR, BN, kMfmaThreads>(
+            sums, C, M, N, m0, n0, n_first, alpha, ep, [&](int r) {
+              return (r / (IP * 16)) * WM + PASS * (IP * 16) + r % (IP * 16);
+            });
+      }(), ...);
+    }(std::make_integer_sequence<int, MT / IP>{});
+    return;
+  }
   using O = LpOut<OutT>;
   if constexpr (EDGE && !TRANS) {
     // As below, without the rows past M and the columns before n_first.

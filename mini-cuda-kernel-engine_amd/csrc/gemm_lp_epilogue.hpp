@@ -1,0 +1,118 @@
+// gemm_lp_epilogue.hpp -- what a 16-bit-input product does with a tile of sums before its
+// one store:
+//
+//   y = act(alpha acc + bias[col]) + residual
+//
+// in fp32, rounded once.  The kernels take it as a template argument: NoEpilogue is the plain
+// product (C = alpha A B + beta C), Epilogue this.
+//
+// The sums leave the accumulation registers as fp32 through LDS, row-major, and a rolled loop
+// reads them back a row at a time.  There the lane's columns do not change, so the bias is
+// loaded once; the residual's loads and the stores are whole rows of 16 bytes a lane; and the
+// activation's code is there once per activation and not once per accumulator (written over
+// the registers, 256 accumulators times four activations are 60 KB of code that each
+// workgroup runs through once).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "device_math.hpp"
+#include "elem.hpp"
+
+namespace mcke_amd {
+
+struct NoEpilogue {
+  static constexpr bool kFused = false;
+};
+
+struct Epilogue {
+  static constexpr bool kFused = true;
+  const void* bias;        // n values of bias_dtype, or null
+  const void* residual;    // m x n values of the output type, or null; may be the output
+  int bias_dtype;
+  int act;
+};
+
+// act(v + bias) + residual for one output.
+template <int ACT> __device__ __forceinline__ float fused_value(float v, float b, float res) {
+  return act_xb<ACT>(v, b) + res;
+}
+
+// Calls f with the activation as a constant.
+template <class F> __device__ __forceinline__ void with_act(int act, F f) {
+  if (act == kActNone) f(std::integral_constant<int, kActNone>{});
+  else if (act == kActRelu) f(std::integral_constant<int, kActRelu>{});
+  else if (act == kActGeluErf) f(std::integral_constant<int, kActGeluErf>{});
+  else f(std::integral_constant<int, kActGeluTanh>{});
+}
+
+// A pass of TR rows by BN columns of fp32 sums in LDS.  16-byte quad q of row r is at
+// q ^ (r % 16): writers put quads of 16 rows side by side, readers take whole rows, and
+// neither meets a bank twice.
+template <int BN> __device__ __forceinline__ int sum_at(int r, int q) {
+  return r * BN + 4 * (q ^ (r & 15));
+}
+
+// Stores the pass: LDS row r is tile row `row_of(r)`, columns n_first .. min(n0 + BN, N) - 1 of
+// the tile at (m0, n0).  THREADS lanes; every lane of the workgroup calls it.
+template <typename OutT, int TR, int BN, int THREADS, class RowOf>
+__device__ __forceinline__ void store_fused(const float* sums, OutT* C, int M, int N, int m0,
+                                            int n0, int n_first, float alpha, const Epilogue& ep,
+                                            RowOf row_of) {
+  constexpr int VE = kVecElems<OutT>;
+  constexpr int kLanes = BN / VE, kRows = THREADS / kLanes, kSteps = TR / kRows;
+  constexpr int U = kSteps < 4 ? kSteps : 4;            // residual loads in flight
+  static_assert(THREADS % kLanes == 0 && TR % kRows == 0 && kSteps % U == 0, "whole steps");
+  const int lr = threadIdx.x / kLanes, lc = VE * (threadIdx.x % kLanes);
+  const int col = n0 + lc;
+  const bool whole = col >= n_first && col + VE <= N;
+  const OutT* res = static_cast<const OutT*>(ep.residual);
+  float b[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e)
+    b[e] = ep.bias && col + e < N ? load_elem(ep.bias, ep.bias_dtype, col + e) : 0.0f;
+
+  with_act(ep.act, [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    for (int s = 0; s < kSteps; s += U) {
+      VecT16<OutT> old[U];
+      if (res && whole) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int row = m0 + row_of(lr + (s + u) * kRows);
+          old[u] = load_vec<OutT>(res + static_cast<int64_t>(row < M ? row : M - 1) * N + col);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = lr + (s + u) * kRows, row = m0 + row_of(r);
+        if (row >= M) continue;
+        float v[VE];
+#pragma unroll
+        for (int q = 0; q < VE / 4; ++q) {
+          const f32x4 a = *reinterpret_cast<const f32x4*>(sums + sum_at<BN>(r, lc / 4 + q));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * q + e] = alpha * a[e];
+        }
+        OutT* p = C + static_cast<int64_t>(row) * N + col;
+        if (whole) {
+          VecT16<OutT> o;
+#pragma unroll
+          for (int e = 0; e < VE; ++e)
+            o[e] = static_cast<OutT>(
+                fused_value<ACT>(v[e], b[e], res ? static_cast<float>(old[u][e]) : 0.0f));
+          *reinterpret_cast<VecT16<OutT>*>(p) = o;
+        } else {
+          const OutT* rp = res + static_cast<int64_t>(row) * N + col;
+#pragma unroll
+          for (int e = 0; e < VE; ++e)
+            if (col + e >= n_first && col + e < N)
+              p[e] = static_cast<OutT>(
+                  fused_value<ACT>(v[e], b[e], res ? static_cast<float>(rp[e]) : 0.0f));
+        }
+      }
+    }
+  });
+}
+
+}  // namespace mcke_amd

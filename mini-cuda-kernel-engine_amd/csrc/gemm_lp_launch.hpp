@@ -1,0 +1,257 @@
+// gemm_lp_launch.hpp -- which kernel a 16-bit-input product runs, by shape and alignment, for
+// the plain product and for the one with an epilogue (gemm_lp_epilogue.hpp).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <string>
+
+#include "common.hpp"
+#include "gemm_lp.hpp"
+#include "gemm_lp_split.hpp"
+
+namespace mcke_amd {
+
+using LpKernel = const void*;
+
+// Direct-to-LDS 16x16x32 kernel for a BM x BN tile: whole tiles with 16-byte aligned
+// operands and K % 64 == 0, or the EDGE form.  Its per-lane source offsets are 32-bit: BM
+// rows of A and 64 rows of B must span less than 4 GiB.
+template <int BM, int BN>
+bool dma_offsets32(int n, int k) {
+  return static_cast<int64_t>(BM) * k * 2 + 4096 < (int64_t{1} << 32) &&
+         static_cast<int64_t>(64) * n * 2 < (int64_t{1} << 32);
+}
+
+inline int64_t tile_count(int m, int n, int bm, int bn) {
+  return static_cast<int64_t>(steps_along(m, bm)) * steps_along(n, bn);
+}
+
+template <class E>
+struct LpArgs {
+  const uint16_t* a;
+  const uint16_t* b;
+  void* c;
+  int m, n, k;
+  float alpha, beta;
+  E ep;
+  hipStream_t s;
+};
+
+template <class E>
+int check_grid(int64_t tiles, int threads) {
+  if (tiles * threads > int64_t{UINT32_MAX})
+    return invalid(std::string(E::kFused ? "launch_gemm_lp_bias_act" : "launch_gemm_lp") +
+                   ": tiles x lanes exceed the grid's 32-bit work size; use a larger tile");
+  return ok();
+}
+
+template <typename T, typename OutT, int BM, int BN, bool EDGE, class E>
+int launch_dma(const LpArgs<E>& x) {
+  const int64_t tiles = tile_count(x.m, x.n, BM, BN);
+  if (int rc = check_grid<E>(tiles, kMfmaThreads)) return rc;
+  gemm_lp_dma16_kernel<T, OutT, BM, BN, EDGE, E>
+      <<<static_cast<unsigned>(tiles), kMfmaThreads, 0, x.s>>>(
+          x.a, x.b, static_cast<OutT*>(x.c), x.m, x.n, x.k, x.alpha, x.beta,
+          steps_along(x.m, BM), steps_along(x.n, BN), x.ep);
+  MCKE_LAUNCH_CHECK("gemm_lp_dma16_kernel");
+  return ok();
+}
+
+template <typename T, typename OutT, int MT, int NW, int WV, class E>
+int launch_split_as(const LpArgs<E>& x) {
+  constexpr int TM = 16 * MT, TN = 16 * NW;
+  const int64_t tiles = tile_count(x.m, x.n, TM, TN);
+  if (int rc = check_grid<E>(tiles, WV * kWave)) return rc;
+  gemm_lp_split_kernel<T, OutT, MT, NW, WV, E>
+      <<<static_cast<unsigned>(tiles), WV * kWave, 0, x.s>>>(
+          x.a, x.b, static_cast<OutT*>(x.c), x.m, x.n, x.k, x.alpha, x.beta,
+          steps_along(x.m, TM), steps_along(x.n, TN), x.ep);
+  MCKE_LAUNCH_CHECK("gemm_lp_split_kernel");
+  return ok();
+}
+
+// The split-K kernel by shape.  Few rows over up to 8192 columns: 32 columns a workgroup
+// and 8 waves, for as many workgroups as there are (16 x 4096 x 4096: 16 x 32 11.9 us,
+// 32 x 64 14.8, 64 x 64 16.4; 16 x 16384 x 4096: 38.6, 25.8, 26.8).  Else 32 x 64 up to
+// four tiles per CU (64 x 4096 x 4096: 15.6 us against 21.3 for 64 x 64; 1628 x 800 x 1109:
+// 14.9 against 17.4), 64 x 64 past that (1531 x 4096 x 1024: 28.2 against 33.3;
+// 4032 x 843 x 2744: 62.7 against 83.8).  Widths of 32 .. 63 take 32 columns.
+template <typename T, typename OutT, class E>
+int launch_split(const LpArgs<E>& x) {
+  if (x.n < 64 || (x.m <= 32 && x.n <= 8192))
+    return x.m <= 16 ? launch_split_as<T, OutT, 1, 2, 8>(x) : launch_split_as<T, OutT, 2, 2, 8>(x);
+  if (tile_count(x.m, x.n, 32, 64) <= 1024) return launch_split_as<T, OutT, 2, 4, 4>(x);
+  return launch_split_as<T, OutT, 4, 4, 4>(x);
+}
+
+// The register-staged kernel's checked forms at the requested tile: what is narrower than
+// any other kernel's tile, or past their 32-bit offsets or grids.
+template <typename T, typename OutT, int BM, int BN, class E>
+int launch_staged(const LpArgs<E>& x, bool vec) {
+  const int64_t tiles = tile_count(x.m, x.n, BM, BN);
+  if (int rc = check_grid<E>(tiles, kMfmaThreads)) return rc;
+  auto* fn = vec ? &gemm_lp_kernel<T, OutT, BM, BN, true, false, E>
+                 : &gemm_lp_kernel<T, OutT, BM, BN, false, false, E>;
+  fn<<<static_cast<unsigned>(tiles), kMfmaThreads, 0, x.s>>>(
+      x.a, x.b, static_cast<OutT*>(x.c), x.m, x.n, x.k, x.alpha, x.beta,
+      steps_along(x.m, BM), steps_along(x.n, BN), x.ep);
+  MCKE_LAUNCH_CHECK("gemm_lp_kernel");
+  return ok();
+}
+
+// Short K over many tiles: the product is its C store, and the register-staged kernel's four
+// waves share a tile's one stage where the split-K kernel has one wave work and three add
+// zeros.  16-byte operands up to 63 of K (fp16 to fp16, 2460 x 1608 x 40: 6.7 us at 64 x 64
+// against 9.9 for split K; up to 1024 tiles they tie, fp32 C, 853 x 1880 x 64 5.5 against 5.4),
+// others up to 7, as their loads are element by element (fp32 C, 2293 x 1737 x 7: 10.3 against
+// 12.8; x 15: 11.6 against 11.7).  128 x 128 tiles where they fill two rounds of CUs or more to 80%
+// (2166 x 3544 x 40: 10.9 us against 12.1 at 64 x 64; 2460 x 1608, 260 tiles: 10.3 against 7.6).
+template <class E> bool short_k(const LpArgs<E>& x, bool vec) {
+  return x.k < (vec ? 64 : 8) && tile_count(x.m, x.n, 32, 64) > 1024;
+}
+
+template <typename T, typename OutT, class E>
+int launch_short_k(const LpArgs<E>& x, bool vec) {
+  const int64_t tiles = tile_count(x.m, x.n, 128, 128), rounds = (tiles + 255) / 256;
+  if (rounds >= 2 && 10 * tiles >= 8 * 256 * rounds)
+    return launch_staged<T, OutT, 128, 128>(x, vec);
+  return launch_staged<T, OutT, 64, 64>(x, vec);
+}
+
+// The WHOLE form.
+template <typename T, typename OutT, int BM, int BN, class E>
+int launch_whole(const LpArgs<E>& x) {
+  const int64_t tiles = tile_count(x.m, x.n, BM, BN);
+  if (int rc = check_grid<E>(tiles, kMfmaThreads)) return rc;
+  gemm_lp_kernel<T, OutT, BM, BN, false, true, E>
+      <<<static_cast<unsigned>(tiles), kMfmaThreads, 0, x.s>>>(
+          x.a, x.b, static_cast<OutT*>(x.c), x.m, x.n, x.k, x.alpha, x.beta,
+          steps_along(x.m, BM), steps_along(x.n, BN), x.ep);
+  MCKE_LAUNCH_CHECK("gemm_lp_kernel");
+  return ok();
+}
+
+template <typename T, typename OutT, int BM, int BN>
+int launch_dma32(const LpArgs<NoEpilogue>& x) {
+  constexpr int kStages = 4;
+  const int64_t tiles = tile_count(x.m, x.n, BM, BN);
+  if (int rc = check_grid<NoEpilogue>(tiles, kMfmaThreads)) return rc;
+  gemm_lp_dma_kernel<T, OutT, BM, BN, kStages>
+      <<<static_cast<unsigned>(tiles), kMfmaThreads, 0, x.s>>>(
+          x.a, x.b, static_cast<OutT*>(x.c), x.m, x.n, x.k, x.alpha, x.beta, x.m / BM, x.n / BN);
+  MCKE_LAUNCH_CHECK("gemm_lp_dma_kernel");
+  return ok();
+}
+
+// The EDGE form at BM x BN, where the shape and the addresses allow it.
+template <int BM, int BN, class E> bool edge_fits(const LpArgs<E>& x) {
+  return x.n >= BN && x.k >= 64 && x.n % 2 == 0 && x.k % 2 == 0 && aligned(x.a, 4) &&
+         aligned(x.b, 4) && aligned(x.c, 4) && dma_offsets32<BM, BN>(x.n, x.k);
+}
+
+// The register-staged kernel's WHOLE form at BM x BN, where the shape and the addresses
+// allow it.
+template <int BM, int BN, typename OutT, class E> bool whole_fits(const LpArgs<E>& x) {
+  return x.n >= BN && x.k >= 64 && aligned(x.a, 2) && aligned(x.b, 2) &&
+         aligned(x.c, sizeof(OutT));
+}
+
+template <typename T, typename OutT, int BM, int BN>
+struct LpTile {
+  // Whole tiles run the requested tile's direct-to-LDS kernel (tiles of 128 and more).
+  // Other shapes run its EDGE form, at 128 x 128 from 208 such tiles on, or from 80 on where
+  // K is long enough to pay for a tile alone on its CU, and at 256 x 256 where they nearly
+  // fill the CUs (fp16 to fp32: 2757 x 432 x 6080, 88 tiles of 128, 49.8 us against 56.9 for
+  // split K; 1628 x 800 x 1110, 91 tiles, 15.9 against 15.2; 300 x 520 x 1032, 15 tiles, 14.4
+  // against 7.6; 4524 x 344 x 96, 108 tiles, 7.5 against 5.8, to fp16 5.9 against 5.5;
+  // 4095 x 4094 x 4090, 256 tiles of 256, 126 us against 206 at 128).  Odd extents run the
+  // register-staged kernel's WHOLE form where its 128 x 128 tiles fill most of the CUs (a tile
+  // alone on its CU takes 1.3 us per 64 of K, so fewer lose to split K: 1531 x 1021 x 2053, 96
+  // tiles, 44.4 us against 29.9; 1700 x 1701 x 1024, 196 tiles, 24.0 against 20.8;
+  // 4032 x 843 x 2744, 224 tiles, 54.5 against 63.9; 1901 x 2001 x 511, 240 tiles, 20.4 against
+  // 22.1; 3001 x 2501 x 901, 480 tiles, 33.1 against 50.0), at 256 x 256 from 192 such tiles on
+  // (4095^3 199 us against 229 at 128 and 406 for split K; 3500 x 3501 x 2001, 196 tiles, 99
+  // against 105).  What is left takes the split-K kernel, as 64 x 64 launches do, but for
+  // short K over many tiles (short_k).  The tile counts here and below are for 256 CUs.
+  template <class E> static int launch(const LpArgs<E>& x, bool vec) {
+    if constexpr (BN >= 128) {
+      if (vec && x.m % BM == 0 && x.n % BN == 0 && x.k % 64 == 0 && x.k > 0 &&
+          dma_offsets32<BM, BN>(x.n, x.k))
+        return launch_dma<T, OutT, BM, BN, false>(x);
+      // (With an epilogue these take the EDGE form.)
+      if constexpr (BM == 128 && !E::kFused)
+        if (vec && x.m % BM == 0 && x.n % BN == 0 && x.k % 64 == 32 &&
+            tile_count(x.m, x.n, BM, BN) >= 80 && dma_offsets32<BM, BN>(x.n, x.k))
+          return launch_dma32<T, OutT, BM, BN>(x);
+      if constexpr (BM == 256)
+        if (edge_fits<256, 256>(x) && tile_count(x.m, x.n, 256, 256) >= 192)
+          return launch_dma<T, OutT, 256, 256, true>(x);
+      const int64_t tiles = tile_count(x.m, x.n, 128, 128);
+      if (edge_fits<128, 128>(x) &&
+          (tiles >= 208 || (tiles >= 80 && x.k >= (sizeof(OutT) == 4 ? 256 : 100))))
+        return launch_dma<T, OutT, 128, 128, true>(x);
+      if constexpr (BM == 256)
+        if (whole_fits<256, 256, OutT>(x) && tile_count(x.m, x.n, 256, 256) >= 192)
+          return launch_whole<T, OutT, 256, 256>(x);
+      if (whole_fits<128, 128, OutT>(x) && tiles >= 208)
+        return launch_whole<T, OutT, 128, 128>(x);
+    }
+    // 16-bit values at 2-byte addresses, per-lane offsets below 4 GiB, and a grid that holds
+    // 32 x 32 tiles of 512 lanes.
+    if (x.n >= 32 && x.k > 0 && tile_count(x.m, x.n, 32, 32) <= int64_t{UINT32_MAX} / 512 &&
+        aligned(x.a, 2) && aligned(x.b, 2) && aligned(x.c, sizeof(OutT)) &&
+        static_cast<int64_t>(64) * x.k * 2 < (int64_t{1} << 32) &&
+        static_cast<int64_t>(64) * x.n * 2 < (int64_t{1} << 32))
+      return short_k(x, vec) ? launch_short_k<T, OutT>(x, vec) : launch_split<T, OutT>(x);
+    // (With an epilogue at most 128 x 128: the checked 256 x 256 form spills as it is.)
+    if constexpr (E::kFused && BM == 256) return launch_staged<T, OutT, 128, 128>(x, vec);
+    else return launch_staged<T, OutT, BM, BN>(x, vec);
+  }
+  // The instantiation whole-tile shapes run, for attribute queries.
+  static LpKernel kernel() {
+    if constexpr (BN >= 128)
+      return reinterpret_cast<LpKernel>(&gemm_lp_dma16_kernel<T, OutT, BM, BN, false>);
+    else
+      return reinterpret_cast<LpKernel>(&gemm_lp_split_kernel<T, OutT, 4, 4, 4>);
+  }
+};
+
+// Instantiated tiles: (bm, bn) with bk = 64 and 256 lanes, so (tm, tn) = (bm/16, bn/16).
+constexpr int kLpTiles[][2] = {{256, 256}, {128, 128}, {64, 64}};
+
+inline int lp_tile_index(const mcke_gemm_tile* t) {
+  if (!t) return -1;
+  for (int i = 0; i < 3; ++i) {
+    const int bm = kLpTiles[i][0], bn = kLpTiles[i][1];
+    if (t->bm == bm && t->bn == bn && t->bk == kLpBK && t->tm == bm / 16 && t->tn == bn / 16)
+      return i;
+  }
+  return -1;
+}
+
+template <typename T, typename OutT>
+struct LpTable {
+  template <class E> static int launch(int ti, const LpArgs<E>& x, bool vec) {
+    switch (ti) {
+      case 0: return LpTile<T, OutT, 256, 256>::launch(x, vec);
+      case 1: return LpTile<T, OutT, 128, 128>::launch(x, vec);
+      default: return LpTile<T, OutT, 64, 64>::launch(x, vec);
+    }
+  }
+  static LpKernel kernel(int ti) {
+    switch (ti) {
+      case 0: return LpTile<T, OutT, 256, 256>::kernel();
+      case 1: return LpTile<T, OutT, 128, 128>::kernel();
+      default: return LpTile<T, OutT, 64, 64>::kernel();
+    }
+  }
+};
+
+// The products with an epilogue, each pair of types in a translation unit with its kernels.
+int launch_fused_bf16_f32(int ti, const LpArgs<Epilogue>& x, bool vec);
+int launch_fused_bf16_bf16(int ti, const LpArgs<Epilogue>& x, bool vec);
+int launch_fused_f16_f32(int ti, const LpArgs<Epilogue>& x, bool vec);
+int launch_fused_f16_f16(int ti, const LpArgs<Epilogue>& x, bool vec);
+
+}  // namespace mcke_amd

@@ -63,10 +63,10 @@ struct LpSplitShape {
   }
 };
 
-template <typename T, typename OutT, int MT, int NW, int WV>
+template <typename T, typename OutT, int MT, int NW, int WV, class E = NoEpilogue>
 __global__ __launch_bounds__(WV * 64) void gemm_lp_split_kernel(
-    const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, OutT* __restrict__ C, int M,
-    int N, int K, float alpha, float beta, int tiles_m, int tiles_n) {
+    const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, OutPtr<OutT, E> C, int M,
+    int N, int K, float alpha, float beta, int tiles_m, int tiles_n, E ep) {
   using S = LpSplitShape<MT, NW, WV>;
   constexpr int L = S::L;
   __shared__ __attribute__((aligned(1024))) char smem[S::kLds];
@@ -257,10 +257,23 @@ __global__ __launch_bounds__(WV * 64) void gemm_lp_split_kernel(
     for (int w = 1; w < S::kFold; ++w)
       s += *reinterpret_cast<const f32x4*>(sums + w * S::kOut + o);
     OutT* p = C + static_cast<int64_t>(row) * N + col;
+    if constexpr (E::kFused) {
+      const OutT* res = static_cast<const OutT*>(ep.residual);
+      with_act(ep.act, [&](auto act) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[j] *= alpha;
-      if (beta != 0.0f && col + j >= n_first) s[j] += beta * O::to_f32(p[j]);
+        for (int j = 0; j < 4; ++j) {
+          if (col + j < n_first) continue;
+          const float b = ep.bias ? load_elem(ep.bias, ep.bias_dtype, col + j) : 0.0f;
+          const float old = res ? O::to_f32(res[static_cast<int64_t>(row) * N + col + j]) : 0.0f;
+          s[j] = fused_value<decltype(act)::value>(alpha * s[j], b, old);
+        }
+      });
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[j] *= alpha;
+        if (beta != 0.0f && col + j >= n_first) s[j] += beta * O::to_f32(p[j]);
+      }
     }
     if (col >= n_first) {
       Pack out;

@@ -1,0 +1,520 @@
+// token_logprobs.hip -- log probabilities of given tokens, the entropy and the most likely
+// alternatives of each row of logits, and the gradient of the first two.
+//
+//   z = scale x,  lse = log sum exp z,  logprob = z[token] - lse
+//   entropy = -sum p log p,  p = exp(z - lse)
+//   alternatives: the top_k largest logits by (value, then lowest index), and their z - lse
+//
+//   d logprob / d z_j = [j == token] - p_j,   d entropy / d z_j = -p_j (log p_j + entropy)
+//
+// One pass over a row carries, per lane, the largest logit m, d = sum 2^u and
+// e = sum u 2^u with u = (x - m) scale log2 e <= 0 (the online softmax with one more sum).
+// Two states join at M = max(m1, m2) with delta = (m - M) scale log2 e:
+//   d -> 2^delta d,   e -> 2^delta (e + delta d)
+// and then lse = scale M + ln d,  entropy = ln d - ln2 e / d, so neither needs p itself.
+// A masked logit (-inf) adds nothing to either; u and delta are held above -1e4, where 2^u is
+// already 0, so that 0 times -inf does not arise.  All arithmetic is fp32.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <string>
+
+#include "common.hpp"
+#include "device_math.hpp"
+#include "elem.hpp"
+
+namespace mcke_amd {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kMaxTop = 64;             // a list lies across a wave, an entry to a lane
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kFar = -1.0e4f;
+
+// ---------------------------------------------------------------------------
+// The sums
+// ---------------------------------------------------------------------------
+struct Sums {
+  float m, d, e;
+};
+
+__device__ __forceinline__ Sums no_sums() { return {-INFINITY, 0.0f, 0.0f}; }
+
+// What a state's exponents move by when the maximum becomes `to`.
+__device__ __forceinline__ float shift_of(float m, float to, float c) {
+  return m == to ? 0.0f : fmaxf((m - to) * c, kFar);
+}
+
+__device__ __forceinline__ Sums moved(Sums s, float to, float c) {
+  const float t = shift_of(s.m, to, c), f = __builtin_amdgcn_exp2f(t);
+  return {to, f * s.d, f * (s.e + t * s.d)};
+}
+
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  a = moved(a, m, c);
+  b = moved(b, m, c);
+  return {m, a.d + b.d, a.e + b.e};
+}
+
+__device__ __forceinline__ Sums wave_join(Sums s, float c) {
+#pragma unroll
+  for (int k = kWave / 2; k >= 1; k >>= 1)
+    s = join(s, Sums{__shfl_xor(s.m, k, 64), __shfl_xor(s.d, k, 64), __shfl_xor(s.e, k, 64)}, c);
+  return s;
+}
+
+template <int VE, bool ENTROPY>
+__device__ __forceinline__ Sums add_values(Sums s, const float (&v)[VE], float m, float c) {
+  if (m > s.m) s = moved(s, m, c);
+  const float from = s.m == -INFINITY ? 0.0f : s.m;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    const float u = (v[i] - from) * c;
+    const float p = __builtin_amdgcn_exp2f(u);
+    s.d += p;
+    if constexpr (ENTROPY) s.e += p * fmaxf(u, kFar);
+  }
+  return s;
+}
+
+// ---------------------------------------------------------------------------
+// The alternatives
+// ---------------------------------------------------------------------------
+// Value and index as one number that orders by value, then by lowest index; -0 counts as +0.
+// 0 is below every key.
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
+  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return static_cast<uint64_t>(o) << 32 | (0xFFFFFFFFu - index);
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t o = static_cast<uint32_t>(k >> 32);
+  return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t k) {
+  return 0xFFFFFFFFu - static_cast<uint32_t>(k);
+}
+
+// A wave's list: lane i holds the i-th best so far.  Elements come in the order of their
+// indices, so one that equals the worst of a full list loses to it.  A NaN is never taken.
+struct TopList {
+  float v;          // lane's entry
+  uint32_t i;
+  int count, k;     // uniform
+  float least;      // uniform: what a new element has to reach
+
+  __device__ __forceinline__ void start(int top_k) {
+    v = 0.0f;
+    i = 0;
+    count = 0;
+    k = top_k;
+    least = -INFINITY;
+  }
+  __device__ __forceinline__ void insert(float x, uint32_t index) {
+    const int lane = threadIdx.x % kWave;
+    const int at = __popcll(__ballot(lane < count && v >= x));
+    const float pv = __shfl_up(v, 1, 64);
+    const uint32_t pi = __shfl_up(i, 1, 64);
+    if (lane > at) {
+      v = pv;
+      i = pi;
+    } else if (lane == at) {
+      v = x;
+      i = index;
+    }
+    if (count < k) ++count;
+    if (count == k) {
+      // The next larger float: past +inf a NaN, which nothing reaches.
+      const float worst =
+          __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), k - 1));
+      const int b = __builtin_bit_cast(int, worst + 0.0f);
+      least = __builtin_bit_cast(float, b >= 0 ? b + 1 : b - 1);
+    }
+  }
+  // The lanes' values v[0 ..], lane l's first one at index first + VE * l.
+  template <int VE>
+  __device__ __forceinline__ void offer(const float (&x)[VE], float m, uint32_t first) {
+    uint64_t hot = __ballot(m >= least);
+    while (hot) {
+      const int l = __ffsll(static_cast<unsigned long long>(hot)) - 1;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float y =
+            __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x[e]), l));
+        if (y >= least) insert(y, first + static_cast<uint32_t>(VE * l + e));
+      }
+      hot &= hot - 1;
+      hot &= __ballot(m >= least);
+    }
+  }
+};
+
+// The top_k largest of n keys in LDS, to `best` in their order; empty keys behind.
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int top_k, uint64_t* best) {
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t mine = keys[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += keys[j] > mine || (keys[j] == mine && j < i);
+    if (rank < top_k) best[rank] = mine;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Kernels
+// ---------------------------------------------------------------------------
+struct RowOut {
+  const int64_t* tokens;
+  float *logprobs, *entropy, *lse, *top_logprobs;
+  int64_t* top_ids;
+};
+
+// A row's results from its sums and its best keys in LDS.
+template <typename T>
+__device__ __forceinline__ void write_row(const RowOut& o, const T* __restrict__ row, int64_t r,
+                                          int64_t vocab, Sums s, const uint64_t* best, int top_k,
+                                          float scale) {
+  const float ln_d = logf(s.d);
+  const bool empty = s.m == -INFINITY && s.d == 0.0f;   // every logit is masked
+  if (threadIdx.x == 0) {
+    if (o.logprobs) {
+      const int64_t t = o.tokens[r];
+      float lp = __builtin_nanf("");                    // no such token
+      if (t < vocab) lp = empty ? -INFINITY : (static_cast<float>(row[t]) - s.m) * scale - ln_d;
+      o.logprobs[r] = lp;
+    }
+    if (o.entropy) o.entropy[r] = empty ? 0.0f : ln_d - kLn2 * (s.e / s.d);
+    if (o.lse) o.lse[r] = empty ? -INFINITY : s.m * scale + ln_d;
+  }
+  for (int i = threadIdx.x; i < top_k; i += kThreads) {
+    const uint64_t k = best[i];
+    const float v = empty ? -INFINITY : (key_value(k) - s.m) * scale - ln_d;
+    if (o.top_logprobs) o.top_logprobs[r * top_k + i] = k ? v : __builtin_nanf("");
+    if (o.top_ids) o.top_ids[r * top_k + i] = k ? static_cast<int64_t>(key_index(k)) : -1;
+  }
+}
+
+// A row without a token is not read.
+__device__ __forceinline__ bool skip_row(const RowOut& o, int64_t r, int top_k, bool write) {
+  if (!o.tokens || o.tokens[r] >= 0) return false;
+  if (write) {
+    if (threadIdx.x == 0) {
+      if (o.logprobs) o.logprobs[r] = 0.0f;
+      if (o.entropy) o.entropy[r] = 0.0f;
+      if (o.lse) o.lse[r] = 0.0f;
+    }
+    for (int i = threadIdx.x; i < top_k; i += kThreads) {
+      if (o.top_logprobs) o.top_logprobs[r * top_k + i] = 0.0f;
+      if (o.top_ids) o.top_ids[r * top_k + i] = -1;
+    }
+  }
+  return true;
+}
+
+// A part of a row as it lies in the workspace.
+struct Part {
+  float m, d, e, unused;
+};
+
+// Workgroup (row, part): vectors part * per_part on, 64 adjacent ones to a wave.  With one
+// part the row's results are written here, else its sums and keys go to the workspace.
+template <typename T, bool ENTROPY>
+__global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ x, RowOut o,
+                                                            Part* __restrict__ parts_out,
+                                                            uint64_t* __restrict__ keys_out,
+                                                            int64_t vocab, int64_t row_stride,
+                                                            int parts, int64_t per_part,
+                                                            float scale, int top_k) {
+  constexpr int VE = kVecElems<T>;
+  __shared__ uint64_t keys[kWaves * kMaxTop], best[kMaxTop];
+  __shared__ Sums waves[kWaves];
+  const int64_t r = blockIdx.x / parts;
+  const int part = static_cast<int>(blockIdx.x % parts);
+  if (skip_row(o, r, top_k, parts == 1)) return;
+  const T* row = x + r * row_stride;
+  const float c = scale * kLog2e;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t all = (vocab + VE - 1) / VE, first = part * per_part;
+  const int64_t end = first + per_part < all ? first + per_part : all;
+
+  Sums s = no_sums();
+  TopList top;
+  top.start(top_k);
+  for (int64_t j0 = first + wave * kWave; j0 < end; j0 += kThreads) {
+    const int64_t j = j0 + lane;
+    VecT16<T> w;
+    if (j >= end) w = load_part<T>(row, 0, -INFINITY);
+    else if ((j + 1) * VE <= vocab) w = load_vec<T>(row + j * VE);
+    else w = load_part<T>(row + j * VE, static_cast<int>(vocab - j * VE), -INFINITY);
+    float v[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] = static_cast<float>(w[e]);
+    float m = v[0];
+#pragma unroll
+    for (int e = 1; e < VE; ++e) m = fmaxf(m, v[e]);
+    s = add_values<VE, ENTROPY>(s, v, m, c);
+    if (top_k > 0) {
+      // Past the end nothing is offered, not even -inf.
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (j * VE + e >= vocab || j >= end) v[e] = __builtin_nanf("");
+      if (j >= end) m = __builtin_nanf("");
+      top.offer<VE>(v, m, static_cast<uint32_t>(j0 * VE));
+    }
+  }
+  s = wave_join(s, c);
+  if (lane == 0) waves[wave] = s;
+  if (lane < top_k) keys[wave * top_k + lane] = lane < top.count ? key_of(top.v, top.i) : 0;
+  __syncthreads();
+  s = waves[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) s = join(s, waves[w], c);
+  rank_keys(keys, kWaves * top_k, top_k, best);
+  __syncthreads();
+  if (parts == 1) {
+    write_row(o, row, r, vocab, s, best, top_k, scale);
+    return;
+  }
+  if (threadIdx.x == 0) parts_out[blockIdx.x] = Part{s.m, s.d, s.e, 0.0f};
+  for (int i = threadIdx.x; i < top_k; i += kThreads)
+    keys_out[static_cast<int64_t>(blockIdx.x) * top_k + i] = best[i];
+}
+
+constexpr int kMaxPartKeys = 1024;   // keys of all parts of a row
+
+// A row's parts joined in their order, a workgroup per row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(
+    const T* __restrict__ x, RowOut o, const Part* __restrict__ parts_in,
+    const uint64_t* __restrict__ keys_in, int64_t vocab, int64_t row_stride, int parts,
+    float scale, int top_k) {
+  __shared__ uint64_t keys[kMaxPartKeys], best[kMaxTop];
+  const int64_t r = blockIdx.x;
+  if (skip_row(o, r, top_k, true)) return;
+  const float c = scale * kLog2e;
+  Sums s = no_sums();
+  for (int p = 0; p < parts; ++p) {
+    const Part q = parts_in[r * parts + p];
+    s = join(s, Sums{q.m, q.d, q.e}, c);
+  }
+  const int n = parts * top_k;
+  for (int i = threadIdx.x; i < n; i += kThreads) keys[i] = keys_in[r * n + i];
+  __syncthreads();
+  rank_keys(keys, n, top_k, best);
+  __syncthreads();
+  write_row(o, x + r * row_stride, r, vocab, s, best, top_k, scale);
+}
+
+// dlogits = scale (g ([j == token] - p_j) - h p_j (log p_j + entropy)), g and h the gradients
+// of the row's logprob and entropy: one 16-byte vector to a lane, a workgroup per kThreads
+// vectors of a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(
+    const T* __restrict__ x, const int64_t* __restrict__ tokens, const float* __restrict__ lse_in,
+    const float* __restrict__ entropy, const float* __restrict__ dlogprobs,
+    const float* __restrict__ dentropy, T* __restrict__ dx, int64_t vocab, int64_t row_stride,
+    int per_row, float scale) {
+  constexpr int VE = kVecElems<T>;
+  const int64_t r = blockIdx.x / per_row;
+  const int64_t at = (static_cast<int64_t>(blockIdx.x % per_row) * kThreads + threadIdx.x) * VE;
+  if (at >= vocab) return;
+  const int n = vocab - at < VE ? static_cast<int>(vocab - at) : VE;
+  const int64_t token = tokens ? tokens[r] : 0;
+  const float lse = lse_in[r];
+  T* out = dx + r * row_stride + at;
+  VecT16<T> w;
+  if (token < 0 || lse == -INFINITY || token >= vocab) {
+    // No token or no probability: no gradient.  No such token: a NaN, as forward.
+    const float none = token < vocab ? 0.0f : __builtin_nanf("");
+#pragma unroll
+    for (int e = 0; e < VE; ++e) w[e] = static_cast<T>(none);
+  } else {
+    const T* in = x + r * row_stride + at;
+    w = n == VE ? load_vec<T>(in) : load_part<T>(in, n, 0.0f);
+    const float g = dlogprobs ? scale * dlogprobs[r] : 0.0f;
+    const float h = dentropy ? scale * dentropy[r] : 0.0f;
+    const float a = dentropy ? -(g + h * entropy[r]) : -g;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float lp = static_cast<float>(w[e]) * scale - lse;
+      float d = __builtin_amdgcn_exp2f(lp * kLog2e) * (a - h * fmaxf(lp, kFar));
+      if (dlogprobs && at + e == token) d += g;
+      w[e] = static_cast<T>(d);
+    }
+  }
+  if (n == VE) *reinterpret_cast<VecT16<T>*>(out) = w;
+  else store_part<T>(out, w, n);
+}
+
+// ---------------------------------------------------------------------------
+// Launchers
+// ---------------------------------------------------------------------------
+// How many workgroups share a row: as many as fill the GPU where there are few rows, at
+// least 2048 logits each, and no more keys than the joining workgroup holds.
+int parts_of(int64_t rows, int64_t vocab, int top_k) {
+  int64_t p = 1024 / (rows > 0 ? rows : 1);
+  const int64_t most = (vocab + 2047) / 2048;
+  if (p > most) p = most;
+  if (p > 64) p = 64;
+  if (top_k > 0 && p > kMaxPartKeys / top_k) p = kMaxPartKeys / top_k;
+  return p < 1 ? 1 : static_cast<int>(p);
+}
+
+struct RowArgs {
+  const void* logits;
+  RowOut o;
+  int64_t rows, vocab, row_stride;
+  float scale;
+  int top_k;
+  void* ws;
+  hipStream_t s;
+};
+
+template <typename T> int logprobs(const RowArgs& a) {
+  const int parts = parts_of(a.rows, a.vocab, a.top_k);
+  const int64_t vecs = (a.vocab + kVecElems<T> - 1) / kVecElems<T>;
+  const int64_t per_part = (vecs + parts - 1) / parts;
+  const T* x = static_cast<const T*>(a.logits);
+  Part* sums = static_cast<Part*>(a.ws);
+  uint64_t* keys = reinterpret_cast<uint64_t*>(sums + (parts > 1 ? a.rows * parts : 0));
+  const unsigned grid = static_cast<unsigned>(a.rows * parts);
+  auto* fn = a.o.entropy ? &logprobs_kernel<T, true> : &logprobs_kernel<T, false>;
+  fn<<<grid, kThreads, 0, a.s>>>(x, a.o, sums, keys, a.vocab, a.row_stride, parts, per_part,
+                                 a.scale, a.top_k);
+  MCKE_LAUNCH_CHECK("logprobs_kernel");
+  if (parts > 1) {
+    logprobs_join_kernel<T><<<static_cast<unsigned>(a.rows), kThreads, 0, a.s>>>(
+        x, a.o, sums, keys, a.vocab, a.row_stride, parts, a.scale, a.top_k);
+    MCKE_LAUNCH_CHECK("logprobs_join_kernel");
+  }
+  return ok();
+}
+
+int check_logits(const char* who, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                 float scale) {
+  const std::string w(who);
+  if (!is_dtype(dtype)) return invalid(w + ": unknown dtype " + std::to_string(dtype));
+  if (rows < 0 || vocab < 0) return invalid(w + ": negative extent");
+  if (vocab > 2147483647LL) return invalid(w + ": vocab exceeds INT32_MAX");
+  if (row_stride < vocab) return invalid(w + ": row_stride is less than vocab");
+  if (rows > 0 && row_stride > INT64_MAX / 16 / rows) return invalid(w + ": extent too large");
+  if (!(scale > 0.0f) || std::isinf(scale * kLog2e))
+    return invalid(w + ": scale must be finite and above zero");
+  return ok();
+}
+
+// Bytes from the first logit to behind the last.
+uint64_t logits_bytes(int dtype, int64_t rows, int64_t vocab, int64_t row_stride) {
+  return dtype_bytes(dtype) * (static_cast<uint64_t>(rows - 1) * row_stride + vocab);
+}
+
+}  // namespace
+}  // namespace mcke_amd
+
+using namespace mcke_amd;
+
+extern "C" {
+
+size_t mcke_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k) {
+  if (rows <= 0 || vocab <= 0 || top_k < 0 || top_k > kMaxTop) return 0;
+  const int parts = parts_of(rows, vocab, top_k);
+  if (parts == 1) return 0;
+  return static_cast<size_t>(rows) * parts * (sizeof(Part) + sizeof(uint64_t) * top_k);
+}
+
+int mcke_launch_token_logprobs(const void* logits, const int64_t* tokens, float* logprobs_out,
+                               float* entropy, float* lse, float* top_logprobs, int64_t* top_ids,
+                               int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                               float scale, int top_k, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  const char* who = "launch_token_logprobs";
+  if (int rc = check_logits(who, dtype, rows, vocab, row_stride, scale)) return rc;
+  if (top_k < 0 || top_k > kMaxTop || top_k > vocab)
+    return invalid("launch_token_logprobs: top_k must be between 0 and 64 and at most vocab");
+  if (rows == 0 || vocab == 0) return ok();
+  if (!logits) return invalid("launch_token_logprobs: null pointer");
+  if (logprobs_out && !tokens)
+    return invalid("launch_token_logprobs: log probabilities need tokens");
+  if (top_k > 0 && !top_logprobs && !top_ids)
+    return invalid("launch_token_logprobs: top_k without an output for the alternatives");
+  if (!logprobs_out && !entropy && !lse && top_k == 0)
+    return invalid("launch_token_logprobs: no output is asked for");
+  if (!aligned(logits, dtype_bytes(dtype)) || !aligned(tokens, 8) || !aligned(logprobs_out, 4) ||
+      !aligned(entropy, 4) || !aligned(lse, 4) || !aligned(top_logprobs, 4) || !aligned(top_ids, 8))
+    return invalid("launch_token_logprobs: a pointer is not aligned to its type");
+  if (rows * parts_of(rows, vocab, top_k) > int64_t{UINT32_MAX} / kThreads)
+    return invalid("launch_token_logprobs: rows exceed the grid's 32-bit work size");
+  const size_t need = mcke_token_logprobs_workspace_bytes(rows, vocab, top_k);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return invalid("launch_token_logprobs: these rows need a 16-byte aligned workspace of " +
+                   std::to_string(need) + " bytes, got " +
+                   std::to_string(workspace ? workspace_bytes : 0));
+  const uint64_t in = logits_bytes(dtype, rows, vocab, row_stride), n = rows, k = top_k;
+  if (top_k == 0) top_logprobs = nullptr, top_ids = nullptr;
+  const void* outs[] = {logprobs_out, entropy, lse, top_logprobs, top_ids,
+                        need > 0 ? workspace : nullptr};
+  const uint64_t out_bytes[] = {4 * n, 4 * n, 4 * n, 4 * n * k, 8 * n * k, need};
+  for (int i = 0; i < 6; ++i) {
+    bool bad = overlap(outs[i], out_bytes[i], logits, in) ||
+               overlap(outs[i], out_bytes[i], tokens, 8 * n);
+    for (int j = 0; j < i; ++j) bad |= overlap(outs[i], out_bytes[i], outs[j], out_bytes[j]);
+    if (bad)
+      return invalid("launch_token_logprobs: an output or the workspace overlaps another operand, "
+                     "which violates the __restrict__ contract");
+  }
+  const RowArgs a{logits, RowOut{tokens, logprobs_out, entropy, lse, top_logprobs, top_ids},
+                 rows, vocab, row_stride, scale, top_k, workspace,
+                 static_cast<hipStream_t>(stream)};
+  if (dtype == MCKE_DTYPE_F32) return logprobs<float>(a);
+  if (dtype == MCKE_DTYPE_F16) return logprobs<_Float16>(a);
+  return logprobs<__bf16>(a);
+}
+
+int mcke_launch_token_logprobs_backward(const void* logits, const int64_t* tokens,
+                                        const float* lse, const float* entropy,
+                                        const float* dlogprobs, const float* dentropy,
+                                        void* dlogits, int dtype, int64_t rows, int64_t vocab,
+                                        int64_t row_stride, float scale, void* stream) {
+  const char* who = "launch_token_logprobs_backward";
+  if (int rc = check_logits(who, dtype, rows, vocab, row_stride, scale)) return rc;
+  if (rows == 0 || vocab == 0) return ok();
+  if (!logits || !lse || !dlogits)
+    return invalid("launch_token_logprobs_backward: null pointer");
+  if (!dlogprobs && !dentropy)
+    return invalid("launch_token_logprobs_backward: no gradient is given");
+  if (dlogprobs && !tokens)
+    return invalid("launch_token_logprobs_backward: dlogprobs need tokens");
+  if (dentropy && !entropy)
+    return invalid("launch_token_logprobs_backward: dentropy needs the entropies");
+  const uint64_t e = dtype_bytes(dtype), n = rows;
+  if (!aligned(logits, e) || !aligned(dlogits, e) || !aligned(tokens, 8) || !aligned(lse, 4) ||
+      !aligned(entropy, 4) || !aligned(dlogprobs, 4) || !aligned(dentropy, 4))
+    return invalid("launch_token_logprobs_backward: a pointer is not aligned to its type");
+  const uint64_t bytes = logits_bytes(dtype, rows, vocab, row_stride);
+  if (overlap(dlogits, bytes, logits, bytes) || overlap(dlogits, bytes, tokens, 8 * n) ||
+      overlap(dlogits, bytes, lse, 4 * n) || overlap(dlogits, bytes, entropy, 4 * n) ||
+      overlap(dlogits, bytes, dlogprobs, 4 * n) || overlap(dlogits, bytes, dentropy, 4 * n))
+    return invalid("launch_token_logprobs_backward: dlogits overlaps an input, which violates the "
+                   "__restrict__ contract");
+  const int64_t per_wg = kThreads * (16 / static_cast<int64_t>(e));
+  const int64_t per_row = (vocab + per_wg - 1) / per_wg;
+  if (rows * per_row > int64_t{UINT32_MAX} / kThreads)
+    return invalid("launch_token_logprobs_backward: rows x vocab exceed the grid's 32-bit work "
+                   "size");
+  const unsigned grid = static_cast<unsigned>(rows * per_row);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  auto launch = [&]<typename T>(T*) {
+    logprobs_backward_kernel<T><<<grid, kThreads, 0, s>>>(
+        static_cast<const T*>(logits), tokens, lse, entropy, dlogprobs, dentropy,
+        static_cast<T*>(dlogits), vocab, row_stride, static_cast<int>(per_row), scale);
+    MCKE_LAUNCH_CHECK("logprobs_backward_kernel");
+    return ok();
+  };
+  if (dtype == MCKE_DTYPE_F32) return launch(static_cast<float*>(nullptr));
+  if (dtype == MCKE_DTYPE_F16) return launch(static_cast<_Float16*>(nullptr));
+  return launch(static_cast<__bf16*>(nullptr));
+}
+
+}  // extern "C"
