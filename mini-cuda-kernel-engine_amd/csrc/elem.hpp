@@ -45,6 +45,35 @@ template <typename T> __device__ __forceinline__ VecT16<T> load_vec(const T* __r
   return *reinterpret_cast<const VecT16<T>*>(p);
 }
 
+// The same, for data that is touched once (non-temporal).
+template <typename T> __device__ __forceinline__ VecT16<T> load_stream(const T* __restrict__ p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const VecT16<T>*>(p));
+}
+template <typename T> __device__ __forceinline__ void store_stream(T* __restrict__ p, VecT16<T> v) {
+  __builtin_nontemporal_store(v, reinterpret_cast<VecT16<T>*>(p));
+}
+
+// N floats from p[c ..] (at P's alignment), or `none` where there is no p.
+template <typename P, int N>
+__device__ __forceinline__ void load_params(float (&v)[N], const P* __restrict__ p, int64_t c,
+                                            float none) {
+  constexpr int VE = kVecElems<P>;
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = none;
+  } else if constexpr (N >= VE) {
+#pragma unroll
+    for (int q = 0; q < N / VE; ++q) {
+      const VecT16<P> w = load_vec<P>(p + c + q * VE);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[q * VE + e] = static_cast<float>(w[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = static_cast<float>(p[c + e]);
+  }
+}
+
 // One element by its dtype, for vectors that are read once per row or launch.
 __device__ __forceinline__ float load_elem(const void* __restrict__ p, int dtype, int64_t i) {
   if (dtype == MCKE_DTYPE_F32) return static_cast<const float*>(p)[i];

@@ -43,6 +43,323 @@ __device__ __forceinline__ f32x2 block_sum2(f32x2 v, f32x2* lds) {
   return s;
 }
 
+// Sums over groups of TPR lanes (a row's), the same bits in every lane of a group.  Groups wider
+// than a wave meet in `lds` (the workgroup's waves), which is free again after the caller's next
+// barrier; every lane of the workgroup calls these.
+template <int TPR, int N, int NW>
+__device__ __forceinline__ void group_sums(float (&v)[N], float (&lds)[N][NW]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = wave_sum<(TPR < kWave ? TPR : kWave)>(v[k]);
+  if constexpr (TPR > kWave) {
+    constexpr int W = TPR / kWave;
+    const int first = (threadIdx.x / TPR) * W;
+    if ((threadIdx.x % kWave) == 0) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) lds[k][threadIdx.x / kWave] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = wave_sum<W>(lds[k][first + threadIdx.x % W]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows that fit in registers: NT-lane workgroups, TPR lanes a row, VPT 16-byte vectors a lane,
+// ROWS rows a lane at once.  x is read once and y written once; a row stays in registers over
+// both reductions.
+// WHOLE: cols is a multiple of the vector.  Otherwise (cols >= one vector) the row's last vector
+// is moved back to end with the row: what it repeats of the vector before it is taken out of
+// the sums again and is stored twice, the same bits.  Loaded and stored element by element instead, the end of
+// each row cost more instructions than the rest of it: 131072 x 500 bf16 69 us against 47.
+// ---------------------------------------------------------------------------
+template <typename T, bool WHOLE> struct RowVectors {
+  static constexpr int VE = kVecElems<T>;
+  int cols;
+  // Whether vector j is the row's, and its first column.
+  __device__ __forceinline__ bool has(int j) const { return j * VE < cols; }
+  __device__ __forceinline__ int col(int j) const {
+    return WHOLE || j * VE + VE <= cols ? j * VE : cols - VE;
+  }
+  // Calls f(e) for the elements of vector j that the one before it has too.
+  template <class F> __device__ __forceinline__ void repeated(int j, F f) const {
+    if constexpr (!WHOLE) {
+      if (has(j) && j * VE + VE > cols) {
+        const int n = (cols + VE - 1) / VE * VE - cols;
+#pragma unroll
+        for (int e = 0; e < VE - 1; ++e)
+          if (e < n) f(e);
+      }
+    }
+  }
+};
+
+template <typename T, typename P, int TPR, int VPT, int NT, int ROWS, bool WHOLE>
+__global__ __launch_bounds__(NT) void ln_fwd_regs_kernel(
+    const T* __restrict__ x, const P* __restrict__ weight, const P* __restrict__ bias,
+    T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows,
+    int cols, float eps) {
+  constexpr int VE = kVecElems<T>;
+  __shared__ float lds[2][ROWS][NT / kWave];
+  const int t = threadIdx.x % TPR;
+  const int64_t r0 =
+      (static_cast<int64_t>(blockIdx.x) * (NT / TPR) + threadIdx.x / TPR) * ROWS;
+  const float n = static_cast<float>(cols);
+  const RowVectors<T, WHOLE> rv{cols};
+
+  // Rows past the end take part in the barriers and in nothing else.
+  float v[ROWS][VPT][VE];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int j = i * TPR + t;
+      VecT16<T> w{};
+      if (r0 + k < rows && rv.has(j)) w = load_stream<T>(x + (r0 + k) * cols + rv.col(j));
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[k][i][e] = static_cast<float>(w[e]);
+    }
+  float mean[ROWS], rstd[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) s += v[k][i][e];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) rv.repeated(i * TPR + t, [&](int e) { s -= v[k][i][e]; });
+    mean[k] = s;
+  }
+  group_sums<TPR, ROWS>(mean, lds[0]);
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    mean[k] /= n;      // (times 1 / n would not be exact where the sum is)
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float qi = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        v[k][i][e] -= mean[k];
+        qi += v[k][i][e] * v[k][i][e];
+      }
+      if (rv.has(i * TPR + t)) q += qi;
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      rv.repeated(i * TPR + t, [&](int e) { q -= v[k][i][e] * v[k][i][e]; });
+    rstd[k] = q;
+  }
+  group_sums<TPR, ROWS>(rstd, lds[1]);
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) rstd[k] = 1.0f / sqrtf(rstd[k] / n + eps);
+
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = i * TPR + t, c = rv.col(j);
+    if (!rv.has(j)) continue;
+    float w[VE], b[VE];
+    load_params<P, VE>(w, weight, c, 1.0f);
+    load_params<P, VE>(b, bias, c, 0.0f);
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      if (r0 + k >= rows) continue;
+      VecT16<T> o;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) o[e] = static_cast<T>(v[k][i][e] * rstd[k] * w[e] + b[e]);
+      store_stream<T>(y + (r0 + k) * cols + c, o);
+    }
+  }
+  if (t == 0) {
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      if (r0 + k >= rows) continue;
+      if (mean_out) mean_out[r0 + k] = mean[k];
+      if (rstd_out) rstd_out[r0 + k] = rstd[k];
+    }
+  }
+}
+
+// The backward pass over rows that fit in registers.  Workgroups walk rows NT / TPR at a time, a
+// lane keeps its columns' sums of dy xhat and dy over all of its rows, and x and dy are read
+// once, each row's behind the one before it.  At the end the groups of a workgroup add up
+// their columns, and the workgroup's sums are rows 2 p and 2 p + 1 of the workspace.  What a
+// row's moved-back last vector repeats is summed up twice to the same bits, and counts once in
+// the row's own sums.
+// PARAMS false: only dx, for rows whose column sums do not fit beside them.
+template <typename T, typename P, int TPR, int VPT, int NT, bool WHOLE, bool PARAMS>
+__global__ __launch_bounds__(NT) void ln_bwd_regs_kernel(
+    const T* __restrict__ dy, const T* __restrict__ x, const P* __restrict__ weight,
+    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx,
+    float* __restrict__ ws, int64_t rows, int cols) {
+  constexpr int VE = kVecElems<T>, G = NT / TPR, NW = NT / kWave;
+  constexpr int kSums = 2 * VPT * VE;                   // of a lane
+  // Groups of a wave add up by lane permutations, those of different waves through LDS.
+  constexpr int L = TPR < kWave ? kWave : TPR;          // lanes that are left to a wave or row
+  constexpr int GL = NT / L;
+  __shared__ float lds[2][2][NW];
+  __shared__ float fold[PARAMS && GL > 1 ? NT * kSums : 1];
+  const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
+  const RowVectors<T, WHOLE> rv{cols};
+  const float inv_n = 1.0f / static_cast<float>(cols);
+
+  // Workgroups of 1024 lanes have 128 registers a lane: they load the weights for each row.
+  constexpr bool KEEP = PARAMS && NT < 1024;
+  float w[KEEP ? VPT : 1][VE], dw[PARAMS ? VPT : 1][VE], db[PARAMS ? VPT : 1][VE];
+  if constexpr (PARAMS) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) dw[i][e] = db[i][e] = 0.0f;
+  }
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int j = i * TPR + t;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) w[i][e] = 0.0f;
+      if (rv.has(j)) load_params<P, VE>(w[i], weight, rv.col(j), 1.0f);
+    }
+  }
+  auto weights = [&](int i) -> const float(&)[VE] {
+    if constexpr (KEEP) {
+      return w[i];
+    } else {
+      const int j = i * TPR + t;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) w[0][e] = 0.0f;
+      if (rv.has(j)) load_params<P, VE>(w[0], weight, rv.col(j), 1.0f);
+      return w[0];
+    }
+  };
+  auto load = [&](int64_t r, VecT16<T> (&xv)[VPT], VecT16<T> (&dv)[VPT], float& m, float& rs) {
+    m = rs = 0.0f;
+    if (r < rows) {
+      m = mean_in[r];
+      rs = rstd_in[r];
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int j = i * TPR + t;
+      xv[i] = VecT16<T>{};
+      dv[i] = VecT16<T>{};
+      if (r < rows && rv.has(j)) {
+        xv[i] = load_stream<T>(x + r * cols + rv.col(j));
+        dv[i] = load_stream<T>(dy + r * cols + rv.col(j));
+      }
+    }
+  };
+
+  const int64_t step = static_cast<int64_t>(gridDim.x) * G;
+  VecT16<T> xv[VPT], dv[VPT];
+  float mean, rstd;
+  load(static_cast<int64_t>(blockIdx.x) * G + g, xv, dv, mean, rstd);
+  int odd = 0;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * G; r0 < rows; r0 += step) {
+    const int64_t r = r0 + g;
+    [[maybe_unused]] VecT16<T> xn[PARAMS ? VPT : 1], dn[PARAMS ? VPT : 1];
+    [[maybe_unused]] float mean_n, rstd_n;
+    if constexpr (PARAMS) load(r + step, xn, dn, mean_n, rstd_n);
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const auto& wi = weights(i);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float d = static_cast<float>(dv[i][e]);
+        const float xhat = (static_cast<float>(xv[i][e]) - mean) * rstd;
+        if constexpr (PARAMS) {
+          dw[i][e] += d * xhat;
+          db[i][e] += d;
+        }
+        s[0] += d * wi[e];
+        s[1] += d * wi[e] * xhat;
+      }
+      rv.repeated(i * TPR + t, [&](int e) {
+        const float dg = static_cast<float>(dv[i][e]) * wi[e];
+        s[0] -= dg;
+        s[1] -= dg * ((static_cast<float>(xv[i][e]) - mean) * rstd);
+      });
+    }
+    if (dx) {
+      group_sums<TPR, 2>(s, lds[odd]);
+      odd ^= 1;
+      const float a = s[0] * inv_n, b = s[1] * inv_n;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int j = i * TPR + t;
+        const auto& wi = weights(i);
+        VecT16<T> o;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float xhat = (static_cast<float>(xv[i][e]) - mean) * rstd;
+          o[e] = static_cast<T>((static_cast<float>(dv[i][e]) * wi[e] - a - xhat * b) * rstd);
+        }
+        if (r < rows && rv.has(j)) store_stream<T>(dx + r * cols + rv.col(j), o);
+      }
+    }
+    if constexpr (PARAMS) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        xv[i] = xn[i];
+        dv[i] = dn[i];
+      }
+      mean = mean_n;
+      rstd = rstd_n;
+    } else {
+      load(r + step, xv, dv, mean, rstd);
+    }
+  }
+  if constexpr (PARAMS) {
+    if (!ws) return;
+
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+#pragma unroll
+        for (int k = TPR; k < kWave; k *= 2) {
+          dw[i][e] += __shfl_xor(dw[i][e], k, 64);
+          db[i][e] += __shfl_xor(db[i][e], k, 64);
+        }
+    if constexpr (GL > 1) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          fold[(2 * (i * VE + e)) * NT + threadIdx.x] = dw[i][e];
+          fold[(2 * (i * VE + e) + 1) * NT + threadIdx.x] = db[i][e];
+        }
+      __syncthreads();
+      if (threadIdx.x >= L) return;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+#pragma unroll
+          for (int k = 1; k < GL; ++k) {
+            dw[i][e] += fold[(2 * (i * VE + e)) * NT + threadIdx.x + k * L];
+            db[i][e] += fold[(2 * (i * VE + e) + 1) * NT + threadIdx.x + k * L];
+          }
+    }
+    if (threadIdx.x >= TPR) return;
+    float* out = ws + 2 * static_cast<int64_t>(blockIdx.x) * cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int j = i * TPR + t;
+      if (!rv.has(j)) continue;
+#pragma unroll
+      for (int q = 0; q < VE / 4; ++q) {
+        float* p = out + rv.col(j) + 4 * q;
+        *reinterpret_cast<f32x4_a4*>(p) =
+            f32x4_a4{dw[i][4 * q], dw[i][4 * q + 1], dw[i][4 * q + 2], dw[i][4 * q + 3]};
+        *reinterpret_cast<f32x4_a4*>(p + cols) =
+            f32x4_a4{db[i][4 * q], db[i][4 * q + 1], db[i][4 * q + 2], db[i][4 * q + 3]};
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Rows of any width: one workgroup per row, three sweeps over it.
 // ---------------------------------------------------------------------------
@@ -108,68 +425,247 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_dx_any_kernel(
   }
 }
 
-// Partial sums of dweight and dbias: workgroup (strip, part) sums rows part, part + parts, ..
-// of one strip of columns, a column to a lane; part p's sums are rows 2 p (dweight) and
-// 2 p + 1 (dbias) of the workspace.
+// dx of rows that do not fit in registers, at least a vector wide: a workgroup per row, two
+// sweeps over it (the second one from the caches).
+constexpr int kWideThreads = 1024;
 template <typename T>
-__global__ __launch_bounds__(kThreads) void ln_bwd_params_any_kernel(
+__global__ __launch_bounds__(kWideThreads) void ln_bwd_dx_wide_kernel(
+    const T* __restrict__ dy, const T* __restrict__ x, const void* __restrict__ weight,
+    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx,
+    int param_dtype, int64_t rows, int64_t cols) {
+  constexpr int VE = kVecElems<T>;
+  __shared__ float lds[2][2][kWideThreads / kWave];
+  const float n = static_cast<float>(cols);
+  int odd = 0;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, odd ^= 1) {
+    const int64_t at = r * cols;
+    const float mean = mean_in[r], rstd = rstd_in[r];
+    float s[2] = {0.0f, 0.0f};
+    for (int64_t c = threadIdx.x * VE; c < cols; c += kWideThreads * VE) {
+      const int64_t from = c + VE <= cols ? c : cols - VE;     // c - from elements are repeated
+      const VecT16<T> dv = load_vec<T>(dy + at + from), xv = load_vec<T>(x + at + from);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float w = weight ? load_elem(weight, param_dtype, from + e) : 1.0f;
+        const float g = from + e >= c ? static_cast<float>(dv[e]) * w : 0.0f;
+        s[0] += g;
+        s[1] += g * ((static_cast<float>(xv[e]) - mean) * rstd);
+      }
+    }
+    group_sums<kWideThreads, 2>(s, lds[odd]);
+    const float a = s[0] / n, b = s[1] / n;
+    for (int64_t c = threadIdx.x * VE; c < cols; c += kWideThreads * VE) {
+      const int64_t from = c + VE <= cols ? c : cols - VE;
+      const VecT16<T> dv = load_vec<T>(dy + at + from), xv = load_vec<T>(x + at + from);
+      VecT16<T> o;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float w = weight ? load_elem(weight, param_dtype, from + e) : 1.0f;
+        const float xhat = (static_cast<float>(xv[e]) - mean) * rstd;
+        o[e] = static_cast<T>((static_cast<float>(dv[e]) * w - a - xhat * b) * rstd);
+      }
+      store_stream<T>(dx + at + from, o);
+    }
+  }
+}
+
+// Partial sums of dweight and dbias, for rows that ln_bwd_regs_kernel does not hold: workgroup
+// (strip, part) sums rows part, part + parts, ... of one strip of columns, a vector to a lane
+// (moved back at the row's end, to the same bits twice), to rows 2 part and 2 part + 1 of the
+// workspace.  Rows narrower than a vector: a column to a lane.
+template <typename T, bool NARROW>
+__global__ __launch_bounds__(kThreads) void ln_bwd_params_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean_in,
     const float* __restrict__ rstd_in, float* __restrict__ ws, int64_t rows, int64_t cols,
     int parts) {
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  constexpr int VE = NARROW ? 1 : kVecElems<T>;
+  int64_t c = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * VE;
   if (c >= cols) return;
-  for (int p = blockIdx.y; p < parts; p += gridDim.y) {
-    float dw = 0.0f, db = 0.0f;
-    for (int64_t r = p; r < rows; r += parts) {
-      const float d = static_cast<float>(dy[r * cols + c]);
-      dw += d * ((static_cast<float>(x[r * cols + c]) - mean_in[r]) * rstd_in[r]);
-      db += d;
+  if (c + VE > cols) c = cols - VE;
+  const int64_t p = blockIdx.y;
+  float dw[VE], db[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) dw[e] = db[e] = 0.0f;
+#pragma unroll 4
+  for (int64_t r = p; r < rows; r += parts) {
+    const float mean = mean_in[r], rstd = rstd_in[r];
+    const T *dp = dy + r * cols + c, *xp = x + r * cols + c;
+    float d[VE], v[VE];
+    if constexpr (NARROW) {
+      d[0] = static_cast<float>(*dp);
+      v[0] = static_cast<float>(*xp);
+    } else {
+      const VecT16<T> dv = load_stream<T>(dp), xv = load_stream<T>(xp);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        d[e] = static_cast<float>(dv[e]);
+        v[e] = static_cast<float>(xv[e]);
+      }
     }
-    ws[(2 * static_cast<int64_t>(p)) * cols + c] = dw;
-    ws[(2 * static_cast<int64_t>(p) + 1) * cols + c] = db;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      dw[e] += d[e] * ((v[e] - mean) * rstd);
+      db[e] += d[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    ws[2 * p * cols + c + e] = dw[e];
+    ws[(2 * p + 1) * cols + c + e] = db[e];
   }
 }
 
-// Folds the parts in a fixed order: 64 columns a workgroup, its waves take parts in turn and
-// their sums meet in LDS.  blockIdx.y 0 is dweight, 1 dbias.
+// Folds the parts in a fixed order: kFoldCols columns a workgroup, kFoldWays lanes a column
+// take the parts in turn and meet in LDS.  blockIdx.y 0 is dweight, 1 dbias.
+constexpr int kFoldCols = 32, kFoldWays = 32;
 template <typename P>
-__global__ __launch_bounds__(kThreads) void ln_bwd_fold_kernel(const float* __restrict__ ws,
-                                                               P* __restrict__ dweight,
-                                                               P* __restrict__ dbias,
-                                                               int64_t cols, int parts) {
-  __shared__ float lds[kWaves][kWave];
+__global__ __launch_bounds__(kFoldCols * kFoldWays) void ln_bwd_fold_kernel(
+    const float* __restrict__ ws, P* __restrict__ dweight, P* __restrict__ dbias, int64_t cols,
+    int parts) {
+  __shared__ float lds[kFoldWays][kFoldCols + 1];
   P* out = blockIdx.y == 0 ? dweight : dbias;
   if (!out) return;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kWave + lane;
+  const int lc = threadIdx.x % kFoldCols, way = threadIdx.x / kFoldCols;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * kFoldCols + lc;
   float s = 0.0f;
-  if (c < cols)
-    for (int p = wave; p < parts; p += kWaves)
+  if (c < cols) {
+#pragma unroll 8
+    for (int p = way; p < parts; p += kFoldWays)
       s += ws[(2 * static_cast<int64_t>(p) + blockIdx.y) * cols + c];
-  lds[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && c < cols) {
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) s += lds[w][lane];
-    out[c] = static_cast<P>(s);
   }
+  lds[way][lc] = s;
+  __syncthreads();
+  // Column `way` of the workgroup, its lanes' sums as a tree.
+  s = wave_sum<kFoldWays>(lds[lc][way]);
+  const int64_t oc = static_cast<int64_t>(blockIdx.x) * kFoldCols + way;
+  if (lc == 0 && oc < cols) out[oc] = static_cast<P>(s);
 }
 
-// How many partial sums of dweight and dbias a launch keeps.
-int ln_parts(int64_t rows, int64_t) { return static_cast<int>(rows < 512 ? rows : 512); }
+// ---------------------------------------------------------------------------
+// Which kernel a row width takes.  `vecs` is the row's 16-byte vectors (the last one may be in
+// part); widths under one vector and over the last entry take the sweeping kernels.
+// ---------------------------------------------------------------------------
+// Calls f with a shape of the forward kernel as constants.  Two rows a lane share the weight's
+// and bias's loads.  bf16 and fp32, 134217728 bytes of x, us (the best of 44 shapes, by width in
+// vectors): 8 44.3, 16 45.6, 32 44.9, 64 45.2, 128 44.5, 256 45.2, 512 45.4 (128 x 4 46.5, 256 x 2
+// 45.6), 1024 90.0 at twice the bytes (256 x 4 one row 92.2), 2048 92.5 (1024 lanes x 2 99.3), 4096
+// 95.6, 8192 106; one row instead of two 1 to 6 us more up to 512 vectors.
+template <int TPR_, int VPT_, int NT_, int ROWS_> struct RowShape {
+  static constexpr int TPR = TPR_, VPT = VPT_, NT = NT_, ROWS = ROWS_;
+};
+template <typename T, class F> int with_forward_shape(int64_t vecs, F f) {
+  if (vecs <= 8) return f(RowShape<8, 1, 256, 2>{});
+  if (vecs <= 16) return f(RowShape<16, 1, 256, 2>{});
+  if (vecs <= 32) return f(RowShape<32, 1, 256, 2>{});
+  if (vecs <= 64) return f(RowShape<64, 1, 256, 2>{});
+  if (vecs <= 128) return f(RowShape<128, 1, 256, 2>{});
+  if (vecs <= 256) return f(RowShape<128, 2, 256, 2>{});
+  if (vecs <= 512) return f(RowShape<512, 1, 512, 2>{});
+  if (vecs <= 1024) return f(RowShape<512, 2, 512, sizeof(T) == 2 ? 2 : 1>{});
+  if (vecs <= 2048) return f(RowShape<512, 4, 512, 1>{});
+  if (vecs <= 4096) return f(RowShape<1024, 4, 1024, 1>{});
+  return f(RowShape<1024, 8, 1024, 1>{});
+}
+constexpr int64_t kMaxForwardVecs = 8192;
+
+// The backward kernel with column sums in registers, and how many workgroups walk the rows
+// (two or three to a CU, as its registers allow; each ends with its sums' store, so more of
+// them cost more than they hide).  At 402653184 bytes of x, dy and dx, us: 8 vectors 68.5 (768
+// workgroups; 512 75.0, 1024 70.1), 32 69.3, 64 69.6, 128 70.1, 256 70.6 (fp32 66.7), 512 73.7
+// (512 x 1 75.8, 256 x 2 77.0), 1024 143 at twice the bytes (512 x 4 155), 2048 147 (256 workgroups;
+// 512 159).  4096 vectors in 16 bits would spill (965): dx and the column sums apart.
+template <int TPR_, int VPT_, int NT_, int WGS_> struct BackShape {
+  static constexpr int TPR = TPR_, VPT = VPT_, NT = NT_, kWorkgroups = WGS_;
+};
+template <bool WHOLE, class F> int with_backward_shape(int64_t vecs, F f) {
+  if (vecs <= 8) return f(BackShape<8, 1, 256, 768>{});
+  if (vecs <= 16) return f(BackShape<16, 1, 256, 768>{});
+  if (vecs <= 32) return f(BackShape<32, 1, 256, 768>{});
+  if (vecs <= 64) return f(BackShape<64, 1, 256, 768>{});
+  if (vecs <= 128) return f(BackShape<128, 1, 512, 512>{});
+  if (vecs <= 256) return f(BackShape<256, 1, 512, 512>{});
+  // 16384 x 4095: 90.6 us, 128 x 4 over 102 (the end's selects cost registers).
+  if (vecs <= 512) {
+    if constexpr (WHOLE) return f(BackShape<128, 4, 256, 512>{});
+    else return f(BackShape<256, 2, 256, 512>{});
+  }
+  if (vecs <= 1024) return f(BackShape<256, 4, 256, 512>{});
+  return f(BackShape<1024, 2, 1024, 256>{});
+}
+constexpr int64_t kMaxBackwardVecs = 2048;
+constexpr int64_t kMaxDxVecs = 4096;      // dx alone, with the row in registers
+
+// Workgroups of a launch over `rows`: each walks two rounds of rows at least (512 x 4096, us:
+// 11.5 with 256 workgroups, 16.3 with 512).
+template <class S> int backward_workgroups(int64_t rows) {
+  const int64_t need = (rows + 2 * (S::NT / S::TPR) - 1) / (2 * (S::NT / S::TPR));
+  return static_cast<int>(need < S::kWorkgroups ? need : S::kWorkgroups);
+}
+
+// Parts of the column sums taken apart: workgroups of one strip for 1024 in all.
+int params_parts(int64_t rows, int64_t cols, int vec) {
+  const int64_t strips = (cols + int64_t{kThreads} * vec - 1) / (int64_t{kThreads} * vec);
+  int64_t parts = 1024 / strips < 1 ? 1 : 1024 / strips;
+  if (parts > 256) parts = 256;
+  return static_cast<int>(parts < rows ? parts : rows);
+}
+
+// How many partial sums of dweight and dbias a launch keeps, `vec` elements to a vector.
+int ln_parts(int64_t rows, int64_t cols, int vec) {
+  if (rows <= 0) return 0;
+  if (cols < vec) return params_parts(rows, cols, 1);
+  const int64_t vecs = (cols + vec - 1) / vec;
+  if (vecs > kMaxBackwardVecs) return params_parts(rows, cols, vec);
+  auto count = [&](auto shape) { return backward_workgroups<decltype(shape)>(rows); };
+  return cols % vec == 0 ? with_backward_shape<true>(vecs, count)
+                         : with_backward_shape<false>(vecs, count);
+}
 
 // One workgroup per row up to the grid's 32-bit work size, which the kernels then walk.
 unsigned row_grid(int64_t rows) {
-  const int64_t most = int64_t{UINT32_MAX} / kThreads;
+  const int64_t most = int64_t{UINT32_MAX} / 1024;
   return static_cast<unsigned>(rows < most ? rows : most);
 }
 
-template <typename T>
-int ln_fwd(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
-           int param_dtype, int64_t rows, int64_t cols, float eps, hipStream_t s) {
-  ln_fwd_any_kernel<T><<<row_grid(rows), kThreads, 0, s>>>(
-      static_cast<const T*>(x), weight, bias, static_cast<T*>(y), mean, rstd, param_dtype, rows,
-      cols, eps);
+struct LnFwdArgs {
+  const void *x, *weight, *bias;
+  void* y;
+  float *mean, *rstd;
+  int param_dtype;
+  int64_t rows, cols;
+  float eps;
+  hipStream_t s;
+};
+
+template <typename T, typename P, bool WHOLE> int ln_fwd_regs(const LnFwdArgs& a) {
+  constexpr int VE = kVecElems<T>;
+  return with_forward_shape<T>((a.cols + VE - 1) / VE, [&](auto shape) {
+    using S = decltype(shape);
+    constexpr int64_t kRows = S::NT / S::TPR * S::ROWS;
+    const int64_t groups = (a.rows + kRows - 1) / kRows;
+    if (groups * S::NT > int64_t{UINT32_MAX})
+      return invalid("launch_layer_norm: rows exceed the grid's 32-bit work size");
+    ln_fwd_regs_kernel<T, P, S::TPR, S::VPT, S::NT, S::ROWS, WHOLE>
+        <<<static_cast<unsigned>(groups), S::NT, 0, a.s>>>(
+            static_cast<const T*>(a.x), static_cast<const P*>(a.weight),
+            static_cast<const P*>(a.bias), static_cast<T*>(a.y), a.mean, a.rstd, a.rows,
+            static_cast<int>(a.cols), a.eps);
+    MCKE_LAUNCH_CHECK("ln_fwd_regs_kernel");
+    return ok();
+  });
+}
+
+template <typename T> int ln_fwd(const LnFwdArgs& a) {
+  constexpr int VE = kVecElems<T>;
+  const bool whole = a.cols % VE == 0;
+  if (a.cols >= VE && a.cols <= kMaxForwardVecs * VE) {
+    if (a.param_dtype == MCKE_DTYPE_F32)
+      return whole ? ln_fwd_regs<T, float, true>(a) : ln_fwd_regs<T, float, false>(a);
+    return whole ? ln_fwd_regs<T, T, true>(a) : ln_fwd_regs<T, T, false>(a);
+  }
+  ln_fwd_any_kernel<T><<<row_grid(a.rows), kThreads, 0, a.s>>>(
+      static_cast<const T*>(a.x), a.weight, a.bias, static_cast<T*>(a.y), a.mean, a.rstd,
+      a.param_dtype, a.rows, a.cols, a.eps);
   MCKE_LAUNCH_CHECK("ln_fwd_any_kernel");
   return ok();
 }
@@ -185,8 +681,8 @@ struct LnBwdArgs {
 };
 
 template <typename P> int ln_fold(const LnBwdArgs& a, int parts) {
-  const dim3 grid(static_cast<unsigned>((a.cols + kWave - 1) / kWave), 2);
-  ln_bwd_fold_kernel<P><<<grid, kThreads, 0, a.s>>>(a.ws, static_cast<P*>(a.dweight),
+  const dim3 grid(static_cast<unsigned>((a.cols + kFoldCols - 1) / kFoldCols), 2);
+  ln_bwd_fold_kernel<P><<<grid, kFoldCols * kFoldWays, 0, a.s>>>(a.ws, static_cast<P*>(a.dweight),
                                                     static_cast<P*>(a.dbias), a.cols, parts);
   MCKE_LAUNCH_CHECK("ln_bwd_fold_kernel");
   return ok();
@@ -198,22 +694,72 @@ int ln_fold_any(const LnBwdArgs& a, int parts) {
   return ln_fold<__bf16>(a, parts);
 }
 
+template <typename T, typename P, bool WHOLE, class S, bool PARAMS>
+int ln_bwd_launch(const LnBwdArgs& a, unsigned grid, float* ws) {
+  ln_bwd_regs_kernel<T, P, S::TPR, S::VPT, S::NT, WHOLE, PARAMS><<<grid, S::NT, 0, a.s>>>(
+      static_cast<const T*>(a.dy), static_cast<const T*>(a.x), static_cast<const P*>(a.weight),
+      a.mean, a.rstd, static_cast<T*>(a.dx), ws, a.rows, static_cast<int>(a.cols));
+  MCKE_LAUNCH_CHECK("ln_bwd_regs_kernel");
+  return ok();
+}
+
+// dx, with the column sums where they are asked for and fit; `summed`: they are in the
+// workspace.
+template <typename T, typename P, bool WHOLE>
+int ln_bwd_rows(const LnBwdArgs& a, int parts, bool* summed) {
+  constexpr int VE = kVecElems<T>;
+  const int64_t vecs = (a.cols + VE - 1) / VE;
+  const bool params = a.dweight || a.dbias;
+  *summed = params && vecs <= kMaxBackwardVecs;
+  if (vecs <= kMaxBackwardVecs)
+    return with_backward_shape<WHOLE>(vecs, [&](auto shape) {
+      using S = decltype(shape);
+      // The workspace and the fold count on it.
+      if (backward_workgroups<S>(a.rows) != parts)
+        return fail(MCKE_STATUS_INTERNAL, "launch_layer_norm_backward: workgroups and parts differ");
+      return ln_bwd_launch<T, P, WHOLE, S, true>(a, parts, params ? a.ws : nullptr);
+    });
+  if (!a.dx) return ok();
+  return ln_bwd_launch<T, P, WHOLE, BackShape<1024, 4, 1024, 0>, false>(a, row_grid(a.rows),
+                                                                        nullptr);
+}
+
 template <typename T> int ln_bwd(const LnBwdArgs& a) {
+  constexpr int VE = kVecElems<T>;
   const T* dy = static_cast<const T*>(a.dy);
   const T* x = static_cast<const T*>(a.x);
-  if (a.dx && a.rows > 0) {
-    ln_bwd_dx_any_kernel<T><<<row_grid(a.rows), kThreads, 0, a.s>>>(
-        dy, x, a.weight, a.mean, a.rstd, static_cast<T*>(a.dx), a.param_dtype, a.rows, a.cols);
-    MCKE_LAUNCH_CHECK("ln_bwd_dx_any_kernel");
+  const bool params = a.dweight || a.dbias;
+  const int parts = ln_parts(a.rows, a.cols, VE);
+  bool summed = false;
+  if (a.rows > 0) {
+    const bool whole = a.cols % VE == 0;
+    int rc = ok();
+    if (a.cols >= VE && a.cols <= kMaxDxVecs * VE) {
+      if (a.param_dtype == MCKE_DTYPE_F32)
+        rc = whole ? ln_bwd_rows<T, float, true>(a, parts, &summed)
+                   : ln_bwd_rows<T, float, false>(a, parts, &summed);
+      else
+        rc = whole ? ln_bwd_rows<T, T, true>(a, parts, &summed) : ln_bwd_rows<T, T, false>(a, parts, &summed);
+    } else if (a.dx && a.cols >= VE) {
+      ln_bwd_dx_wide_kernel<T><<<row_grid(a.rows), kWideThreads, 0, a.s>>>(
+          dy, x, a.weight, a.mean, a.rstd, static_cast<T*>(a.dx), a.param_dtype, a.rows, a.cols);
+      MCKE_LAUNCH_CHECK("ln_bwd_dx_wide_kernel");
+    } else if (a.dx) {
+      ln_bwd_dx_any_kernel<T><<<row_grid(a.rows), kThreads, 0, a.s>>>(
+          dy, x, a.weight, a.mean, a.rstd, static_cast<T*>(a.dx), a.param_dtype, a.rows, a.cols);
+      MCKE_LAUNCH_CHECK("ln_bwd_dx_any_kernel");
+    }
+    if (rc) return rc;
   }
-  if (!a.dweight && !a.dbias) return ok();
-  const int parts = ln_parts(a.rows, a.cols);
-  if (parts > 0) {
-    const dim3 grid(static_cast<unsigned>((a.cols + kThreads - 1) / kThreads),
+  if (!params) return ok();
+  if (parts > 0 && !summed) {
+    const int vec = a.cols < VE ? 1 : VE;
+    const dim3 grid(static_cast<unsigned>((a.cols + int64_t{kThreads} * vec - 1) /
+                                          (int64_t{kThreads} * vec)),
                     static_cast<unsigned>(parts));
-    ln_bwd_params_any_kernel<T><<<grid, kThreads, 0, a.s>>>(dy, x, a.mean, a.rstd, a.ws, a.rows,
-                                                            a.cols, parts);
-    MCKE_LAUNCH_CHECK("ln_bwd_params_any_kernel");
+    auto* fn = a.cols < VE ? &ln_bwd_params_kernel<T, true> : &ln_bwd_params_kernel<T, false>;
+    fn<<<grid, kThreads, 0, a.s>>>(dy, x, a.mean, a.rstd, a.ws, a.rows, a.cols, parts);
+    MCKE_LAUNCH_CHECK("ln_bwd_params_kernel");
   }
   return ln_fold_any(a, parts);
 }
@@ -268,17 +814,18 @@ int mcke_launch_layer_norm(const void* x, const void* weight, const void* bias, 
       return invalid("launch_layer_norm: an output overlaps another operand, which violates the "
                      "__restrict__ contract");
   }
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == MCKE_DTYPE_F32)
-    return ln_fwd<float>(x, weight, bias, y, mean, rstd, param_dtype, rows, cols, eps, s);
-  if (dtype == MCKE_DTYPE_F16)
-    return ln_fwd<_Float16>(x, weight, bias, y, mean, rstd, param_dtype, rows, cols, eps, s);
-  return ln_fwd<__bf16>(x, weight, bias, y, mean, rstd, param_dtype, rows, cols, eps, s);
+  const LnFwdArgs a{x, weight, bias, y, mean, rstd, param_dtype, rows, cols, eps,
+                    static_cast<hipStream_t>(stream)};
+  if (dtype == MCKE_DTYPE_F32) return ln_fwd<float>(a);
+  if (dtype == MCKE_DTYPE_F16) return ln_fwd<_Float16>(a);
+  return ln_fwd<__bf16>(a);
 }
 
 size_t mcke_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0 || cols > kMaxCols) return 0;
-  return 2 * sizeof(float) * static_cast<size_t>(ln_parts(rows, cols)) * static_cast<size_t>(cols);
+  // The most that any type needs.
+  const int p32 = ln_parts(rows, cols, 4), p16 = ln_parts(rows, cols, 8);
+  return 2 * sizeof(float) * static_cast<size_t>(p32 > p16 ? p32 : p16) * static_cast<size_t>(cols);
 }
 
 int mcke_launch_layer_norm_backward(const void* dy, const void* x, const void* weight,
