@@ -66,29 +66,35 @@ __device__ __forceinline__ Sums wave_join(Sums s, float c) {
   return s;
 }
 
-template <int VE, bool ENTROPY>
-__device__ __forceinline__ Sums add_values(Sums s, const float (&v)[VE], float m, float c) {
-  if (m > s.m) s = moved(s, m, c);
-  const float from = s.m == -INFINITY ? 0.0f : s.m;
+// Takes in N values whose largest is m.
+template <int N, bool ENTROPY>
+__device__ __forceinline__ void add_values(Sums& s, const float (&v)[N], float m, float c) {
+  const float to = fmaxf(s.m, m);
+  s = moved(s, to, c);
+  const float from = to == -INFINITY ? 0.0f : to;
 #pragma unroll
-  for (int i = 0; i < VE; ++i) {
+  for (int i = 0; i < N; ++i) {
+    // The difference before the product: a product alone, rounded at the size of z, would move
+    // large logits by much of a unit.
     const float u = (v[i] - from) * c;
     const float p = __builtin_amdgcn_exp2f(u);
     s.d += p;
     if constexpr (ENTROPY) s.e += p * fmaxf(u, kFar);
   }
-  return s;
 }
 
 // ---------------------------------------------------------------------------
 // The alternatives
 // ---------------------------------------------------------------------------
-// Value and index as one number that orders by value, then by lowest index; -0 counts as +0.
-// 0 is below every key.
-__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
+// A value's bits in an order that whole numbers have too; -0 counts as +0.  Above 0 for every
+// value.
+__device__ __forceinline__ uint32_t order_of(float v) {
   const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
-  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return static_cast<uint64_t>(o) << 32 | (0xFFFFFFFFu - index);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+// Value and index as one number that orders by value, then by lowest index.
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
+  return static_cast<uint64_t>(order_of(v)) << 32 | (0xFFFFFFFFu - index);
 }
 __device__ __forceinline__ float key_value(uint64_t k) {
   const uint32_t o = static_cast<uint32_t>(k >> 32);
@@ -96,6 +102,27 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t k) {
   return 0xFFFFFFFFu - static_cast<uint32_t>(k);
+}
+
+// How many leading bits of order_of() tell two values of T apart.
+template <typename T> constexpr int kOrderBits = 32;
+template <> constexpr int kOrderBits<__bf16> = 16;
+template <> constexpr int kOrderBits<_Float16> = 19;     // sign, 8 bits of exponent, 10
+
+// The k-th largest of a wave's 64 * PER numbers (to their leading BITS, the others 0): the
+// largest t that k of them reach, bit by bit.  Every lane of the wave has the same.
+template <int BITS, int PER>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[PER], int k) {
+  uint32_t t = 0;
+#pragma unroll 1
+  for (int b = 31; b >= 32 - BITS; --b) {
+    const uint32_t up = t | 1u << b;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) n += __popcll(__ballot(v[i] >= up));
+    if (n >= k) t = up;
+  }
+  return t;
 }
 
 // A wave's list: lane i holds the i-th best so far.  Elements come in the order of their
@@ -152,13 +179,13 @@ struct TopList {
   }
 };
 
-// The top_k largest of n keys in LDS, to `best` in their order; empty keys behind.
+// The top_k largest of n different keys in LDS, to `best` in their order; 0 behind them.
 __device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int top_k, uint64_t* best) {
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t mine = keys[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += keys[j] > mine || (keys[j] == mine && j < i);
-    if (rank < top_k) best[rank] = mine;
+    for (int j = 0; j < n; ++j) rank += keys[j] > mine;
+    if (mine && rank < top_k) best[rank] = mine;
   }
 }
 
@@ -171,18 +198,16 @@ struct RowOut {
   int64_t* top_ids;
 };
 
-// A row's results from its sums and its best keys in LDS.
-template <typename T>
-__device__ __forceinline__ void write_row(const RowOut& o, const T* __restrict__ row, int64_t r,
-                                          int64_t vocab, Sums s, const uint64_t* best, int top_k,
+// A row's results from its sums, its best keys in LDS and its token's logit.
+__device__ __forceinline__ void write_row(const RowOut& o, int64_t r, int64_t vocab, int64_t token,
+                                          float logit, Sums s, const uint64_t* best, int top_k,
                                           float scale) {
   const float ln_d = logf(s.d);
   const bool empty = s.m == -INFINITY && s.d == 0.0f;   // every logit is masked
   if (threadIdx.x == 0) {
     if (o.logprobs) {
-      const int64_t t = o.tokens[r];
       float lp = __builtin_nanf("");                    // no such token
-      if (t < vocab) lp = empty ? -INFINITY : (static_cast<float>(row[t]) - s.m) * scale - ln_d;
+      if (token < vocab) lp = empty ? -INFINITY : (logit - s.m) * scale - ln_d;
       o.logprobs[r] = lp;
     }
     if (o.entropy) o.entropy[r] = empty ? 0.0f : ln_d - kLn2 * (s.e / s.d);
@@ -196,21 +221,23 @@ __device__ __forceinline__ void write_row(const RowOut& o, const T* __restrict__
   }
 }
 
-// A row without a token is not read.
-__device__ __forceinline__ bool skip_row(const RowOut& o, int64_t r, int top_k, bool write) {
-  if (!o.tokens || o.tokens[r] >= 0) return false;
-  if (write) {
-    if (threadIdx.x == 0) {
-      if (o.logprobs) o.logprobs[r] = 0.0f;
-      if (o.entropy) o.entropy[r] = 0.0f;
-      if (o.lse) o.lse[r] = 0.0f;
-    }
-    for (int i = threadIdx.x; i < top_k; i += kThreads) {
-      if (o.top_logprobs) o.top_logprobs[r * top_k + i] = 0.0f;
-      if (o.top_ids) o.top_ids[r * top_k + i] = -1;
-    }
+__device__ __forceinline__ void write_no_row(const RowOut& o, int64_t r, int top_k) {
+  if (threadIdx.x == 0) {
+    if (o.logprobs) o.logprobs[r] = 0.0f;
+    if (o.entropy) o.entropy[r] = 0.0f;
+    if (o.lse) o.lse[r] = 0.0f;
   }
-  return true;
+  for (int i = threadIdx.x; i < top_k; i += kThreads) {
+    if (o.top_logprobs) o.top_logprobs[r * top_k + i] = 0.0f;
+    if (o.top_ids) o.top_ids[r * top_k + i] = -1;
+  }
+}
+
+// The row's token (0 where there are none) and its logit.
+template <typename T>
+__device__ __forceinline__ float token_logit(const RowOut& o, const T* row, int64_t vocab,
+                                             int64_t token) {
+  return o.logprobs && token >= 0 && token < vocab ? static_cast<float>(row[token]) : 0.0f;
 }
 
 // A part of a row as it lies in the workspace.
@@ -218,8 +245,53 @@ struct Part {
   float m, d, e, unused;
 };
 
-// Workgroup (row, part): vectors part * per_part on, 64 adjacent ones to a wave.  With one
-// part the row's results are written here, else its sums and keys go to the workspace.
+constexpr int kMaxKeys = 1024;       // candidates of a part, or keys of all parts of a row
+
+template <typename T>
+__device__ __forceinline__ VecT16<T> load_logits(const T* row, int64_t j, int64_t vocab) {
+  constexpr int VE = kVecElems<T>;
+  if ((j + 1) * VE <= vocab) return load_vec<T>(row + j * VE);
+  return load_part<T>(row + j * VE, static_cast<int>(vocab - j * VE), -INFINITY);
+}
+
+// The alternatives of vectors first .. end - 1 of a row, in any order and with any ties: a list
+// per wave, elements in the order of their indices.  Returns how many keys it put down.
+template <typename T>
+__device__ __noinline__ int list_keys(const T* row, int64_t first, int64_t end, int64_t vocab,
+                                      int top_k, uint64_t* keys) {
+  constexpr int VE = kVecElems<T>;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  TopList top;
+  top.start(top_k);
+  for (int64_t j0 = first + wave * kWave; j0 < end; j0 += kThreads) {
+    const int64_t j = j0 + lane;
+    float v[VE], m = __builtin_nanf("");
+#pragma unroll
+    for (int e = 0; e < VE; ++e) v[e] = m;              // past the end nothing is offered
+    if (j < end) {
+      const VecT16<T> w = load_logits<T>(row, j, vocab);
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (j * VE + e < vocab) v[e] = static_cast<float>(w[e]);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) m = fmaxf(m, v[e]);
+    }
+    top.offer<VE>(v, m, static_cast<uint32_t>(j0 * VE));
+  }
+  if (lane < top_k) keys[wave * top_k + lane] = lane < top.count ? key_of(top.v, top.i) : 0;
+  return kWaves * top_k;
+}
+
+// Workgroup (row, part): vectors part * per_part on, a vector to a lane, kUnroll of them in
+// flight behind the ones at work.  With one part the row's results are written here, else its
+// sums and keys go to the workspace.
+//
+// Alternatives cost the pass nothing per logit: a lane has the largest of its own logits in
+// its sums.  The top_k-th largest of those 256 is a bound that at least top_k logits reach and
+// few others do, and only lanes whose largest reaches it have any, so their vectors are read
+// again (from the caches), the logits that reach the bound are put down and ranked.  Rows in
+// which more than kMaxKeys reach it (ties, masks, sorted rows) take list_keys instead.
+constexpr int kUnroll = 4;
 template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ x, RowOut o,
                                                             Part* __restrict__ parts_out,
@@ -227,84 +299,167 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
                                                             int64_t vocab, int64_t row_stride,
                                                             int parts, int64_t per_part,
                                                             float scale, int top_k) {
-  constexpr int VE = kVecElems<T>;
-  __shared__ uint64_t keys[kWaves * kMaxTop], best[kMaxTop];
+  constexpr int VE = kVecElems<T>, U = kUnroll;
+  __shared__ uint64_t keys[kMaxKeys], best[kMaxTop];
+  __shared__ uint32_t largest[kThreads];
   __shared__ Sums waves[kWaves];
+  __shared__ int hot[kThreads], hot_count, key_count;
   const int64_t r = blockIdx.x / parts;
   const int part = static_cast<int>(blockIdx.x % parts);
-  if (skip_row(o, r, top_k, parts == 1)) return;
   const T* row = x + r * row_stride;
+  const int64_t token = o.tokens ? o.tokens[r] : 0;
   const float c = scale * kLog2e;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int t = threadIdx.x, lane = t % kWave, wave = t / kWave;
   const int64_t all = (vocab + VE - 1) / VE, first = part * per_part;
   const int64_t end = first + per_part < all ? first + per_part : all;
 
+  if (token < 0) {                                      // nothing of the row is used
+    if (parts == 1) write_no_row(o, r, top_k);
+    return;
+  }
   Sums s = no_sums();
-  TopList top;
-  top.start(top_k);
-  for (int64_t j0 = first + wave * kWave; j0 < end; j0 += kThreads) {
-    const int64_t j = j0 + lane;
-    VecT16<T> w;
-    if (j >= end) w = load_part<T>(row, 0, -INFINITY);
-    else if ((j + 1) * VE <= vocab) w = load_vec<T>(row + j * VE);
-    else w = load_part<T>(row + j * VE, static_cast<int>(vocab - j * VE), -INFINITY);
+  auto take = [&](const VecT16<T>& w) {
     float v[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e) v[e] = static_cast<float>(w[e]);
     float m = v[0];
 #pragma unroll
     for (int e = 1; e < VE; ++e) m = fmaxf(m, v[e]);
-    s = add_values<VE, ENTROPY>(s, v, m, c);
-    if (top_k > 0) {
-      // Past the end nothing is offered, not even -inf.
+    add_values<VE, ENTROPY>(s, v, m, c);
+  };
+  // Whole rounds of U vectors a lane: one behind the other, then what is left.
+  const int64_t whole = vocab / VE < end ? vocab / VE : end;
+  const int rounds = static_cast<int>((whole > first ? whole - first : 0) / (U * kThreads));
+  const T* at = row + (first + t) * VE;
+  if (rounds > 0) {
+    VecT16<T> w[U];
 #pragma unroll
-      for (int e = 0; e < VE; ++e)
-        if (j * VE + e >= vocab || j >= end) v[e] = __builtin_nanf("");
-      if (j >= end) m = __builtin_nanf("");
-      top.offer<VE>(v, m, static_cast<uint32_t>(j0 * VE));
+    for (int u = 0; u < U; ++u) w[u] = load_stream<T>(at + u * (kThreads * VE));
+    for (int i = 0; i < rounds; ++i) {
+      VecT16<T> n[U];
+      // The last round loads itself again.
+      const T* next = at + (i + 1 < rounds ? U * kThreads * VE : 0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) n[u] = load_stream<T>(next + u * (kThreads * VE));
+      float v[U * VE];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) v[u * VE + e] = static_cast<float>(w[u][e]);
+      float m = v[0];
+#pragma unroll
+      for (int e = 1; e < U * VE; ++e) m = fmaxf(m, v[e]);
+      add_values<U * VE, ENTROPY>(s, v, m, c);
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = n[u];
+      at = next;
     }
   }
+  for (int64_t j = first + static_cast<int64_t>(rounds) * U * kThreads + t; j < end; j += kThreads)
+    take(load_logits<T>(row, j, vocab));
+  const float logit = token_logit<T>(o, row, vocab, token);
+
+  if (t == 0) hot_count = key_count = 0;
+  if (t < kMaxTop) best[t] = 0;
+  largest[t] = order_of(s.m);
+  const uint32_t mine = largest[t];
   s = wave_join(s, c);
   if (lane == 0) waves[wave] = s;
-  if (lane < top_k) keys[wave * top_k + lane] = lane < top.count ? key_of(top.v, top.i) : 0;
   __syncthreads();
   s = waves[0];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) s = join(s, waves[w], c);
-  rank_keys(keys, kWaves * top_k, top_k, best);
-  __syncthreads();
+
+  if (top_k > 0) {
+    uint32_t v[kWaves];
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) v[i] = largest[i * kWave + lane];
+    const uint32_t bound = kth_largest<kOrderBits<T>, kWaves>(v, top_k);
+    if (mine >= bound && first + t < end) hot[atomicAdd(&hot_count, 1)] = t;
+    __syncthreads();
+    // A lane has per_lane vectors at most, the last one possibly past the end.
+    const int per_lane = static_cast<int>((end - first + kThreads - 1) / kThreads);
+    const int items = hot_count * per_lane;
+    for (int i = t; i < items; i += kThreads) {
+      const int64_t j = first + hot[i / per_lane] + static_cast<int64_t>(i % per_lane) * kThreads;
+      if (j >= end) continue;
+      const VecT16<T> w = load_logits<T>(row, j, vocab);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float y = static_cast<float>(w[e]);
+        if (y == y && order_of(y) >= bound && j * VE + e < vocab) {
+          const int n = atomicAdd(&key_count, 1);
+          if (n < kMaxKeys) keys[n] = key_of(y, static_cast<uint32_t>(j * VE + e));
+        }
+      }
+    }
+    __syncthreads();
+    int n = key_count;
+    if (n > kMaxKeys) {
+      __syncthreads();                                  // everybody has read the count
+      n = list_keys<T>(row, first, end, vocab, top_k, keys);
+      __syncthreads();
+    }
+    rank_keys(keys, n, top_k, best);
+    __syncthreads();
+  }
   if (parts == 1) {
-    write_row(o, row, r, vocab, s, best, top_k, scale);
+    write_row(o, r, vocab, token, logit, s, best, top_k, scale);
     return;
   }
-  if (threadIdx.x == 0) parts_out[blockIdx.x] = Part{s.m, s.d, s.e, 0.0f};
-  for (int i = threadIdx.x; i < top_k; i += kThreads)
+  if (t == 0) parts_out[blockIdx.x] = Part{s.m, s.d, s.e, 0.0f};
+  for (int i = t; i < top_k; i += kThreads)
     keys_out[static_cast<int64_t>(blockIdx.x) * top_k + i] = best[i];
 }
 
-constexpr int kMaxPartKeys = 1024;   // keys of all parts of a row
-
-// A row's parts joined in their order, a workgroup per row.
+// A row's parts joined, a workgroup per row.  Keys: the top_k-th largest of the parts' first few
+// is a bound for all of them, and those that reach it are ranked.
+constexpr int kMaxParts = 64;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(
     const T* __restrict__ x, RowOut o, const Part* __restrict__ parts_in,
     const uint64_t* __restrict__ keys_in, int64_t vocab, int64_t row_stride, int parts,
     float scale, int top_k) {
-  __shared__ uint64_t keys[kMaxPartKeys], best[kMaxTop];
+  __shared__ uint64_t keys[kMaxKeys], best[kMaxTop];
+  __shared__ int key_count;
   const int64_t r = blockIdx.x;
-  if (skip_row(o, r, top_k, true)) return;
+  const int64_t token = o.tokens ? o.tokens[r] : 0;
+  const int t = threadIdx.x, lane = t % kWave;
+  if (token < 0) {
+    write_no_row(o, r, top_k);
+    return;
+  }
+  const float logit = token_logit<T>(o, x + r * row_stride, vocab, token);
   const float c = scale * kLog2e;
   Sums s = no_sums();
-  for (int p = 0; p < parts; ++p) {
-    const Part q = parts_in[r * parts + p];
-    s = join(s, Sums{q.m, q.d, q.e}, c);
+  if (lane < parts) {
+    const Part q = parts_in[r * parts + lane];
+    s = Sums{q.m, q.d, q.e};
   }
-  const int n = parts * top_k;
-  for (int i = threadIdx.x; i < n; i += kThreads) keys[i] = keys_in[r * n + i];
-  __syncthreads();
-  rank_keys(keys, n, top_k, best);
-  __syncthreads();
-  write_row(o, x + r * row_stride, r, vocab, s, best, top_k, scale);
+  s = wave_join(s, c);
+  if (top_k > 0) {
+    if (t == 0) key_count = 0;
+    if (t < kMaxTop) best[t] = 0;
+    const uint64_t* in = keys_in + r * parts * top_k;
+    // The first `few` of each part: at least top_k of them together, 256 at most.
+    const int few = kThreads / parts < top_k ? kThreads / parts : top_k;
+    uint32_t v[kWaves];
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      const int k = i * kWave + lane;
+      v[i] = k < parts * few ? static_cast<uint32_t>(in[k / few * top_k + k % few] >> 32) : 0;
+    }
+    const uint32_t bound = kth_largest<kOrderBits<T>, kWaves>(v, top_k);
+    __syncthreads();
+    for (int i = t; i < parts * top_k; i += kThreads) {
+      const uint64_t k = in[i];
+      if (k && k >> 32 >= bound) keys[atomicAdd(&key_count, 1)] = k;
+    }
+    __syncthreads();
+    rank_keys(keys, key_count, top_k, best);
+    __syncthreads();
+  }
+  write_row(o, r, vocab, token, logit, s, best, top_k, scale);
 }
 
 // dlogits = scale (g ([j == token] - p_j) - h p_j (log p_j + entropy)), g and h the gradients
@@ -357,8 +512,8 @@ int parts_of(int64_t rows, int64_t vocab, int top_k) {
   int64_t p = 1024 / (rows > 0 ? rows : 1);
   const int64_t most = (vocab + 2047) / 2048;
   if (p > most) p = most;
-  if (p > 64) p = 64;
-  if (top_k > 0 && p > kMaxPartKeys / top_k) p = kMaxPartKeys / top_k;
+  if (p > kMaxParts) p = kMaxParts;
+  if (top_k > 0 && p > kMaxKeys / top_k) p = kMaxKeys / top_k;
   return p < 1 ? 1 : static_cast<int>(p);
 }
 
