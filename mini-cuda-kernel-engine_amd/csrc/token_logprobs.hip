@@ -282,16 +282,17 @@ __device__ __noinline__ int list_keys(const T* row, int64_t first, int64_t end, 
   return kWaves * top_k;
 }
 
-// Workgroup (row, part): vectors part * per_part on, a vector to a lane, kUnroll of them in
-// flight behind the ones at work.  With one part the row's results are written here, else its
-// sums and keys go to the workspace.
+// Workgroup (row, part): vectors part * per_part on, in rounds of kUnroll vectors a lane, each
+// round's loads a round ahead of its work.  With one part the row's results are written here,
+// else its sums and keys go to the workspace.
 //
-// Alternatives cost the pass nothing per logit: a lane has the largest of its own logits in
-// its sums.  The top_k-th largest of those 256 is a bound that at least top_k logits reach and
-// few others do, and only lanes whose largest reaches it have any, so their vectors are read
-// again (from the caches), the logits that reach the bound are put down and ranked.  Rows in
-// which more than kMaxKeys reach it (ties, masks, sorted rows) take list_keys instead.
-constexpr int kUnroll = 4;
+// Alternatives cost the pass next to nothing per logit: a lane has the largest of its own logits in
+// its sums, and keeps it for each quarter of its rounds.  The top_k-th largest of the lanes' is
+// a bound that at least top_k logits reach and few others do; only quarters whose largest
+// reaches it have any, so those are read again (from the caches) and the logits that reach the
+// bound are put down and ranked.  Rows in which more than kMaxKeys reach it (ties, masks, sorted
+// rows) take list_keys instead.
+constexpr int kUnroll = 4, kQuarters = 4;
 template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ x, RowOut o,
                                                             Part* __restrict__ parts_out,
@@ -299,48 +300,52 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
                                                             int64_t vocab, int64_t row_stride,
                                                             int parts, int64_t per_part,
                                                             float scale, int top_k) {
-  constexpr int VE = kVecElems<T>, U = kUnroll;
+  constexpr int VE = kVecElems<T>, U = kUnroll, kRound = U * kThreads;
   __shared__ uint64_t keys[kMaxKeys], best[kMaxTop];
   __shared__ uint32_t largest[kThreads];
   __shared__ Sums waves[kWaves];
-  __shared__ int hot[kThreads], hot_count, key_count;
+  __shared__ int hot[kQuarters * kThreads], hot_count, key_count;
   const int64_t r = blockIdx.x / parts;
   const int part = static_cast<int>(blockIdx.x % parts);
   const T* row = x + r * row_stride;
-  const int64_t token = o.tokens ? o.tokens[r] : 0;
   const float c = scale * kLog2e;
   const int t = threadIdx.x, lane = t % kWave, wave = t / kWave;
   const int64_t all = (vocab + VE - 1) / VE, first = part * per_part;
   const int64_t end = first + per_part < all ? first + per_part : all;
+  const int n_vecs = static_cast<int>(end > first ? end - first : 0);
+  const int rounds = (n_vecs + kRound - 1) / kRound;
+  const int quarter = (rounds + kQuarters - 1) / kQuarters;        // rounds of one
 
+  // Round i: vectors first + i * kRound + u * kThreads + t.  Only the last one can leave the row.
+  auto load = [&](int i, VecT16<T> (&w)[U]) {
+    const int64_t j = first + static_cast<int64_t>(i) * kRound + t;
+    if ((first + (i + 1) * static_cast<int64_t>(kRound)) * VE <= vocab && (i + 1) * kRound <= n_vecs) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = load_stream<T>(row + (j + u * kThreads) * VE);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        w[u] = j + u * kThreads < end ? load_logits<T>(row, j + u * kThreads, vocab)
+                                      : load_part<T>(row, 0, -INFINITY);
+    }
+  };
+  VecT16<T> w[U];
+  load(0, w);
+  const int64_t token = o.tokens ? o.tokens[r] : 0;
   if (token < 0) {                                      // nothing of the row is used
     if (parts == 1) write_no_row(o, r, top_k);
     return;
   }
+  const float logit = token_logit<T>(o, row, vocab, token);
   Sums s = no_sums();
-  auto take = [&](const VecT16<T>& w) {
-    float v[VE];
+  float quarter_m[kQuarters];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) v[e] = static_cast<float>(w[e]);
-    float m = v[0];
-#pragma unroll
-    for (int e = 1; e < VE; ++e) m = fmaxf(m, v[e]);
-    add_values<VE, ENTROPY>(s, v, m, c);
-  };
-  // Whole rounds of U vectors a lane: one behind the other, then what is left.
-  const int64_t whole = vocab / VE < end ? vocab / VE : end;
-  const int rounds = static_cast<int>((whole > first ? whole - first : 0) / (U * kThreads));
-  const T* at = row + (first + t) * VE;
-  if (rounds > 0) {
-    VecT16<T> w[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = load_stream<T>(at + u * (kThreads * VE));
-    for (int i = 0; i < rounds; ++i) {
+  for (int q = 0; q < kQuarters; ++q) {
+    quarter_m[q] = -INFINITY;
+    const int stop = (q + 1) * quarter < rounds ? (q + 1) * quarter : rounds;
+    for (int i = q * quarter; i < stop; ++i) {
       VecT16<T> n[U];
-      // The last round loads itself again.
-      const T* next = at + (i + 1 < rounds ? U * kThreads * VE : 0);
-#pragma unroll
-      for (int u = 0; u < U; ++u) n[u] = load_stream<T>(next + u * (kThreads * VE));
+      if (i + 1 < rounds) load(i + 1, n);
       float v[U * VE];
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -349,20 +354,18 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
       float m = v[0];
 #pragma unroll
       for (int e = 1; e < U * VE; ++e) m = fmaxf(m, v[e]);
+      quarter_m[q] = fmaxf(quarter_m[q], m);
       add_values<U * VE, ENTROPY>(s, v, m, c);
+      if (i + 1 < rounds) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = n[u];
-      at = next;
+        for (int u = 0; u < U; ++u) w[u] = n[u];
+      }
     }
   }
-  for (int64_t j = first + static_cast<int64_t>(rounds) * U * kThreads + t; j < end; j += kThreads)
-    take(load_logits<T>(row, j, vocab));
-  const float logit = token_logit<T>(o, row, vocab, token);
 
   if (t == 0) hot_count = key_count = 0;
   if (t < kMaxTop) best[t] = 0;
   largest[t] = order_of(s.m);
-  const uint32_t mine = largest[t];
   s = wave_join(s, c);
   if (lane == 0) waves[wave] = s;
   __syncthreads();
@@ -375,13 +378,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) v[i] = largest[i * kWave + lane];
     const uint32_t bound = kth_largest<kOrderBits<T>, kWaves>(v, top_k);
-    if (mine >= bound && first + t < end) hot[atomicAdd(&hot_count, 1)] = t;
+    const int per_hot = quarter * U;                    // vectors of a lane's quarter
+#pragma unroll
+    for (int q = 0; q < kQuarters; ++q)
+      if (order_of(quarter_m[q]) >= bound && q * quarter < rounds)
+        hot[atomicAdd(&hot_count, 1)] = q * per_hot * kThreads + t;
     __syncthreads();
-    // A lane has per_lane vectors at most, the last one possibly past the end.
-    const int per_lane = static_cast<int>((end - first + kThreads - 1) / kThreads);
-    const int items = hot_count * per_lane;
+    const int items = hot_count * per_hot;
     for (int i = t; i < items; i += kThreads) {
-      const int64_t j = first + hot[i / per_lane] + static_cast<int64_t>(i % per_lane) * kThreads;
+      const int h = i / per_hot;
+      const int64_t j = first + hot[h] + static_cast<int64_t>(i - h * per_hot) * kThreads;
       if (j >= end) continue;
       const VecT16<T> w = load_logits<T>(row, j, vocab);
 #pragma unroll
@@ -463,44 +469,62 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(
 }
 
 // dlogits = scale (g ([j == token] - p_j) - h p_j (log p_j + entropy)), g and h the gradients
-// of the row's logprob and entropy: one 16-byte vector to a lane, a workgroup per kThreads
-// vectors of a row.
+// of the row's logprob and entropy: a workgroup per kBackVecs * kThreads vectors of a row, a lane's
+// loads all out before the row's own values are looked at.
+constexpr int kBackVecs = 2;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(
     const T* __restrict__ x, const int64_t* __restrict__ tokens, const float* __restrict__ lse_in,
     const float* __restrict__ entropy, const float* __restrict__ dlogprobs,
     const float* __restrict__ dentropy, T* __restrict__ dx, int64_t vocab, int64_t row_stride,
     int per_row, float scale) {
-  constexpr int VE = kVecElems<T>;
+  constexpr int VE = kVecElems<T>, V = kBackVecs;
   const int64_t r = blockIdx.x / per_row;
-  const int64_t at = (static_cast<int64_t>(blockIdx.x % per_row) * kThreads + threadIdx.x) * VE;
-  if (at >= vocab) return;
-  const int n = vocab - at < VE ? static_cast<int>(vocab - at) : VE;
+  const int64_t at0 =
+      (static_cast<int64_t>(blockIdx.x % per_row) * (V * kThreads) + threadIdx.x) * VE;
+  const T* in = x + r * row_stride;
+  T* out = dx + r * row_stride;
+  VecT16<T> w[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int64_t at = at0 + i * (kThreads * VE);
+    if (at + VE <= vocab) w[i] = load_stream<T>(in + at);
+    else if (at < vocab) w[i] = load_part<T>(in + at, static_cast<int>(vocab - at), 0.0f);
+  }
   const int64_t token = tokens ? tokens[r] : 0;
   const float lse = lse_in[r];
-  T* out = dx + r * row_stride + at;
-  VecT16<T> w;
-  if (token < 0 || lse == -INFINITY || token >= vocab) {
-    // No token or no probability: no gradient.  No such token: a NaN, as forward.
-    const float none = token < vocab ? 0.0f : __builtin_nanf("");
+  // No token or no probability: no gradient.  No such token: a NaN, as forward.
+  const bool none = token < 0 || lse == -INFINITY || token >= vocab;
+  const float instead = token < vocab ? 0.0f : __builtin_nanf("");
+  const float g = dlogprobs ? scale * dlogprobs[r] : 0.0f;
+  const float h = dentropy ? scale * dentropy[r] : 0.0f;
+  const float a = dentropy ? -(g + h * entropy[r]) : -g;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) w[e] = static_cast<T>(none);
-  } else {
-    const T* in = x + r * row_stride + at;
-    w = n == VE ? load_vec<T>(in) : load_part<T>(in, n, 0.0f);
-    const float g = dlogprobs ? scale * dlogprobs[r] : 0.0f;
-    const float h = dentropy ? scale * dentropy[r] : 0.0f;
-    const float a = dentropy ? -(g + h * entropy[r]) : -g;
+  for (int i = 0; i < V; ++i) {
+    const int64_t at = at0 + i * (kThreads * VE);
+    if (at >= vocab) break;
+    VecT16<T> y;
+    if (none) {
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      const float lp = static_cast<float>(w[e]) * scale - lse;
-      float d = __builtin_amdgcn_exp2f(lp * kLog2e) * (a - h * fmaxf(lp, kFar));
-      if (dlogprobs && at + e == token) d += g;
-      w[e] = static_cast<T>(d);
+      for (int e = 0; e < VE; ++e) y[e] = static_cast<T>(instead);
+    } else {
+      float d[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float lp = static_cast<float>(w[i][e]) * scale - lse;
+        d[e] = __builtin_amdgcn_exp2f(lp * kLog2e) * (a - h * fmaxf(lp, kFar));
+      }
+      if (dlogprobs && token >= at && token < at + VE) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          if (at + e == token) d[e] += g;
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) y[e] = static_cast<T>(d[e]);
     }
+    if (at + VE <= vocab) store_stream<T>(out + at, y);
+    else store_part<T>(out + at, y, static_cast<int>(vocab - at));
   }
-  if (n == VE) *reinterpret_cast<VecT16<T>*>(out) = w;
-  else store_part<T>(out, w, n);
 }
 
 // ---------------------------------------------------------------------------
@@ -653,7 +677,7 @@ int mcke_launch_token_logprobs_backward(const void* logits, const int64_t* token
       overlap(dlogits, bytes, dlogprobs, 4 * n) || overlap(dlogits, bytes, dentropy, 4 * n))
     return invalid("launch_token_logprobs_backward: dlogits overlaps an input, which violates the "
                    "__restrict__ contract");
-  const int64_t per_wg = kThreads * (16 / static_cast<int64_t>(e));
+  const int64_t per_wg = kBackVecs * kThreads * (16 / static_cast<int64_t>(e));
   const int64_t per_row = (vocab + per_wg - 1) / per_wg;
   if (rows * per_row > int64_t{UINT32_MAX} / kThreads)
     return invalid("launch_token_logprobs_backward: rows x vocab exceed the grid's 32-bit work "
