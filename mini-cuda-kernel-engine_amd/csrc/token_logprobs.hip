@@ -104,25 +104,35 @@ __device__ __forceinline__ uint32_t key_index(uint64_t k) {
   return 0xFFFFFFFFu - static_cast<uint32_t>(k);
 }
 
-// How many leading bits of order_of() tell two values of T apart.
+// How many leading bits of order_of() tell two values of T apart (an even number).
 template <typename T> constexpr int kOrderBits = 32;
 template <> constexpr int kOrderBits<__bf16> = 16;
-template <> constexpr int kOrderBits<_Float16> = 19;     // sign, 8 bits of exponent, 10
+template <> constexpr int kOrderBits<_Float16> = 20;     // sign, 8 bits of exponent, 10, and one
 
 // The k-th largest of a wave's 64 * PER numbers (to their leading BITS, the others 0): the
-// largest t that k of them reach, bit by bit.  Every lane of the wave has the same.
+// largest t that k of them reach, two bits at a time.  Every lane of the wave has the same.
 template <int BITS, int PER>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[PER], int k) {
   uint32_t t = 0;
 #pragma unroll 1
-  for (int b = 31; b >= 32 - BITS; --b) {
-    const uint32_t up = t | 1u << b;
-    int n = 0;
+  for (int b = 30; b >= 32 - BITS; b -= 2) {
+    uint32_t up = t;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) n += __popcll(__ballot(v[i] >= up));
-    if (n >= k) t = up;
+    for (uint32_t d = 1; d < 4; ++d) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) n += __popcll(__ballot(v[i] >= (t | d << b)));
+      up += n >= k ? 1u << b : 0u;                       // the counts fall with d
+    }
+    t = up;
   }
   return t;
+}
+
+// The least value whose order_of() reaches a bound of kth_largest.
+__device__ __forceinline__ float least_value(uint32_t bound) {
+  if (bound < 0x00800000u) return -INFINITY;             // up to order_of(-inf)
+  return __builtin_bit_cast(float, bound & 0x80000000u ? bound & 0x7FFFFFFFu : ~bound);
 }
 
 // A wave's list: lane i holds the i-th best so far.  Elements come in the order of their
@@ -184,6 +194,7 @@ __device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int top_k
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t mine = keys[i];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) rank += keys[j] > mine;
     if (mine && rank < top_k) best[rank] = mine;
   }
@@ -365,38 +376,49 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
 
   if (t == 0) hot_count = key_count = 0;
   if (t < kMaxTop) best[t] = 0;
-  largest[t] = order_of(s.m);
+  const uint32_t mine = order_of(s.m);
+  largest[t] = mine;
   s = wave_join(s, c);
   if (lane == 0) waves[wave] = s;
   __syncthreads();
   s = waves[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) s = join(s, waves[w], c);
+  for (int i = 1; i < kWaves; ++i) s = join(s, waves[i], c);
 
   if (top_k > 0) {
     uint32_t v[kWaves];
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) v[i] = largest[i * kWave + lane];
     const uint32_t bound = kth_largest<kOrderBits<T>, kWaves>(v, top_k);
-    const int per_hot = quarter * U;                    // vectors of a lane's quarter
-#pragma unroll
-    for (int q = 0; q < kQuarters; ++q)
-      if (order_of(quarter_m[q]) >= bound && q * quarter < rounds)
-        hot[atomicAdd(&hot_count, 1)] = q * per_hot * kThreads + t;
-    __syncthreads();
-    const int items = hot_count * per_hot;
-    for (int i = t; i < items; i += kThreads) {
-      const int h = i / per_hot;
-      const int64_t j = first + hot[h] + static_cast<int64_t>(i - h * per_hot) * kThreads;
-      if (j >= end) continue;
-      const VecT16<T> w = load_logits<T>(row, j, vocab);
+    const float least = least_value(bound);
+    auto put = [&](const VecT16<T>& w, int64_t j) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         const float y = static_cast<float>(w[e]);
-        if (y == y && order_of(y) >= bound && j * VE + e < vocab) {
+        if (y >= least && j * VE + e < vocab) {         // never a NaN
           const int n = atomicAdd(&key_count, 1);
           if (n < kMaxKeys) keys[n] = key_of(y, static_cast<uint32_t>(j * VE + e));
         }
+      }
+    };
+    if (rounds <= 1) {                                  // the lane still has its vectors
+      if (mine >= bound) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (first + u * kThreads + t < end) put(w[u], first + u * kThreads + t);
+      }
+    } else {
+      const int per_hot = quarter * U;                  // vectors of a lane's quarter
+#pragma unroll
+      for (int q = 0; q < kQuarters; ++q)
+        if (order_of(quarter_m[q]) >= bound && q * quarter < rounds)
+          hot[atomicAdd(&hot_count, 1)] = q * per_hot * kThreads + t;
+      __syncthreads();
+      const int items = hot_count * per_hot;
+      for (int i = t; i < items; i += kThreads) {
+        const int h = i / per_hot;
+        const int64_t j = first + hot[h] + static_cast<int64_t>(i - h * per_hot) * kThreads;
+        if (j < end) put(load_logits<T>(row, j, vocab), j);
       }
     }
     __syncthreads();
@@ -418,54 +440,56 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     keys_out[static_cast<int64_t>(blockIdx.x) * top_k + i] = best[i];
 }
 
-// A row's parts joined, a workgroup per row.  Keys: the top_k-th largest of the parts' first few
-// is a bound for all of them, and those that reach it are ranked.
-constexpr int kMaxParts = 64;
+// A row's parts joined, a workgroup per row.  Keys: the top_k-th largest of the lanes' largest is
+// a bound again, and those that reach it are ranked.
+constexpr int kMaxParts = 64, kKeysPerLane = kMaxKeys / kThreads;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(
     const T* __restrict__ x, RowOut o, const Part* __restrict__ parts_in,
     const uint64_t* __restrict__ keys_in, int64_t vocab, int64_t row_stride, int parts,
     float scale, int top_k) {
   __shared__ uint64_t keys[kMaxKeys], best[kMaxTop];
+  __shared__ uint32_t largest[kThreads];
   __shared__ int key_count;
   const int64_t r = blockIdx.x;
-  const int64_t token = o.tokens ? o.tokens[r] : 0;
   const int t = threadIdx.x, lane = t % kWave;
-  if (token < 0) {
-    write_no_row(o, r, top_k);
-    return;
-  }
-  const float logit = token_logit<T>(o, x + r * row_stride, vocab, token);
-  const float c = scale * kLog2e;
+  const int n = parts * top_k;
+  uint64_t key[kKeysPerLane];
+#pragma unroll
+  for (int i = 0; i < kKeysPerLane; ++i)
+    key[i] = t + i * kThreads < n ? keys_in[r * n + t + i * kThreads] : 0;
   Sums s = no_sums();
   if (lane < parts) {
     const Part q = parts_in[r * parts + lane];
     s = Sums{q.m, q.d, q.e};
   }
-  s = wave_join(s, c);
+  const int64_t token = o.tokens ? o.tokens[r] : 0;
+  if (token < 0) {
+    write_no_row(o, r, top_k);
+    return;
+  }
+  const float logit = token_logit<T>(o, x + r * row_stride, vocab, token);
   if (top_k > 0) {
     if (t == 0) key_count = 0;
     if (t < kMaxTop) best[t] = 0;
-    const uint64_t* in = keys_in + r * parts * top_k;
-    // The first `few` of each part: at least top_k of them together, 256 at most.
-    const int few = kThreads / parts < top_k ? kThreads / parts : top_k;
+    uint64_t most = key[0];
+#pragma unroll
+    for (int i = 1; i < kKeysPerLane; ++i) most = key[i] > most ? key[i] : most;
+    largest[t] = static_cast<uint32_t>(most >> 32);
+    __syncthreads();
     uint32_t v[kWaves];
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const int k = i * kWave + lane;
-      v[i] = k < parts * few ? static_cast<uint32_t>(in[k / few * top_k + k % few] >> 32) : 0;
-    }
+    for (int i = 0; i < kWaves; ++i) v[i] = largest[i * kWave + lane];
     const uint32_t bound = kth_largest<kOrderBits<T>, kWaves>(v, top_k);
-    __syncthreads();
-    for (int i = t; i < parts * top_k; i += kThreads) {
-      const uint64_t k = in[i];
-      if (k && k >> 32 >= bound) keys[atomicAdd(&key_count, 1)] = k;
-    }
+#pragma unroll
+    for (int i = 0; i < kKeysPerLane; ++i)
+      if (key[i] && key[i] >> 32 >= bound) keys[atomicAdd(&key_count, 1)] = key[i];
     __syncthreads();
     rank_keys(keys, key_count, top_k, best);
     __syncthreads();
   }
-  write_row(o, r, vocab, token, logit, s, best, top_k, scale);
+  const float c = scale * kLog2e;
+  write_row(o, r, vocab, token, logit, wave_join(s, c), best, top_k, scale);
 }
 
 // dlogits = scale (g ([j == token] - p_j) - h p_j (log p_j + entropy)), g and h the gradients
