@@ -426,24 +426,28 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void gemm_lp_kernel(
     constexpr int TR = BM * IP / MT;
     static_assert(TR * BN * 4 <= 2 * S::kBytes, "a pass must fit the stages");
     float* sums = reinterpret_cast<float*>(smem);
+    [&]<int... PASS>(std::integer_sequence<int, PASS...>) {
+      ([&] {
+        auto st = fused_store<OutT, TR, BN, kMfmaThreads>(
+            ep,
+            [=](int r) { return (r / (IP * 32)) * WM + PASS * (IP * 32) + r % (IP * 32); }, M, N,
+            m0, n0, n_first);
+        st.begin();
+        if constexpr (PASS > 0) __syncthreads();
 #pragma unroll
-    for (int pass = 0; pass < MT / IP; ++pass) {
-      if (pass > 0) __syncthreads();
+        for (int i = 0; i < IP; ++i)
 #pragma unroll
-      for (int i = 0; i < IP; ++i)
+          for (int r = 0; r < 16; ++r) {
+            const int row = wm * (IP * 32) + i * 32 + 8 * (r / 4) + 4 * h + (r % 4);
+            const int col = wn * WN + NT * c;
+            float* p = sums + sum_at<BN>(row, col / 4) + col % 4;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int row = wm * (IP * 32) + i * 32 + 8 * (r / 4) + 4 * h + (r % 4);
-          const int col = wn * WN + NT * c;
-          float* p = sums + sum_at<BN>(row, col / 4) + col % 4;
-#pragma unroll
-          for (int j = 0; j < NT; ++j) p[j] = acc[pass * IP + i][j][r];
-        }
-      __syncthreads();
-      store_fused<OutT, TR, BN, kMfmaThreads>(sums, C, M, N, m0, n0, n_first, alpha, ep, [&](int r) {
-        return (r / (IP * 32)) * WM + pass * (IP * 32) + r % (IP * 32);
-      });
-    }
+            for (int j = 0; j < NT; ++j) p[j] = acc[PASS * IP + i][j][r];
+          }
+        __syncthreads();
+        st.finish(sums, C, alpha);
+      }(), ...);
+    }(std::make_integer_sequence<int, MT / IP>{});
   } else {
     lp_store_c<OutT, BM, BN, VEC, WHOLE>(acc, C, M, N, m0, n0, n_first, wm, wn, h, c, alpha, beta);
   }
@@ -1326,6 +1330,11 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void gemm_lp_dma16_kernel(
     float* sums = reinterpret_cast<float*>(smem);
     [&]<int... PASS>(std::integer_sequence<int, PASS...>) {
       ([&] {
+        auto st = fused_store<OutT, TR, BN, kMfmaThreads>(
+            ep,
+            [=](int r) { return (r / (IP * 16)) * WM + PASS * (IP * 16) + r % (IP * 16); }, M, N,
+            m0, n0, n_first);
+        st.begin();
         __syncthreads();   // the stage buffers, or the pass before, have been read
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1341,10 +1350,7 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void gemm_lp_dma16_kernel(
           __builtin_amdgcn_sched_barrier(0);
         }
         __syncthreads();
-        store_fused<OutT, TR, BN, kMfmaThreads>(
-            sums, C, M, N, m0, n0, n_first, alpha, ep, [&](int r) {
-              return (r / (IP * 16)) * WM + PASS * (IP * 16) + r % (IP * 16);
-            });
+        st.finish(sums, C, alpha);
       }(), ...);
     }(std::make_integer_sequence<int, MT / IP>{});
     return;

@@ -58,12 +58,12 @@ int launch_dma(const LpArgs<E>& x) {
   return ok();
 }
 
-template <typename T, typename OutT, int MT, int NW, int WV, class E>
+template <typename T, typename OutT, int MT, int NW, int WV, int AHEAD = 1, class E>
 int launch_split_as(const LpArgs<E>& x) {
   constexpr int TM = 16 * MT, TN = 16 * NW;
   const int64_t tiles = tile_count(x.m, x.n, TM, TN);
   if (int rc = check_grid<E>(tiles, WV * kWave)) return rc;
-  gemm_lp_split_kernel<T, OutT, MT, NW, WV, E>
+  gemm_lp_split_kernel<T, OutT, MT, NW, WV, E, AHEAD>
       <<<static_cast<unsigned>(tiles), WV * kWave, 0, x.s>>>(
           x.a, x.b, static_cast<OutT*>(x.c), x.m, x.n, x.k, x.alpha, x.beta,
           steps_along(x.m, TM), steps_along(x.n, TN), x.ep);
@@ -83,6 +83,35 @@ int launch_split(const LpArgs<E>& x) {
     return x.m <= 16 ? launch_split_as<T, OutT, 1, 2, 8>(x) : launch_split_as<T, OutT, 2, 2, 8>(x);
   if (tile_count(x.m, x.n, 32, 64) <= 1024) return launch_split_as<T, OutT, 2, 4, 4>(x);
   return launch_split_as<T, OutT, 4, 4, 4>(x);
+}
+
+// Few rows (tokens) with an epilogue: bound by reading B, which a CU takes in at 8 to 9 bytes a
+// clock at most, more of it from whole 128-byte lines.  So as many workgroups as there are CUs
+// where N allows it, then 64 columns each (with bias and GELU, bf16, us; MT x NW, waves,
+// chunks ahead):
+//   rows 1, K 4096:   N 16384  1x4 4w 25.2, 1x2 8w 41, 128 x 128 tiles 48   N 12288  1x4 4w two ahead
+//     22.6, one 23.8   N 8192  1x2 8w 13.6, 1x4 13.6   N 4096  1x1 8w two ahead 11.4, 1x2 8w 11.8
+//   rows 1, K 16384:  N 4096  1x1 53.8, 1x2 61      N 1000  1x1 28, 1x2 31
+//   rows 32:          32 x 4096 x 16384  1x2 two ahead 62.6, one 66.8    32 x 8192 x 4096  1x4 8w
+//     15.4, 2x2 8w 16.2      32 x 16384 x 4096  2x4 4w 29.0, 4x4 4w 29.9
+//   rows 64:          64 x 4096 x 16384  2x2 8w two ahead 66.5, one 72.8, 1x4 8w 70.0
+//     64 x 8192 x 4096  2x4 8w 17.3, 2x4 4w 19.8    64 x 16384 x 4096  4x4 8w 37.4, 4w 40.4
+template <typename T, typename OutT, class E>
+int launch_few_rows(const LpArgs<E>& x) {
+  if (x.m <= 16) {
+    if (x.n <= 4096) return launch_split_as<T, OutT, 1, 1, 8, 2>(x);
+    if (x.n <= 8192) return launch_split_as<T, OutT, 1, 2, 8>(x);
+    if (x.n < 16384) return launch_split_as<T, OutT, 1, 4, 4, 2>(x);
+    return launch_split_as<T, OutT, 1, 4, 4>(x);
+  }
+  if (x.m <= 32) {
+    if (x.n <= 4096) return launch_split_as<T, OutT, 1, 2, 8, 2>(x);
+    if (x.n <= 8192) return launch_split_as<T, OutT, 1, 4, 8>(x);
+    return launch_split_as<T, OutT, 2, 4, 4>(x);
+  }
+  if (x.n <= 4096) return launch_split_as<T, OutT, 2, 2, 8, 2>(x);
+  if (x.n <= 8192) return launch_split_as<T, OutT, 2, 4, 8>(x);
+  return launch_split_as<T, OutT, 4, 4, 8>(x);
 }
 
 // The register-staged kernel's checked forms at the requested tile: what is narrower than
@@ -157,6 +186,15 @@ template <int BM, int BN, typename OutT, class E> bool whole_fits(const LpArgs<E
          aligned(x.c, sizeof(OutT));
 }
 
+// Whether the split-K kernel's limits hold: 16-bit values at 2-byte addresses, per-lane offsets
+// below 4 GiB, and a grid that holds 32 x 32 tiles of 512 lanes.
+template <typename OutT, class E> bool split_fits(const LpArgs<E>& x) {
+  return x.k > 0 && tile_count(x.m, x.n, 32, 32) <= int64_t{UINT32_MAX} / 512 &&
+         aligned(x.a, 2) && aligned(x.b, 2) && aligned(x.c, sizeof(OutT)) &&
+         static_cast<int64_t>(64) * x.k * 2 < (int64_t{1} << 32) &&
+         static_cast<int64_t>(64) * x.n * 2 < (int64_t{1} << 32);
+}
+
 template <typename T, typename OutT, int BM, int BN>
 struct LpTile {
   // Whole tiles run the requested tile's direct-to-LDS kernel (tiles of 128 and more).
@@ -175,6 +213,9 @@ struct LpTile {
   // against 105).  What is left takes the split-K kernel, as 64 x 64 launches do, but for
   // short K over many tiles (short_k).  The tile counts here and below are for 256 CUs.
   template <class E> static int launch(const LpArgs<E>& x, bool vec) {
+    if constexpr (E::kFused)
+      if (x.m <= 64 && x.n >= 64 && x.k >= 64 && split_fits<OutT>(x))
+        return launch_few_rows<T, OutT>(x);
     if constexpr (BN >= 128) {
       if (vec && x.m % BM == 0 && x.n % BN == 0 && x.k % 64 == 0 && x.k > 0 &&
           dma_offsets32<BM, BN>(x.n, x.k))
@@ -197,12 +238,7 @@ struct LpTile {
       if (whole_fits<128, 128, OutT>(x) && tiles >= 208)
         return launch_whole<T, OutT, 128, 128>(x);
     }
-    // 16-bit values at 2-byte addresses, per-lane offsets below 4 GiB, and a grid that holds
-    // 32 x 32 tiles of 512 lanes.
-    if (x.n >= 32 && x.k > 0 && tile_count(x.m, x.n, 32, 32) <= int64_t{UINT32_MAX} / 512 &&
-        aligned(x.a, 2) && aligned(x.b, 2) && aligned(x.c, sizeof(OutT)) &&
-        static_cast<int64_t>(64) * x.k * 2 < (int64_t{1} << 32) &&
-        static_cast<int64_t>(64) * x.n * 2 < (int64_t{1} << 32))
+    if (x.n >= 32 && split_fits<OutT>(x))
       return short_k(x, vec) ? launch_short_k<T, OutT>(x, vec) : launch_split<T, OutT>(x);
     // (With an epilogue at most 128 x 128: the checked 256 x 256 form spills as it is.)
     if constexpr (E::kFused && BM == 256) return launch_staged<T, OutT, 128, 128>(x, vec);

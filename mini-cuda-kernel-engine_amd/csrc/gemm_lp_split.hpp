@@ -54,16 +54,17 @@ struct LpSplitShape {
   // takes no more LDS than the slots.
   static constexpr int kFold = kOut * 4 * WV <= kSlots ? WV : WV / 2;
   static constexpr int kLds = kSlots > kFold * kOut * 4 ? kSlots : kFold * kOut * 4;
-  static_assert(kLds <= 64 * 1024, "two workgroups or more per CU");
+  static_assert(kLds <= 80 * 1024, "two workgroups or more per CU");
   static constexpr int kARow = 64, kBRow = 32 * NW;
-  static_assert(NW == 2 || NW == 4, "column blocks are swizzled in twos or fours");
+  static_assert(NW == 1 || NW == 2 || NW == 4, "column blocks are swizzled in twos or fours");
   static __host__ __device__ constexpr int aswz(int r) { return (r >> 2) & 3; }
   static __host__ __device__ constexpr int bswz(int s) {
-    return NW == 2 ? (s >> 2) & 1 : (s >> 1) & 3;
+    return NW == 1 ? 0 : NW == 2 ? (s >> 2) & 1 : (s >> 1) & 3;
   }
 };
 
-template <typename T, typename OutT, int MT, int NW, int WV, class E = NoEpilogue>
+// AHEAD: chunks of a wave's loads in flight behind the one at work.
+template <typename T, typename OutT, int MT, int NW, int WV, class E = NoEpilogue, int AHEAD = 1>
 __global__ __launch_bounds__(WV * 64) void gemm_lp_split_kernel(
     const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, OutPtr<OutT, E> C, int M,
     int N, int K, float alpha, float beta, int tiles_m, int tiles_n, E ep) {
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(WV * 64) void gemm_lp_split_kernel(
   // eight: element by element).  Loaded element by element as a whole, after the loop, the
   // remainder took up to 1.8 us, much of a short product's time: fp16 to fp16, 33 x 2200 x 16
   // 5.7 -> 4.1 us, 2460 x 1608 x 40 14.9 -> 10.7.
-  u32x4 v[L];
+  u32x4 v[AHEAD][L];
   const int rem = K % S::KC;
   if (rem != 0 && wave == chunks % WV) {
     const int past = 8 - rem % 8;        // of a cut eight, what lies past the end
@@ -197,19 +198,69 @@ __global__ __launch_bounds__(WV * 64) void gemm_lp_split_kernel(
       w[S::NA + u] = u32x4{0u, 0u, 0u, 0u};
       if (b_k[u] < rem) w[S::NA + u] = *reinterpret_cast<const u32x4_a2*>(bp + b_src[u]);
     }
-    if (n_it > 0) load(0, v);
+    if (n_it > 0) {
+      load(0, v[0]);
+#pragma unroll
+      for (int p = 1; p < AHEAD; ++p) load(p < n_it ? p : n_it - 1, v[p]);
+    }
     to_slot(w);
     written();
     compute();
   } else if (n_it > 0) {
-    load(0, v);
+    load(0, v[0]);
+#pragma unroll
+    for (int p = 1; p < AHEAD; ++p) load(p < n_it ? p : n_it - 1, v[p]);
   }
-  for (int it = 0; it < n_it; ++it) {
-    // The slot's last reads have been waited for by the MFMAs that used them.
-    to_slot(v);
-    load(it + 1 < n_it ? it + 1 : it, v);
-    written();
-    compute();
+  if constexpr (AHEAD == 1) {
+    for (int it = 0; it < n_it; ++it) {
+      // The slot's last reads have been waited for by the MFMAs that used them.
+      to_slot(v[0]);
+      load(it + 1 < n_it ? it + 1 : it, v[0]);
+      written();
+      compute();
+    }
+  } else {
+    int it = 0;
+    for (; it + AHEAD <= n_it; it += AHEAD) {
+#pragma unroll
+      for (int p = 0; p < AHEAD; ++p) {
+        to_slot(v[p]);
+        load(it + p + AHEAD < n_it ? it + p + AHEAD : n_it - 1, v[p]);
+        written();
+        compute();
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < AHEAD - 1; ++p) {
+      if (it + p < n_it) {
+        to_slot(v[p]);
+        written();
+        compute();
+      }
+    }
+  }
+
+  // With an epilogue: this lane's bias (its columns are the same in every turn below) and
+  // residual, on their way while the waves' sums meet.
+  using O = LpOut<OutT>;
+  struct Pack { OutT v[4]; };   // four adjacent columns at any address
+  constexpr int kTurns = (S::kOut / 4 + S::kThreads - 1) / S::kThreads;
+  [[maybe_unused]] float bias[4];
+  [[maybe_unused]] Pack old[kTurns];
+  if constexpr (E::kFused) {
+    static_assert(S::kThreads % (S::TN / 4) == 0, "a lane keeps its columns");
+    const int col = n0 + 4 * (threadIdx.x % (S::TN / 4));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      bias[j] = ep.bias ? load_elem(ep.bias, ep.bias_dtype, col + j) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const int row_t = (threadIdx.x + i * S::kThreads) / (S::TN / 4);
+      const int row = m0 + row_t < M ? m0 + row_t : M - 1;
+      if (ep.residual)
+        __builtin_memcpy(&old[i], static_cast<const OutT*>(ep.residual) +
+                                      static_cast<int64_t>(row) * N + col, sizeof(Pack));
+    }
   }
 
   // The waves' sums.  While there are more than fit, the upper half hands its own to the
@@ -245,8 +296,38 @@ __global__ __launch_bounds__(WV * 64) void gemm_lp_split_kernel(
   }
   if (wave < S::kFold) put(wave);
   __syncthreads();
-  using O = LpOut<OutT>;
-  struct Pack { OutT v[4]; };   // four adjacent columns at any address
+  if constexpr (E::kFused) {
+#pragma unroll
+    for (int turn = 0; turn < kTurns; ++turn) {
+      const int q = turn * S::kThreads + threadIdx.x;
+      if (q >= S::kOut / 4) break;
+      const int rt = q / (S::TN / 4), cq = q % (S::TN / 4);
+      const int row = m0 + rt, col = n0 + 4 * cq;
+      if (row >= M || col + 3 < n_first) continue;
+      const int o =
+          (((rt / 16) * NW + cq / 4) * 4 + rt % 4) * 64 + 16 * ((rt / 4) % 4) + 4 * (cq % 4);
+      f32x4 s = *reinterpret_cast<const f32x4*>(sums + o);
+#pragma unroll
+      for (int w = 1; w < S::kFold; ++w)
+        s += *reinterpret_cast<const f32x4*>(sums + w * S::kOut + o);
+      Pack out;
+      with_act(ep.act, [&](auto act) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          out.v[j] = O::from_f32(fused_value<decltype(act)::value>(
+              alpha * s[j], bias[j], ep.residual ? O::to_f32(old[turn].v[j]) : 0.0f));
+      });
+      OutT* p = C + static_cast<int64_t>(row) * N + col;
+      if (col >= n_first) {
+        __builtin_memcpy(p, &out, sizeof(out));
+      } else {
+#pragma unroll
+        for (int j = 1; j < 4; ++j)
+          if (col + j >= n_first) p[j] = out.v[j];
+      }
+    }
+    return;
+  }
   for (int q = threadIdx.x; q < S::kOut / 4; q += S::kThreads) {
     const int rt = q / (S::TN / 4), cq = q % (S::TN / 4);
     const int row = m0 + rt, col = n0 + 4 * cq;
@@ -257,23 +338,10 @@ __global__ __launch_bounds__(WV * 64) void gemm_lp_split_kernel(
     for (int w = 1; w < S::kFold; ++w)
       s += *reinterpret_cast<const f32x4*>(sums + w * S::kOut + o);
     OutT* p = C + static_cast<int64_t>(row) * N + col;
-    if constexpr (E::kFused) {
-      const OutT* res = static_cast<const OutT*>(ep.residual);
-      with_act(ep.act, [&](auto act) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (col + j < n_first) continue;
-          const float b = ep.bias ? load_elem(ep.bias, ep.bias_dtype, col + j) : 0.0f;
-          const float old = res ? O::to_f32(res[static_cast<int64_t>(row) * N + col + j]) : 0.0f;
-          s[j] = fused_value<decltype(act)::value>(alpha * s[j], b, old);
-        }
-      });
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j] *= alpha;
-        if (beta != 0.0f && col + j >= n_first) s[j] += beta * O::to_f32(p[j]);
-      }
+    for (int j = 0; j < 4; ++j) {
+      s[j] *= alpha;
+      if (beta != 0.0f && col + j >= n_first) s[j] += beta * O::to_f32(p[j]);
     }
     if (col >= n_first) {
       Pack out;
