@@ -259,9 +259,12 @@ def exported_symbols() -> list[str]:
     return sorted(n for n in dir(_lib) if n.startswith("mcke_"))
 
 
+_OK = Status()                           # what every launch that succeeds returns
+
+
 def _st(rc: int) -> Status:
     if rc == 0:
-        return Status()
+        return _OK
     msg = lib().mcke_last_error()
     return Status(StatusCode(rc), msg.decode() if msg else "")
 
@@ -272,8 +275,9 @@ def _ptr(p) -> int | None:
         return None
     if isinstance(p, DeviceBuffer):
         return p.ptr
-    if hasattr(p, "data_ptr"):           # a torch tensor on the GPU
-        return int(p.data_ptr())
+    data_ptr = getattr(p, "data_ptr", None)
+    if data_ptr is not None:             # a torch tensor on the GPU
+        return data_ptr()
     return int(p)
 
 
@@ -592,8 +596,8 @@ def launch_gemm_lp_bias_act(a, b, bias, residual, y, ab_dtype, y_dtype, bias_dty
     reference counterpart."""
     tile = gemm_lp_default_tile(m, n, k) if tile is None else tile
     return _st(lib().mcke_launch_gemm_lp_bias_act(
-        _ptr(a), _ptr(b), _ptr(bias), _ptr(residual), _ptr(y), int(ab_dtype), int(y_dtype),
-        int(bias_dtype), m, n, k, alpha, int(act), C.byref(tile), _sh(stream)))
+        _ptr(a), _ptr(b), _ptr(bias), _ptr(residual), _ptr(y), ab_dtype, y_dtype,
+        bias_dtype, m, n, k, alpha, act, C.byref(tile), _sh(stream)))
 
 
 # ---------------------------------------------------------------------------
@@ -605,7 +609,7 @@ def launch_layer_norm(x, weight, bias, y, mean, rstd, dtype, param_dtype, rows: 
     """y = (x - mean) * rstd * weight + bias over each row; weight, bias, mean and rstd may be
     None."""
     return _st(lib().mcke_launch_layer_norm(_ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean),
-                                            _ptr(rstd), int(dtype), int(param_dtype), rows, cols,
+                                            _ptr(rstd), dtype, param_dtype, rows, cols,
                                             eps, _sh(stream)))
 
 
@@ -620,7 +624,7 @@ def launch_layer_norm_backward(dy, x, weight, mean, rstd, dx, dweight, dbias, dt
     workspace is for the latter two."""
     return _st(lib().mcke_launch_layer_norm_backward(
         _ptr(dy), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight),
-        _ptr(dbias), int(dtype), int(param_dtype), rows, cols, _ptr(workspace), workspace_bytes,
+        _ptr(dbias), dtype, param_dtype, rows, cols, _ptr(workspace), workspace_bytes,
         _sh(stream)))
 
 
@@ -637,7 +641,7 @@ def launch_token_logprobs(logits, tokens, logprobs, entropy, lse, top_logprobs, 
     row to leave out."""
     return _st(lib().mcke_launch_token_logprobs(
         _ptr(logits), _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(lse), _ptr(top_logprobs),
-        _ptr(top_ids), int(dtype), rows, vocab, row_stride, scale, top_k, _ptr(workspace),
+        _ptr(top_ids), dtype, rows, vocab, row_stride, scale, top_k, _ptr(workspace),
         workspace_bytes, _sh(stream)))
 
 
@@ -648,7 +652,7 @@ def launch_token_logprobs_backward(logits, tokens, lse, entropy, dlogprobs, dent
     may be None."""
     return _st(lib().mcke_launch_token_logprobs_backward(
         _ptr(logits), _ptr(tokens), _ptr(lse), _ptr(entropy), _ptr(dlogprobs), _ptr(dentropy),
-        _ptr(dlogits), int(dtype), rows, vocab, row_stride, scale, _sh(stream)))
+        _ptr(dlogits), dtype, rows, vocab, row_stride, scale, _sh(stream)))
 
 
 # ---------------------------------------------------------------------------
