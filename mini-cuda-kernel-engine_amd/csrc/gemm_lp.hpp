@@ -289,7 +289,9 @@ __device__ __forceinline__ void lp_store_c(const f32x16 (&acc)[BM / 64][BN / 64]
 // 14 bytes per clock and CU at 128 x 128); each operand is read half as often as by 64 x 64
 // tiles, which is what it gains on the split-K kernel: 4095 x 4095 x 1023, fp16 to fp32, 136
 // -> 65.6 us (524 TFLOP/s).
-template <typename T, typename OutT, int BM, int BN, bool VEC, bool WHOLE, class E = NoEpilogue>
+// AHEAD 2: two stages of loads in registers, each a K step longer on its way.
+template <typename T, typename OutT, int BM, int BN, bool VEC, bool WHOLE, class E = NoEpilogue,
+          int AHEAD = 1>
 __global__ __launch_bounds__(kMfmaThreads, 1) void gemm_lp_kernel(
     const uint16_t* __restrict__ A, const uint16_t* __restrict__ B, OutPtr<OutT, E> C,
     int M, int N, int K, float alpha, float beta, int tiles_m, int tiles_n, E ep) {
@@ -357,6 +359,59 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void gemm_lp_kernel(
   }
 
   constexpr int kLoads = S::kAChunks + S::KR;
+  if constexpr (AHEAD == 2) {
+    // Step ks multiplies its stage, puts stage ks + 1 (in `have`) into LDS and loads stage
+    // ks + 2 into `get`.  Past the end the last stage is loaded again and put where nobody reads.
+    auto load_stage = [&](typename S::Regs& to, int st) {
+      const int k = (st < ksteps ? st : ksteps - 1) * kLpBK - k_short;
+#pragma unroll
+      for (int l = 0; l < S::kAChunks; ++l) S::template load_a<VEC, WHOLE>(to, l, A, M, K, m0, k);
+#pragma unroll
+      for (int l = 0; l < S::KR; ++l) S::template load_b<VEC, WHOLE>(to, l, B, N, K, n0, k);
+    };
+    auto step = [&](int ks, typename S::Regs& have, typename S::Regs& get) {
+      const char* stage = smem + (ks & 1) * S::kBytes;
+      char* next_stage = smem + ((ks + 1) & 1) * S::kBytes;
+      load_stage(get, ks + 2);
+      u32x4 av[MT], bv[NT];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int q = 2 * s + h;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          av[i] = *reinterpret_cast<const u32x4*>(stage + a_row[i] + 16 * (q ^ a_x[i]));
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          bv[j] = *reinterpret_cast<const u32x4*>(stage + b_row[j] + 16 * (q ^ b_x[j]));
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int jj = 0; jj < NT; ++jj) {
+            const int j = mfma_snake_col(i, jj, NT);
+            acc[i][j] = MF::run(av[i], bv[j], acc[i][j]);
+          }
+        if (s == 2) {
+#pragma unroll
+          for (int i = 0; i < S::kAChunks; ++i) S::store_a(have, i, next_stage);
+        } else if (s == 3) {
+          S::store_b(have, next_stage);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // A bare barrier: __syncthreads() would wait for the loads on their way.
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+    typename S::Regs R2;
+    if (ksteps > 0) load_stage(R, 1);
+    int ks = 0;
+    for (; ks + 2 <= ksteps; ks += 2) {
+      step(ks, R, R2);
+      step(ks + 1, R2, R);
+    }
+    if (ks < ksteps) step(ks, R, R2);
+  } else
   for (int ks = 0; ks < ksteps; ++ks) {
     const char* stage = smem + (ks & 1) * S::kBytes;
     char* next_stage = smem + ((ks + 1) & 1) * S::kBytes;

@@ -149,11 +149,11 @@ int launch_short_k(const LpArgs<E>& x, bool vec) {
 }
 
 // The WHOLE form.
-template <typename T, typename OutT, int BM, int BN, class E>
+template <typename T, typename OutT, int BM, int BN, int AHEAD = 1, class E>
 int launch_whole(const LpArgs<E>& x) {
   const int64_t tiles = tile_count(x.m, x.n, BM, BN);
   if (int rc = check_grid<E>(tiles, kMfmaThreads)) return rc;
-  gemm_lp_kernel<T, OutT, BM, BN, false, true, E>
+  gemm_lp_kernel<T, OutT, BM, BN, false, true, E, AHEAD>
       <<<static_cast<unsigned>(tiles), kMfmaThreads, 0, x.s>>>(
           x.a, x.b, static_cast<OutT*>(x.c), x.m, x.n, x.k, x.alpha, x.beta,
           steps_along(x.m, BM), steps_along(x.n, BN), x.ep);
@@ -184,6 +184,34 @@ template <int BM, int BN, class E> bool edge_fits(const LpArgs<E>& x) {
 template <int BM, int BN, typename OutT, class E> bool whole_fits(const LpArgs<E>& x) {
   return x.n >= BN && x.k >= 64 && aligned(x.a, 2) && aligned(x.b, 2) &&
          aligned(x.c, sizeof(OutT));
+}
+
+// Odd extents with an epilogue: the register-staged kernel's WHOLE form, at 128 x 128 with two
+// stages of loads in registers, where there are enough tiles (fp16 to fp32, GELU and residual,
+// us; 256 x 256, 128 x 128 two ahead, one ahead, 64 x 64, split K 64 x 64):
+//   4001^3 217 236 244 362 374 (256 tiles of 256, one round)     3216 x 3091 x 10672 462 360 424 566 694
+//   1635 x 12638 x 3991 404 293 306 452 487      613 x 5107 x 5864 271 80 106 115 138
+//   1531 x 2053 x 1021 (204 tiles of 128) 86 31.4 35.5 34.7 39.7     x 1024 79 26.2 30.2 25.2 33.4
+//   1300 x 1901 x 4095 (165) 208 69 85 73 84     x 1024 77 24.4 28.3 21.7 28.8
+//   1200 x 1701 x 513 (140) 62 20.1 21.8 15.6 23.3      1000 x 1501 x 2001 (384 tiles of 64) 125 41 48
+//     32 32       700 x 701 x 3001 (121) 164 53 64 42 27
+// A tile of 256 takes as long as 3.7 rounds of 128.  `rc`: the launch's result, if there is one.
+template <typename T, typename OutT, class E> bool launch_odd(const LpArgs<E>& x, int* rc) {
+  const int64_t tiles = tile_count(x.m, x.n, 128, 128);
+  if (whole_fits<128, 128, OutT>(x) && (tiles >= 208 || (tiles >= 140 && x.k >= 2048))) {
+    const int64_t t256 = tile_count(x.m, x.n, 256, 256);
+    const int64_t rounds256 = (t256 + 255) / 256, rounds = (tiles + 255) / 256;
+    if (whole_fits<256, 256, OutT>(x) && t256 >= 192 && 37 * rounds256 < 10 * rounds)
+      *rc = launch_whole<T, OutT, 256, 256>(x);
+    else
+      *rc = launch_whole<T, OutT, 128, 128, 2>(x);
+    return true;
+  }
+  if (whole_fits<64, 64, OutT>(x) && tile_count(x.m, x.n, 64, 64) >= 448) {
+    *rc = launch_whole<T, OutT, 64, 64>(x);
+    return true;
+  }
+  return false;
 }
 
 // Whether the split-K kernel's limits hold: 16-bit values at 2-byte addresses, per-lane offsets
@@ -232,11 +260,14 @@ struct LpTile {
       if (edge_fits<128, 128>(x) &&
           (tiles >= 208 || (tiles >= 80 && x.k >= (sizeof(OutT) == 4 ? 256 : 100))))
         return launch_dma<T, OutT, 128, 128, true>(x);
-      if constexpr (BM == 256)
+      if constexpr (E::kFused)
+        if (int rc = 0; launch_odd<T, OutT>(x, &rc)) return rc;
+      if constexpr (BM == 256 && !E::kFused)
         if (whole_fits<256, 256, OutT>(x) && tile_count(x.m, x.n, 256, 256) >= 192)
           return launch_whole<T, OutT, 256, 256>(x);
-      if (whole_fits<128, 128, OutT>(x) && tiles >= 208)
-        return launch_whole<T, OutT, 128, 128>(x);
+      if constexpr (!E::kFused)
+        if (whole_fits<128, 128, OutT>(x) && tiles >= 208)
+          return launch_whole<T, OutT, 128, 128>(x);
     }
     if (x.n >= 32 && split_fits<OutT>(x))
       return short_k(x, vec) ? launch_short_k<T, OutT>(x, vec) : launch_split<T, OutT>(x);
