@@ -198,7 +198,7 @@ template <int BM, int BN, typename OutT, class E> bool whole_fits(const LpArgs<E
 // A tile of 256 takes as long as 3.7 rounds of 128.  `rc`: the launch's result, if there is one.
 template <typename T, typename OutT, class E> bool launch_odd(const LpArgs<E>& x, int* rc) {
   const int64_t tiles = tile_count(x.m, x.n, 128, 128);
-  if (whole_fits<128, 128, OutT>(x) && (tiles >= 208 || (tiles >= 140 && x.k >= 2048))) {
+  if (whole_fits<128, 128, OutT>(x) && (tiles >= 200 || (tiles >= 140 && x.k >= 2048))) {
     const int64_t t256 = tile_count(x.m, x.n, 256, 256);
     const int64_t rounds256 = (t256 + 255) / 256, rounds = (tiles + 255) / 256;
     if (whole_fits<256, 256, OutT>(x) && t256 >= 192 && 37 * rounds256 < 10 * rounds)

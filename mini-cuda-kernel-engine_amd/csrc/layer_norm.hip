@@ -529,7 +529,7 @@ __global__ __launch_bounds__(kFoldCols * kFoldWays) void ln_bwd_fold_kernel(
   const int64_t c = static_cast<int64_t>(blockIdx.x) * kFoldCols + lc;
   float s = 0.0f;
   if (c < cols) {
-#pragma unroll 8
+#pragma unroll 16
     for (int p = way; p < parts; p += kFoldWays)
       s += ws[(2 * static_cast<int64_t>(p) + blockIdx.y) * cols + c];
   }

@@ -52,17 +52,23 @@ __device__ __forceinline__ Sums moved(Sums s, float to, float c) {
   return {to, f * s.d, f * (s.e + t * s.d)};
 }
 
-__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  a = moved(a, m, c);
-  b = moved(b, m, c);
-  return {m, a.d + b.d, a.e + b.e};
-}
-
+// The states of a wave's lanes, or of the workgroup's waves, as one: each moved to the largest
+// m, then added up in a fixed order.
 __device__ __forceinline__ Sums wave_join(Sums s, float c) {
+  s = moved(s, wave_max(s.m), c);
+  return {s.m, wave_sum(s.d), wave_sum(s.e)};
+}
+__device__ __forceinline__ Sums block_join(const Sums (&waves)[kWaves], float c) {
+  float m = waves[0].m;
 #pragma unroll
-  for (int k = kWave / 2; k >= 1; k >>= 1)
-    s = join(s, Sums{__shfl_xor(s.m, k, 64), __shfl_xor(s.d, k, 64), __shfl_xor(s.e, k, 64)}, c);
+  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, waves[w].m);
+  Sums s{m, 0.0f, 0.0f};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const Sums q = moved(waves[w], m, c);
+    s.d += q.d;
+    s.e += q.e;
+  }
   return s;
 }
 
@@ -104,35 +110,51 @@ __device__ __forceinline__ uint32_t key_index(uint64_t k) {
   return 0xFFFFFFFFu - static_cast<uint32_t>(k);
 }
 
-// How many leading bits of order_of() tell two values of T apart (an even number).
-template <typename T> constexpr int kOrderBits = 32;
-template <> constexpr int kOrderBits<__bf16> = 16;
-template <> constexpr int kOrderBits<_Float16> = 20;     // sign, 8 bits of exponent, 10, and one
+// A value that at least k of the workgroup's logits reach, and few more: the k-th largest of the
+// largest of each quad of lanes, up to kQuadTop, else of each lane (20 of 64 quads: some 24 of
+// normally distributed logits reach it).  A value's rank is how many are larger, counted from
+// LDS, and the bound is the least of those that rank below k.  (Bisecting the values' bits with
+// ballots took 2770 cycles for 256 of them: each count passes through a scalar register.)
+// Every lane calls it, with m its largest logit and not a NaN; `lds` holds kThreads floats, and
+// `mins` kWaves.  -inf, which every logit reaches, where k of them have no logits.
+constexpr int kQuadTop = 24;
 
-// The k-th largest of a wave's 64 * PER numbers (to their leading BITS, the others 0): the
-// largest t that k of them reach, two bits at a time.  Every lane of the wave has the same.
-template <int BITS, int PER>
-__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[PER], int k) {
-  uint32_t t = 0;
-#pragma unroll 1
-  for (int b = 30; b >= 32 - BITS; b -= 2) {
-    uint32_t up = t;
+template <int N>
+__device__ __forceinline__ int count_larger(const float* lds, float v) {
+  int n = 0;
+#pragma unroll 8
+  for (int i = 0; i < N; i += 4) {
+    const f32x4 o = *reinterpret_cast<const f32x4*>(lds + i);
 #pragma unroll
-    for (uint32_t d = 1; d < 4; ++d) {
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) n += __popcll(__ballot(v[i] >= (t | d << b)));
-      up += n >= k ? 1u << b : 0u;                       // the counts fall with d
-    }
-    t = up;
+    for (int e = 0; e < 4; ++e) n += o[e] > v;
   }
-  return t;
+  return n;
 }
 
-// The least value whose order_of() reaches a bound of kth_largest.
-__device__ __forceinline__ float least_value(uint32_t bound) {
-  if (bound < 0x00800000u) return -INFINITY;             // up to order_of(-inf)
-  return __builtin_bit_cast(float, bound & 0x80000000u ? bound & 0x7FFFFFFFu : ~bound);
+// The first half, before a barrier of the workgroup.
+__device__ __forceinline__ void put_largest(float m, int k, float* lds) {
+  if (k > kQuadTop) {
+    lds[threadIdx.x] = m;
+  } else {
+    m = wave_max<4>(m);
+    if (threadIdx.x % 4 == 0) lds[threadIdx.x / 4] = m;
+  }
+}
+
+// The second, behind it.
+__device__ __forceinline__ float bound_of(float m, int k, const float* lds, float* mins) {
+  const int lane = threadIdx.x % kWave;
+  if (k <= kQuadTop) {                                   // every wave for itself
+    const float v = lds[lane];
+    return -wave_max(count_larger<kThreads / 4>(lds, v) < k ? -v : -INFINITY);
+  }
+  const float least = -wave_max(count_larger<kThreads>(lds, m) < k ? -m : -INFINITY);
+  if (lane == 0) mins[threadIdx.x / kWave] = least;
+  __syncthreads();
+  float all = mins[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) all = fminf(all, mins[w]);
+  return all;
 }
 
 // A wave's list: lane i holds the i-th best so far.  Elements come in the order of their
@@ -189,14 +211,46 @@ struct TopList {
   }
 };
 
-// The top_k largest of n different keys in LDS, to `best` in their order; 0 behind them.
-__device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int top_k, uint64_t* best) {
+// The keys a workgroup has put down, in an order that does not matter to what comes of them.
+constexpr int kMaxKeys = 1024;
+struct KeyList {
+  uint64_t keys[kMaxKeys];
+  int count;               // past kMaxKeys only counted
+
+  // Before the first key and a barrier: what rank_keys reads past the end of a short list is 0.
+  __device__ __forceinline__ void clear() {
+    if (threadIdx.x < kWave + 16) keys[threadIdx.x] = 0;
+    if (threadIdx.x == 0) count = 0;
+  }
+  __device__ __forceinline__ void put(uint64_t key) {
+    const int at = atomicAdd(&count, 1);
+    if (at < kMaxKeys) keys[at] = key;
+  }
+};
+
+// Calls out(i, key) for the top_k largest of n keys, all different, in their order, each from some
+// lane, and with key 0 for what is left of top_k.
+template <class F>
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, int top_k, F out) {
+  if (n <= kWave) {                                      // a key to a lane of the first wave
+    if (threadIdx.x >= kWave) return;
+    const int i = threadIdx.x;
+    const uint64_t mine = keys[i];
+    int rank = 0;
+    for (int j = 0; j < n; j += 16) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) rank += keys[j + e] > mine;
+    }
+    if (i >= n) rank = i;
+    if (rank < top_k) out(rank, mine);
+    return;
+  }
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t mine = keys[i];
     int rank = 0;
 #pragma unroll 8
     for (int j = 0; j < n; ++j) rank += keys[j] > mine;
-    if (mine && rank < top_k) best[rank] = mine;
+    if (rank < top_k) out(rank, mine);
   }
 }
 
@@ -209,13 +263,13 @@ struct RowOut {
   int64_t* top_ids;
 };
 
-// A row's results from its sums, its best keys in LDS and its token's logit.
+// A row's results from its sums, its n keys and its token's logit.
 __device__ __forceinline__ void write_row(const RowOut& o, int64_t r, int64_t vocab, int64_t token,
-                                          float logit, Sums s, const uint64_t* best, int top_k,
-                                          float scale) {
+                                          float logit, Sums s, const uint64_t* keys, int n,
+                                          int top_k, float scale) {
   const float ln_d = logf(s.d);
   const bool empty = s.m == -INFINITY && s.d == 0.0f;   // every logit is masked
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == kThreads - 1) {                    // the first wave ranks meanwhile
     if (o.logprobs) {
       float lp = __builtin_nanf("");                    // no such token
       if (token < vocab) lp = empty ? -INFINITY : (logit - s.m) * scale - ln_d;
@@ -224,12 +278,12 @@ __device__ __forceinline__ void write_row(const RowOut& o, int64_t r, int64_t vo
     if (o.entropy) o.entropy[r] = empty ? 0.0f : ln_d - kLn2 * (s.e / s.d);
     if (o.lse) o.lse[r] = empty ? -INFINITY : s.m * scale + ln_d;
   }
-  for (int i = threadIdx.x; i < top_k; i += kThreads) {
-    const uint64_t k = best[i];
+  if (top_k == 0) return;
+  rank_keys(keys, n, top_k, [&](int i, uint64_t k) {
     const float v = empty ? -INFINITY : (key_value(k) - s.m) * scale - ln_d;
     if (o.top_logprobs) o.top_logprobs[r * top_k + i] = k ? v : __builtin_nanf("");
     if (o.top_ids) o.top_ids[r * top_k + i] = k ? static_cast<int64_t>(key_index(k)) : -1;
-  }
+  });
 }
 
 __device__ __forceinline__ void write_no_row(const RowOut& o, int64_t r, int top_k) {
@@ -256,7 +310,6 @@ struct Part {
   float m, d, e, unused;
 };
 
-constexpr int kMaxKeys = 1024;       // candidates of a part, or keys of all parts of a row
 
 template <typename T>
 __device__ __forceinline__ VecT16<T> load_logits(const T* row, int64_t j, int64_t vocab) {
@@ -266,10 +319,11 @@ __device__ __forceinline__ VecT16<T> load_logits(const T* row, int64_t j, int64_
 }
 
 // The alternatives of vectors first .. end - 1 of a row, in any order and with any ties: a list
-// per wave, elements in the order of their indices.  Returns how many keys it put down.
+// per wave, elements in the order of their indices.  Returns how many keys the waves put down;
+// every lane of the workgroup calls it, and a barrier follows.
 template <typename T>
 __device__ __noinline__ int list_keys(const T* row, int64_t first, int64_t end, int64_t vocab,
-                                      int top_k, uint64_t* keys) {
+                                      int top_k, KeyList* list, int* counts) {
   constexpr int VE = kVecElems<T>;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   TopList top;
@@ -289,8 +343,54 @@ __device__ __noinline__ int list_keys(const T* row, int64_t first, int64_t end, 
     }
     top.offer<VE>(v, m, static_cast<uint32_t>(j0 * VE));
   }
-  if (lane < top_k) keys[wave * top_k + lane] = lane < top.count ? key_of(top.v, top.i) : 0;
-  return kWaves * top_k;
+  if (lane == 0) counts[wave] = top.count;
+  if (threadIdx.x < kWave + 16) list->keys[threadIdx.x] = 0;
+  __syncthreads();
+  int before = 0, n = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += counts[w];
+    n += counts[w];
+  }
+  if (lane < top.count) list->keys[before + lane] = key_of(top.v, top.i);
+  return n;
+}
+
+typedef uint32_t u32x4_of __attribute__((ext_vector_type(4)));
+
+// Logit i of a dword of T.
+template <typename T> __device__ __forceinline__ float value_of(uint32_t d, int i) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, d);
+  else
+    return static_cast<float>(
+        __builtin_bit_cast(T, static_cast<uint16_t>(i ? d >> 16 : d & 0xFFFFu)));
+}
+
+// Puts down the logits of a lane's vectors j, j + kThreads, ... that reach `least`.  Which do is a
+// bit each of one number, whose few bits a loop picks out.
+template <typename T, int N>
+__device__ __forceinline__ void put_keys(const VecT16<T> (&w)[N], int64_t j, int64_t end,
+                                         int64_t vocab, float least, KeyList& list) {
+  constexpr int VE = kVecElems<T>, PER = VE / 4;         // logits of a dword
+  static_assert(N * VE <= 32, "a bit each");
+  uint32_t hit = 0;
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      hit |= static_cast<float>(w[u][e]) >= least ? 1u << (u * VE + e) : 0u;   // never a NaN
+  while (hit) {
+    const int k = __ffs(hit) - 1;
+    hit &= hit - 1;
+    const int64_t ju = j + k / VE * kThreads, index = ju * VE + k % VE;
+    if (ju >= end || index >= vocab) continue;
+    uint32_t d = 0;
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        d = k / PER == 4 * u + i ? __builtin_bit_cast(u32x4_of, w[u])[i] : d;
+    list.put(key_of(value_of<T>(d, k % PER), static_cast<uint32_t>(index)));
+  }
 }
 
 // Workgroup (row, part): vectors part * per_part on, in rounds of kUnroll vectors a lane, each
@@ -301,8 +401,8 @@ __device__ __noinline__ int list_keys(const T* row, int64_t first, int64_t end, 
 // its sums, and keeps it for each quarter of its rounds.  The top_k-th largest of the lanes' is
 // a bound that at least top_k logits reach and few others do; only quarters whose largest
 // reaches it have any, so those are read again (from the caches) and the logits that reach the
-// bound are put down and ranked.  Rows in which more than kMaxKeys reach it (ties, masks, sorted
-// rows) take list_keys instead.
+// bound are put down and ranked.  Where more than kMaxKeys reach it (ties, masks, sorted rows)
+// list_keys does it instead.
 constexpr int kUnroll = 4, kQuarters = 4;
 template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ x, RowOut o,
@@ -312,10 +412,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
                                                             int parts, int64_t per_part,
                                                             float scale, int top_k) {
   constexpr int VE = kVecElems<T>, U = kUnroll, kRound = U * kThreads;
-  __shared__ uint64_t keys[kMaxKeys], best[kMaxTop];
-  __shared__ uint32_t largest[kThreads];
+  __shared__ KeyList list;
+  __shared__ __attribute__((aligned(16))) float largest[kThreads];
+  __shared__ float mins[kWaves];
   __shared__ Sums waves[kWaves];
-  __shared__ int hot[kQuarters * kThreads], hot_count, key_count;
+  __shared__ int hot[kQuarters * kThreads], hot_count, wave_counts[kWaves];
   const int64_t r = blockIdx.x / parts;
   const int part = static_cast<int>(blockIdx.x % parts);
   const T* row = x + r * row_stride;
@@ -374,70 +475,53 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     }
   }
 
-  if (t == 0) hot_count = key_count = 0;
-  if (t < kMaxTop) best[t] = 0;
-  const uint32_t mine = order_of(s.m);
-  largest[t] = mine;
+  if (t == 0) hot_count = 0;
+  list.clear();
+  const float mine = s.m;
+  if (top_k > 0) put_largest(mine, top_k, largest);
   s = wave_join(s, c);
   if (lane == 0) waves[wave] = s;
   __syncthreads();
-  s = waves[0];
-#pragma unroll
-  for (int i = 1; i < kWaves; ++i) s = join(s, waves[i], c);
+  s = block_join(waves, c);
 
+  int n_keys = 0;
   if (top_k > 0) {
-    uint32_t v[kWaves];
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) v[i] = largest[i * kWave + lane];
-    const uint32_t bound = kth_largest<kOrderBits<T>, kWaves>(v, top_k);
-    const float least = least_value(bound);
-    auto put = [&](const VecT16<T>& w, int64_t j) {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float y = static_cast<float>(w[e]);
-        if (y >= least && j * VE + e < vocab) {         // never a NaN
-          const int n = atomicAdd(&key_count, 1);
-          if (n < kMaxKeys) keys[n] = key_of(y, static_cast<uint32_t>(j * VE + e));
-        }
-      }
-    };
+    const float least = bound_of(mine, top_k, largest, mins);
     if (rounds <= 1) {                                  // the lane still has its vectors
-      if (mine >= bound) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (first + u * kThreads + t < end) put(w[u], first + u * kThreads + t);
-      }
+      if (mine >= least) put_keys<T, U>(w, first + t, end, vocab, least, list);
     } else {
       const int per_hot = quarter * U;                  // vectors of a lane's quarter
 #pragma unroll
       for (int q = 0; q < kQuarters; ++q)
-        if (order_of(quarter_m[q]) >= bound && q * quarter < rounds)
+        if (quarter_m[q] >= least && q * quarter < rounds)
           hot[atomicAdd(&hot_count, 1)] = q * per_hot * kThreads + t;
       __syncthreads();
       const int items = hot_count * per_hot;
       for (int i = t; i < items; i += kThreads) {
         const int h = i / per_hot;
         const int64_t j = first + hot[h] + static_cast<int64_t>(i - h * per_hot) * kThreads;
-        if (j < end) put(load_logits<T>(row, j, vocab), j);
+        if (j >= end) continue;
+        const VecT16<T> one[1] = {load_logits<T>(row, j, vocab)};
+        put_keys<T, 1>(one, j, end, vocab, least, list);
       }
     }
     __syncthreads();
-    int n = key_count;
-    if (n > kMaxKeys) {
+    n_keys = list.count;
+    if (n_keys > kMaxKeys) {
       __syncthreads();                                  // everybody has read the count
-      n = list_keys<T>(row, first, end, vocab, top_k, keys);
+      n_keys = list_keys<T>(row, first, end, vocab, top_k, &list, wave_counts);
       __syncthreads();
     }
-    rank_keys(keys, n, top_k, best);
-    __syncthreads();
   }
   if (parts == 1) {
-    write_row(o, r, vocab, token, logit, s, best, top_k, scale);
+    write_row(o, r, vocab, token, logit, s, list.keys, n_keys, top_k, scale);
     return;
   }
-  if (t == 0) parts_out[blockIdx.x] = Part{s.m, s.d, s.e, 0.0f};
-  for (int i = t; i < top_k; i += kThreads)
-    keys_out[static_cast<int64_t>(blockIdx.x) * top_k + i] = best[i];
+  if (t == kThreads - 1) parts_out[blockIdx.x] = Part{s.m, s.d, s.e, 0.0f};
+  if (top_k > 0)
+    rank_keys(list.keys, n_keys, top_k, [&](int i, uint64_t k) {
+      keys_out[static_cast<int64_t>(blockIdx.x) * top_k + i] = k;
+    });
 }
 
 // A row's parts joined, a workgroup per row.  Keys: the top_k-th largest of the lanes' largest is
@@ -448,9 +532,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(
     const T* __restrict__ x, RowOut o, const Part* __restrict__ parts_in,
     const uint64_t* __restrict__ keys_in, int64_t vocab, int64_t row_stride, int parts,
     float scale, int top_k) {
-  __shared__ uint64_t keys[kMaxKeys], best[kMaxTop];
-  __shared__ uint32_t largest[kThreads];
-  __shared__ int key_count;
+  __shared__ KeyList list;
+  __shared__ __attribute__((aligned(16))) float largest[kThreads];
+  __shared__ float mins[kWaves];
   const int64_t r = blockIdx.x;
   const int t = threadIdx.x, lane = t % kWave;
   const int n = parts * top_k;
@@ -470,26 +554,22 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(
   }
   const float logit = token_logit<T>(o, x + r * row_stride, vocab, token);
   if (top_k > 0) {
-    if (t == 0) key_count = 0;
-    if (t < kMaxTop) best[t] = 0;
+    list.clear();
     uint64_t most = key[0];
 #pragma unroll
     for (int i = 1; i < kKeysPerLane; ++i) most = key[i] > most ? key[i] : most;
-    largest[t] = static_cast<uint32_t>(most >> 32);
+    const float m = most ? key_value(most) : -INFINITY;
+    put_largest(m, top_k, largest);
     __syncthreads();
-    uint32_t v[kWaves];
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) v[i] = largest[i * kWave + lane];
-    const uint32_t bound = kth_largest<kOrderBits<T>, kWaves>(v, top_k);
+    const float least = bound_of(m, top_k, largest, mins);
 #pragma unroll
     for (int i = 0; i < kKeysPerLane; ++i)
-      if (key[i] && key[i] >> 32 >= bound) keys[atomicAdd(&key_count, 1)] = key[i];
-    __syncthreads();
-    rank_keys(keys, key_count, top_k, best);
+      if (key[i] && key_value(key[i]) >= least) list.put(key[i]);
     __syncthreads();
   }
   const float c = scale * kLog2e;
-  write_row(o, r, vocab, token, logit, wave_join(s, c), best, top_k, scale);
+  write_row(o, r, vocab, token, logit, wave_join(s, c), list.keys, top_k > 0 ? list.count : 0, top_k,
+            scale);
 }
 
 // dlogits = scale (g ([j == token] - p_j) - h p_j (log p_j + entropy)), g and h the gradients
