@@ -186,26 +186,43 @@ template <int BM, int BN, typename OutT, class E> bool whole_fits(const LpArgs<E
          aligned(x.c, sizeof(OutT));
 }
 
-// Odd extents with an epilogue: the register-staged kernel's WHOLE form, at 128 x 128 with two
-// stages of loads in registers, where there are enough tiles (fp16 to fp32, GELU and residual,
-// us; 256 x 256, 128 x 128 two ahead, one ahead, 64 x 64, split K 64 x 64):
-//   4001^3 217 236 244 362 374 (256 tiles of 256, one round)     3216 x 3091 x 10672 462 360 424 566 694
-//   1635 x 12638 x 3991 404 293 306 452 487      613 x 5107 x 5864 271 80 106 115 138
-//   1531 x 2053 x 1021 (204 tiles of 128) 86 31.4 35.5 34.7 39.7     x 1024 79 26.2 30.2 25.2 33.4
-//   1300 x 1901 x 4095 (165) 208 69 85 73 84     x 1024 77 24.4 28.3 21.7 28.8
-//   1200 x 1701 x 513 (140) 62 20.1 21.8 15.6 23.3      1000 x 1501 x 2001 (384 tiles of 64) 125 41 48
-//     32 32       700 x 701 x 3001 (121) 164 53 64 42 27
-// A tile of 256 takes as long as 3.7 rounds of 128.  `rc`: the launch's result, if there is one.
+// Odd extents with an epilogue: the register-staged kernel's WHOLE form, with two stages of loads
+// in registers at 128 x 128 and 64 x 128.  By tiles of 128 x 128 (t), fp16 to fp32 with GELU and
+// residual, us:
+//                        t    256   128, 128 one ahead   64 x 128   64    split K 64 x 64
+//   4001^3             1024   217   236     240            274     362      374
+//   1635 x 12638 x 3991 1287  404   287     304            331     455      487
+//   3216 x 3091 x 10672 650   462   350     415            426     568      694
+//   2501 x 2501 x 1001  400          41                     48      52       66
+//   613 x 5107 x 5864   200   271    78     106             92     114      138
+//   1531 x 2053 x 1021  204    86    31      35             28      34       40
+//   3001 x 1201 x 901   240    82    29      33             27      31       37
+//   1300 x 1901 x 4095  165   208    73      85             73      70       81
+//   1200 x 1701 x 513   140    62    20      22             19      15       22
+//   900 x 1501 x 4001    96          65                     45      54       56
+//   1000 x 1301 x 2001   88          41                     27      31       31
+//   300 x 3001 x 2001    72          39                     27      30       24
+// A tile of 256 takes as long as 3.7 rounds of 128; 64 x 128 is for one round of its tiles, one to a
+// CU.  `rc`: the launch's result, if there is one.
 template <typename T, typename OutT, class E> bool launch_odd(const LpArgs<E>& x, int* rc) {
   const int64_t tiles = tile_count(x.m, x.n, 128, 128);
-  if (whole_fits<128, 128, OutT>(x) && (tiles >= 200 || (tiles >= 140 && x.k >= 2048))) {
-    const int64_t t256 = tile_count(x.m, x.n, 256, 256);
-    const int64_t rounds256 = (t256 + 255) / 256, rounds = (tiles + 255) / 256;
-    if (whole_fits<256, 256, OutT>(x) && t256 >= 192 && 37 * rounds256 < 10 * rounds)
-      *rc = launch_whole<T, OutT, 256, 256>(x);
-    else
-      *rc = launch_whole<T, OutT, 128, 128, 2>(x);
-    return true;
+  if (whole_fits<128, 128, OutT>(x)) {
+    if (tiles >= 200) {
+      const int64_t t256 = tile_count(x.m, x.n, 256, 256);
+      const int64_t rounds256 = (t256 + 255) / 256, rounds = (tiles + 255) / 256;
+      if (whole_fits<256, 256, OutT>(x) && t256 >= 192 && 37 * rounds256 < 10 * rounds)
+        *rc = launch_whole<T, OutT, 256, 256>(x);
+      else if (tiles <= 256 && x.k < 2048)
+        *rc = launch_whole<T, OutT, 64, 128, 2>(x);
+      else
+        *rc = launch_whole<T, OutT, 128, 128, 2>(x);
+      return true;
+    }
+    const int64_t halves = tile_count(x.m, x.n, 64, 128);
+    if (halves >= 170 && halves <= 256) {
+      *rc = launch_whole<T, OutT, 64, 128, 2>(x);
+      return true;
+    }
   }
   if (whole_fits<64, 64, OutT>(x) && tile_count(x.m, x.n, 64, 64) >= 448) {
     *rc = launch_whole<T, OutT, 64, 64>(x);

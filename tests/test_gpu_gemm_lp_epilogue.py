@@ -108,6 +108,38 @@ def test_exact_sums(gpu, i, shape, which):
     assert torch.equal(run(gpu, a, b, bias, res, ab, yt, bt, RELU, in_place=True), y.to(TORCH[yt]))
 
 
+# The kernels for few rows at each of their widths (up to 16, 32 and 64 rows; 4096, 8192 and 16384
+# columns), with K chunks that the waves share unevenly; odd extents at 256 x 256, 128 x 128 with
+# two stages ahead (K of two, three and four steps), 64 x 128 and 64 x 64.
+MORE = [(1, 200, 2000), (2, 300, 4090), (16, 4096, 96), (3, 5001, 131), (2, 9000, 70),
+        (1, 16400, 96), (20, 300, 200), (25, 5003, 77), (30, 8500, 64), (50, 130, 333),
+        (64, 4100, 65), (33, 8300, 66), (3701, 3701, 65), (2100, 2301, 67), (2100, 2301, 131),
+        (2101, 2303, 200), (900, 2101, 65), (900, 2101, 130), (1201, 1701, 69)]
+
+
+@pytest.mark.parametrize("i,shape", enumerate(MORE), ids=[f"{s[0]}x{s[1]}x{s[2]}" for s in MORE])
+def test_exact_sums_of_more_kernels(gpu, i, shape):
+    for which in (i % 4, (i + 1) % 4):
+        ab = (BF16, F16)[which % 2]
+        yt, bt = (ab, F32)[which // 2], (F32, ab)[i % 2]
+        a, b, bias, res = _operands(*shape, ab, yt, bt, i, quarters=True)
+        for act, bb, rr in ((NONE, bias, res), (RELU, None, res), (RELU, bias, None)):
+            y, _ = _want(a, b, bb, rr, act, 1.0, yt)
+            assert torch.equal(run(gpu, a, b, bb, rr, ab, yt, bt, act), y.to(TORCH[yt])), act
+        y, _ = _want(a, b, bias, res, NONE, 1.0, yt)
+        got = run(gpu, a, b, bias, res, ab, yt, bt, NONE, shift=1, in_place=True)
+        assert torch.equal(got, y.to(TORCH[yt]))
+
+
+@pytest.mark.parametrize("i,shape", enumerate(MORE), ids=[f"{s[0]}x{s[1]}x{s[2]}" for s in MORE])
+def test_activations_of_more_kernels(gpu, i, shape):
+    ab, yt, bt = _types(i)
+    a, b, bias, res = _operands(*shape, ab, yt, bt, 70 + i)
+    for act in (ERF, TANH):
+        check("y", run(gpu, a, b, bias, res, ab, yt, bt, act),
+              *_want(a, b, bias, res, act, 1.0, yt))
+
+
 @pytest.mark.parametrize("act", [NONE, RELU, ERF, TANH])
 @pytest.mark.parametrize("i,shape", enumerate(SHAPES), ids=[f"{s[0]}x{s[1]}x{s[2]}" for s in SHAPES])
 def test_activations(gpu, i, shape, act):
