@@ -276,7 +276,9 @@ def _ptr(p) -> int | None:
     if isinstance(p, DeviceBuffer):
         return p.ptr
     data_ptr = getattr(p, "data_ptr", None)
-    if data_ptr is not None:             # a torch tensor on the GPU
+    if data_ptr is not None:             # a torch tensor
+        if not getattr(p, "is_cuda", True) and not p.is_pinned():
+            raise ValueError("a tensor in host memory where a kernel reads or writes device memory")
         return data_ptr()
     return int(p)
 

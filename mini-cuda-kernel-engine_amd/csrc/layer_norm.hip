@@ -547,20 +547,25 @@ __global__ __launch_bounds__(kFoldCols * kFoldWays) void ln_bwd_fold_kernel(
 // ---------------------------------------------------------------------------
 // Calls f with a shape of the forward kernel as constants.  Two rows a lane share the weight's
 // and bias's loads.  bf16 and fp32, 134217728 bytes of x, us (the best of 44 shapes, by width in
-// vectors): 8 44.3, 16 45.6, 32 44.9, 64 45.2, 128 44.5, 256 45.2, 512 45.4 (128 x 4 46.5, 256 x 2
-// 45.6), 1024 90.0 at twice the bytes (256 x 4 one row 92.2), 2048 92.5 (1024 lanes x 2 99.3), 4096
-// 95.6, 8192 106; one row instead of two 1 to 6 us more up to 512 vectors.
+// vectors): 8 44.3, 16 45.6, 32 44.9, 64 45.2, 128 44.5, 256 45.2, 512 45.1 (128 x 4 one row 45.6,
+// 512 x 1 48.6; 16384 x 4095: 50.7 and 49.2), 1024 90.0 at twice the bytes (256 x 4 one row 92.2),
+// 2048 92.5 (1024 lanes x 2 99.3), 4096 95.6, 8192 106; one row instead of two 1 to 6 us more up to
+// 512 vectors.  Non-temporal loads and stores: 45.1; stores alone 46.2, loads alone 47.8,
+// neither 48.4.
 template <int TPR_, int VPT_, int NT_, int ROWS_> struct RowShape {
   static constexpr int TPR = TPR_, VPT = VPT_, NT = NT_, ROWS = ROWS_;
 };
-template <typename T, class F> int with_forward_shape(int64_t vecs, F f) {
+template <typename T, bool WHOLE, class F> int with_forward_shape(int64_t vecs, F f) {
   if (vecs <= 8) return f(RowShape<8, 1, 256, 2>{});
   if (vecs <= 16) return f(RowShape<16, 1, 256, 2>{});
   if (vecs <= 32) return f(RowShape<32, 1, 256, 2>{});
   if (vecs <= 64) return f(RowShape<64, 1, 256, 2>{});
   if (vecs <= 128) return f(RowShape<128, 1, 256, 2>{});
   if (vecs <= 256) return f(RowShape<128, 2, 256, 2>{});
-  if (vecs <= 512) return f(RowShape<512, 1, 512, 2>{});
+  if (vecs <= 512) {
+    if constexpr (WHOLE) return f(RowShape<256, 2, 256, 2>{});
+    else return f(RowShape<512, 1, 512, 2>{});
+  }
   if (vecs <= 1024) return f(RowShape<512, 2, 512, sizeof(T) == 2 ? 2 : 1>{});
   if (vecs <= 2048) return f(RowShape<512, 4, 512, 1>{});
   if (vecs <= 4096) return f(RowShape<1024, 4, 1024, 1>{});
@@ -639,7 +644,7 @@ struct LnFwdArgs {
 
 template <typename T, typename P, bool WHOLE> int ln_fwd_regs(const LnFwdArgs& a) {
   constexpr int VE = kVecElems<T>;
-  return with_forward_shape<T>((a.cols + VE - 1) / VE, [&](auto shape) {
+  return with_forward_shape<T, WHOLE>((a.cols + VE - 1) / VE, [&](auto shape) {
     using S = decltype(shape);
     constexpr int64_t kRows = S::NT / S::TPR * S::ROWS;
     const int64_t groups = (a.rows + kRows - 1) / kRows;

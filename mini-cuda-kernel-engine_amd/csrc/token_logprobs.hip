@@ -677,14 +677,14 @@ template <typename T> int logprobs(const RowArgs& a) {
 
 int check_logits(const char* who, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
                  float scale) {
-  const std::string w(who);
-  if (!is_dtype(dtype)) return invalid(w + ": unknown dtype " + std::to_string(dtype));
-  if (rows < 0 || vocab < 0) return invalid(w + ": negative extent");
-  if (vocab > 2147483647LL) return invalid(w + ": vocab exceeds INT32_MAX");
-  if (row_stride < vocab) return invalid(w + ": row_stride is less than vocab");
-  if (rows > 0 && row_stride > INT64_MAX / 16 / rows) return invalid(w + ": extent too large");
+  auto no = [&](const std::string& what) { return invalid(std::string(who) + ": " + what); };
+  if (!is_dtype(dtype)) return no("unknown dtype " + std::to_string(dtype));
+  if (rows < 0 || vocab < 0) return no("negative extent");
+  if (vocab > 2147483647LL) return no("vocab exceeds INT32_MAX");
+  if (row_stride < vocab) return no("row_stride is less than vocab");
+  if (rows > 0 && row_stride > INT64_MAX / 16 / rows) return no("extent too large");
   if (!(scale > 0.0f) || std::isinf(scale * kLog2e))
-    return invalid(w + ": scale must be finite and above zero");
+    return no("scale must be finite and above zero");
   return ok();
 }
 

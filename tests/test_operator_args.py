@@ -28,6 +28,16 @@ def _refused(m, st, part):
     assert part in st.message, st.message
 
 
+def test_host_tensors_are_refused(mcke):
+    """A tensor that a kernel could not read is refused before its address is taken."""
+    import torch
+    x = torch.zeros(4, 8)
+    with pytest.raises(ValueError, match="host memory"):
+        mcke.launch_layer_norm(x, None, None, x, None, None, 0, 0, 4, 8, 1e-5)
+    with pytest.raises(ValueError, match="host memory"):
+        mcke.launch_row_softmax_f32(x, x, 4, 8, mcke.SoftmaxVariant.kOnlineOnePass)
+
+
 # ---------------------------------------------------------------------------
 # Layer norm
 # ---------------------------------------------------------------------------
