@@ -72,21 +72,33 @@ __device__ __forceinline__ Sums block_join(const Sums (&waves)[kWaves], float c)
   return s;
 }
 
-// Takes in N values whose largest is m.
+// Takes in N values whose largest is m, at one fused multiply-add an exponent: with r = from c
+// rounded and lo = from c - r (exact, by another one), the exponents are v c - r - lo, and what
+// all of them have in common comes out of the sums as 2^-lo:
+//   sum 2^u = 2^-lo d,  sum u 2^u = 2^-lo (e - lo d)   with  d = sum 2^(v c - r), e = sum (v c - r) 2^(v c - r)
+// The multiply-add rounds once, at the size of its result, so large logits lose nothing to the
+// product.  lo stays below 32 as |r| is held to 2^30 with a smaller c: past that two logits that
+// differ are 64 apart in the exponent either way, and the smaller one's 2^u is nothing.
+// (Difference, then product: 4096 x 32768 bf16 with the top 20 55.0 us, this 52.8.)
 template <int N, bool ENTROPY>
 __device__ __forceinline__ void add_values(Sums& s, const float (&v)[N], float m, float c) {
+  constexpr float kMost = 1073741824.0f;
   const float to = fmaxf(s.m, m);
   s = moved(s, to, c);
   const float from = to == -INFINITY ? 0.0f : to;
+  const float cc = fabsf(from * c) > kMost ? kMost / fabsf(from) : c;
+  const float r = from * cc, lo = __builtin_fmaf(from, cc, -r);
+  float d = 0.0f, e = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    // The difference before the product: a product alone, rounded at the size of z, would move
-    // large logits by much of a unit.
-    const float u = (v[i] - from) * c;
+    const float u = __builtin_fmaf(v[i], cc, -r);
     const float p = __builtin_amdgcn_exp2f(u);
-    s.d += p;
-    if constexpr (ENTROPY) s.e += p * fmaxf(u, kFar);
+    d += p;
+    if constexpr (ENTROPY) e += p * fmaxf(u, kFar);
   }
+  const float f = __builtin_amdgcn_exp2f(-lo);
+  s.d += f * d;
+  if constexpr (ENTROPY) s.e += f * (e - lo * d);
 }
 
 // ---------------------------------------------------------------------------

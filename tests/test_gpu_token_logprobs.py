@@ -64,7 +64,7 @@ def _reference(x, tokens, scale, k):
 
     def lp_of(ids):
         zi = z.gather(1, ids)
-        lp = zi - lse
+        lp = zi - M - ln_d                            # lse itself may swallow ln_d, in 64 bits too
         far = torch.where(zi > -INF, M - zi, 0.0)
         return lp, torch.where(lp > -INF, 2 * U * far + R + 3 * U * ln_d + U * lp.abs(), 0.0)
 
@@ -231,9 +231,9 @@ def test_any_alignment(gpu, shift, pad):
 
 
 def test_large_logits(gpu):
-    """Logits of 1e4 and more, whose exponentials' arguments need the difference before the
-    product."""
-    for mag in (1e4, 1e6):
+    """Logits of 1e4 and more, whose exponentials' arguments must not be rounded at the logits'
+    size; from 1e9 on any two that differ are far apart."""
+    for mag in (1e4, 1e6, -1e6, 1e9, 1e12, -1e12, 1e30, -3e38):
         x, tokens = _logits(3, 5000, F32, 8)
         x = x + mag
         compare(run(gpu, x, tokens, 1.0, 5), _reference(x, tokens, 1.0, 5))
