@@ -205,7 +205,7 @@ struct TopList {
       least = __builtin_bit_cast(float, b >= 0 ? b + 1 : b - 1);
     }
   }
-  // The lanes' values v[0 ..], lane l's first one at index first + VE * l.
+  // The lanes' values x[0 ..], lane l's first one at index first + VE * l, m the lane's largest.
   template <int VE>
   __device__ __forceinline__ void offer(const float (&x)[VE], float m, uint32_t first) {
     uint64_t hot = __ballot(m >= least);
@@ -321,7 +321,6 @@ __device__ __forceinline__ float token_logit(const RowOut& o, const T* row, int6
 struct Part {
   float m, d, e, unused;
 };
-
 
 template <typename T>
 __device__ __forceinline__ VecT16<T> load_logits(const T* row, int64_t j, int64_t vocab) {
