@@ -264,6 +264,7 @@ __global__ __launch_bounds__(NT) void ln_bwd_regs_kernel(
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const auto& wi = weights(i);
+      float s1 = 0.0f;
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
         const float d = static_cast<float>(dv[i][e]);
@@ -273,8 +274,11 @@ __global__ __launch_bounds__(NT) void ln_bwd_regs_kernel(
           db[i][e] += d;
         }
         s[0] += d * wi[e];
-        s[1] += d * wi[e] * xhat;
+        s1 += d * wi[e] * xhat;
       }
+      // A lane without vector i has zeros there: its (0 - mean) rstd is not a value of the row,
+      // and may be past fp32's range.
+      if (rv.has(i * TPR + t)) s[1] += s1;
       rv.repeated(i * TPR + t, [&](int e) {
         const float dg = static_cast<float>(dv[i][e]) * wi[e];
         s[0] -= dg;

@@ -231,6 +231,20 @@ def test_special_values(gpu, cols):
         assert same_bits(y[r], clean[0][r])
 
 
+@pytest.mark.parametrize("cols", [100, 99, 8])
+def test_large_constant_rows_backward(gpu, cols):
+    """Equal values of 2^120: their sum is exact and finite and xhat is 0 everywhere, while
+    mean * rstd is past fp32's range; lanes that hold none of the row add nothing to it."""
+    x = torch.full((3, cols), 2.0**120)
+    dy = (torch.arange(3 * cols).reshape(3, cols) % 5 - 2).float()
+    _, mean, rstd = run_forward(gpu, x, None, None, F32, F32)
+    assert (mean == 2.0**120).all() and 2.0**120 * float(rstd[0]) > torch.finfo(torch.float32).max
+    got = run_backward(gpu, dy, x, None, mean, rstd, F32, F32)
+    for name, g, r, t in zip(("dx", "dweight", "dbias"), got,
+                             *_backward(dy, x, None, mean, rstd, F32, F32)):
+        check(name, g, r, t)
+
+
 def test_gradient_against_differences(gpu):
     """dx, dweight and dbias of sum(dy y) against central differences of the forward formula in
     64 bits: with steps of 1e-4 their own error is below 1e-7 of the largest gradient."""
