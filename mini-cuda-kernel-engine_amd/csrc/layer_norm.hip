@@ -582,11 +582,12 @@ constexpr int64_t kMaxForwardVecs = 8192;
 // them cost more than they hide).  At 402653184 bytes of x, dy and dx, us: 8 vectors 68.5 (768
 // workgroups; 512 75.0, 1024 70.1), 32 69.3, 64 69.6, 128 70.1, 256 70.6 (fp32 66.7), 512 73.7
 // (512 x 1 75.8, 256 x 2 77.0), 1024 143 at twice the bytes (512 x 4 155), 2048 147 (256 workgroups;
-// 512 159).  4096 vectors in 16 bits would spill (965): dx and the column sums apart.
+// 512 159).  8192 rows of 640 and 768 vectors 55.5 and 61.5 (256 x 4 58.1 and 62.3).  4096 vectors
+// in 16 bits would spill (965): dx and the column sums apart.
 template <int TPR_, int VPT_, int NT_, int WGS_> struct BackShape {
   static constexpr int TPR = TPR_, VPT = VPT_, NT = NT_, kWorkgroups = WGS_;
 };
-template <bool WHOLE, class F> int with_backward_shape(int64_t vecs, F f) {
+template <int VE, bool WHOLE, class F> int with_backward_shape(int64_t vecs, F f) {
   if (vecs <= 8) return f(BackShape<8, 1, 256, 768>{});
   if (vecs <= 16) return f(BackShape<16, 1, 256, 768>{});
   if (vecs <= 32) return f(BackShape<32, 1, 256, 768>{});
@@ -598,7 +599,14 @@ template <bool WHOLE, class F> int with_backward_shape(int64_t vecs, F f) {
     if constexpr (WHOLE) return f(BackShape<128, 4, 256, 512>{});
     else return f(BackShape<256, 2, 256, 512>{});
   }
-  if (vecs <= 1024) return f(BackShape<256, 4, 256, 512>{});
+  if (vecs <= 768) return f(BackShape<256, 3, 256, 512>{});
+  // A row's end takes 256 x 4 over 256 registers in 16 bits, one workgroup a CU: 8192 x 6143 110 us
+  // (256 x 3 74.6), 8192 x 8191 129 (512 x 2 112, with 512 workgroups 120; 1024 x 1 115).  fp32 has
+  // them: 8192 x 4095 79.1, 512 x 2 85.4.
+  if (vecs <= 1024) {
+    if constexpr (WHOLE || VE == 4) return f(BackShape<256, 4, 256, 512>{});
+    else return f(BackShape<512, 2, 512, 256>{});
+  }
   return f(BackShape<1024, 2, 1024, 256>{});
 }
 constexpr int64_t kMaxBackwardVecs = 2048;
@@ -626,8 +634,12 @@ int ln_parts(int64_t rows, int64_t cols, int vec) {
   const int64_t vecs = (cols + vec - 1) / vec;
   if (vecs > kMaxBackwardVecs) return params_parts(rows, cols, vec);
   auto count = [&](auto shape) { return backward_workgroups<decltype(shape)>(rows); };
-  return cols % vec == 0 ? with_backward_shape<true>(vecs, count)
-                         : with_backward_shape<false>(vecs, count);
+  const bool whole = cols % vec == 0;
+  if (vec == 4)
+    return whole ? with_backward_shape<4, true>(vecs, count)
+                 : with_backward_shape<4, false>(vecs, count);
+  return whole ? with_backward_shape<8, true>(vecs, count)
+               : with_backward_shape<8, false>(vecs, count);
 }
 
 // One workgroup per row up to the grid's 32-bit work size, which the kernels then walk.
@@ -721,7 +733,7 @@ int ln_bwd_rows(const LnBwdArgs& a, int parts, bool* summed) {
   const bool params = a.dweight || a.dbias;
   *summed = params && vecs <= kMaxBackwardVecs;
   if (vecs <= kMaxBackwardVecs)
-    return with_backward_shape<WHOLE>(vecs, [&](auto shape) {
+    return with_backward_shape<VE, WHOLE>(vecs, [&](auto shape) {
       using S = decltype(shape);
       // The workspace and the fold count on it.
       if (backward_workgroups<S>(a.rows) != parts)

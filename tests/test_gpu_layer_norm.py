@@ -149,6 +149,16 @@ def test_backward_many_rows(gpu, rows, cols):
         check(name, g, r, t)
 
 
+# Widths of 513 to 1024 vectors, whole and not, in either element size, and rows enough for a
+# workgroup to walk several of them.
+@pytest.mark.parametrize("dt", DTYPES, ids=ID.get)
+@pytest.mark.parametrize("rows,cols", [(5, 2500), (3, 2501), (4, 3500), (3, 3501), (5, 4999),
+                                       (3, 5000), (1500, 6143), (3, 6500), (5, 6501),
+                                       (1100, 8191), (2, 8192)])
+def test_backward_between_powers_of_two(gpu, rows, cols, dt):
+    test_backward(gpu, rows, cols, dt)
+
+
 @pytest.mark.parametrize("dt", DTYPES, ids=ID.get)
 @pytest.mark.parametrize("shift", [1, 3])
 @pytest.mark.parametrize("rows,cols", [(5, 64), (9, 1024), (3, 4099), (2, 16384)])
