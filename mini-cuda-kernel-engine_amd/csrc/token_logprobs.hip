@@ -404,7 +404,7 @@ __device__ __forceinline__ void put_keys(const VecT16<T> (&w)[N], int64_t j, int
   }
 }
 
-// Workgroup (row, part): vectors part * per_part on, in rounds of kUnroll vectors a lane, each
+// Workgroup (row, part): vectors part * per_part on, in rounds of U vectors a lane, each
 // round's loads a round ahead of its work.  With one part the row's results are written here,
 // else its sums and keys go to the workspace.
 //
@@ -415,14 +415,14 @@ __device__ __forceinline__ void put_keys(const VecT16<T> (&w)[N], int64_t j, int
 // bound are put down and ranked.  Where more than kMaxKeys reach it (ties, masks, sorted rows)
 // list_keys does it instead.
 constexpr int kUnroll = 4, kQuarters = 4;
-template <typename T, bool ENTROPY>
+template <typename T, int U, bool ENTROPY>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict__ x, RowOut o,
                                                             Part* __restrict__ parts_out,
                                                             uint64_t* __restrict__ keys_out,
                                                             int64_t vocab, int64_t row_stride,
                                                             int parts, int64_t per_part,
                                                             float scale, int top_k) {
-  constexpr int VE = kVecElems<T>, U = kUnroll, kRound = U * kThreads;
+  constexpr int VE = kVecElems<T>, kRound = U * kThreads;
   __shared__ KeyList list;
   __shared__ __attribute__((aligned(16))) float largest[kThreads];
   __shared__ float mins[kWaves];
@@ -645,9 +645,15 @@ __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(
 // ---------------------------------------------------------------------------
 // Launchers
 // ---------------------------------------------------------------------------
-// How many workgroups share a row: as many as fill the GPU where there are few rows, at
-// least 2048 logits each, and no more keys than the joining workgroup holds.
+// How many workgroups share a row: one where a row is short or there is one for each CU, as the
+// second launch costs more than the others save; else as many as fill the GPU, at least 2048
+// logits each, and no more keys than the joining workgroup holds.  One workgroup and split, without
+// and with the top 20, us: 64 x 32768 bf16 6.1 and 7.4, 8.9 and 12.1; 64 x 50264 8.6 and 7.8,
+// 11.3 and 13.0; 128 x 64000 9.3 and 10.1, 12.2 and 16.2; 128 x 131072 14.3 and 11.8, 18.4 and
+// 18.1; 256 x 131072 15.7 and 16.7, 19.7 and 23.0; 512 x 131072 fp32 40.4 and 43.6, 47.1 and 52.9.
+// What it costs: 256 x 262144 fp32 49.0 and 43.5.
 int parts_of(int64_t rows, int64_t vocab, int top_k) {
+  if (vocab <= 32768 || rows >= 256 || (rows >= 128 && vocab <= 65536)) return 1;
   int64_t p = 1024 / (rows > 0 ? rows : 1);
   const int64_t most = (vocab + 2047) / 2048;
   if (p > most) p = most;
@@ -666,6 +672,10 @@ struct RowArgs {
   hipStream_t s;
 };
 
+template <typename T, int U> auto* logprobs_kernel_for(bool entropy) {
+  return entropy ? &logprobs_kernel<T, U, true> : &logprobs_kernel<T, U, false>;
+}
+
 template <typename T> int logprobs(const RowArgs& a) {
   const int parts = parts_of(a.rows, a.vocab, a.top_k);
   const int64_t vecs = (a.vocab + kVecElems<T> - 1) / kVecElems<T>;
@@ -674,7 +684,10 @@ template <typename T> int logprobs(const RowArgs& a) {
   Part* sums = static_cast<Part*>(a.ws);
   uint64_t* keys = reinterpret_cast<uint64_t*>(sums + (parts > 1 ? a.rows * parts : 0));
   const unsigned grid = static_cast<unsigned>(a.rows * parts);
-  auto* fn = a.o.entropy ? &logprobs_kernel<T, true> : &logprobs_kernel<T, false>;
+  // A short row takes as few vectors a lane as hold it: 4096 x 1000 bf16 10.2 us, with four 15.8.
+  auto* fn = logprobs_kernel_for<T, kUnroll>(a.o.entropy);
+  if (per_part <= kThreads) fn = logprobs_kernel_for<T, 1>(a.o.entropy);
+  else if (per_part <= 2 * kThreads) fn = logprobs_kernel_for<T, 2>(a.o.entropy);
   fn<<<grid, kThreads, 0, a.s>>>(x, a.o, sums, keys, a.vocab, a.row_stride, parts, per_part,
                                  a.scale, a.top_k);
   MCKE_LAUNCH_CHECK("logprobs_kernel");

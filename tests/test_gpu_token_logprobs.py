@@ -128,6 +128,22 @@ def test_forward(gpu, rows, vocab, dt):
     compare(got, _reference(x, tokens, scale, k))
 
 
+# Rows of one, two and four vectors a lane, whole up to 32768 logits, and shared by workgroups from
+# there on where there are few of them.
+@pytest.mark.parametrize("dt", DTYPES, ids=ID.get)
+@pytest.mark.parametrize("rows,vocab", [(7, 1024), (5, 1025), (6, 2051), (5, 3000), (4, 4096),
+                                        (3, 4097), (3, 32768), (40, 32769), (130, 65537),
+                                        (127, 33003), (128, 40001), (260, 33003)])
+def test_vectors_a_lane_and_parts(gpu, rows, vocab, dt):
+    test_forward(gpu, rows, vocab, dt)
+
+
+@pytest.mark.parametrize("k", [1, 20, 64])
+@pytest.mark.parametrize("rows,vocab", [(2, 2049), (3, 4095), (1, 32768), (33, 50003), (260, 2500)])
+def test_top_k_of_more_rows(gpu, rows, vocab, k):
+    test_top_k(gpu, rows, vocab, k)
+
+
 @pytest.mark.parametrize("k", [1, 2, 20, 63, 64])
 @pytest.mark.parametrize("rows,vocab", [(1, 64), (1, 70000), (33, 5000), (1025, 300)])
 def test_top_k(gpu, rows, vocab, k):
@@ -219,6 +235,17 @@ def test_optional_outputs(gpu, rows, vocab):
     assert all(same_bits(got[n], full[n]) for n in got) and "logprobs" not in got
     got = run(gpu, x, tokens, 1.0, 0)
     compare(got, _reference(x, tokens, 1.0, 0))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,vocab", [(2, 2600), (2, 4800), (3, 40000)])
+def test_ties_orders_and_masks_of_more_rows(gpu, rows, vocab, kind):
+    test_ties_orders_and_masks(gpu, rows, vocab, kind)
+
+
+@pytest.mark.parametrize("rows,vocab", [(8, 40000), (9, 2500), (9, 3600)])
+def test_special_rows_of_more_widths(gpu, rows, vocab):
+    test_special_rows(gpu, rows, vocab)
 
 
 @pytest.mark.parametrize("shift,pad", [(1, 0), (3, 1), (0, 7)])
@@ -344,11 +371,12 @@ def test_gradient_against_differences(gpu):
     check("dlogits", got, want, tol + (64 * U + 1e-7) * want.abs().max())
 
 
-def test_captured(gpu):
-    """Forward (with parts and their join) and backward, captured: every replay gives the eager
-    bits, with eager work between them and outputs and workspace overwritten."""
+@pytest.mark.parametrize("vocab", [20011, 50021])
+def test_captured(gpu, vocab):
+    """Forward (whole rows, and parts with their join) and backward, captured: every replay gives
+    the eager bits, with eager work between them and outputs and workspace overwritten."""
     m = gpu
-    rows, vocab, k = 3, 20011, 10
+    rows, k = 3, 10
     x, tokens = _logits(rows, vocab, BF16, 31)
     eager = run(m, x, tokens, 1.0, k)
     g, h = torch.ones(rows), torch.full((rows,), 0.5)
@@ -357,7 +385,7 @@ def test_captured(gpu):
     outs = {n: out(m, eager[n].shape, eager[n].dtype) for n in NAMES}
     grad = out(m, x.shape, x.dtype)
     nbytes = m.token_logprobs_workspace_bytes(rows, vocab, k)
-    assert nbytes > 0
+    assert (nbytes > 0) == (vocab == 50021)
     ws = workspace(m, nbytes)
 
     def launch(stream):
@@ -372,7 +400,7 @@ def test_captured(gpu):
             graph.replay()
             assert all(same_bits(outs[n].get(), eager[n]) for n in NAMES), i
             assert same_bits(grad.get(), egrad), i
-            for o in (*outs.values(), grad, ws):
+            for o in (*outs.values(), grad, *([ws] if ws else [])):
                 o.buf.upload(np.full(o.buf.nbytes, 0xA5, np.uint8))
             again = run(m, x, tokens, 1.0, k)
             assert all(same_bits(again[n], eager[n]) for n in NAMES)
