@@ -52,11 +52,17 @@ __device__ __forceinline__ Sums moved(Sums s, float to, float c) {
   return {to, f * s.d, f * (s.e + t * s.d)};
 }
 
+__device__ __forceinline__ float first_lane(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+
 // The states of a wave's lanes, or of the workgroup's waves, as one: each moved to the largest
-// m, then added up in a fixed order.
+// m, then added up in a fixed order.  A lane's own product and its neighbour's go into one
+// multiply-add, which rounds the one and not the other: the lanes' sums differ in their last bit,
+// and every lane takes the first one's.
 __device__ __forceinline__ Sums wave_join(Sums s, float c) {
   s = moved(s, wave_max(s.m), c);
-  return {s.m, wave_sum(s.d), wave_sum(s.e)};
+  return {s.m, first_lane(wave_sum(s.d)), first_lane(wave_sum(s.e))};
 }
 __device__ __forceinline__ Sums block_join(const Sums (&waves)[kWaves], float c) {
   float m = waves[0].m;

@@ -257,6 +257,17 @@ def test_any_alignment(gpu, shift, pad):
         assert all(same_bits(a[n], b[n]) for n in NAMES)
 
 
+@pytest.mark.parametrize("rows,vocab,k", [(3, 60001, 40), (1, 131072, 64), (2, 50000, 64),
+                                          (40, 70000, 20), (3, 20000, 64)])
+def test_same_bits_on_every_run(gpu, rows, vocab, k):
+    """Which lane writes an alternative depends on the order of the keys, its value does not."""
+    x, tokens = _logits(rows, vocab, BF16, 8)
+    first = run(gpu, x, tokens, 1.0, k)
+    for _ in range(6):
+        again = run(gpu, x, tokens, 1.0, k)
+        assert all(same_bits(again[n], first[n]) for n in NAMES)
+
+
 def test_large_logits(gpu):
     """Logits of 1e4 and more, whose exponentials' arguments must not be rounded at the logits'
     size; from 1e9 on any two that differ are far apart."""
