@@ -257,6 +257,25 @@ def test_any_alignment(gpu, shift, pad):
         assert all(same_bits(a[n], b[n]) for n in NAMES)
 
 
+@pytest.mark.parametrize("dt", [BF16, F16], ids=ID.get)
+@pytest.mark.parametrize("rows,vocab,pad", [(4, 8193, 0), (5, 16384, 1), (5, 16385, 0), (4, 16391, 2),
+                                            (3, 24577, 4), (3, 60001, 0), (40, 40003, 0),
+                                            (130, 66001, 0), (7, 2049, 0), (7, 4097, 0)])
+def test_rows_at_odd_addresses(gpu, rows, vocab, pad, dt):
+    """Every other row starts off a 4-byte address (all of them, or all but those, with the buffer
+    moved by an element): the bits of rows that start at 16 bytes, for one round of vectors and
+    several, whole rows and shared ones, rounds that end with the row and an element before."""
+    x, tokens = _logits(rows, vocab, dt, vocab)
+    x[-1, -1] = x[-1].max() + 1                      # the last logit there is
+    x[1, 0] = x[1].max() + 1
+    tokens[-1], tokens[1] = vocab - 1, 0
+    for k in (0, 20, 40):
+        want = run(gpu, x, tokens, 1.0, k, pad=-vocab % 8)
+        for shift in (0, 1):
+            got = run(gpu, x, tokens, 1.0, k, pad=pad, shift=shift)
+            assert all(same_bits(got[n], want[n]) for n in got), (k, shift)
+
+
 @pytest.mark.parametrize("rows,vocab,k", [(3, 60001, 40), (1, 131072, 64), (2, 50000, 64),
                                           (40, 70000, 20), (3, 20000, 64)])
 def test_same_bits_on_every_run(gpu, rows, vocab, k):
