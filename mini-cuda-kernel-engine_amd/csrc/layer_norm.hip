@@ -519,8 +519,9 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_params_kernel(
   }
 }
 
-// Folds the parts in a fixed order: kFoldCols columns a workgroup, kFoldWays lanes a column
-// take the parts in turn and meet in LDS.  blockIdx.y 0 is dweight, 1 dbias.
+// Folds the parts in a fixed order: kFoldCols columns a workgroup at a time, kFoldWays lanes a
+// column take the parts in turn and meet in LDS.  blockIdx.y 0 is dweight, 1 dbias.  Workgroups walk
+// the columns: 32 lanes a column are past the grid's 32-bit work size from 2^27 columns on.
 constexpr int kFoldCols = 32, kFoldWays = 32;
 template <typename P>
 __global__ __launch_bounds__(kFoldCols * kFoldWays) void ln_bwd_fold_kernel(
@@ -530,19 +531,25 @@ __global__ __launch_bounds__(kFoldCols * kFoldWays) void ln_bwd_fold_kernel(
   P* out = blockIdx.y == 0 ? dweight : dbias;
   if (!out) return;
   const int lc = threadIdx.x % kFoldCols, way = threadIdx.x / kFoldCols;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kFoldCols + lc;
-  float s = 0.0f;
-  if (c < cols) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kFoldCols;
+  for (int64_t c0 = static_cast<int64_t>(blockIdx.x) * kFoldCols;;) {
+    const int64_t c = c0 + lc;
+    float s = 0.0f;
+    if (c < cols) {
 #pragma unroll 16
-    for (int p = way; p < parts; p += kFoldWays)
-      s += ws[(2 * static_cast<int64_t>(p) + blockIdx.y) * cols + c];
+      for (int p = way; p < parts; p += kFoldWays)
+        s += ws[(2 * static_cast<int64_t>(p) + blockIdx.y) * cols + c];
+    }
+    lds[way][lc] = s;
+    __syncthreads();
+    // Column `way` of the workgroup's, its lanes' sums as a tree.
+    s = wave_sum<kFoldWays>(lds[lc][way]);
+    const int64_t oc = c0 + way;
+    if (lc == 0 && oc < cols) out[oc] = static_cast<P>(s);
+    c0 += step;
+    if (c0 >= cols) return;
+    __syncthreads();   // lds is written again
   }
-  lds[way][lc] = s;
-  __syncthreads();
-  // Column `way` of the workgroup, its lanes' sums as a tree.
-  s = wave_sum<kFoldWays>(lds[lc][way]);
-  const int64_t oc = static_cast<int64_t>(blockIdx.x) * kFoldCols + way;
-  if (lc == 0 && oc < cols) out[oc] = static_cast<P>(s);
 }
 
 // ---------------------------------------------------------------------------
@@ -642,10 +649,11 @@ int ln_parts(int64_t rows, int64_t cols, int vec) {
                : with_backward_shape<8, false>(vecs, count);
 }
 
-// One workgroup per row up to the grid's 32-bit work size, which the kernels then walk.
-unsigned row_grid(int64_t rows) {
+// A workgroup of up to 1024 lanes per row, or per strip of columns, up to the grid's 32-bit work
+// size; the kernels walk what is left.
+unsigned grid_of_1024(int64_t n) {
   const int64_t most = int64_t{UINT32_MAX} / 1024;
-  return static_cast<unsigned>(rows < most ? rows : most);
+  return static_cast<unsigned>(n < most ? n : most);
 }
 
 struct LnFwdArgs {
@@ -684,7 +692,7 @@ template <typename T> int ln_fwd(const LnFwdArgs& a) {
       return whole ? ln_fwd_regs<T, float, true>(a) : ln_fwd_regs<T, float, false>(a);
     return whole ? ln_fwd_regs<T, T, true>(a) : ln_fwd_regs<T, T, false>(a);
   }
-  ln_fwd_any_kernel<T><<<row_grid(a.rows), kThreads, 0, a.s>>>(
+  ln_fwd_any_kernel<T><<<grid_of_1024(a.rows), kThreads, 0, a.s>>>(
       static_cast<const T*>(a.x), a.weight, a.bias, static_cast<T*>(a.y), a.mean, a.rstd,
       a.param_dtype, a.rows, a.cols, a.eps);
   MCKE_LAUNCH_CHECK("ln_fwd_any_kernel");
@@ -702,7 +710,7 @@ struct LnBwdArgs {
 };
 
 template <typename P> int ln_fold(const LnBwdArgs& a, int parts) {
-  const dim3 grid(static_cast<unsigned>((a.cols + kFoldCols - 1) / kFoldCols), 2);
+  const dim3 grid(grid_of_1024((a.cols + kFoldCols - 1) / kFoldCols), 2);
   ln_bwd_fold_kernel<P><<<grid, kFoldCols * kFoldWays, 0, a.s>>>(a.ws, static_cast<P*>(a.dweight),
                                                     static_cast<P*>(a.dbias), a.cols, parts);
   MCKE_LAUNCH_CHECK("ln_bwd_fold_kernel");
@@ -741,7 +749,7 @@ int ln_bwd_rows(const LnBwdArgs& a, int parts, bool* summed) {
       return ln_bwd_launch<T, P, WHOLE, S, true>(a, parts, params ? a.ws : nullptr);
     });
   if (!a.dx) return ok();
-  return ln_bwd_launch<T, P, WHOLE, BackShape<1024, 4, 1024, 0>, false>(a, row_grid(a.rows),
+  return ln_bwd_launch<T, P, WHOLE, BackShape<1024, 4, 1024, 0>, false>(a, grid_of_1024(a.rows),
                                                                         nullptr);
 }
 
@@ -762,11 +770,11 @@ template <typename T> int ln_bwd(const LnBwdArgs& a) {
       else
         rc = whole ? ln_bwd_rows<T, T, true>(a, parts, &summed) : ln_bwd_rows<T, T, false>(a, parts, &summed);
     } else if (a.dx && a.cols >= VE) {
-      ln_bwd_dx_wide_kernel<T><<<row_grid(a.rows), kWideThreads, 0, a.s>>>(
+      ln_bwd_dx_wide_kernel<T><<<grid_of_1024(a.rows), kWideThreads, 0, a.s>>>(
           dy, x, a.weight, a.mean, a.rstd, static_cast<T*>(a.dx), a.param_dtype, a.rows, a.cols);
       MCKE_LAUNCH_CHECK("ln_bwd_dx_wide_kernel");
     } else if (a.dx) {
-      ln_bwd_dx_any_kernel<T><<<row_grid(a.rows), kThreads, 0, a.s>>>(
+      ln_bwd_dx_any_kernel<T><<<grid_of_1024(a.rows), kThreads, 0, a.s>>>(
           dy, x, a.weight, a.mean, a.rstd, static_cast<T*>(a.dx), a.param_dtype, a.rows, a.cols);
       MCKE_LAUNCH_CHECK("ln_bwd_dx_any_kernel");
     }
@@ -785,7 +793,7 @@ template <typename T> int ln_bwd(const LnBwdArgs& a) {
   return ln_fold_any(a, parts);
 }
 
-// The widest row: column strips of 64 lanes stay within the grid's 32-bit work size.
+// The widest row: a lane per column of it is within the grid's 32-bit work size.
 constexpr int64_t kMaxCols = int64_t{1} << 30;
 
 int check_types(const char* who, int dtype, int param_dtype) {

@@ -348,3 +348,18 @@ def test_offsets_past_32_bits(gpu):
     got = torch.from_numpy(got).view(torch.bfloat16)
     assert same_bits(got[0], b)                       # a constant row: the bias
     assert same_bits(got[1:], want[0])
+
+
+def test_more_columns_than_a_grid_of_their_sums(gpu):
+    """Past 2^27 columns the sums' fold walks them.  Quarters, a mean of a quarter and rstd of 1
+    and 2: every product and sum is exact, and so is its bf16 value (at most 7 bits)."""
+    m = gpu
+    rows, cols = 2, (1 << 27) + 4099
+    i = torch.arange(cols, dtype=torch.int32)
+    x = torch.stack([(i % 7 - 3), (i % 5 - 2)]).to(torch.bfloat16) / 4
+    dy = torch.stack([(i % 3 - 1), (i // 1021 % 3 - 1)]).to(torch.bfloat16)
+    mean, rstd = torch.full((rows,), 0.25), torch.tensor([1.0, 2.0])
+    _, dw, db = run_backward(m, dy, x, None, mean, rstd, BF16, BF16, want=(False, True, True))
+    assert torch.equal(db, dy[0] + dy[1])
+    del db
+    assert torch.equal(dw, dy[0] * (x[0] - 0.25) + dy[1] * (x[1] - 0.25) * 2)
