@@ -277,7 +277,7 @@ def _ptr(p) -> int | None:
         return p.ptr
     data_ptr = getattr(p, "data_ptr", None)
     if data_ptr is not None:             # a torch tensor
-        if not getattr(p, "is_cuda", True) and not p.is_pinned():
+        if not getattr(p, "is_cuda", True) and p.numel() and not p.is_pinned():
             raise ValueError("a tensor in host memory where a kernel reads or writes device memory")
         return data_ptr()
     return int(p)
@@ -494,7 +494,9 @@ def launch_activation_f32(x, y, n: int, act, vector_width: int, stream=None) -> 
 
 
 def max_vector_width_f32(p, cols: int) -> int:
-    return int(lib().mcke_max_vector_width_f32(_ptr(p), cols))
+    """Looks at the address alone: p may be in host memory."""
+    at = p.data_ptr() if hasattr(p, "data_ptr") else _ptr(p)
+    return int(lib().mcke_max_vector_width_f32(at, cols))
 
 
 def row_reduce_workspace_bytes(rows: int, cols: int, variant) -> int:

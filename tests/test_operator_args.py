@@ -38,6 +38,18 @@ def test_host_tensors_are_refused(mcke):
         mcke.launch_row_softmax_f32(x, x, 4, 8, mcke.SoftmaxVariant.kOnlineOnePass)
 
 
+def test_host_tensors_that_no_kernel_reads(mcke):
+    """The query of an address's vector width takes any tensor, and a launch of nothing empty
+    ones."""
+    import torch
+    x = torch.zeros(64)
+    for t in (x, x[1:], x[2:]):
+        assert mcke.max_vector_width_f32(t, 64) == mcke.max_vector_width_f32(t.data_ptr(), 64)
+    e = torch.empty(0, 8)
+    assert mcke.launch_row_softmax_f32(e, e, 0, 8, mcke.SoftmaxVariant.kOnlineOnePass).ok()
+    assert mcke.launch_layer_norm(e, None, None, e, None, None, 0, 0, 0, 8, 1e-5).ok()
+
+
 # ---------------------------------------------------------------------------
 # Layer norm
 # ---------------------------------------------------------------------------
