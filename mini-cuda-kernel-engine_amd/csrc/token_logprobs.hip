@@ -464,8 +464,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
   // 16-bit rows off 4-byte addresses: vectors at 2-byte addresses take the load units twice, so they
   // are read an element early and shifted into place, the same lanes' the same bits (bf16, data
   // past the caches: 4096 x 50257 83.5 -> 74.2 us beside 71.3 for 50256, 2048 x 131071 104 -> 89.2).
-  // The element before row 0 is nobody's.
-  const bool odd = sizeof(T) == 2 && r > 0 && reinterpret_cast<uintptr_t>(row) / 2 % 2 == 1;
+  // What lies before the row is not its own and is not read: the row's first vector is loaded from
+  // its second element on, and the first one by itself.
+  const bool odd = sizeof(T) == 2 && reinterpret_cast<uintptr_t>(row) / 2 % 2 == 1;
   const T* from = odd ? row - 1 : row;
   // Rounds that lie in the row, in an odd one with an element behind them.
   const int64_t whole = (vocab - (odd ? 1 : 0)) / VE - first;
@@ -477,7 +478,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
     const int64_t j = first + static_cast<int64_t>(i) * kRound + t;
     if (i < full) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = load_stream<T>(from + (j + u * kThreads) * VE);
+      for (int u = 0; u < U; ++u)
+        w[u] = load_stream<T>(from + (j + u * kThreads) * VE + (u == 0 && odd && j == 0 ? 2 : 0));
       if constexpr (sizeof(T) == 2) {
         if (odd && lane >= kWave - U) {
           const int64_t behind = j - lane + kWave + (lane - (kWave - U)) * kThreads;
@@ -491,14 +493,17 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
                                       : load_part<T>(row, 0, -INFINITY);
     }
   };
-  VecT16<T> w[U];
-  uint32_t after = 0;
-  load(0, w, after);
+  // Before any load of the row: without a token it is not read.  (Behind the first ones no faster:
+  // 4 x 131072 bf16 9.75 us and 9.87, with the top 20; half the rows without a token, 2048 x 131072
+  // 61.8 and 60.2.)
   const int64_t token = o.tokens ? o.tokens[r] : 0;
-  if (token < 0) {                                      // nothing of the row is used
+  if (token < 0) {
     if (parts == 1) write_no_row(o, r, top_k);
     return;
   }
+  VecT16<T> w[U];
+  uint32_t after = 0;
+  load(0, w, after);
   const float logit = token_logit<T>(o, row, vocab, token);
   Sums s = no_sums();
   float quarter_m[kQuarters];
@@ -512,6 +517,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(const T* __restrict_
       // Before the next loads are out: behind them it takes 98 registers for 82.
       if constexpr (sizeof(T) == 2) {
         if (odd && i < full) {
+          if (i == 0 && first + t == 0) {
+            const u32x4_of d = __builtin_bit_cast(u32x4_of, w[0]);
+            const uint32_t d0 = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row)) << 16;
+            w[0] = __builtin_bit_cast(VecT16<T>, u32x4_of{d0, d[0], d[1], d[2]});
+          }
 #pragma unroll
           for (int u = 0; u < U; ++u)
             w[u] = shifted<T>(w[u], __builtin_amdgcn_readlane(after, kWave - U + u));
@@ -635,7 +645,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(
 
 // dlogits = scale (g ([j == token] - p_j) - h p_j (log p_j + entropy)), g and h the gradients
 // of the row's logprob and entropy: a workgroup per kBackVecs * kThreads vectors of a row, a lane's
-// loads all out before the row's own values are looked at.
+// loads all out before the row's own values but its token are looked at.  A row without a token is
+// not read (2048 x 131072 bf16: half the rows without one 169 -> 130 us, none 84.6 -> 86.5 at 1024
+// rows, with the loads behind the token).
 constexpr int kBackVecs = 2;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(
@@ -649,14 +661,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(
       (static_cast<int64_t>(blockIdx.x % per_row) * (V * kThreads) + threadIdx.x) * VE;
   const T* in = x + r * row_stride;
   T* out = dx + r * row_stride;
-  VecT16<T> w[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int64_t at = at0 + i * (kThreads * VE);
-    if (at + VE <= vocab) w[i] = load_stream<T>(in + at);
-    else if (at < vocab) w[i] = load_part<T>(in + at, static_cast<int>(vocab - at), 0.0f);
-  }
   const int64_t token = tokens ? tokens[r] : 0;
+  VecT16<T> w[V];
+  if (token >= 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int64_t at = at0 + i * (kThreads * VE);
+      if (at + VE <= vocab) w[i] = load_stream<T>(in + at);
+      else if (at < vocab) w[i] = load_part<T>(in + at, static_cast<int>(vocab - at), 0.0f);
+    }
+  }
   const float lse = lse_in[r];
   // No token or no probability: no gradient.  No such token: a NaN, as forward.
   const bool none = token < 0 || lse == -INFINITY || token >= vocab;

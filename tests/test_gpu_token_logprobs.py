@@ -276,6 +276,20 @@ def test_rows_at_odd_addresses(gpu, rows, vocab, pad, dt):
             assert all(same_bits(got[n], want[n]) for n in got), (k, shift)
 
 
+@pytest.mark.parametrize("dt", [BF16, F16], ids=ID.get)
+@pytest.mark.parametrize("vocab", [2048, 2049, 4101, 16385, 60001])
+def test_first_logits_of_rows_at_odd_addresses(gpu, vocab, dt):
+    """A row's first logit, its largest and its token, at odd addresses with NaN before it: the
+    bits of aligned rows, the first row's too."""
+    x, tokens = _logits(4, vocab, dt, 15)
+    x[:, 0] = x.amax(1) + 1
+    tokens[:] = 0
+    want = run(gpu, x, tokens, 1.0, 20)
+    for pad, shift in ((1, 1), (-vocab % 8, 1), (-vocab % 2 + 1, 0)):
+        got = run(gpu, x, tokens, 1.0, 20, pad=pad, shift=shift)
+        assert all(same_bits(got[n], want[n]) for n in got), (pad, shift)
+
+
 @pytest.mark.parametrize("rows,vocab,k", [(3, 60001, 40), (1, 131072, 64), (2, 50000, 64),
                                           (40, 70000, 20), (3, 20000, 64)])
 def test_same_bits_on_every_run(gpu, rows, vocab, k):
@@ -489,3 +503,26 @@ def test_offsets_past_32_bits(gpu):
                                         1, None))
         m.device_synchronize()
         assert same_bits(torch.from_numpy(got).view(torch.bfloat16), wgrad[r])
+
+
+def test_rows_without_a_token_cost_no_reads(gpu):
+    """The gradient of rows without a token is written and nothing of them read: half the bytes
+    of a row with one (measured: 0.6 of the time; read all the same, 0.99)."""
+    m = gpu
+    rows, vocab = 1024, 131072
+    x = Dev(m, torch.ones(rows, vocab, dtype=torch.bfloat16))
+    dx = m.DeviceBuffer(2 * rows * vocab)
+    lse, g = Dev(m, torch.full((rows,), 12.78)), Dev(m, torch.ones(rows))
+    some, none = (Dev(m, torch.full((rows,), t, dtype=torch.int64)) for t in (5, -1))
+    e0, e1 = m.Event(), m.Event()
+    best = {}
+    for _ in range(12):
+        for name, tokens in (("some", some), ("none", none)):
+            e0.record()
+            for _ in range(4):
+                m.launch_token_logprobs_backward(x, tokens, lse, None, g, None, dx, BF16, rows,
+                                                 vocab, vocab).throw_if_error()
+            e1.record()
+            e1.synchronize()
+            best[name] = min(best.get(name, INF), e0.elapsed_ms(e1))
+    assert best["none"] < 0.85 * best["some"], best
