@@ -3,8 +3,11 @@
 //
 //   y = act(alpha acc + bias[col]) + residual
 //
-// in fp32, rounded once.  The kernels take it as a template argument: NoEpilogue is the plain
-// product (C = alpha A B + beta C), Epilogue this.
+// in fp32, rounded once to the output's type.  alpha acc is rounded to fp32 before the bias is added,
+// as the plain product that stores it and the fp32 product's epilogue do, and what is absent adds -0,
+// which changes nothing: with the sums of the plain product (few rows and odd extents take other
+// kernels) a fp32 output has the bits of that product and mcke_launch_bias_act_f32.  The kernels take
+// it as a template argument: NoEpilogue is the plain product (C = alpha A B + beta C), Epilogue this.
 //
 // The sums leave the accumulation registers as fp32 through LDS, row-major, and a rolled loop
 // reads them back a row at a time.  There the lane's columns do not change, so the bias is
@@ -33,8 +36,13 @@ struct Epilogue {
   int act;
 };
 
-// act(v + bias) + residual for one output.
+// act(v + bias) + residual for one output, v = alpha acc: a register's value behind the empty asm, so
+// that the product does not go into one multiply-add with the bias.  (The activation's extra
+// operation a value, bf16 with GELU_erf and residual, us: 4096^3 123.9 -> 124.5-125.4, 8192 x 4096 x
+// 128 82.7 -> 84.1; a volatile asm, which orders them too, 125.2 and 85.3.)
+constexpr float kAbsent = -0.0f;
 template <int ACT> __device__ __forceinline__ float fused_value(float v, float b, float res) {
+  asm("" : "+v"(v));
   return act_xb<ACT>(v, b) + res;
 }
 
@@ -103,7 +111,7 @@ struct FusedStore {
     float b[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e)
-      b[e] = ep.bias && col + e < N ? load_elem(ep.bias, ep.bias_dtype, col + e) : 0.0f;
+      b[e] = ep.bias && col + e < N ? load_elem(ep.bias, ep.bias_dtype, col + e) : kAbsent;
     with_act(ep.act, [&](auto act) {
       constexpr int ACT = decltype(act)::value;
 #pragma unroll 1
@@ -125,7 +133,7 @@ struct FusedStore {
           VecT16<OutT> o;
 #pragma unroll
           for (int e = 0; e < VE; ++e) {
-            float old_e = 0.0f;
+            float old_e = kAbsent;
             if (res && inside) old_e = static_cast<float>(old[u][e]);
             else if (res && col + e < N)
               old_e = static_cast<float>(res[static_cast<int64_t>(row) * N + col + e]);

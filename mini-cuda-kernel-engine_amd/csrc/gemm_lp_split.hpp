@@ -252,7 +252,7 @@ __global__ __launch_bounds__(WV * 64) void gemm_lp_split_kernel(
     const int col = n0 + 4 * (threadIdx.x % (S::TN / 4));
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      bias[j] = ep.bias ? load_elem(ep.bias, ep.bias_dtype, col + j) : 0.0f;
+      bias[j] = ep.bias ? load_elem(ep.bias, ep.bias_dtype, col + j) : kAbsent;
 #pragma unroll
     for (int i = 0; i < kTurns; ++i) {
       const int row_t = (threadIdx.x + i * S::kThreads) / (S::TN / 4);
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(WV * 64) void gemm_lp_split_kernel(
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           out.v[j] = O::from_f32(fused_value<decltype(act)::value>(
-              alpha * s[j], bias[j], ep.residual ? O::to_f32(old[turn].v[j]) : 0.0f));
+              alpha * s[j], bias[j], ep.residual ? O::to_f32(old[turn].v[j]) : kAbsent));
       });
       OutT* p = C + static_cast<int64_t>(row) * N + col;
       if (col >= n_first) {

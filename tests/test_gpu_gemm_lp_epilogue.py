@@ -182,6 +182,30 @@ def test_bits_of_the_two_launches(gpu, shape):
         assert torch.equal(got.nan_to_num(7.0), y.get().nan_to_num(7.0)), act
 
 
+@pytest.mark.parametrize("alpha", [1.0, 0.7, -1.3])
+@pytest.mark.parametrize("shape", [(1, 4096, 512), (512, 512, 96), (2048, 2048, 128),
+                                   (1901, 2001, 131)])
+def test_bits_of_the_two_launches_at_any_alpha(gpu, shape, alpha):
+    """The product with alpha is rounded before the bias is added, as a launch that stores it
+    does, and where there is no residual nothing is added: also the zeros keep their signs (of
+    empty rows, and of GELU far below zero).  Without a bias too, the plain product's bits."""
+    m = gpu
+    M, N, K = shape
+    a, b, bias, _ = _operands(M, N, K, BF16, F32, F32, 4)
+    a[M // 2] = 0
+    bias[::3] -= 40
+    bias[1::3] = -0.0
+    da, db, dbias = Dev(m, a), Dev(m, b), Dev(m, bias)
+    c, y = out(m, (M, N), torch.float32), out(m, (M, N), torch.float32)
+    m.launch_gemm_lp(da, db, c, BF16, F32, M, N, K, alpha, 0.0).throw_if_error()
+    m.device_synchronize()
+    assert same_bits(run(m, a, b, None, None, BF16, F32, F32, NONE, alpha), c.get())
+    for act in (NONE, RELU, ERF, TANH):
+        m.launch_bias_act_f32(c, dbias, y, M, N, act, 1).throw_if_error()
+        m.device_synchronize()
+        assert same_bits(run(m, a, b, bias, None, BF16, F32, F32, act, alpha), y.get()), act
+
+
 @pytest.mark.parametrize("shape", [(4, 64, 128), (300, 520, 130), (2048, 2048, 64)])
 def test_special_values(gpu, shape):
     """A NaN or infinity in a row of A spoils that row alone, one in the residual its element."""
