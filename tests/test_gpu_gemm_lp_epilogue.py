@@ -132,12 +132,54 @@ def test_exact_sums_of_more_kernels(gpu, i, shape):
 
 
 @pytest.mark.parametrize("i,shape", enumerate(MORE), ids=[f"{s[0]}x{s[1]}x{s[2]}" for s in MORE])
+def test_exact_sums_of_more_kernels_in_the_other_types(gpu, i, shape):
+    for which in ((i + 2) % 4, (i + 3) % 4):
+        ab = (BF16, F16)[which % 2]
+        yt, bt = (ab, F32)[which // 2], (F32, ab)[i % 2]
+        a, b, bias, res = _operands(*shape, ab, yt, bt, i, quarters=True)
+        y, _ = _want(a, b, bias, res, RELU, 1.0, yt)
+        assert torch.equal(run(gpu, a, b, bias, res, ab, yt, bt, RELU), y.to(TORCH[yt]))
+
+
+@pytest.mark.parametrize("i,shape", enumerate(MORE), ids=[f"{s[0]}x{s[1]}x{s[2]}" for s in MORE])
 def test_activations_of_more_kernels(gpu, i, shape):
     ab, yt, bt = _types(i)
     a, b, bias, res = _operands(*shape, ab, yt, bt, 70 + i)
     for act in (ERF, TANH):
         check("y", run(gpu, a, b, bias, res, ab, yt, bt, act),
               *_want(a, b, bias, res, act, 1.0, yt))
+
+
+# (shape, tile): 192 tiles of 256 and more that are ragged in M, N, K or all of them, whole tiles of
+# 256; short K over many tiles of 128, in vectors and not; narrower than 32 columns at tiles of 128
+# and 256.
+LARGE = [((3500, 3590, 66), 0), ((3585, 3584, 128), 0), ((3584, 3602, 64), 0), ((2048, 2048, 64), 0),
+         ((2166, 3544, 40), 1), ((2166, 3543, 7), 1), ((300, 31, 100), 1), ((517, 9, 64), 0)]
+LARGE_IDS = [f"{s[0]}x{s[1]}x{s[2]}" for s, _ in LARGE]
+
+
+@pytest.mark.parametrize("which", range(4), ids=["bf16", "f16", "bf16-f32", "f16-f32"])
+@pytest.mark.parametrize("i,case", enumerate(LARGE), ids=LARGE_IDS)
+def test_exact_sums_of_large_tiles(gpu, i, case, which):
+    shape, tile = case[0], gpu.LP_TILES[case[1]]
+    ab = (BF16, F16)[which % 2]
+    yt, bt = (ab, F32)[which // 2], (F32, ab)[(i + which) % 2]
+    a, b, bias, res = _operands(*shape, ab, yt, bt, 90 + i, quarters=True)
+    for act, bb, rr, in_place in ((RELU, bias, res, False), (NONE, bias, res, True),
+                                  (NONE, None, None, False)):
+        y, _ = _want(a, b, bb, rr, act, 1.0, yt)
+        got = run(gpu, a, b, bb, rr, ab, yt, bt, act, tile=tile, in_place=in_place)
+        assert torch.equal(got, y.to(TORCH[yt])), (act, in_place)
+
+
+@pytest.mark.parametrize("i,case", enumerate(LARGE), ids=LARGE_IDS)
+def test_activations_of_large_tiles(gpu, i, case):
+    shape, tile = case[0], gpu.LP_TILES[case[1]]
+    ab, yt, bt = _types(i)
+    a, b, bias, res = _operands(*shape, ab, yt, bt, 80 + i)
+    for act in (ERF, TANH):
+        check("y", run(gpu, a, b, bias, res, ab, yt, bt, act, 0.7, tile, in_place=act == TANH),
+              *_want(a, b, bias, res, act, 0.7, yt))
 
 
 @pytest.mark.parametrize("act", [NONE, RELU, ERF, TANH])
