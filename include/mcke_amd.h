@@ -317,8 +317,8 @@ int mcke_launch_layer_norm_backward(const void* dy, const void* x, const void* w
  * rows == 0 or vocab == 0 is a no-op. */
 
 /* Bytes of workspace that few long rows need, which several workgroups share (0 for many rows and
- * for short ones); its contents on entry do not matter, and two launches that may run at the same
- * time need one each. */
+ * for short ones), the most that any dtype takes; its contents on entry do not matter, and two
+ * launches that may run at the same time need one each. */
 size_t mcke_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k);
 
 int mcke_launch_token_logprobs(const void* logits, const int64_t* tokens, float* logprobs,

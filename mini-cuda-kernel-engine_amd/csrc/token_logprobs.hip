@@ -709,21 +709,43 @@ __global__ __launch_bounds__(kThreads) void logprobs_backward_kernel(
 // ---------------------------------------------------------------------------
 // Launchers
 // ---------------------------------------------------------------------------
-// How many workgroups share a row: one where a row is short or there is one for each CU, as the
-// second launch costs more than the others save; else as many as fill the GPU, at least 2048
-// logits each, and no more keys than the joining workgroup holds.  One workgroup and split, without
-// and with the top 20, us: 64 x 32768 bf16 6.1 and 7.4, 8.9 and 12.1; 64 x 50264 8.6 and 7.8,
-// 11.3 and 13.0; 128 x 64000 9.3 and 10.1, 12.2 and 16.2; 128 x 131072 14.3 and 11.8, 18.4 and
-// 18.1; 256 x 131072 15.7 and 16.7, 19.7 and 23.0; 512 x 131072 fp32 40.4 and 43.6, 47.1 and 52.9.
-// What it costs: 256 x 262144 fp32 49.0 and 43.5.
-int parts_of(int64_t rows, int64_t vocab, int top_k) {
-  if (vocab <= 32768 || rows >= 256 || (rows >= 128 && vocab <= 65536)) return 1;
+// How many workgroups share a row: one where that is sooner done than the second launch, else as
+// many as fill the GPU, at least 2048 logits each, and no more keys than the joining workgroup
+// holds.  One workgroup's time goes by the row's bytes; what sharing costs grows with the rows, whose
+// workgroups fill the GPU anyway, and with alternatives, which every part ranks (above kQuadTop by a
+// longer count).  Up to 32768 logits of any type a row stays whole.  One workgroup and shared, us:
+//                     no alternatives              top 20                       top 64
+//   16 x 32768   bf16   6.1   6.7                    8.5  10.1                   11.8  17.3
+//   16 x 50264          8.0   7.3                   10.8  10.0                   15.3  17.9
+//   64 x 50264          8.2   7.6                   11.1  12.9                   15.8  22.1
+//   64 x 100000        12.4   9.4                   16.4  15.6                   22.1  24.7
+//   128 x 65536         9.1   9.6                   12.1  15.7                   16.7  23.2
+//   128 x 131072       14.6  12.1                   18.8  18.2                   24.6  26.3
+//   250 x 131072       15.6  17.0                   19.9  23.1                   26.0  30.6
+//   250 x 262144       27.4  27.2                   33.1  33.0                   42.9  43.4
+//   64 x 32768   fp32   8.0   7.4                   10.7  12.1                   15.3  21.0
+//   64 x 65536         13.0   8.3                   17.0  13.7                   22.4  22.6
+//   128 x 32768         8.3   8.4                   11.2  13.7                   15.7  20.9
+//   128 x 65536        13.4  10.8                   17.4  16.4                   22.9  24.5
+//   250 x 65536        14.8  15.2                   18.7  21.0                   24.6  27.9
+//   256 x 262144       48.2  44.0                   57.1  53.5                   72.8  66.8
+//   400 x 262144       60.3  71.5                   71.1  85.4                   92.5 104.5
+int64_t whole_row_bytes(int64_t rows, int top_k) {
+  return 1000 * (72 + rows * rows / 160 + (top_k == 0 ? 0 : rows < 80 ? rows : 80) +
+                 (top_k > kQuadTop ? 80 : 0));
+}
+int parts_of(int64_t rows, int64_t vocab, int top_k, int64_t elem_bytes) {
+  if (rows > 256 || vocab <= 32768 || vocab * elem_bytes <= whole_row_bytes(rows, top_k)) return 1;
   int64_t p = 1024 / (rows > 0 ? rows : 1);
   const int64_t most = (vocab + 2047) / 2048;
   if (p > most) p = most;
   if (p > kMaxParts) p = kMaxParts;
   if (top_k > 0 && p > kMaxKeys / top_k) p = kMaxKeys / top_k;
   return p < 1 ? 1 : static_cast<int>(p);
+}
+size_t workspace_of(int64_t rows, int top_k, int parts) {
+  if (parts == 1) return 0;
+  return static_cast<size_t>(rows) * parts * (sizeof(Part) + sizeof(uint64_t) * top_k);
 }
 
 struct RowArgs {
@@ -741,7 +763,7 @@ template <typename T, int U> auto* logprobs_kernel_for(bool entropy) {
 }
 
 template <typename T> int logprobs(const RowArgs& a) {
-  const int parts = parts_of(a.rows, a.vocab, a.top_k);
+  const int parts = parts_of(a.rows, a.vocab, a.top_k, sizeof(T));
   const int64_t vecs = (a.vocab + kVecElems<T> - 1) / kVecElems<T>;
   const int64_t per_part = (vecs + parts - 1) / parts;
   const T* x = static_cast<const T*>(a.logits);
@@ -789,10 +811,9 @@ using namespace mcke_amd;
 extern "C" {
 
 size_t mcke_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k) {
-  if (rows <= 0 || vocab <= 0 || top_k < 0 || top_k > kMaxTop) return 0;
-  const int parts = parts_of(rows, vocab, top_k);
-  if (parts == 1) return 0;
-  return static_cast<size_t>(rows) * parts * (sizeof(Part) + sizeof(uint64_t) * top_k);
+  if (rows <= 0 || vocab <= 0 || vocab > 2147483647LL || top_k < 0 || top_k > kMaxTop) return 0;
+  // The most that any type needs: where 16-bit rows are shared, those of fp32 are, by as many.
+  return workspace_of(rows, top_k, parts_of(rows, vocab, top_k, 4));
 }
 
 int mcke_launch_token_logprobs(const void* logits, const int64_t* tokens, float* logprobs_out,
@@ -815,9 +836,10 @@ int mcke_launch_token_logprobs(const void* logits, const int64_t* tokens, float*
   if (!aligned(logits, dtype_bytes(dtype)) || !aligned(tokens, 8) || !aligned(logprobs_out, 4) ||
       !aligned(entropy, 4) || !aligned(lse, 4) || !aligned(top_logprobs, 4) || !aligned(top_ids, 8))
     return invalid("launch_token_logprobs: a pointer is not aligned to its type");
-  if (rows * parts_of(rows, vocab, top_k) > int64_t{UINT32_MAX} / kThreads)
+  const int parts = parts_of(rows, vocab, top_k, static_cast<int64_t>(dtype_bytes(dtype)));
+  if (rows * parts > int64_t{UINT32_MAX} / kThreads)
     return invalid("launch_token_logprobs: rows exceed the grid's 32-bit work size");
-  const size_t need = mcke_token_logprobs_workspace_bytes(rows, vocab, top_k);
+  const size_t need = workspace_of(rows, top_k, parts);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return invalid("launch_token_logprobs: these rows need a 16-byte aligned workspace of " +
                    std::to_string(need) + " bytes, got " +

@@ -138,6 +138,18 @@ def test_vectors_a_lane_and_parts(gpu, rows, vocab, dt):
     test_forward(gpu, rows, vocab, dt)
 
 
+@pytest.mark.parametrize("rows,vocab,k,dt", [
+    (r, v, k, dt) for r, v in ((1, 40000), (1, 70001), (16, 50003), (64, 60001))
+    for k in (0, 20, 40) for dt in DTYPES] + [
+        (65, 130003, 20, BF16), (65, 130003, 40, BF16), (130, 131077, 0, F16), (256, 131073, 0, F32),
+        (257, 131073, 0, F32), (200, 66001, 1, F32), (200, 66001, 0, F32)])
+def test_whole_and_shared_rows(gpu, rows, vocab, k, dt):
+    """Rows that one workgroup takes, or several, by their bytes, their number and the
+    alternatives, with a workspace for any type."""
+    x, tokens = _logits(rows, vocab, dt, rows + vocab)
+    compare(run(gpu, x, tokens, 1.0, k, pad=3, shift=1), _reference(x, tokens, 1.0, k))
+
+
 @pytest.mark.parametrize("k", [1, 20, 64])
 @pytest.mark.parametrize("rows,vocab", [(2, 2049), (3, 4095), (1, 32768), (33, 50003), (260, 2500)])
 def test_top_k_of_more_rows(gpu, rows, vocab, k):
