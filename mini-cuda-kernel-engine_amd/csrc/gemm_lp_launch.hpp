@@ -85,8 +85,8 @@ int launch_split(const LpArgs<E>& x) {
   return launch_split_as<T, OutT, 4, 4, 4>(x);
 }
 
-// Few rows (tokens) with an epilogue: bound by reading B, which a CU takes in at 8 to 9 bytes a
-// clock at most, more of it from whole 128-byte lines.  So as many workgroups as there are CUs
+// Few rows (tokens) with an epilogue: bound by reading B, of which these kernels' loads bring 8 to 9
+// bytes a clock to a CU, more of it from whole 128-byte lines.  So as many workgroups as there are CUs
 // where N allows it, then 64 columns each (with bias and GELU, bf16, us; MT x NW, waves,
 // chunks ahead):
 //   rows 1, K 4096:   N 16384  1x4 4w 25.2, 1x2 8w 41, 128 x 128 tiles 48   N 12288  1x4 4w two ahead
@@ -96,6 +96,17 @@ int launch_split(const LpArgs<E>& x) {
 //     15.4, 2x2 8w 16.2      32 x 16384 x 4096  2x4 4w 29.0, 4x4 4w 29.9
 //   rows 64:          64 x 4096 x 16384  2x2 8w two ahead 66.5, one 72.8, 1x4 8w 70.0
 //     64 x 8192 x 4096  2x4 8w 17.3, 2x4 4w 19.8    64 x 16384 x 4096  4x4 8w 37.4, 4w 40.4
+// Past 16384 columns each workgroup's A comes to a second round of workgroups: from 33 rows on, and
+// from 17 on where N is odd, the other products' kernels (bf16 with bias, these and those, us):
+//   K 4096:   64 x 16384  35.7  48.7   64 x 16400  51.7  48.9   64 x 24576  62.8  51.3   64 x 131072  306  236
+//     33 x 16384  31.4  48.3   33 x 24576  52.5  50.9   33 x 131072  262  234   32 x 24576  53.7  50.7
+//     32 x 50304  94.5  95.6   32 x 50257  118  101     16 x 50257  104  99     1 x 50257  92.4  99.5
+//   K 1024:   64 x 16384  10.6  14.5   64 x 24576  17.9  14.8   33 x 24576  16.2  14.3
+//     32 x 24576  13.0  14.0   32 x 50304  24.5  32.6   32 x 50257  29.8  28.7   17 x 50257  26.9  28.3
+template <class E> bool few_rows(const LpArgs<E>& x) {
+  return x.m <= 64 && x.n >= 64 && x.k >= 64 &&
+         (x.n <= 16384 || x.m <= 16 || (x.m <= 32 && x.n % 2 == 0));
+}
 template <typename T, typename OutT, class E>
 int launch_few_rows(const LpArgs<E>& x) {
   if (x.m <= 16) {
@@ -259,8 +270,7 @@ struct LpTile {
   // short K over many tiles (short_k).  The tile counts here and below are for 256 CUs.
   template <class E> static int launch(const LpArgs<E>& x, bool vec) {
     if constexpr (E::kFused)
-      if (x.m <= 64 && x.n >= 64 && x.k >= 64 && split_fits<OutT>(x))
-        return launch_few_rows<T, OutT>(x);
+      if (few_rows(x) && split_fits<OutT>(x)) return launch_few_rows<T, OutT>(x);
     if constexpr (BN >= 128) {
       if (vec && x.m % BM == 0 && x.n % BN == 0 && x.k % 64 == 0 && x.k > 0 &&
           dma_offsets32<BM, BN>(x.n, x.k))

@@ -150,6 +150,22 @@ def test_activations_of_more_kernels(gpu, i, shape):
               *_want(a, b, bias, res, act, 1.0, yt))
 
 
+# Up to 64 rows on either side of 16384 columns, even and odd widths.
+WIDE = [(64, 16384, 96), (64, 16386, 130), (33, 16500, 70), (40, 16385, 77), (32, 16402, 66),
+        (17, 16401, 300), (16, 16385, 65), (1, 20001, 67)]
+
+
+@pytest.mark.parametrize("i,shape", enumerate(WIDE), ids=[f"{s[0]}x{s[1]}x{s[2]}" for s in WIDE])
+def test_few_rows_over_many_columns(gpu, i, shape):
+    for which in range(4):
+        ab = (BF16, F16)[which % 2]
+        yt, bt = (ab, F32)[which // 2], (F32, ab)[i % 2]
+        a, b, bias, res = _operands(*shape, ab, yt, bt, 60 + i, quarters=True)
+        y, _ = _want(a, b, bias, res, RELU, 1.0, yt)
+        got = run(gpu, a, b, bias, res, ab, yt, bt, RELU, in_place=which > 1)
+        assert torch.equal(got, y.to(TORCH[yt])), which
+
+
 # (shape, tile): 192 tiles of 256 and more that are ragged in M, N, K or all of them, whole tiles of
 # 256; short K over many tiles of 128, in vectors and not; narrower than 32 columns at tiles of 128
 # and 256.
