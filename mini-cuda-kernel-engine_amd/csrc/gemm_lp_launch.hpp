@@ -213,8 +213,17 @@ template <int BM, int BN, typename OutT, class E> bool whole_fits(const LpArgs<E
 //   900 x 1501 x 4001    96          65                     45      54       56
 //   1000 x 1301 x 2001   88          41                     27      31       31
 //   300 x 3001 x 2001    72          39                     27      30       24
-// A tile of 256 takes as long as 3.7 rounds of 128; 64 x 128 is for one round of its tiles, one to a
-// CU.  `rc`: the launch's result, if there is one.
+// A tile of 256 takes as long as 3.7 rounds of 128.  64 x 128 is for one round of its tiles, one to a
+// CU, and for up to two a CU (200 .. 256 tiles of 128) below 2048 of K, where 128 x 128 has one tile a
+// CU and too few K steps to cover its ends (64 x 128, 128 x 128 and 64 x 64, fp16 to fp32 with GELU and
+// residual; bf16 to bf16 within 1 us of it):
+//   K                       1021             2047             2049             4095
+//   1535 x 1931, t 192   27  29  26       42  43  41       41  40  39       72  69  70
+//   1531 x 2053, t 204   28  30  33       42  43  56       41  41  54       73  69 101
+//   2047 x 2047, t 256   29  30  33       44  44  55       43  41  53       75  70 101
+//   2301 x 2047, t 288   36  40  45       59  61  74       57  59  70      103 104 132
+//   the same to bf16     42  41  45       64  62  74       61  59  71      108 104 132
+// `rc`: the launch's result, if there is one.
 template <typename T, typename OutT, class E> bool launch_odd(const LpArgs<E>& x, int* rc) {
   const int64_t tiles = tile_count(x.m, x.n, 128, 128);
   if (whole_fits<128, 128, OutT>(x)) {

@@ -54,9 +54,9 @@ struct LpSplitShape {
   // takes no more LDS than the slots.
   static constexpr int kFold = kOut * 4 * WV <= kSlots ? WV : WV / 2;
   static constexpr int kLds = kSlots > kFold * kOut * 4 ? kSlots : kFold * kOut * 4;
-  static_assert(kLds <= 80 * 1024, "two workgroups or more per CU");
+  static_assert(kLds <= 64 * 1024, "two workgroups or more per CU");
   static constexpr int kARow = 64, kBRow = 32 * NW;
-  static_assert(NW == 1 || NW == 2 || NW == 4, "column blocks are swizzled in twos or fours");
+  static_assert(NW == 1 || NW == 2 || NW == 4, "one column block, or a swizzle of two or four");
   static __host__ __device__ constexpr int aswz(int r) { return (r >> 2) & 3; }
   static __host__ __device__ constexpr int bswz(int s) {
     return NW == 1 ? 0 : NW == 2 ? (s >> 2) & 1 : (s >> 1) & 3;
