@@ -249,13 +249,16 @@ int mcke_launch_gemm_lp_vendor(const void* a, const void* b, void* c, int ab_dty
 /* No reference counterpart: the 16-bit product with its bias, activation and residual in the
  * epilogue, as the layers of a transformer chain them,
  *   y[i,j] = act(alpha * (A B)[i,j] + bias[j]) + residual[i,j],
- * computed in fp32 from the fp32 sums and rounded once.  y and residual (m x n, row-major)
- * are of y_dtype: MCKE_DTYPE_F32 or ab_dtype.  bias (n values of bias_dtype, MCKE_DTYPE_F32 or
- * ab_dtype) and residual may be null.  residual may be y itself (the residual stream updated
- * in place); apart from that y overlaps no operand.  activation is an mcke_activation value,
- * with the meaning it has in mcke_launch_bias_act_f32 (a NaN becomes 0 under ReLU).  m == 0
- * or n == 0 is a no-op; k == 0 gives act(bias) + residual.  Other validation, tiles, and the
- * choice of kernel by shape and alignment as mcke_launch_gemm_lp.  Forward only, as every
+ * computed in fp32 from the fp32 sums (alpha times the sum rounded to fp32 before the bias is
+ * added) and rounded once to y_dtype.  y and residual (m x n, row-major) are of y_dtype:
+ * MCKE_DTYPE_F32 or ab_dtype.  bias (n values of bias_dtype, MCKE_DTYPE_F32 or ab_dtype) and
+ * residual may be null.  residual may be y itself (the residual stream updated in place); apart
+ * from that y overlaps no operand.  activation is an mcke_activation value, with the meaning it
+ * has in mcke_launch_bias_act_f32 (a NaN becomes 0 under ReLU).  m == 0 or n == 0 is a no-op;
+ * k == 0 gives act(bias) + residual.  Other validation, tiles, and the choice of kernel by shape
+ * and alignment as mcke_launch_gemm_lp; where that takes its checked kernel at a 256 x 256 tile
+ * (n < 32, or past 2^25) this takes 128 x 128, so m or n above 2^31 - 128 is refused there.  Up to
+ * 64 rows have kernels of their own, also with neither bias nor residual.  Forward only, as every
  * product here. */
 int mcke_launch_gemm_lp_bias_act(const void* a, const void* b, const void* bias,
                                  const void* residual, void* y, int ab_dtype, int y_dtype,
