@@ -228,6 +228,10 @@ def test_gemm_lp_bias_act_refusals(cpu_only):
     _refused(m, f(res=E + 2), "without being it")
     _refused(m, f(M=1 << 18, N=1 << 18, K=64, res=None, bias=None, y=BIG, a=BIG >> 2, b=BIG >> 3,
                   tile=m.GemmTile(64, 64, 64, 4, 4)), "32-bit work size")
-    for long in (dict(M=1, N=(1 << 31) - 1), dict(M=(1 << 31) - 1, N=1)):
-        _refused(m, f(**long, K=1, res=None, bias=None, y=BIG, a=BIG >> 2, b=BIG >> 3),
-                 "32-bit work size")
+
+
+@pytest.mark.parametrize("M,N", [(1, (1 << 31) - 1), ((1 << 31) - 1, 1)])
+def test_gemm_lp_bias_act_grid_at_int32_max(cpu_only, M, N):
+    m = cpu_only
+    _refused(m, m.launch_gemm_lp_bias_act(BIG >> 2, BIG >> 3, None, None, BIG, 2, 2, 0, M, N, 1, 1.0,
+                                          3, m.LP_TILES[0]), "32-bit work size")
