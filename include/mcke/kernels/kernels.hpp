@@ -244,4 +244,87 @@ struct GemmKernelAttrs {
       vocab, row_stride, scale, stream));
 }
 
+// ---------------------------------------------------------------------------
+// Embedding, bias + activation kept in 8 bits, cross entropy of hidden states.  No
+// reference counterparts; formulas, optional (null) operands and special rows are
+// those of mcke_amd.h.
+// ---------------------------------------------------------------------------
+[[nodiscard]] inline Status launch_embedding(const std::int64_t* tokens, const void* table,
+                                            void* out, DType table_dtype, DType out_dtype,
+                                            std::int64_t rows, std::int64_t vocab,
+                                            std::int64_t cols, float scale,
+                                            rt::StreamHandle stream) {
+  return detail::status_of(mcke_launch_embedding(tokens, table, out, static_cast<int>(table_dtype),
+                                                 static_cast<int>(out_dtype), rows, vocab, cols,
+                                                 scale, stream));
+}
+
+[[nodiscard]] inline std::size_t embedding_backward_workspace_bytes(std::int64_t rows,
+                                                                   std::int64_t vocab,
+                                                                   std::int64_t cols) noexcept {
+  return mcke_embedding_backward_workspace_bytes(rows, vocab, cols);
+}
+
+[[nodiscard]] inline Status launch_embedding_backward(
+    const std::int64_t* tokens, const void* dout, void* dtable, DType dout_dtype,
+    DType table_dtype, std::int64_t rows, std::int64_t vocab, std::int64_t cols, float scale,
+    bool accumulate, void* workspace, std::size_t workspace_bytes, rt::StreamHandle stream) {
+  return detail::status_of(mcke_launch_embedding_backward(
+      tokens, dout, dtable, static_cast<int>(dout_dtype), static_cast<int>(table_dtype), rows,
+      vocab, cols, scale, accumulate ? 1 : 0, workspace, workspace_bytes, stream));
+}
+
+[[nodiscard]] inline Status launch_bias_act_checkpoint8(
+    const void* x, const void* bias, void* y, std::uint8_t* codes, std::uint8_t* exponents,
+    DType dtype, DType bias_dtype, std::int64_t rows, std::int64_t cols, Activation act,
+    rt::StreamHandle stream) {
+  return detail::status_of(mcke_launch_bias_act_checkpoint8(
+      x, bias, y, codes, exponents, static_cast<int>(dtype), static_cast<int>(bias_dtype), rows,
+      cols, static_cast<int>(act), stream));
+}
+
+[[nodiscard]] inline std::size_t bias_act_checkpoint8_backward_workspace_bytes(
+    std::int64_t rows, std::int64_t cols) noexcept {
+  return mcke_bias_act_checkpoint8_backward_workspace_bytes(rows, cols);
+}
+
+[[nodiscard]] inline Status launch_bias_act_checkpoint8_backward(
+    const void* dy, const std::uint8_t* codes, const std::uint8_t* exponents, void* dx, void* y,
+    void* dbias, DType dtype, DType bias_dtype, std::int64_t rows, std::int64_t cols,
+    Activation act, void* workspace, std::size_t workspace_bytes, rt::StreamHandle stream) {
+  return detail::status_of(mcke_launch_bias_act_checkpoint8_backward(
+      dy, codes, exponents, dx, y, dbias, static_cast<int>(dtype), static_cast<int>(bias_dtype),
+      rows, cols, static_cast<int>(act), workspace, workspace_bytes, stream));
+}
+
+[[nodiscard]] inline std::size_t linear_cross_entropy_workspace_bytes(std::int64_t rows,
+                                                                     std::int64_t vocab,
+                                                                     std::int64_t dim) noexcept {
+  return mcke_linear_cross_entropy_workspace_bytes(rows, vocab, dim);
+}
+
+[[nodiscard]] inline Status launch_linear_cross_entropy(
+    const void* hidden, const void* weight, const std::int64_t* targets, float* loss, float* lse,
+    DType dtype, std::int64_t rows, std::int64_t vocab, std::int64_t dim, float scale,
+    void* workspace, std::size_t workspace_bytes, rt::StreamHandle stream) {
+  return detail::status_of(mcke_launch_linear_cross_entropy(
+      hidden, weight, targets, loss, lse, static_cast<int>(dtype), rows, vocab, dim, scale,
+      workspace, workspace_bytes, stream));
+}
+
+[[nodiscard]] inline std::size_t linear_cross_entropy_backward_workspace_bytes(
+    std::int64_t rows, std::int64_t vocab, std::int64_t dim) noexcept {
+  return mcke_linear_cross_entropy_backward_workspace_bytes(rows, vocab, dim);
+}
+
+[[nodiscard]] inline Status launch_linear_cross_entropy_backward(
+    const void* hidden, const void* weight, const std::int64_t* targets, const float* lse,
+    const float* dloss, const float* dlse, void* dhidden, void* dweight, DType dtype,
+    std::int64_t rows, std::int64_t vocab, std::int64_t dim, float scale, void* workspace,
+    std::size_t workspace_bytes, rt::StreamHandle stream) {
+  return detail::status_of(mcke_launch_linear_cross_entropy_backward(
+      hidden, weight, targets, lse, dloss, dlse, dhidden, dweight, static_cast<int>(dtype), rows,
+      vocab, dim, scale, workspace, workspace_bytes, stream));
+}
+
 }  // namespace mcke::kernels

@@ -343,6 +343,110 @@ int mcke_launch_token_logprobs_backward(const void* logits, const int64_t* token
                                         void* dlogits, int dtype, int64_t rows, int64_t vocab,
                                         int64_t row_stride, float scale, void* stream);
 
+/* ---- embedding -----------------------------------------------------------------
+ * No reference counterpart; where tokens enter and their gradients leave.  table and dtable
+ * (vocab x cols, row-major) are of table_dtype; out and dout (rows x cols) of table_dtype or
+ * MCKE_DTYPE_F32; any alignment of their type; tokens are rows values.  rows up to 2^31 - 1, vocab up to
+ * 2^31 - 2, cols up to 2^24.  scale is finite (sqrt(cols) in some models).  Arithmetic is fp32,
+ * each output is rounded once, and the same input gives the same bits on every run. */
+
+/* out[r] = scale * table[tokens[r]].  A row with tokens[r] < 0 (padding) is zeros, one with
+ * tokens[r] >= vocab NaN.  rows == 0 or cols == 0 is a no-op. */
+int mcke_launch_embedding(const int64_t* tokens, const void* table, void* out, int table_dtype,
+                          int out_dtype, int64_t rows, int64_t vocab, int64_t cols, float scale,
+                          void* stream);
+
+/* Bytes of workspace for the sorted tokens (0 for rows == 0); its contents on entry do not matter,
+ * and two launches that may run at the same time need one each. */
+size_t mcke_embedding_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t cols);
+
+/* The gradient in the table:
+ *   dtable[v] = scale * sum over r with tokens[r] == v, in the order of r, of dout[r]
+ * zeros for tokens that are not there; accumulate != 0 adds to dtable instead, and touches the
+ * rows of tokens that are there alone (tied weights: the loss's gradient is there already).
+ * Tokens outside 0 .. vocab - 1 add nothing; their rows of dout are not read.  A 16-byte aligned
+ * workspace is needed (see above).  vocab == 0 or cols == 0 is a no-op. */
+int mcke_launch_embedding_backward(const int64_t* tokens, const void* dout, void* dtable,
+                                   int dout_dtype, int table_dtype, int64_t rows, int64_t vocab,
+                                   int64_t cols, float scale, int accumulate, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* ---- bias + activation, its input kept in 8 bits ---------------------------------------
+ * No reference counterpart; mcke_launch_bias_act_f32 for training, whose backward pass needs the
+ * activation's input: kept in 8 bits instead of dtype.  x, y, dy and dx (rows x cols, row-major)
+ * are of dtype (MCKE_DTYPE_F32, F16 or BF16); bias and dbias (cols values) of bias_dtype,
+ * MCKE_DTYPE_F32 or dtype; any alignment of their type.  rows up to 2^31 - 1, cols up to 2^24.
+ *   codes (rows x cols bytes): u = x + bias (rounded to fp32) times 2^-E in e4m3 (OCP, to nearest,
+ *     ties to even)
+ *   exponents (rows x ceil(cols / 32) bytes): E + 127 of each 32 columns of a row, the smallest
+ *     E >= -126 with |u| <= 448 * 2^E for their finite values
+ * so a value is restored within 2^-4 of itself, or 2^-10 * 2^E where that is more.  An infinite or
+ * NaN u is kept as NaN.  Arithmetic is fp32, each output is rounded once, and the same input gives
+ * the same bits on every run. */
+
+/* y = act(u), codes and exponents of u.  bias null is none; y null saves alone.  activation is an
+ * mcke_activation value, with the meaning it has in mcke_launch_bias_act_f32.  No output overlaps
+ * an operand.  rows == 0 or cols == 0 is a no-op. */
+int mcke_launch_bias_act_checkpoint8(const void* x, const void* bias, void* y, uint8_t* codes,
+                                     uint8_t* exponents, int dtype, int bias_dtype, int64_t rows,
+                                     int64_t cols, int activation, void* stream);
+
+/* Bytes of workspace that dbias needs (0 for rows == 0); its contents on entry do not matter, and
+ * two launches that may run at the same time need one each. */
+size_t mcke_bias_act_checkpoint8_backward_workspace_bytes(int64_t rows, int64_t cols);
+
+/* From the restored u:
+ *   dx = dy * act'(u), dbias = sum over rows of dx (before it is rounded), y = act(u) once more
+ * Any of dx, y and dbias may be null, not all; they are overwritten.  dy is for dx and dbias.  With
+ * MCKE_ACT_NONE, y is u itself.  dbias needs a 16-byte aligned workspace (see above).  Where u was
+ * kept as NaN, y and dx are NaN (0 under ReLU).  rows == 0 gives a dbias of zeros; cols == 0 is a
+ * no-op. */
+int mcke_launch_bias_act_checkpoint8_backward(const void* dy, const uint8_t* codes,
+                                              const uint8_t* exponents, void* dx, void* y,
+                                              void* dbias, int dtype, int bias_dtype, int64_t rows,
+                                              int64_t cols, int activation, void* workspace,
+                                              size_t workspace_bytes, void* stream);
+
+/* ---- cross entropy of hidden states ------------------------------------------------
+ * No reference counterpart; the last product and its loss in one, where the logits would be the
+ * largest tensor of a training step: they are never kept.  hidden (rows x dim, row-major) and
+ * weight (vocab x dim, row-major: as a layer or a tied embedding holds it) are of dtype,
+ * MCKE_DTYPE_BF16 or MCKE_DTYPE_F16; hidden at any alignment of its type, weight 16-byte aligned if dim is a
+ * multiple of 64 (other widths are copied a piece at a time, and run slower).  rows and vocab up
+ * to 2^24, dim up to 2^16; vocab and dim > 0.  scale > 0 multiplies the logits.  With
+ * z = scale * hidden[r] . weight[j]:
+ *   lse = log sum exp z, loss = lse - z[targets[r]]
+ * Products are summed in fp32, and the same input gives the same bits on every run.
+ *
+ * A row with targets[r] < 0 (padding) is not read: its loss, lse and dhidden are 0, and it adds
+ * nothing to dweight.  targets[r] >= vocab gives a NaN loss and NaN gradients.  rows == 0 is a no-op
+ * forward. */
+
+/* Bytes of workspace of either launch, for dtypes of 16 bits; its contents on entry do not matter,
+ * and two launches that may run at the same time need one each. */
+size_t mcke_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim);
+size_t mcke_linear_cross_entropy_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim);
+
+/* loss and lse (rows values; a backward pass needs the latter); either may be null, not both. */
+int mcke_launch_linear_cross_entropy(const void* hidden, const void* weight, const int64_t* targets,
+                                     float* loss, float* lse, int dtype, int64_t rows,
+                                     int64_t vocab, int64_t dim, float scale, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/* The gradients, from what the forward pass had and gave:
+ *   dz[j] = scale * ((dloss + dlse) * p_j - dloss * [j == targets[r]]), p = exp(z - lse)
+ *   dhidden = dz weight, dweight = dz^T hidden
+ * dloss or dlse (rows values) may be null, not both; dhidden (as hidden) or dweight (as weight, at
+ * any alignment of its type) may be null, not both; they are overwritten.  dz is rounded to dtype
+ * once, relative to the largest gradient of a row in fp16.  rows == 0 gives a
+ * dweight of zeros. */
+int mcke_launch_linear_cross_entropy_backward(const void* hidden, const void* weight,
+                                              const int64_t* targets, const float* lse,
+                                              const float* dloss, const float* dlse, void* dhidden,
+                                              void* dweight, int dtype, int64_t rows, int64_t vocab,
+                                              int64_t dim, float scale, void* workspace,
+                                              size_t workspace_bytes, void* stream);
+
 /* ---- runtime: rt::Stream / rt::Event / raw device memory ------------------
  * reference include/mcke/runtime/stream.hpp:82-306, src/core/device.cpp:56-168,
  * src/memory/allocator.cpp:44-73, src/tensor/tensor.cpp:108-138. */

@@ -212,6 +212,25 @@ def lib() -> C.CDLL:
         "mcke_launch_token_logprobs_backward": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP,
                                                           C.c_int, _I64, _I64, _I64, C.c_float,
                                                           _VP]),
+        "mcke_launch_embedding": (C.c_int, [_VP, _VP, _VP, C.c_int, C.c_int, _I64, _I64, _I64,
+                                            C.c_float, _VP]),
+        "mcke_embedding_backward_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64]),
+        "mcke_launch_embedding_backward": (C.c_int, [_VP, _VP, _VP, C.c_int, C.c_int, _I64, _I64,
+                                                     _I64, C.c_float, C.c_int, _VP, C.c_size_t,
+                                                     _VP]),
+        "mcke_launch_bias_act_checkpoint8": (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_int, C.c_int,
+                                                       _I64, _I64, C.c_int, _VP]),
+        "mcke_bias_act_checkpoint8_backward_workspace_bytes": (C.c_size_t, [_I64, _I64]),
+        "mcke_launch_bias_act_checkpoint8_backward": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _VP,
+                                                                C.c_int, C.c_int, _I64, _I64,
+                                                                C.c_int, _VP, C.c_size_t, _VP]),
+        "mcke_linear_cross_entropy_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64]),
+        "mcke_linear_cross_entropy_backward_workspace_bytes": (C.c_size_t, [_I64, _I64, _I64]),
+        "mcke_launch_linear_cross_entropy": (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_int, _I64, _I64,
+                                                       _I64, C.c_float, _VP, C.c_size_t, _VP]),
+        "mcke_launch_linear_cross_entropy_backward": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP,
+                                                                _VP, C.c_int, _I64, _I64, _I64,
+                                                                C.c_float, _VP, C.c_size_t, _VP]),
         "mcke_rt_get_device_count": (C.c_int, [C.POINTER(C.c_int)]),
         "mcke_rt_set_device": (C.c_int, [C.c_int]),
         "mcke_rt_get_device": (C.c_int, [C.POINTER(C.c_int)]),
@@ -657,6 +676,84 @@ def launch_token_logprobs_backward(logits, tokens, lse, entropy, dlogprobs, dent
     return _st(lib().mcke_launch_token_logprobs_backward(
         _ptr(logits), _ptr(tokens), _ptr(lse), _ptr(entropy), _ptr(dlogprobs), _ptr(dentropy),
         _ptr(dlogits), dtype, rows, vocab, row_stride, scale, _sh(stream)))
+
+
+# ---------------------------------------------------------------------------
+# Embedding, bias + activation kept in 8 bits, cross entropy of hidden states (no
+# reference counterparts; see include/mcke_amd.h)
+# ---------------------------------------------------------------------------
+def launch_embedding(tokens, table, out, table_dtype, out_dtype, rows: int, vocab: int, cols: int,
+                     scale: float = 1.0, stream=None) -> Status:
+    """out[r] = scale * table[tokens[r]]; zeros for a negative token."""
+    return _st(lib().mcke_launch_embedding(_ptr(tokens), _ptr(table), _ptr(out), table_dtype,
+                                           out_dtype, rows, vocab, cols, scale, _sh(stream)))
+
+
+def embedding_backward_workspace_bytes(rows: int, vocab: int, cols: int) -> int:
+    return int(lib().mcke_embedding_backward_workspace_bytes(rows, vocab, cols))
+
+
+def launch_embedding_backward(tokens, dout, dtable, dout_dtype, table_dtype, rows: int, vocab: int,
+                              cols: int, scale: float = 1.0, accumulate: bool = False,
+                              workspace=None, workspace_bytes: int = 0, stream=None) -> Status:
+    """The table's gradient, each token's rows of dout added up in their order; accumulate adds
+    to dtable, else all of it is written."""
+    return _st(lib().mcke_launch_embedding_backward(
+        _ptr(tokens), _ptr(dout), _ptr(dtable), dout_dtype, table_dtype, rows, vocab, cols, scale,
+        accumulate, _ptr(workspace), workspace_bytes, _sh(stream)))
+
+
+def launch_bias_act_checkpoint8(x, bias, y, codes, exponents, dtype, bias_dtype, rows: int,
+                                cols: int, act, stream=None) -> Status:
+    """y = act(x + bias), with x + bias kept as e4m3 codes (rows x cols bytes) and an exponent for
+    each 32 columns of a row (rows x ceil(cols / 32) bytes); bias and y may be None."""
+    return _st(lib().mcke_launch_bias_act_checkpoint8(
+        _ptr(x), _ptr(bias), _ptr(y), _ptr(codes), _ptr(exponents), dtype, bias_dtype, rows, cols,
+        act, _sh(stream)))
+
+
+def bias_act_checkpoint8_backward_workspace_bytes(rows: int, cols: int) -> int:
+    return int(lib().mcke_bias_act_checkpoint8_backward_workspace_bytes(rows, cols))
+
+
+def launch_bias_act_checkpoint8_backward(dy, codes, exponents, dx, y, dbias, dtype, bias_dtype,
+                                         rows: int, cols: int, act, workspace=None,
+                                         workspace_bytes: int = 0, stream=None) -> Status:
+    """From what launch_bias_act_checkpoint8 kept: dx = dy * act'(u), dbias, and y = act(u) once
+    more.  Any of the three may be None; dy is for the first two and the workspace for dbias."""
+    return _st(lib().mcke_launch_bias_act_checkpoint8_backward(
+        _ptr(dy), _ptr(codes), _ptr(exponents), _ptr(dx), _ptr(y), _ptr(dbias), dtype, bias_dtype,
+        rows, cols, act, _ptr(workspace), workspace_bytes, _sh(stream)))
+
+
+def linear_cross_entropy_workspace_bytes(rows: int, vocab: int, dim: int) -> int:
+    return int(lib().mcke_linear_cross_entropy_workspace_bytes(rows, vocab, dim))
+
+
+def launch_linear_cross_entropy(hidden, weight, targets, loss, lse, dtype, rows: int, vocab: int,
+                                dim: int, scale: float = 1.0, workspace=None,
+                                workspace_bytes: int = 0, stream=None) -> Status:
+    """Each row's loss = lse - z[target] and lse = log sum exp z over z = scale * hidden weight^T,
+    which is not kept; a negative target marks a row to leave out.  loss or lse may be None."""
+    return _st(lib().mcke_launch_linear_cross_entropy(
+        _ptr(hidden), _ptr(weight), _ptr(targets), _ptr(loss), _ptr(lse), dtype, rows, vocab, dim,
+        scale, _ptr(workspace), workspace_bytes, _sh(stream)))
+
+
+def linear_cross_entropy_backward_workspace_bytes(rows: int, vocab: int, dim: int) -> int:
+    return int(lib().mcke_linear_cross_entropy_backward_workspace_bytes(rows, vocab, dim))
+
+
+def launch_linear_cross_entropy_backward(hidden, weight, targets, lse, dloss, dlse, dhidden,
+                                         dweight, dtype, rows: int, vocab: int, dim: int,
+                                         scale: float = 1.0, workspace=None,
+                                         workspace_bytes: int = 0, stream=None) -> Status:
+    """The gradients of launch_linear_cross_entropy in the hidden states and in the weights;
+    dloss or dlse, and dhidden or dweight, may be None."""
+    return _st(lib().mcke_launch_linear_cross_entropy_backward(
+        _ptr(hidden), _ptr(weight), _ptr(targets), _ptr(lse), _ptr(dloss), _ptr(dlse),
+        _ptr(dhidden), _ptr(dweight), dtype, rows, vocab, dim, scale, _ptr(workspace),
+        workspace_bytes, _sh(stream)))
 
 
 # ---------------------------------------------------------------------------

@@ -1,0 +1,335 @@
+// gemm_lp_any.hpp -- the main loop of a 16-bit product whose operands lie either way:
+//
+//   acc[m][n] += sum over k of A(m, k) B(k, n),   bf16 or fp16, fp32 accumulation
+//
+// each operand with its k contiguous (kAlongK: rows of A[m][k], of B[n][k], as a layer's weights
+// [out][in] and activations are) or with its other index contiguous (kAcrossK: A[k][m],
+// B[k][n]).  A layer's three products, y = x W^T, dx = dy W and dW = dy^T x, are one of these
+// each, with no transposed copy.
+//
+// A workgroup of four waves (2 x 2) owns BM x BN, a wave MT x NT blocks of 16 x 16
+// (v_mfma_f32_16x16x32).  K goes in stages of 64 (two steps of 32), each operand's stage straight
+// from memory into LDS (global_load_lds_dwordx4):
+//   kAlongK   rows of 128 bytes, 16-byte chunk c of row r at c ^ (r % 8); a fragment is one
+//             ds_read_b128;
+//   kAcrossK  64 rows (one k each) of 2 BM or 2 BN bytes, chunk c of row k at
+//             c ^ (4 (k % 4) + 2 ((k / 8) % 2)); a fragment is two ds_read_b64_tr_b16.
+// Neither read meets a bank twice.  A has three stage buffers and B two: 160 KB at 256 x 256.
+//
+// Stage p is two steps; a step computes on fragments read in the step before it:
+//   step 2 p      MFMAs of k half 0; reads of half 1; DMA of A stage p + 2
+//   step 2 p + 1  wait for A and B of stage p + 1, barrier; MFMAs of half 1; reads of
+//                 half 0 of stage p + 1; DMA of B stage p + 2 into the buffer of stage p
+// so a stage has two to three steps to land, and there is one barrier per 64 of K.  Each wave
+// waits for its own reads before that barrier, which makes every buffer of stage p free behind it.
+// Past the end the DMA repeats the last stage into buffers that nobody reads, which keeps the
+// count of loads in flight the same in every step.
+//
+// K is a multiple of 64 here.  Rows past an operand's end along M and N repeat its last row and are
+// not to be stored.  Along K both operands have whole stages: kAlongK rows are as long, and of a
+// kAcrossK operand the last stage may lie elsewhere (`tail`), where rows of a matrix that ends inside
+// it are followed by zeros.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <utility>
+
+#include "gemm_lp.hpp"
+
+namespace mcke_amd {
+
+enum class Along { kAlongK, kAcrossK };
+
+// An operand's memory, 16-byte aligned, `row` elements between neighbouring rows.  `extent`: its
+// rows (kAlongK), or how many elements of a row may be read (kAcrossK; a multiple of 8, at least
+// 8).
+struct LpOperand {
+  const uint16_t* p;
+  int64_t row;
+  int64_t extent;
+  const uint16_t* tail = nullptr;
+  int64_t tail_stage = -1;     // the stage that is at `tail`
+};
+
+template <int B, Along L> struct LpAnyOperand {
+  static constexpr bool kAcross = L == Along::kAcrossK;
+  static constexpr int kBuf = B * 128;               // one stage, either way: B x 64 values
+  static constexpr int kDma = kBuf / 1024 / 4;       // DMA instructions per wave and stage
+  static constexpr int kBlocks = B / 32;             // 16-wide blocks of a wave
+  static constexpr int kRow = kAcross ? 2 * B : 128; // an LDS row
+  static constexpr int kLanes = kRow / 16;           // lanes a row of a DMA instruction
+  static constexpr int kReads = kBlocks * (kAcross ? 2 : 1);
+  static_assert(kLanes <= 32 && (!kAcross || B >= 128), "the swizzle takes 16 chunks a row");
+  static __host__ __device__ constexpr int swz(int r) {
+    return kAcross ? 4 * (r % 4) + 2 * ((r / 8) % 2) : r % 8;
+  }
+
+  // A lane's sources, relative to the stage's uniform base.
+  const char* base;
+  const char* tail;
+  int64_t tail_stage;
+  int64_t step;                                      // bytes between stages
+  uint32_t src[kDma];
+  uint32_t off[2];                                   // fragment addresses in a buffer
+
+  // A DMA instruction's immediate offset (1 KB times its index, modulo four) moves its source too:
+  // the offsets have it taken off, and are kept positive by 3 KB that the base gives back.
+  static constexpr uint32_t kBias = 3072;
+
+  // The workgroup's rows or columns begin at `first`, the wave's at `wave_first` of them.
+  __device__ __forceinline__ void begin(const LpOperand& o, int64_t first, int wave_first,
+                                        int wave) {
+    const int lane = threadIdx.x % kWave, g = lane / 16, r16 = lane % 16;
+    if constexpr (!kAcross) {
+      base = reinterpret_cast<const char*>(o.p + first * o.row) - kBias;
+      step = 128;
+      const int64_t last = o.extent - 1 - first;
+#pragma unroll
+      for (int q = 0; q < kDma; ++q) {
+        const int rt = 8 * (wave * kDma + q) + lane / 8;
+        const int64_t r = rt < last ? rt : last;
+        src[q] = static_cast<uint32_t>(r * o.row * 2) + 16u * ((lane % 8) ^ swz(rt)) + kBias -
+                 1024u * (q % 4);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        off[s] = (wave_first + r16) * kRow + 16 * ((4 * s + g) ^ (r16 % 8));
+    } else {
+      base = reinterpret_cast<const char*>(o.p) - kBias;
+      tail = reinterpret_cast<const char*>(o.tail) - kBias;
+      tail_stage = o.tail_stage;
+      step = 64 * o.row * 2;
+#pragma unroll
+      for (int q = 0; q < kDma; ++q) {
+        const int rt = (64 / kLanes) * (wave * kDma + q) + lane / kLanes;
+        const int64_t col = first + 8 * ((lane % kLanes) ^ swz(rt));
+        src[q] = static_cast<uint32_t>(rt * o.row * 2) +
+                 static_cast<uint32_t>(2 * (col + 8 <= o.extent ? col : o.extent - 8)) + kBias -
+                 1024u * (q % 4);
+      }
+      // Lane r16 = 4 jq + qa of group g reads row 8 g + 4 t + jq at columns 4 qa of its block and
+      // receives column r16 of rows 8 g + 4 t .. + 3.
+      // Block b's chunks differ from block 0's in bits that the wave's first chunk does not have,
+      // and buffers begin at multiples of 1 KB: the blocks' addresses are one, xor 32 b.
+      const int jq = r16 / 4, qa = r16 % 4, k = 8 * g + jq, col = wave_first + 4 * qa;
+      off[0] = k * kRow + 16 * ((col / 8) ^ swz(k)) + (col % 8) * 2;
+    }
+  }
+
+  // Instruction Q of stage p, whose uniform source is `from`, into the buffer at LDS `buf`.
+  template <int Q>
+  __device__ __forceinline__ void dma(const char* from, uint32_t buf, uint32_t wave) const {
+    lds_dma16<(Q % 4) * 1024>(src[Q], from, buf + (wave * kDma + Q / 4 * 4) * 1024);
+  }
+  __device__ __forceinline__ const char* source(int64_t p) const {
+    if constexpr (kAcross)
+      if (p == tail_stage) return tail;
+    return base + p * step;
+  }
+
+  struct Frags {
+    u32x4 whole[kAcross ? 1 : kBlocks];
+    u32x2 half[kAcross ? kBlocks : 1][2];
+  };
+  // Read RR of half S of the stage at LDS `buf`.
+  template <int S, int RR> __device__ __forceinline__ void read(uint32_t buf, Frags& f) const {
+    if constexpr (kAcross)
+      f.half[RR / 2][RR % 2] =
+          lds_read_tr16<(32 * S + 4 * (RR % 2)) * kRow>((buf + off[0]) ^ (32 * (RR / 2)));
+    else
+      f.whole[RR] = lds_read128<RR * 16 * kRow>(buf + off[S]);
+  }
+  template <int I> static __device__ __forceinline__ void touch(Frags& f) {
+    if constexpr (kAcross) {
+      asm volatile("" : "+v"(f.half[I][0]));
+      asm volatile("" : "+v"(f.half[I][1]));
+    } else {
+      asm volatile("" : "+v"(f.whole[I]));
+    }
+  }
+  static __device__ __forceinline__ u32x4 get(const Frags& f, int i) {
+    if constexpr (kAcross)
+      return u32x4{f.half[i][0][0], f.half[i][0][1], f.half[i][1][0], f.half[i][1][1]};
+    else
+      return f.whole[i];
+  }
+};
+
+template <int BM, int BN, Along LA, Along LB> struct LpAnyShape {
+  using OA = LpAnyOperand<BM, LA>;
+  using OB = LpAnyOperand<BN, LB>;
+  static constexpr int kABufs = 3, kBBufs = 2;
+  static constexpr int kBBase = kABufs * OA::kBuf;
+  static constexpr int kLdsBytes = kBBase + kBBufs * OB::kBuf;
+  static constexpr int MT = BM / 32, NT = BN / 32;
+  static constexpr int kMfmas = MT * NT;
+  static constexpr int kReads = OB::kReads + OA::kReads;       // B's blocks first, then A's
+  // Reads in the first three quarters of a step, so that those of step 2 p have come back at the
+  // barrier behind it.
+  static constexpr int read_slot(int rr) { return rr * (3 * kMfmas) / (4 * kReads); }
+  static constexpr int dma_slot(int ii, int n) { return ii * kMfmas / n + (kMfmas / n) / 2; }
+  static_assert(kLdsBytes <= 160 * 1024, "LDS holds 160 KiB");
+  // Block row i of an even step waits for B's reads and A block i's, issued in the step before; A
+  // reads behind them and this step's so far may be outstanding (lgkmcnt counts to 15).
+  static constexpr int wait_before_row(int i) {
+    int n = (OA::kReads / MT) * (MT - 1 - i);
+    for (int rr = 0; rr < kReads; ++rr) n += read_slot(rr) < i * NT ? 1 : 0;
+    return n < 15 ? n : 15;
+  }
+};
+
+// What a step needs besides the fragments.
+struct LpAnyStep {
+  uint32_t a_read, b_read;       // LDS buffers that are read
+  uint32_t dma_buf;              // LDS buffer that is filled
+  const char* dma_from;
+};
+
+// MFMA IDX of a step, on the fragments cur, with the reads (of half RS, into next) and the DMA
+// (of A or of B) that go out behind it.  The product is transposed: a lane holds four
+// neighbouring columns of a row.
+template <typename T, class S, int PARITY, int IDX>
+__device__ __forceinline__ void lp_any_slot(
+    f32x4 (&acc)[S::MT][S::NT], typename S::OA::Frags& ca, typename S::OB::Frags& cb,
+    typename S::OA::Frags& na, typename S::OB::Frags& nb, const typename S::OA& oa,
+    const typename S::OB& ob, const LpAnyStep& sp, uint32_t wave) {
+  constexpr int NT = S::NT, RS = 1 - PARITY;
+  constexpr int i = IDX / NT, jj = IDX % NT, j = mfma_snake_col(i, jj, NT);
+  if constexpr (jj == 0) {
+    if constexpr (PARITY == 0) lds_wait_n<S::wait_before_row(i)>();
+    S::OA::template touch<i>(ca);
+    if constexpr (i == 0) {
+      [&]<int... J>(std::integer_sequence<int, J...>) {
+        (S::OB::template touch<J>(cb), ...);
+      }(std::make_integer_sequence<int, NT>{});
+    }
+  }
+  acc[i][j] = LpMfma16<T>::run(S::OB::get(cb, j), S::OA::get(ca, i), acc[i][j]);
+  __builtin_amdgcn_sched_barrier(0);
+  [&]<int... RR>(std::integer_sequence<int, RR...>) {
+    ([&] {
+      if constexpr (S::read_slot(RR) == IDX) {
+        if constexpr (RR < S::OB::kReads) ob.template read<RS, RR>(sp.b_read, nb);
+        else oa.template read<RS, RR - S::OB::kReads>(sp.a_read, na);
+      }
+    }(), ...);
+  }(std::make_integer_sequence<int, S::kReads>{});
+  if constexpr (PARITY == 0) {
+    [&]<int... Q>(std::integer_sequence<int, Q...>) {
+      ([&] {
+        if constexpr (S::dma_slot(Q, S::OA::kDma) == IDX)
+          oa.template dma<Q>(sp.dma_from, sp.dma_buf, wave);
+      }(), ...);
+    }(std::make_integer_sequence<int, S::OA::kDma>{});
+  } else {
+    [&]<int... Q>(std::integer_sequence<int, Q...>) {
+      ([&] {
+        if constexpr (S::dma_slot(Q, S::OB::kDma) == IDX)
+          ob.template dma<Q>(sp.dma_from, sp.dma_buf, wave);
+      }(), ...);
+    }(std::make_integer_sequence<int, S::OB::kDma>{});
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The products of stages first .. first + stages - 1 (stages >= 1) of the tile at (m0, n0) into
+// acc, from zero.  `smem`: S::kLdsBytes, 1024-byte aligned; free behind the caller's next barrier.
+// Lane (g, r16), register e of block (i, j): row wm BM/2 + 16 i + r16, column
+// wn BN/2 + 16 j + 4 g + e of the tile.
+template <typename T, int BM, int BN, Along LA, Along LB>
+__device__ __forceinline__ void lp_any_loop(f32x4 (&acc)[BM / 32][BN / 32], char* smem,
+                                            const LpOperand& A, const LpOperand& B, int64_t m0,
+                                            int64_t n0, int64_t first, int stages) {
+  using S = LpAnyShape<BM, BN, LA, LB>;
+  constexpr int MT = S::MT, NT = S::NT;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wm = wave / 2, wn = wave % 2;
+  typename S::OA oa;
+  typename S::OB ob;
+  oa.begin(A, m0, wm * (BM / 2), wave);
+  ob.begin(B, n0, wn * (BN / 2), wave);
+  const uint32_t lds0 = lds_addr(smem), ldsb = lds0 + S::kBBase;
+  const uint32_t w = static_cast<uint32_t>(wave);
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  // The accumulators are in the accumulation registers from here on: left to itself the compiler
+  // keeps some elsewhere and moves them back and forth in every stage.
+  auto pin = [&] {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) asm volatile("" : "+a"(acc[i][j]));
+  };
+  pin();
+
+  auto stage = [&](int p) { return first + (p < stages ? p : stages - 1); };
+  auto dma_a = [&](int p, uint32_t buf) {
+    [&]<int... Q>(std::integer_sequence<int, Q...>) {
+      (oa.template dma<Q>(oa.source(stage(p)), buf, w), ...);
+    }(std::make_integer_sequence<int, S::OA::kDma>{});
+  };
+  auto dma_b = [&](int p, uint32_t buf) {
+    [&]<int... Q>(std::integer_sequence<int, Q...>) {
+      (ob.template dma<Q>(ob.source(stage(p)), buf, w), ...);
+    }(std::make_integer_sequence<int, S::OB::kDma>{});
+  };
+  dma_a(0, lds0);
+  dma_b(0, ldsb);
+  dma_a(1, lds0 + S::OA::kBuf);
+  dma_b(1, ldsb + S::OB::kBuf);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(S::OA::kDma + S::OB::kDma) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  typename S::OA::Frags fa[2];
+  typename S::OB::Frags fb[2];
+  [&]<int... RR>(std::integer_sequence<int, RR...>) {
+    (ob.template read<0, RR>(ldsb, fb[0]), ...);
+  }(std::make_integer_sequence<int, S::OB::kReads>{});
+  [&]<int... RR>(std::integer_sequence<int, RR...>) {
+    (oa.template read<0, RR>(lds0, fa[0]), ...);
+  }(std::make_integer_sequence<int, S::OA::kReads>{});
+
+  uint32_t abuf = 0;               // A buffer of stage p
+  for (int p = 0; p < stages; ++p) {
+    const uint32_t a1 = abuf == 2 ? 0 : abuf + 1, a2 = a1 == 2 ? 0 : a1 + 1;
+    const uint32_t bcur = ldsb + (p % 2) * S::OB::kBuf, bnext = ldsb + ((p + 1) % 2) * S::OB::kBuf;
+    const LpAnyStep even{lds0 + abuf * S::OA::kBuf, bcur, lds0 + a2 * S::OA::kBuf,
+                         oa.source(stage(p + 2))};
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+      (lp_any_slot<T, S, 0, I>(acc, fa[0], fb[0], fa[1], fb[1], oa, ob, even, w),
+       ...);
+    }(std::make_integer_sequence<int, S::kMfmas>{});
+    // Of the loads in flight only A's of stage p + 2 may be outstanding, and none of this wave's
+    // reads.  A bare s_barrier: __syncthreads() would wait for all loads.
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(S::OA::kDma) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const LpAnyStep odd{lds0 + a1 * S::OA::kBuf, bnext, bcur, ob.source(stage(p + 2))};
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+      (lp_any_slot<T, S, 1, I>(acc, fa[1], fb[1], fa[0], fb[0], oa, ob, odd, w),
+       ...);
+    }(std::make_integer_sequence<int, S::kMfmas>{});
+    abuf = a1;
+    pin();
+  }
+  // The last stage's reads of the next one go unused, but they land in these registers: named
+  // behind the wait, those hold nothing else before it.
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  [&]<int... I>(std::integer_sequence<int, I...>) {
+    (S::OA::template touch<I>(fa[0]), ...);
+  }(std::make_integer_sequence<int, MT>{});
+  [&]<int... I>(std::integer_sequence<int, I...>) {
+    (S::OB::template touch<I>(fb[0]), ...);
+  }(std::make_integer_sequence<int, NT>{});
+  // They are read by acc_get, inline asm that the hazard checks do not see into: 16 cycles for the
+  // last MFMA's results.
+  pin();
+  asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
+}
+
+}  // namespace mcke_amd

@@ -1,0 +1,936 @@
+// linear_cross_entropy.hip -- softmax cross entropy of hidden states and a vocabulary's weights,
+// and its gradients, without the logits being kept.
+//
+//   z = scale H W^T (H: rows x dim, W: vocab x dim, as layers hold it)
+//   lse = log sum exp z,  loss = lse - z[target]
+//   dz = scale ((dloss + dlse) p - dloss [j == target]),  p = exp(z - lse)
+//   dH = dz W,  dW = dz^T H
+//
+// Forward.  Each tile of logits stays in the accumulation registers: a wave reduces its rows to
+// (largest logit, sum of exponentials against it) and stores those two numbers and the target's
+// logit.  A second launch joins them.  What is written is 16 bytes for 128 (or 64) logits.
+//
+// Backward.  The vocabulary goes in pieces.  For each, the logits are computed once more (the
+// third of three products: the alternative is to keep them), become dz in 16 bits, and two more
+// products take dz: dH adds up over the pieces in fp32, dW's rows are the piece's own.  dz is
+// rounded to the operands' type because the matrix cores take it so: at most half a step
+// relative to each value, as the rounding of a stored logit's gradient would be.  It is stored
+// relative to the largest gradient m of a row, as 2^14 dz / m, and the fp32 sums are multiplied by m
+// 2^-14.  With that, fp16 keeps all bits of p down to 4e-9 (dloss is often 1 / rows, and its
+// own smallest full value is 6e-5); and where all rows have the same dloss, as under a mean, the
+// target's - dloss is -2^14 with no rounding, in either type.  (It is the largest term of dH,
+// and rounds to the same side in all rows: 2047 rows, 32001 tokens, fp16, off by 3.5e-4 of the
+// gradients' size with a power of two for m, 2.4e-4 like this; 2.1e-4 is the outputs' own rounding.)
+//
+// Rows without a target (target < 0) are not read.  The rows that have one are copied side by
+// side first, which skips the products of the others, ends them at whole stages of K with zeros,
+// and makes rows of any width and alignment whole 16-byte vectors.  (16384 x 4096: 0.3 ms of a
+// pass.)  How many there are is known on the device alone: the launches cover all rows, and
+// workgroups past the last one end.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <string>
+
+#include "common.hpp"
+#include "device_math.hpp"
+#include "elem.hpp"
+#include "gemm_lp_any.hpp"
+
+namespace mcke_amd {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kPrepThreads = 1024;
+constexpr int kThreads = 256;
+
+// Device-side facts that the launches of a call share.
+struct Meta {
+  int rows;            // that have a target
+  float factor;        // what dz is stored times, and what takes it out again
+  float unfactor;
+  int pad;
+};
+
+// The rows that have a target, packed.
+struct Rows {
+  Meta* meta;
+  int* from;           // packed row -> row
+  int* rank;           // row -> packed row, or -1
+  int* target;         // of packed rows; -2 where it is past the vocabulary (NaN results)
+  float* lse2;         // lse log2 e                                   (backward)
+  float* cp;           // what p and the target's 1 are multiplied by  (backward)
+  float* ct;
+};
+
+// ---------------------------------------------------------------------------
+// Rows that have a target, in order; one workgroup.
+// ---------------------------------------------------------------------------
+template <bool BACKWARD>
+__global__ __launch_bounds__(kPrepThreads) void lce_rows_kernel(
+    const int64_t* __restrict__ targets, const float* __restrict__ lse,
+    const float* __restrict__ dloss, const float* __restrict__ dlse, int rows, int64_t vocab,
+    float scale, Rows out, float* __restrict__ loss_out, float* __restrict__ lse_out) {
+  __shared__ int waves[kPrepThreads / kWave];
+  __shared__ float most[kPrepThreads / kWave];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  float factor = 1.0f, unfactor = 1.0f;
+  if constexpr (BACKWARD) {
+    float m = 0.0f;
+    for (int r = threadIdx.x; r < rows; r += kPrepThreads) {
+      if (targets[r] < 0) continue;
+      const float a = dloss ? scale * dloss[r] : 0.0f, b = dlse ? scale * dlse[r] : 0.0f;
+      const float big = __builtin_fabsf(a) + __builtin_fabsf(b);
+      m = fmaxf(m, big < __builtin_inff() ? big : 0.0f);
+    }
+    m = wave_max(m);
+    if (lane == 0) most[wave] = m;
+    __syncthreads();
+    m = wave_max<16>(most[threadIdx.x % 16]);
+    if (m > 0.0f) {
+      m = fmaxf(m, 0x1p-100f);     // (2^14 / m stays finite)
+      factor = 0x1p14f / m;
+      unfactor = m * 0x1p-14f;
+    }
+    static_assert(kPrepThreads / kWave == 16, "one value of each wave");
+  }
+  int count = 0;
+  for (int r0 = 0; r0 < rows; r0 += kPrepThreads) {
+    const int r = r0 + threadIdx.x;
+    const int64_t t = r < rows ? targets[r] : -1;
+    const uint64_t set = __ballot(t >= 0);
+    if (lane == 0) waves[wave] = __popcll(set);
+    __syncthreads();
+    int before = count + __popcll(set & ((uint64_t{1} << lane) - 1));
+    for (int w = 0; w < kPrepThreads / kWave; ++w) {
+      if (w < wave) before += waves[w];
+      count += waves[w];
+    }
+    if (r < rows) {
+      out.rank[r] = t >= 0 ? before : -1;
+      if (t >= 0) {
+        out.from[before] = r;
+        out.target[before] = t < vocab ? static_cast<int>(t) : -2;
+        if constexpr (BACKWARD) {
+          const float a = dloss ? scale * dloss[r] * factor : 0.0f;
+          const float b = dlse ? scale * dlse[r] * factor : 0.0f;
+          out.lse2[before] = lse[r] * kLog2e;
+          out.cp[before] = t < vocab ? a + b : __builtin_nanf("");
+          out.ct[before] = a;
+        }
+      } else {
+        if (loss_out) loss_out[r] = 0.0f;
+        if (lse_out) lse_out[r] = 0.0f;
+      }
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *out.meta = Meta{count, factor, unfactor, 0};
+}
+
+// Packed rows: row k of `to` (`width` values, a multiple of 64) is row from[k] of x (`cols`
+// values) with zeros behind it, and behind the last row are rows of zeros up to the next multiple
+// of 64 (64 at least).  from null: the `given` rows as they are, and zeros up to `rows`.  A
+// workgroup a row.
+__global__ __launch_bounds__(kThreads) void lce_pack_kernel(const uint16_t* __restrict__ x,
+                                                            const int* __restrict__ from,
+                                                            const Meta* __restrict__ meta,
+                                                            uint16_t* __restrict__ to, int64_t given,
+                                                            int64_t rows, int cols, int width) {
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8), aligned(2)));
+  for (int64_t k = blockIdx.x; k < rows; k += gridDim.x) {
+    const uint16_t* row = nullptr;
+    if (!from) {
+      if (k < given) row = x + k * cols;
+    } else {
+      const int n = meta->rows, up = n > 0 ? (n + 63) / 64 * 64 : 64;
+      if (k >= up) return;
+      if (k < n) row = x + static_cast<int64_t>(from[k]) * cols;
+    }
+    for (int c = 8 * threadIdx.x; c < width; c += 8 * kThreads) {
+      u16x8 v{};
+      if (row && c + 8 <= cols) {
+        v = *reinterpret_cast<const u16x8*>(row + c);
+      } else if (row) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < cols) v[e] = row[c + e];
+      }
+      *reinterpret_cast<u16x8*>(to + k * width + c) = v;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Tiles
+// ---------------------------------------------------------------------------
+// The tile of this workgroup, or false where the rows that have a target end before it.
+template <int BM>
+__device__ __forceinline__ bool tile_of_rows(int n, int tiles_n, int& tm, int& tn) {
+  const int tiles_m = n > 0 ? (n + BM - 1) / BM : 1;
+  if (static_cast<int>(blockIdx.x) >= tiles_m * tiles_n) return false;
+  mfma_tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  return true;
+}
+
+__device__ __forceinline__ float across_groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float across_groups_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+struct Logits {
+  const uint16_t* hidden;      // packed rows, `width` apart
+  const uint16_t* weight;      // the piece's rows, `width` apart
+  int width;                   // a multiple of 64
+  int64_t piece;               // rows of the piece
+  int64_t first;               // its first row in the vocabulary
+  float scale;
+};
+
+template <int BM, int BN, typename T>
+__device__ __forceinline__ void logits_tile(f32x4 (&acc)[BM / 32][BN / 32], char* smem,
+                                            const Logits& l, int n, int64_t m0, int64_t n0) {
+  const LpOperand A{l.hidden, l.width, n > 0 ? n : 1};
+  const LpOperand B{l.weight, l.width, l.piece};
+  lp_any_loop<T, BM, BN, Along::kAlongK, Along::kAlongK>(acc, smem, A, B, m0, n0, 0, l.width / 64);
+}
+
+// (largest, sum) of each row's part in the tile: wave column wn of vocabulary tile `tile` is
+// entry 2 tile + wn, `stride` values apart.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(kMfmaThreads, 1) void lce_stats_kernel(
+    Logits l, const Meta* __restrict__ meta, const int* __restrict__ target,
+    float* __restrict__ largest, float* __restrict__ sums, float* __restrict__ at_target,
+    int64_t stride, int tile0, int tiles_n) {
+  using S = LpAnyShape<BM, BN, Along::kAlongK, Along::kAlongK>;
+  constexpr int MT = S::MT, NT = S::NT, WN = BN / 2;
+  __shared__ __attribute__((aligned(1024))) char smem[S::kLdsBytes];
+  const int n = __builtin_amdgcn_readfirstlane(meta->rows);
+  int tm, tn;
+  if (!tile_of_rows<BM>(n, tiles_n, tm, tn)) return;
+  const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+  f32x4 acc[MT][NT];
+  logits_tile<BM, BN, T>(acc, smem, l, n, m0, n0);
+
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
+  const float c = l.scale * kLog2e;
+  // Columns of the wave that are in the vocabulary, less this lane's 4 g.
+  const bool cut = n0 + BN > l.piece;
+  const int left = static_cast<int>(cut ? l.piece - n0 - wn * WN - 4 * g : BN);
+  const int64_t at = 2 * static_cast<int64_t>(tile0 + tn) + wn;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t row = m0 + wm * (BM / 2) + 16 * i + r16;
+    float v[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = acc_get(acc[i][j][e]);
+    if (cut) {
+      int past = left;
+      asm("" : "+v"(past));        // (kept over the rows, the 4 NT comparisons fill the scalar file)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (16 * j + e >= past) v[j][e] = -__builtin_inff();
+    }
+    float m = v[0][0];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, v[j][e]);
+    m = across_groups_max(m);
+    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((v[j][e] - ref) * c);
+    s = across_groups_sum(s);
+    if (g == 0 && row < n) {
+      largest[at * stride + row] = m;
+      sums[at * stride + row] = s;
+    }
+    // The target's column, where it is one of this wave's.
+    const int64_t t = (row < n ? target[row] : -1) - (l.first + n0 + wn * WN);
+    if (__ballot(t >= 0 && t < WN)) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (t == 16 * j + 4 * g + e) at_target[row] = v[j][e];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// loss and lse of packed rows from their parts: 64 rows a workgroup (a row to a lane), the parts
+// dealt to its waves.
+constexpr int kJoinWaves = 16;
+
+__global__ __launch_bounds__(kJoinWaves * kWave) void lce_join_kernel(
+    const float* __restrict__ largest, const float* __restrict__ sums,
+    const float* __restrict__ at_target, const int* __restrict__ from,
+    const int* __restrict__ target, const Meta* __restrict__ meta, float* __restrict__ loss,
+    float* __restrict__ lse_out, int64_t stride, int parts, float scale) {
+  __shared__ float lm[kJoinWaves][kWave], ls[kJoinWaves][kWave];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWave + lane;
+  const int n = meta->rows;
+  const float c = scale * kLog2e;
+  if (static_cast<int64_t>(blockIdx.x) * kWave >= n) return;
+  float m = -__builtin_inff(), s = 0.0f;
+  auto add = [&](float m2, float s2) {
+    // (An empty part has no largest logit; -inf against itself moves nothing.)
+    const float to = fmaxf(m, m2);
+    const float f = m == to ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
+    const float f2 = m2 == to ? 1.0f : __builtin_amdgcn_exp2f((m2 - to) * c);
+    s = f * s + f2 * s2;
+    m = to;
+  };
+  if (row < n) {
+#pragma unroll 8
+    for (int p = wave; p < parts; p += kJoinWaves) add(largest[p * stride + row], sums[p * stride + row]);
+  }
+  lm[wave][lane] = m;
+  ls[wave][lane] = s;
+  __syncthreads();
+  if (wave > 0 || row >= n) return;
+  for (int w = 1; w < kJoinWaves; ++w) add(lm[w][lane], ls[w][lane]);
+  const float lse = __builtin_fmaf(kLn2, __builtin_amdgcn_logf(s), scale * m);
+  if (lse_out) lse_out[from[row]] = lse;
+  if (loss) loss[from[row]] = target[row] < 0 ? __builtin_nanf("") : lse - scale * at_target[row];
+}
+
+// dz of a tile, row-major (`ld` values a row), zeros in rows and columns that pad it.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows rows,
+                                                                uint16_t* __restrict__ dz,
+                                                                int64_t ld, int tiles_n) {
+  using S = LpAnyShape<BM, BN, Along::kAlongK, Along::kAlongK>;
+  using O = LpOut<T>;
+  constexpr int MT = S::MT, NT = S::NT, WM = BM / 2, WN = BN / 2;
+  __shared__ __attribute__((aligned(1024))) char smem[S::kLdsBytes];
+  const int n = __builtin_amdgcn_readfirstlane(rows.meta->rows);
+  int tm, tn;
+  if (!tile_of_rows<BM>(n, tiles_n, tm, tn)) return;
+  const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+  f32x4 acc[MT][NT];
+  logits_tile<BM, BN, T>(acc, smem, l, n, m0, n0);
+
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
+  const float c = l.scale * kLog2e;
+  const bool cut = n0 + BN > l.piece;
+  const int left = static_cast<int>(cut ? l.piece - n0 - wn * WN - 4 * g : BN);
+  // Through LDS, so that the stores are whole rows: chunk q of tile row r at q ^ (r % kChunks).
+  struct alignas(8) Quad { T v[4]; };
+  constexpr int kRowBytes = BN * 2, kChunks = kRowBytes / 16, kSwz = kChunks < 32 ? kChunks : 32;
+  static_assert(BM * kRowBytes <= S::kLdsBytes, "the tile must fit the stage buffers");
+  __syncthreads();
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int rt = wm * WM + 16 * i + r16;
+    const int64_t row = m0 + rt;
+    const bool have = row < n;
+    const float lse2 = have ? rows.lse2[row] : 0.0f, cp = have ? rows.cp[row] : 0.0f;
+    const float ct = have ? rows.ct[row] : 0.0f;
+    const int64_t t = (have ? rows.target[row] : -1) - (l.first + n0 + wn * WN) - 4 * g;
+    // Columns from `past` on, and rows without a target, are zeros whatever their exponentials
+    // are.
+    int past = have ? left : 0;
+    asm("" : "+v"(past));          // (as in the statistics)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      Quad o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p =
+            __builtin_amdgcn_exp2f(__builtin_fmaf(acc_get(acc[i][j][e]), c, -lse2));
+        float v = cp * p;
+        if (t == 16 * j + e) v -= ct;
+        if (16 * j + e >= past) v = 0.0f;
+        o.v[e] = O::from_f32(v);
+      }
+      const int col = wn * WN + 16 * j + 4 * g;
+      *reinterpret_cast<Quad*>(smem + rt * kRowBytes + (((col / 8) ^ (rt % kSwz)) * 16) +
+                               (col % 8) * 2) = o;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();
+  constexpr int kRowsPerPass = kMfmaThreads / kChunks;
+  const int q = threadIdx.x % kChunks;
+  const int up = n > 0 ? (n + 63) / 64 * 64 : 64;
+#pragma unroll 4
+  for (int r0 = 0; r0 < BM; r0 += kRowsPerPass) {
+    const int rt = r0 + threadIdx.x / kChunks;
+    const u32x4 v =
+        *reinterpret_cast<const u32x4*>(smem + rt * kRowBytes + ((q ^ (rt % kSwz)) * 16));
+    if (m0 + rt < up) *reinterpret_cast<u32x4*>(dz + (m0 + rt) * ld + n0 + 8 * q) = v;
+  }
+}
+
+// dH's sums over part blockIdx.y of a piece: acc = dz W, written or added to the part's sums.
+// Where the piece ends inside a stage of 64 rows, `tail` is that stage with zeros behind it (dz has
+// zeros there, but what lies behind the weights is not the caller's to read).
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(kMfmaThreads, 1) void lce_dh_kernel(
+    const uint16_t* __restrict__ dz, int64_t ld, const uint16_t* __restrict__ weight,
+    const uint16_t* __restrict__ tail, int width, int64_t piece, const Meta* __restrict__ meta, float* __restrict__ out, int64_t part_stride,
+    int stages_per_part, bool add, int tiles_n) {
+  using S = LpAnyShape<BM, BN, Along::kAlongK, Along::kAcrossK>;
+  constexpr int MT = S::MT, NT = S::NT;
+  __shared__ __attribute__((aligned(1024))) char smem[S::kLdsBytes];
+  const int n = __builtin_amdgcn_readfirstlane(meta->rows);
+  int tm, tn;
+  if (!tile_of_rows<BM>(n, tiles_n, tm, tn)) return;
+  const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+  const int all = static_cast<int>((piece + 63) / 64);
+  const int first = blockIdx.y * stages_per_part;
+  const int stages = all - first < stages_per_part ? all - first : stages_per_part;
+  if (stages <= 0) return;
+  const LpOperand A{dz, ld, n > 0 ? n : 1};
+  const LpOperand B{weight, width, width, tail, piece % 64 ? all - 1 : -1};
+  f32x4 acc[MT][NT];
+  lp_any_loop<T, BM, BN, Along::kAlongK, Along::kAcrossK>(acc, smem, A, B, m0, n0, first, stages);
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
+  out += blockIdx.y * part_stride;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t row = m0 + wm * (BM / 2) + 16 * i + r16;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int64_t col = n0 + wn * (BN / 2) + 16 * j + 4 * g;
+      if (row < n && col < width) {
+        f32x4* p = reinterpret_cast<f32x4*>(out + row * width + col);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc_get(acc[i][j][e]);
+        if (add) v += *p;
+        *p = v;
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// dH from its parts' sums, the factor taken out; zeros for rows without a target.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void lce_dh_store_kernel(
+    const float* __restrict__ sums, int64_t part_stride, int parts, const int* __restrict__ rank,
+    const Meta* __restrict__ meta, T* __restrict__ dhidden, int rows, int cols, int width) {
+  const float unfactor = meta->unfactor;
+  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    const int k = rank[r];
+    for (int c = 8 * threadIdx.x; c < cols; c += 8 * kThreads) {
+      float v[8] = {};
+      if (k >= 0) {
+        const float* p = sums + static_cast<int64_t>(k) * width + c;
+        for (int s = 0; s < parts; ++s, p += part_stride) {
+          const f32x4 a = *reinterpret_cast<const f32x4*>(p);
+          const f32x4 b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] += a[e];
+            v[4 + e] += b[e];
+          }
+        }
+      }
+      VecT16<T> o;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(v[e] * unfactor);
+      T* to = dhidden + static_cast<int64_t>(r) * cols + c;
+      if (c + 8 <= cols) *reinterpret_cast<VecT16<T>*>(to) = o;
+      else store_part<T>(to, o, cols - c);
+    }
+  }
+}
+
+// dW's rows of a piece: dz^T H, the factor taken out.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(kMfmaThreads, 1) void lce_dw_kernel(
+    const uint16_t* __restrict__ dz, int64_t ld, const uint16_t* __restrict__ hidden, int width,
+    const Meta* __restrict__ meta, T* __restrict__ dweight, int64_t piece, int cols, int tiles_m,
+    int tiles_n) {
+  using S = LpAnyShape<BM, BN, Along::kAcrossK, Along::kAcrossK>;
+  using O = LpOut<T>;
+  constexpr int MT = S::MT, NT = S::NT, WM = BM / 2, WN = BN / 2;
+  __shared__ __attribute__((aligned(1024))) char smem[S::kLdsBytes];
+  int tm, tn;
+  mfma_tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+  const int n = __builtin_amdgcn_readfirstlane(meta->rows), stages = n > 0 ? (n + 63) / 64 : 1;
+  const LpOperand A{dz, ld, ld};
+  const LpOperand B{hidden, width, width};
+  f32x4 acc[MT][NT];
+  lp_any_loop<T, BM, BN, Along::kAcrossK, Along::kAcrossK>(acc, smem, A, B, m0, n0, 0, stages);
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
+  const float unfactor = meta->unfactor;
+  struct alignas(8) Quad { T v[4]; };
+  constexpr int kRowBytes = BN * 2, kChunks = kRowBytes / 16, kSwz = kChunks < 32 ? kChunks : 32;
+  __syncthreads();
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int rt = wm * WM + 16 * i + r16;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      Quad o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o.v[e] = O::from_f32(unfactor * acc_get(acc[i][j][e]));
+      const int col = wn * WN + 16 * j + 4 * g;
+      *reinterpret_cast<Quad*>(smem + rt * kRowBytes + (((col / 8) ^ (rt % kSwz)) * 16) +
+                               (col % 8) * 2) = o;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();
+  constexpr int kRowsPerPass = kMfmaThreads / kChunks;
+  const int q = threadIdx.x % kChunks;
+  const int64_t col = n0 + 8 * q;
+#pragma unroll 4
+  for (int r0 = 0; r0 < BM; r0 += kRowsPerPass) {
+    const int rt = r0 + threadIdx.x / kChunks;
+    const u32x4 v =
+        *reinterpret_cast<const u32x4*>(smem + rt * kRowBytes + ((q ^ (rt % kSwz)) * 16));
+    if (m0 + rt >= piece) continue;
+    T* to = dweight + (m0 + rt) * cols + col;
+    if (col + 8 <= cols) {
+      *reinterpret_cast<u32x4_a2*>(to) = v;
+    } else {
+      const VecT16<T> w = __builtin_bit_cast(VecT16<T>, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < cols) to[e] = w[e];
+    }
+  }
+}
+
+// No rows: the weights have no gradient.
+__global__ __launch_bounds__(kThreads) void lce_zero_kernel(uint16_t* __restrict__ p, int64_t n) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * kThreads)
+    p[i] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// Plans: tiles, pieces and the workspace, by the extents alone
+// ---------------------------------------------------------------------------
+constexpr int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
+constexpr int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+constexpr int64_t kPieceAlign = 256;
+constexpr int64_t kPieceValues = int64_t{1} << 26;     // of dz, and of a padded piece of W
+
+enum class Tile { k64x128, k128, k256 };
+
+// 256 x 256 where such tiles are most of the CUs' or more; 64 rows at 64 x 128.
+Tile tile_of(int64_t rows, int64_t cols) {
+  if (rows <= 64) return Tile::k64x128;
+  if (rows > 128 && ceil_div(rows, 256) * ceil_div(cols, 256) >= 192) return Tile::k256;
+  return Tile::k128;
+}
+int tile_rows(Tile t) { return t == Tile::k64x128 ? 64 : t == Tile::k128 ? 128 : 256; }
+int tile_cols(Tile t) { return t == Tile::k256 ? 256 : 128; }
+
+struct Plan {
+  int64_t rows, vocab, dim;
+  int64_t width;             // dim, a multiple of 64
+  int64_t up;                // rows, a multiple of 64
+  bool pad;                  // the weights need a padded copy
+  int64_t piece, pieces;     // rows of W at once
+  Tile tile;                 // of the logits
+  int64_t at;                // bytes of workspace so far
+
+  Plan(int64_t r, int64_t v, int64_t d, bool backward) : rows(r), vocab(v), dim(d), at(0) {
+    width = round_up(d, 64);
+    up = round_up(r, 64);
+    pad = d % 64 != 0;
+    int64_t most = round_up(v, kPieceAlign);
+    auto limit = [&](int64_t per_row) {
+      int64_t m = kPieceValues / per_row / kPieceAlign * kPieceAlign;
+      if (m < kPieceAlign) m = kPieceAlign;
+      if (m < most) most = m;
+    };
+    if (backward) limit(up);
+    if (pad) limit(width);
+    piece = round_up(ceil_div(v, ceil_div(v, most)), kPieceAlign);
+    pieces = ceil_div(v, piece);
+    tile = tile_of(r, backward ? (piece < v ? piece : v) : v);
+  }
+  int64_t take(int64_t bytes) {
+    const int64_t from = at;
+    at += round_up(bytes, 256);
+    return from;
+  }
+};
+
+struct RowsAt {
+  int64_t meta, from, rank, target, lse2, cp, ct, hidden, weight;
+  RowsAt(Plan& p, bool backward) {
+    meta = p.take(sizeof(Meta));
+    from = p.take(4 * p.up);
+    rank = p.take(4 * p.up);
+    target = p.take(4 * p.up);
+    lse2 = cp = ct = 0;
+    if (backward) {
+      lse2 = p.take(4 * p.up);
+      cp = p.take(4 * p.up);
+      ct = p.take(4 * p.up);
+    }
+    hidden = p.take(2 * p.up * p.width);
+    // A padded piece of the weights, or the last stage of 64 of their rows.
+    weight = p.pad ? p.take(2 * p.piece * p.width)
+             : backward && p.vocab % 64 ? p.take(2 * 64 * p.width) : 0;
+  }
+  Rows rows(char* ws) const {
+    return {reinterpret_cast<Meta*>(ws + meta),     reinterpret_cast<int*>(ws + from),
+            reinterpret_cast<int*>(ws + rank),      reinterpret_cast<int*>(ws + target),
+            reinterpret_cast<float*>(ws + lse2),    reinterpret_cast<float*>(ws + cp),
+            reinterpret_cast<float*>(ws + ct)};
+  }
+};
+
+struct FwdPlan : Plan {
+  RowsAt r;
+  int64_t stride, parts, largest, sums, at_target;
+  FwdPlan(int64_t rows, int64_t vocab, int64_t dim) : Plan(rows, vocab, dim, false), r(*this, false) {
+    stride = up;
+    parts = 2 * ceil_div(vocab, tile_cols(tile));
+    largest = take(4 * parts * stride);
+    sums = take(4 * parts * stride);
+    at_target = take(4 * up);
+  }
+};
+
+struct BwdPlan : Plan {
+  RowsAt r;
+  Tile dh_tile, dw_tile;
+  int64_t dz, ld, parts, stages_per_part, dh, part_stride;
+  BwdPlan(int64_t rows, int64_t vocab, int64_t dim) : Plan(rows, vocab, dim, true), r(*this, true) {
+    ld = piece;
+    dz = take(2 * up * ld);
+    dh_tile = tile_of(rows, dim);
+    // Few tiles of dH share a piece's stages: up to two workgroups a CU, at least 8 stages each.
+    const int64_t tiles = ceil_div(rows, tile_rows(dh_tile)) * ceil_div(dim, tile_cols(dh_tile));
+    const int64_t stages = ceil_div(piece < vocab ? piece : vocab, 64);
+    parts = (dh_tile == Tile::k256 ? 256 : 512) / tiles;
+    if (parts > 16) parts = 16;
+    if (parts > ceil_div(stages, 8)) parts = ceil_div(stages, 8);
+    if (parts < 1) parts = 1;
+    stages_per_part = ceil_div(stages, parts);
+    parts = ceil_div(stages, stages_per_part);
+    part_stride = up * width;
+    dh = take(4 * parts * part_stride);
+    dw_tile = rows > 128 && ceil_div(piece, 256) * ceil_div(dim, 256) >= 192 ? Tile::k256 : Tile::k128;
+  }
+};
+
+// f(std::integral_constant<int, BM>, BN) for a tile.
+template <class F> int with_tile(Tile t, F f) {
+  using I64 = std::integral_constant<int, 64>;
+  using I128 = std::integral_constant<int, 128>;
+  using I256 = std::integral_constant<int, 256>;
+  if (t == Tile::k64x128) return f(I64{}, I128{});
+  if (t == Tile::k128) return f(I128{}, I128{});
+  return f(I256{}, I256{});
+}
+
+int launch_pack(const void* x, const int* from, const Meta* meta, void* to, int64_t given,
+                int64_t rows, int64_t cols, int64_t width, hipStream_t s) {
+  const int64_t most = 65536;
+  lce_pack_kernel<<<static_cast<unsigned>(rows < most ? rows : most), kThreads, 0, s>>>(
+      static_cast<const uint16_t*>(x), from, meta, static_cast<uint16_t*>(to), given,
+      rows, static_cast<int>(cols), static_cast<int>(width));
+  MCKE_LAUNCH_CHECK("lce_pack_kernel");
+  return ok();
+}
+
+// Calls f(piece's rows of W (`width` apart), its first row, how many) for each piece.
+template <class F>
+int for_pieces(const Plan& p, const RowsAt& r, const void* weight, char* ws, hipStream_t s, F f) {
+  for (int64_t i = 0; i < p.pieces; ++i) {
+    const int64_t first = i * p.piece, n = p.vocab - first < p.piece ? p.vocab - first : p.piece;
+    const uint16_t* w = static_cast<const uint16_t*>(weight) + first * p.dim;
+    if (p.pad) {
+      if (int rc = launch_pack(w, nullptr, nullptr, ws + r.weight, n, round_up(n, 64),
+                               p.dim, p.width, s)) return rc;
+      w = reinterpret_cast<const uint16_t*>(ws + r.weight);
+    }
+    if (int rc = f(w, first, n)) return rc;
+  }
+  return ok();
+}
+
+template <typename T>
+int lce_forward(const void* hidden, const void* weight, const int64_t* targets, float* loss,
+                float* lse, const FwdPlan& p, float scale, char* ws, hipStream_t s) {
+  const Rows rows = p.r.rows(ws);
+  lce_rows_kernel<false><<<1, kPrepThreads, 0, s>>>(targets, nullptr, nullptr, nullptr,
+                                                    static_cast<int>(p.rows), p.vocab, scale, rows,
+                                                    loss, lse);
+  MCKE_LAUNCH_CHECK("lce_rows_kernel");
+  uint16_t* packed = reinterpret_cast<uint16_t*>(ws + p.r.hidden);
+  if (int rc = launch_pack(hidden, rows.from, rows.meta, packed, p.rows, p.up, p.dim, p.width,
+                           s)) return rc;
+  float* largest = reinterpret_cast<float*>(ws + p.largest);
+  float* sums = reinterpret_cast<float*>(ws + p.sums);
+  float* at_target = reinterpret_cast<float*>(ws + p.at_target);
+  const int rc = for_pieces(p, p.r, weight, ws, s, [&](const uint16_t* w, int64_t first, int64_t n) {
+    return with_tile(p.tile, [&](auto bm, auto bn) {
+      constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
+      const int64_t tiles_n = ceil_div(n, BN), tiles = ceil_div(p.rows, BM) * tiles_n;
+      lce_stats_kernel<T, BM, BN><<<static_cast<unsigned>(tiles), kMfmaThreads, 0, s>>>(
+          Logits{packed, w, static_cast<int>(p.width), n, first, scale}, rows.meta, rows.target,
+          largest, sums, at_target, p.stride, static_cast<int>(first / BN),
+          static_cast<int>(tiles_n));
+      MCKE_LAUNCH_CHECK("lce_stats_kernel");
+      return ok();
+    });
+  });
+  if (rc) return rc;
+  lce_join_kernel<<<static_cast<unsigned>(ceil_div(p.rows, kWave)), kJoinWaves * kWave, 0, s>>>(
+      largest, sums, at_target, rows.from, rows.target, rows.meta, loss, lse, p.stride,
+      static_cast<int>(p.parts), scale);
+  MCKE_LAUNCH_CHECK("lce_join_kernel");
+  return ok();
+}
+
+struct BwdArgs {
+  const void* hidden;
+  const void* weight;
+  const int64_t* targets;
+  const float* lse;
+  const float* dloss;
+  const float* dlse;
+  void* dhidden;
+  void* dweight;
+  float scale;
+  char* ws;
+  hipStream_t s;
+};
+
+template <typename T> int lce_backward(const BwdArgs& a, const BwdPlan& p) {
+  const Rows rows = p.r.rows(a.ws);
+  lce_rows_kernel<true><<<1, kPrepThreads, 0, a.s>>>(a.targets, a.lse, a.dloss, a.dlse,
+                                                     static_cast<int>(p.rows), p.vocab, a.scale,
+                                                     rows, nullptr, nullptr);
+  MCKE_LAUNCH_CHECK("lce_rows_kernel");
+  uint16_t* packed = reinterpret_cast<uint16_t*>(a.ws + p.r.hidden);
+  if (int rc = launch_pack(a.hidden, rows.from, rows.meta, packed, p.rows, p.up, p.dim,
+                           p.width, a.s))
+    return rc;
+  // Where the vocabulary ends inside a stage: padded pieces have their zeros, else a copy.
+  uint16_t* tail = nullptr;
+  const int64_t tail_rows = p.vocab % 64, tail_at = p.vocab - tail_rows;
+  if (tail_rows > 0) {
+    tail = reinterpret_cast<uint16_t*>(a.ws + p.r.weight);
+    if (p.pad)
+      tail += (tail_at - (p.pieces - 1) * p.piece) * p.width;
+    else if (int rc = launch_pack(static_cast<const uint16_t*>(a.weight) + tail_at * p.dim, nullptr,
+                                  nullptr, tail, tail_rows, 64, p.dim, p.width, a.s))
+      return rc;
+  }
+  uint16_t* dz = reinterpret_cast<uint16_t*>(a.ws + p.dz);
+  float* dh = reinterpret_cast<float*>(a.ws + p.dh);
+  const int width = static_cast<int>(p.width);
+  const int rc =
+      for_pieces(p, p.r, a.weight, a.ws, a.s, [&](const uint16_t* w, int64_t first, int64_t n) {
+        int rc = with_tile(p.tile, [&](auto bm, auto bn) {
+          constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
+          const int64_t tiles_n = ceil_div(n, BN), tiles = ceil_div(p.rows, BM) * tiles_n;
+          lce_dz_kernel<T, BM, BN><<<static_cast<unsigned>(tiles), kMfmaThreads, 0, a.s>>>(
+              Logits{packed, w, width, n, first, a.scale}, rows, dz, p.ld,
+              static_cast<int>(tiles_n));
+          MCKE_LAUNCH_CHECK("lce_dz_kernel");
+          return ok();
+        });
+        if (rc) return rc;
+        if (a.dhidden) {
+          rc = with_tile(p.dh_tile, [&](auto bm, auto bn) {
+            constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
+            const int64_t tiles_n = ceil_div(p.dim, BN), tiles = ceil_div(p.rows, BM) * tiles_n;
+            lce_dh_kernel<T, BM, BN>
+                <<<dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(p.parts)),
+                   kMfmaThreads, 0, a.s>>>(dz, p.ld, w, tail, width, n, rows.meta, dh, p.part_stride,
+                                           static_cast<int>(p.stages_per_part), first > 0,
+                                           static_cast<int>(tiles_n));
+            MCKE_LAUNCH_CHECK("lce_dh_kernel");
+            return ok();
+          });
+          if (rc) return rc;
+        }
+        if (!a.dweight) return ok();
+        auto dw = [&](auto bt) {
+          constexpr int B = decltype(bt)::value;
+          const int64_t tiles_m = ceil_div(n, B), tiles_n = ceil_div(p.dim, B);
+          lce_dw_kernel<T, B, B><<<static_cast<unsigned>(tiles_m * tiles_n), kMfmaThreads, 0, a.s>>>(
+              dz, p.ld, packed, width, rows.meta, static_cast<T*>(a.dweight) + first * p.dim, n,
+              static_cast<int>(p.dim), static_cast<int>(tiles_m), static_cast<int>(tiles_n));
+          MCKE_LAUNCH_CHECK("lce_dw_kernel");
+          return ok();
+        };
+        return p.dw_tile == Tile::k256 ? dw(std::integral_constant<int, 256>{})
+                                       : dw(std::integral_constant<int, 128>{});
+      });
+  if (rc) return rc;
+  if (!a.dhidden) return ok();
+  const int64_t blocks = p.rows < 65536 ? p.rows : 65536;
+  lce_dh_store_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, a.s>>>(
+      dh, p.part_stride, static_cast<int>(p.parts), rows.rank, rows.meta,
+      static_cast<T*>(a.dhidden), static_cast<int>(p.rows), static_cast<int>(p.dim), width);
+  MCKE_LAUNCH_CHECK("lce_dh_store_kernel");
+  return ok();
+}
+
+constexpr int64_t kMaxRows = int64_t{1} << 24, kMaxVocab = int64_t{1} << 24,
+                  kMaxDim = int64_t{1} << 16;
+
+bool extents_fit(int64_t rows, int64_t vocab, int64_t dim) {
+  return rows <= kMaxRows && vocab <= kMaxVocab && dim <= kMaxDim;
+}
+
+int check_args(const std::string& who, int dtype, int64_t rows, int64_t vocab, int64_t dim,
+               float scale) {
+  if (dtype != MCKE_DTYPE_F16 && dtype != MCKE_DTYPE_BF16)
+    return invalid(who + ": dtype must be MCKE_DTYPE_BF16 or MCKE_DTYPE_F16, got " +
+                   std::to_string(dtype));
+  if (rows < 0 || vocab < 0 || dim < 0) return invalid(who + ": negative extent");
+  if (!extents_fit(rows, vocab, dim))
+    return invalid(who + ": too large: rows and vocab up to 2^24, dim up to 2^16");
+  if (!(scale > 0.0f) || !std::isfinite(scale) || !std::isfinite(scale * kLog2e))
+    return invalid(who + ": scale must be finite and > 0");
+  const Tile t = tile_of(rows, vocab);
+  if (ceil_div(rows, tile_rows(t)) * ceil_div(vocab, tile_cols(t)) > int64_t{INT32_MAX} / kThreads)
+    return invalid(who + ": rows x vocab exceed the grid's 32-bit work size");
+  return ok();
+}
+
+int check_workspace(const std::string& who, const void* ws, size_t bytes, size_t need) {
+  if (!ws || bytes < need || !aligned(ws, 16))
+    return invalid(who + ": needs a 16-byte aligned workspace of " + std::to_string(need) +
+                   " bytes, got " + std::to_string(ws ? bytes : 0));
+  return ok();
+}
+
+int check_weight(const std::string& who, const void* weight, int64_t dim) {
+  if (dim % 64 == 0 && !aligned(weight, 16))
+    return invalid(who + ": weight must be 16-byte aligned where dim is a multiple of 64");
+  return ok();
+}
+
+}  // namespace
+}  // namespace mcke_amd
+
+using namespace mcke_amd;
+
+extern "C" {
+
+size_t mcke_linear_cross_entropy_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim) {
+  if (rows <= 0 || vocab <= 0 || dim <= 0 || !extents_fit(rows, vocab, dim)) return 0;
+  return static_cast<size_t>(FwdPlan(rows, vocab, dim).at);
+}
+
+size_t mcke_linear_cross_entropy_backward_workspace_bytes(int64_t rows, int64_t vocab,
+                                                          int64_t dim) {
+  if (rows <= 0 || vocab <= 0 || dim <= 0 || !extents_fit(rows, vocab, dim)) return 0;
+  return static_cast<size_t>(BwdPlan(rows, vocab, dim).at);
+}
+
+int mcke_launch_linear_cross_entropy(const void* hidden, const void* weight, const int64_t* targets,
+                                     float* loss, float* lse, int dtype, int64_t rows,
+                                     int64_t vocab, int64_t dim, float scale, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  const std::string who = "launch_linear_cross_entropy";
+  if (int rc = check_args(who, dtype, rows, vocab, dim, scale)) return rc;
+  if (rows == 0) return ok();
+  if (vocab == 0 || dim == 0) return invalid(who + ": vocab and dim must be > 0");
+  if (!hidden || !weight || !targets) return invalid(who + ": null pointer");
+  if (!loss && !lse) return invalid(who + ": no output is asked for");
+  if (!aligned(hidden, 2) || !aligned(weight, 2) || !aligned(targets, 8) || !aligned(loss, 4) ||
+      !aligned(lse, 4))
+    return invalid(who + ": a pointer is not aligned to its type");
+  if (int rc = check_weight(who, weight, dim)) return rc;
+  const FwdPlan p(rows, vocab, dim);
+  const size_t need = static_cast<size_t>(p.at);
+  if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
+  const uint64_t n = rows, h = 2 * n * dim, w = 2 * static_cast<uint64_t>(vocab) * dim;
+  const void* outs[] = {loss, lse, workspace};
+  const uint64_t out_bytes[] = {4 * n, 4 * n, need};
+  for (int i = 0; i < 3; ++i) {
+    bool bad = overlap(outs[i], out_bytes[i], hidden, h) ||
+               overlap(outs[i], out_bytes[i], weight, w) ||
+               overlap(outs[i], out_bytes[i], targets, 8 * n);
+    for (int j = 0; j < i; ++j) bad |= overlap(outs[i], out_bytes[i], outs[j], out_bytes[j]);
+    if (bad)
+      return invalid(who + ": an output or the workspace overlaps another operand, which violates "
+                           "the __restrict__ contract");
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  return dtype == MCKE_DTYPE_F16
+             ? lce_forward<_Float16>(hidden, weight, targets, loss, lse, p, scale, ws, s)
+             : lce_forward<__bf16>(hidden, weight, targets, loss, lse, p, scale, ws, s);
+}
+
+int mcke_launch_linear_cross_entropy_backward(const void* hidden, const void* weight,
+                                              const int64_t* targets, const float* lse,
+                                              const float* dloss, const float* dlse, void* dhidden,
+                                              void* dweight, int dtype, int64_t rows, int64_t vocab,
+                                              int64_t dim, float scale, void* workspace,
+                                              size_t workspace_bytes, void* stream) {
+  const std::string who = "launch_linear_cross_entropy_backward";
+  if (int rc = check_args(who, dtype, rows, vocab, dim, scale)) return rc;
+  if (!dhidden && !dweight) return invalid(who + ": no gradient is asked for");
+  if (vocab == 0 || dim == 0) {
+    if (rows == 0) return ok();
+    return invalid(who + ": vocab and dim must be > 0");
+  }
+  if (rows > 0 && (!hidden || !weight || !targets || !lse)) return invalid(who + ": null pointer");
+  if (rows > 0 && !dloss && !dlse) return invalid(who + ": no gradient is given");
+  if (!aligned(hidden, 2) || !aligned(weight, 2) || !aligned(dhidden, 2) || !aligned(dweight, 2) ||
+      !aligned(targets, 8) || !aligned(lse, 4) || !aligned(dloss, 4) || !aligned(dlse, 4))
+    return invalid(who + ": a pointer is not aligned to its type");
+  if (rows == 0) {
+    if (!dweight) return ok();
+    lce_zero_kernel<<<1024, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        static_cast<uint16_t*>(dweight), vocab * dim);
+    MCKE_LAUNCH_CHECK("lce_zero_kernel");
+    return ok();
+  }
+  if (int rc = check_weight(who, weight, dim)) return rc;
+  const BwdPlan p(rows, vocab, dim);
+  const size_t need = static_cast<size_t>(p.at);
+  if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
+  const uint64_t n = rows, h = 2 * n * dim, w = 2 * static_cast<uint64_t>(vocab) * dim;
+  const void* outs[] = {dhidden, dweight, workspace};
+  const uint64_t out_bytes[] = {h, w, need};
+  for (int i = 0; i < 3; ++i) {
+    bool bad = overlap(outs[i], out_bytes[i], hidden, h) ||
+               overlap(outs[i], out_bytes[i], weight, w) ||
+               overlap(outs[i], out_bytes[i], targets, 8 * n) ||
+               overlap(outs[i], out_bytes[i], lse, 4 * n) ||
+               overlap(outs[i], out_bytes[i], dloss, 4 * n) ||
+               overlap(outs[i], out_bytes[i], dlse, 4 * n);
+    for (int j = 0; j < i; ++j) bad |= overlap(outs[i], out_bytes[i], outs[j], out_bytes[j]);
+    if (bad)
+      return invalid(who + ": an output or the workspace overlaps another operand, which violates "
+                           "the __restrict__ contract");
+  }
+  const BwdArgs a{hidden,  weight,  targets, lse,   dloss, dlse, dhidden,
+                  dweight, scale,   static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
+  return dtype == MCKE_DTYPE_F16 ? lce_backward<_Float16>(a, p) : lce_backward<__bf16>(a, p);
+}
+
+}  // extern "C"
