@@ -31,75 +31,44 @@ constexpr int64_t kMaxCols = int64_t{1} << 24;
 int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
 
 // ---------------------------------------------------------------------------
-// Slopes.  Beyond |u| = 10 both GELUs' are 1, or less than 1e-20 from 0, so the argument is held
-// there, where no power of it and no exponential overflows; a NaN passes through.
+// Activations with their slopes.  Beyond |v| = 10 both GELUs' slopes are 1, or less than 1e-20 from
+// 0, so the argument of what needs it is held there, where no power of it and no exponential
+// overflows; a NaN passes through.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float held10(float v) {
   return v > 10.0f ? 10.0f : v < -10.0f ? -10.0f : v;
 }
 
-// d/dv [0.5 v (1 + tanh z)] with q = 0.5 (1 + tanh z) = 1 / (1 + exp(-2 z)), z = sqrt(2/pi)
-// (v + 0.044715 v^3):  q + v q (1 - q) 2 z'.  1 - q is e q with e = exp(-2 z): no cancellation
-// where q is near 1, and with v held e is below 2^127.
-__device__ __forceinline__ float gelu_tanh_slope(float v) {
-  constexpr float c1 = -2.30220818520f;     // -2 log2(e) sqrt(2/pi)
-  constexpr float c2 = -0.102943241596f;    // 0.044715 c1
-  constexpr float d1 = 1.5957691216057308f; // 2 sqrt(2/pi)
-  constexpr float d2 = 0.21406444881780073f;// 3 * 0.044715 d1
-  v = held10(v);
-  const float v2 = v * v;
-  const float e = __builtin_amdgcn_exp2f(v * __builtin_fmaf(c2, v2, c1));
-  const float q = __builtin_amdgcn_rcpf(1.0f + e);
-  return __builtin_fmaf(v * __builtin_fmaf(d2, v2, d1), (e * q) * q, q);
-}
-
-// Phi(v) + v phi(v), Phi through erfc of |v| (device_math.hpp).
-__device__ __forceinline__ float gelu_erf_slope(float v) {
-  constexpr float kLog2e = 1.4426950408889634f;
-  v = held10(v);
-  const float half = 0.5f * erfc_nonneg(__builtin_fabsf(v) * 0.70710678118654752440f);
-  const float cdf = v >= 0.0f ? 1.0f - half : half;
-  const float pdf = 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * v * v);
-  return __builtin_fmaf(v, pdf, cdf);
-}
-
-template <int ACT> __device__ __forceinline__ float act_slope(float v) {
-  if constexpr (ACT == kActNone) return v != v ? v : 1.0f;    // (a lost value has no gradient)
-  else if constexpr (ACT == kActRelu) return v > 0.0f ? 1.0f : 0.0f;
-  else if constexpr (ACT == kActGeluErf) return gelu_erf_slope(v);
-  else return gelu_tanh_slope(v);
-}
-
-// ---------------------------------------------------------------------------
-// A lane's vector of a row: columns j VE on.  Rows that are not whole vectors end in one that is
-// cut at `n` and goes element by element.
-// ---------------------------------------------------------------------------
-template <int VE> struct Bytes;
-template <> struct Bytes<4> {
-  typedef unsigned type __attribute__((aligned(1)));
-};
-template <> struct Bytes<8> {
-  typedef unsigned type __attribute__((ext_vector_type(2), aligned(1)));
-};
-
-template <typename T>
-__device__ __forceinline__ void load_row(float (&v)[kVecElems<T>], const T* __restrict__ p, int n) {
-  constexpr int VE = kVecElems<T>;
-  VecT16<T> w;
-  if (n == VE) w = load_stream<T>(p);
-  else w = load_part<T>(p, n, 0.0f);
-#pragma unroll
-  for (int e = 0; e < VE; ++e) v[e] = static_cast<float>(w[e]);
-}
-
-template <typename T>
-__device__ __forceinline__ void store_row(T* __restrict__ p, const float (&v)[kVecElems<T>], int n) {
-  constexpr int VE = kVecElems<T>;
-  VecT16<T> w;
-#pragma unroll
-  for (int e = 0; e < VE; ++e) w[e] = static_cast<T>(v[e]);
-  if (n == VE) store_stream<T>(p, w);
-  else store_part<T>(p, w, n);
+template <int ACT> __device__ __forceinline__ void act_and_slope(float v, float& y, float& slope) {
+  if constexpr (ACT == kActNone) {
+    y = v;
+    slope = v != v ? v : 1.0f;          // (a lost value has no gradient)
+  } else if constexpr (ACT == kActRelu) {
+    y = v > 0.0f ? v : 0.0f;
+    slope = v > 0.0f ? 1.0f : 0.0f;
+  } else if constexpr (ACT == kActGeluErf) {
+    // Phi through erfc of |v| (device_math.hpp); slope = Phi(v) + v phi(v).
+    constexpr float kLog2e = 1.4426950408889634f;
+    const float half = 0.5f * erfc_nonneg(__builtin_fabsf(v) * 0.70710678118654752440f);
+    const float h = held10(v);
+    const float pdf = 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * h * h);
+    const float cdf = v >= 0.0f ? 1.0f - half : half;
+    y = v * cdf;
+    slope = __builtin_fmaf(h, pdf, cdf);
+  } else {
+    // q = 0.5 (1 + tanh z) = 1 / (1 + e), e = exp(-2 z), z = sqrt(2/pi) (v + 0.044715 v^3):
+    // y = v q, slope = q + v q (1 - q) 2 z'.  1 - q is e q: no cancellation where q is near 1, and
+    // with v held e is below 2^127.
+    constexpr float c1 = -2.30220818520f;     // -2 log2(e) sqrt(2/pi)
+    constexpr float c2 = -0.102943241596f;    // 0.044715 c1
+    constexpr float d1 = 1.5957691216057308f; // 2 sqrt(2/pi)
+    constexpr float d2 = 0.21406444881780073f;// 3 * 0.044715 d1
+    const float h = held10(v), h2 = h * h;
+    const float e = __builtin_amdgcn_exp2f(h * __builtin_fmaf(c2, h2, c1));
+    const float q = __builtin_amdgcn_rcpf(1.0f + e);
+    y = v * q;
+    slope = __builtin_fmaf(h * __builtin_fmaf(d2, h2, d1), (e * q) * q, q);
+  }
 }
 
 struct Layout {
@@ -109,75 +78,80 @@ struct Layout {
   int bias_dtype;
 };
 
-template <int VE>
-__device__ __forceinline__ void load_bias(float (&b)[VE], const Layout& l, int c, int n) {
-#pragma unroll
-  for (int e = 0; e < VE; ++e)
-    b[e] = l.bias && e < n ? load_elem(l.bias, l.bias_dtype, c + e) : -0.0f;
-}
-
 // ---------------------------------------------------------------------------
-// Forward.  32 columns are 4 (16-bit types) or 8 neighbouring lanes.
+// Forward.  32 columns are 4 (16-bit types) or 8 neighbouring lanes.  A row's last vector is
+// moved back to end with it (WHOLE false): its first values are the lane's before it, and count
+// and are saved there.
 // ---------------------------------------------------------------------------
-template <typename T, int ACT>
+template <typename T, int ACT, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void checkpoint8_fwd_kernel(
     const T* __restrict__ x, T* __restrict__ y, uint8_t* __restrict__ codes,
     uint8_t* __restrict__ exponents, Layout l) {
   constexpr int VE = kVecElems<T>, LB = kBlock / VE;
-  const int t = threadIdx.x & ((1 << l.tpr_log2) - 1);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads >> l.tpr_log2);
-  const int64_t c64 = ((static_cast<int64_t>(blockIdx.y) << l.tpr_log2) + t) * VE;
+  const int t = threadIdx.x & ((1 << l.tpr_log2) - 1), group = threadIdx.x >> l.tpr_log2;
+  const int groups = kThreads >> l.tpr_log2;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * groups;
+  const int64_t j = (static_cast<int64_t>(blockIdx.y) << l.tpr_log2) + t;
   // Lanes behind the row hold zeros: their block's exponent wants them.
-  const int c = c64 < l.cols ? static_cast<int>(c64) : l.cols;
-  const int n = l.cols - c < VE ? l.cols - c : VE;
+  const Cols<VE, WHOLE> at(j, l.cols);
   float b[VE];
-  load_bias<VE>(b, l, c, n);
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * (kThreads >> l.tpr_log2) +
-                   (threadIdx.x >> l.tpr_log2);
-       r < l.rows; r += step) {
-    float v[VE], u[VE];
-    load_row<T>(v, x + r * l.cols + c, n);
-    float most = 0.0f;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) b[e] = -0.0f;
+  if (l.bias && at.any) {
+    if (l.bias_dtype == MCKE_DTYPE_F32) at.load(b, static_cast<const float*>(l.bias));
+    else at.load(b, static_cast<const T*>(l.bias));
+  }
+
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * groups + group; r < l.rows; r += step) {
+    float xv[VE], u[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) xv[e] = 0.0f;
+    if (at.any) at.load_stream(xv, x + r * l.cols);
+    float most = 0.0f, any = 0.0f;                // `any`: not finite where a value is not
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
-      u[e] = v[e] + b[e];
-      const float a = __builtin_fabsf(u[e]);
-      most = fmaxf(most, a < __builtin_inff() && e < n ? a : 0.0f);
+      u[e] = xv[e] + b[e];
+      any += u[e];
+      if (WHOLE || (e >= at.skip && e < at.n)) most = fmaxf(most, __builtin_fabsf(u[e]));
+    }
+    if (__ballot(!(__builtin_fabsf(any) < __builtin_inff()))) {
+      most = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float a = __builtin_fabsf(u[e]);
+        if (!(a < __builtin_inff()))
+          u[e] = __builtin_nanf("");
+        else if (WHOLE || (e >= at.skip && e < at.n))
+          most = fmaxf(most, a);
+      }
     }
     most = wave_max<LB>(most);
     const int bits = __builtin_bit_cast(int, most);
-    int ex = (bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0);   // 1.75: 448 = 1.75 * 2^8
+    // 1.75: 448 = 1.75 * 2^8.
+    int ex = (bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0);
     ex = ex < 1 ? 1 : ex;
     const float inv = __builtin_bit_cast(float, (254 - ex) << 23);
-    int packed[VE / 4];
+    typedef unsigned Packed __attribute__((ext_vector_type(VE / 4), aligned(1)));
+    Packed packed;
 #pragma unroll
     for (int q = 0; q < VE / 4; ++q) {
-      float s[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float w = u[4 * q + e];
-        s[e] = __builtin_fabsf(w) < __builtin_inff() ? w * inv : __builtin_nanf("");
-      }
-      int p = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
-      packed[q] = __builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], p, true);
+      const int p = __builtin_amdgcn_cvt_pk_fp8_f32(u[4 * q] * inv, u[4 * q + 1] * inv, 0, false);
+      packed[q] = static_cast<unsigned>(
+          __builtin_amdgcn_cvt_pk_fp8_f32(u[4 * q + 2] * inv, u[4 * q + 3] * inv, p, true));
     }
-    uint8_t* to = codes + r * l.cols + c;
-    if (n == VE) {
-      using B = typename Bytes<VE>::type;
-      if constexpr (VE == 4) *reinterpret_cast<B*>(to) = static_cast<unsigned>(packed[0]);
-      else *reinterpret_cast<B*>(to) = B{static_cast<unsigned>(packed[0]),
-                                         static_cast<unsigned>(packed[VE / 4 - 1])};
+    if (!at.any) continue;
+    uint8_t* to = codes + r * l.cols + at.c;
+    if (WHOLE || (at.skip == 0 && at.n == VE)) {
+      *reinterpret_cast<Packed*>(to) = packed;
     } else {
-#pragma unroll
-      for (int e = 0; e < VE; ++e)
-        if (e < n) to[e] = static_cast<uint8_t>(packed[e / 4] >> (8 * (e % 4)));
+      at.template each<false>(
+          [&](int e) { to[e] = static_cast<uint8_t>(packed[e / 4] >> (8 * (e % 4))); });
     }
-    if (t % LB == 0 && n > 0)
-      exponents[r * l.blocks + c / kBlock] = static_cast<uint8_t>(ex);
+    if (t % LB == 0) exponents[r * l.blocks + j / LB] = static_cast<uint8_t>(ex);
     if (y) {
 #pragma unroll
-      for (int e = 0; e < VE; ++e) v[e] = act_xb<ACT>(v[e], b[e]);
-      store_row<T>(y + r * l.cols + c, v, n);
+      for (int e = 0; e < VE; ++e) u[e] = act_xb<ACT>(xv[e], b[e]);
+      at.store_stream_again(y + r * l.cols, u);
     }
   }
 }
@@ -186,67 +160,80 @@ __global__ __launch_bounds__(kThreads) void checkpoint8_fwd_kernel(
 // Backward.  Workgroup (p, columns) walks the rows p per, p per + 1, .. of its part; a lane
 // keeps its columns' sums of dx, and the workgroup's are row p of the workspace.
 // ---------------------------------------------------------------------------
-template <typename T, int ACT>
+template <typename T, int ACT, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void checkpoint8_bwd_kernel(
     const T* __restrict__ dy, const uint8_t* __restrict__ codes,
     const uint8_t* __restrict__ exponents, T* __restrict__ dx, T* __restrict__ y,
     float* __restrict__ partials, Layout l, int64_t per) {
   constexpr int VE = kVecElems<T>;
+  constexpr int U = 4;                            // rows whose loads are in flight
   __shared__ float fold[kThreads * VE];
   const int tpr = 1 << l.tpr_log2, groups = kThreads >> l.tpr_log2;
   const int t = threadIdx.x & (tpr - 1), g = threadIdx.x >> l.tpr_log2;
-  const int64_t c64 = ((static_cast<int64_t>(blockIdx.y) << l.tpr_log2) + t) * VE;
-  const int c = c64 < l.cols ? static_cast<int>(c64) : l.cols;
-  const int n = l.cols - c < VE ? l.cols - c : VE;
+  const Cols<VE, WHOLE> at((static_cast<int64_t>(blockIdx.y) << l.tpr_log2) + t, l.cols);
   const int64_t r0 = blockIdx.x * per, r1 = r0 + per < l.rows ? r0 + per : l.rows;
+  // A vector that is moved back may begin in the block before: its values from `turn` on are the
+  // second block's.
+  const int block = at.c / kBlock;
+  [[maybe_unused]] const int turn = kBlock - at.c % kBlock;
+  [[maybe_unused]] const int block2 = WHOLE ? block : (at.c + at.n - 1) / kBlock;
   float sum[VE];
 #pragma unroll
   for (int e = 0; e < VE; ++e) sum[e] = 0.0f;
-  if (n > 0) {
-#pragma unroll 2
-    for (int64_t r = r0 + g; r < r1; r += groups) {
-      const uint8_t* from = codes + r * l.cols + c;
-      int packed[VE / 4];
-      if (n == VE) {
-        using B = typename Bytes<VE>::type;
-        const B w = *reinterpret_cast<const B*>(from);
-        if constexpr (VE == 4) {
-          packed[0] = static_cast<int>(w);
+  if (at.any) {
+    for (int64_t rb = r0 + g; rb < r1; rb += U * groups) {
+      typedef unsigned Packed __attribute__((ext_vector_type(VE / 4), aligned(1)));
+      Packed packed[U];
+      int ex[U], ex2[U];
+      PackT<T, VE> d[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        // (Past the part its last row again, for nothing.)
+        const int64_t r = rb + k * groups < r1 ? rb + k * groups : rb;
+        const uint8_t* from = codes + r * l.cols + at.c;
+        if (WHOLE || at.n == VE) {
+          packed[k] = *reinterpret_cast<const Packed*>(from);
         } else {
-          packed[0] = static_cast<int>(w[0]);
-          packed[1] = static_cast<int>(w[1]);
+          packed[k] = Packed{};
+          at.template each<true>([&](int e) {
+            packed[k][e / 4] |= static_cast<unsigned>(from[e]) << (8 * (e % 4));
+          });
         }
-      } else {
-#pragma unroll
-        for (int q = 0; q < VE / 4; ++q) packed[q] = 0;
-#pragma unroll
-        for (int e = 0; e < VE; ++e)
-          if (e < n) packed[e / 4] |= from[e] << (8 * (e % 4));
+        ex[k] = exponents[r * l.blocks + block];
+        ex2[k] = WHOLE ? ex[k] : exponents[r * l.blocks + block2];
+        if (dy) d[k] = at.load_raw(dy + r * l.cols);
       }
-      const int ex = exponents[r * l.blocks + c / kBlock];
-      const float scale = __builtin_bit_cast(float, ex << 23);
-      float d[VE];
-      if (dy) load_row<T>(d, dy + r * l.cols + c, n);
-      float u[VE];
 #pragma unroll
-      for (int q = 0; q < VE / 4; ++q) {
-        u[4 * q + 0] = scale * __builtin_amdgcn_cvt_f32_fp8(packed[q], 0);
-        u[4 * q + 1] = scale * __builtin_amdgcn_cvt_f32_fp8(packed[q], 1);
-        u[4 * q + 2] = scale * __builtin_amdgcn_cvt_f32_fp8(packed[q], 2);
-        u[4 * q + 3] = scale * __builtin_amdgcn_cvt_f32_fp8(packed[q], 3);
-      }
-      if (dy) {
+      for (int k = 0; k < U; ++k) {
+        const int64_t r = rb + k * groups;
+        if (r >= r1) break;
+        float u[VE], s[VE], v[VE];
+#pragma unroll
+        for (int q = 0; q < VE / 4; ++q) {
+          const int p = static_cast<int>(packed[k][q]);
+          u[4 * q + 0] = __builtin_amdgcn_cvt_f32_fp8(p, 0);
+          u[4 * q + 1] = __builtin_amdgcn_cvt_f32_fp8(p, 1);
+          u[4 * q + 2] = __builtin_amdgcn_cvt_f32_fp8(p, 2);
+          u[4 * q + 3] = __builtin_amdgcn_cvt_f32_fp8(p, 3);
+        }
+        const float scale = __builtin_bit_cast(float, ex[k] << 23);
+        const float scale2 = __builtin_bit_cast(float, ex2[k] << 23);
+        int second = turn;
+        if constexpr (!WHOLE) asm("" : "+v"(second));   // (kept as masks, these fill the scalar file)
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-          d[e] *= act_slope<ACT>(u[e]);
-          sum[e] += d[e];
+          u[e] *= WHOLE || e < second ? scale : scale2;
+          act_and_slope<ACT>(u[e], v[e], s[e]);
         }
-        if (dx) store_row<T>(dx + r * l.cols + c, d, n);
-      }
-      if (y) {
+        if (dy) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) u[e] = act_xb<ACT>(u[e], -0.0f);
-        store_row<T>(y + r * l.cols + c, u, n);
+          for (int e = 0; e < VE; ++e) {
+            s[e] *= static_cast<float>(d[k][e]);
+            sum[e] += s[e];
+          }
+          if (dx) at.store_stream_again(dx + r * l.cols, s);
+        }
+        if (y) at.store_stream_again(y + r * l.cols, v);
       }
     }
   }
@@ -261,30 +248,31 @@ __global__ __launch_bounds__(kThreads) void checkpoint8_bwd_kernel(
 #pragma unroll
       for (int e = 0; e < VE; ++e) sum[e] += fold[e * kThreads + k * tpr + t];
   }
-  float* to = partials + static_cast<int64_t>(blockIdx.x) * l.cols + c;
-#pragma unroll
-  for (int e = 0; e < VE; ++e)
-    if (e < n) to[e] = sum[e];
+  if (at.any) at.store(partials + static_cast<int64_t>(blockIdx.x) * l.cols, sum);
 }
 
-// dbias from the workgroups' sums: kWays lanes a column, each every kWays-th part, then a tree.
-constexpr int kFoldCols = 32, kFoldWays = 8;
+// dbias from the workgroups' sums: kFoldWays lanes a column, each every kFoldWays-th part, then a
+// tree.
+constexpr int kFoldCols = 32, kFoldWays = 32;
 
 __global__ __launch_bounds__(kFoldCols * kFoldWays) void checkpoint8_fold_kernel(
     const float* __restrict__ partials, void* __restrict__ dbias, int dtype, int64_t cols,
     int parts) {
-  __shared__ float lds[kFoldWays][kFoldCols];
+  __shared__ float lds[kFoldWays][kFoldCols + 1];
   const int lc = threadIdx.x % kFoldCols, way = threadIdx.x / kFoldCols;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kFoldCols + lc;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * kFoldCols;
   float s = 0.0f;
-  if (c < cols) {
+  if (c0 + lc < cols) {
 #pragma unroll 8
-    for (int p = way; p < parts; p += kFoldWays) s += partials[static_cast<int64_t>(p) * cols + c];
+    for (int p = way; p < parts; p += kFoldWays)
+      s += partials[static_cast<int64_t>(p) * cols + c0 + lc];
   }
   lds[way][lc] = s;
   __syncthreads();
-  if (way > 0 || c >= cols) return;
-  for (int w = 1; w < kFoldWays; ++w) s += lds[w][lc];
+  // Column `way` of the workgroup's, its lanes' sums as a tree.
+  s = wave_sum<kFoldWays>(lds[lc][way]);
+  const int64_t c = c0 + way;
+  if (lc > 0 || c >= cols) return;
   if (dtype == MCKE_DTYPE_F32) static_cast<float*>(dbias)[c] = s;
   else if (dtype == MCKE_DTYPE_F16) static_cast<_Float16*>(dbias)[c] = static_cast<_Float16>(s);
   else static_cast<__bf16*>(dbias)[c] = static_cast<__bf16>(s);
@@ -300,13 +288,13 @@ int lanes_log2(int64_t cols, int ve) {
   return log2;
 }
 
+constexpr int64_t kParts = 1024;
+
 // Parts of the rows whose sums of dx are kept apart.  (Of rows and cols alone: the workspace is
 // sized without the type.)
 int64_t parts_of(int64_t rows, int64_t cols) {
-  const int64_t tiles = ceil_div(cols, 2048);
-  int64_t parts = ceil_div(1024, tiles);
-  if (parts > 256) parts = 256;
-  const int64_t some = ceil_div(rows, 4);
+  const int64_t tiles = ceil_div(cols, 2048), at_once = cols < 512 ? 2048 / cols : 4;
+  const int64_t parts = ceil_div(kParts, tiles), some = ceil_div(rows, at_once);
   return parts < some ? parts : some;
 }
 
@@ -376,9 +364,10 @@ int mcke_launch_bias_act_checkpoint8(const void* x, const void* bias, void* y, u
   const dim3 grid(static_cast<unsigned>(groups < most ? groups : most), static_cast<unsigned>(gy));
   return with_types(dtype, activation, [&](auto t, auto act) {
     using T = decltype(t);
-    checkpoint8_fwd_kernel<T, decltype(act)::value>
-        <<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            static_cast<const T*>(x), static_cast<T*>(y), codes, exponents, l);
+    auto* fn = cols % kVecElems<T> == 0 ? &checkpoint8_fwd_kernel<T, decltype(act)::value, true>
+                                        : &checkpoint8_fwd_kernel<T, decltype(act)::value, false>;
+    fn<<<grid, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        static_cast<const T*>(x), static_cast<T*>(y), codes, exponents, l);
     MCKE_LAUNCH_CHECK("checkpoint8_fwd_kernel");
     return ok();
   });
@@ -432,7 +421,9 @@ int mcke_launch_bias_act_checkpoint8_backward(const void* dy, const uint8_t* cod
     const void* grad = dx || dbias ? dy : nullptr;
     const int rc = with_types(dtype, activation, [&](auto t, auto act) {
       using T = decltype(t);
-      checkpoint8_bwd_kernel<T, decltype(act)::value><<<grid, kThreads, 0, s>>>(
+      auto* fn = cols % kVecElems<T> == 0 ? &checkpoint8_bwd_kernel<T, decltype(act)::value, true>
+                                          : &checkpoint8_bwd_kernel<T, decltype(act)::value, false>;
+      fn<<<grid, kThreads, 0, s>>>(
           static_cast<const T*>(grad), codes, exponents, static_cast<T*>(dx), static_cast<T*>(y),
           dbias ? static_cast<float*>(workspace) : nullptr, l, per);
       MCKE_LAUNCH_CHECK("checkpoint8_bwd_kernel");

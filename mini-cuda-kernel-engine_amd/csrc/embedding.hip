@@ -10,11 +10,13 @@
 // order.  So no sum depends on the order of atomics, and a token that is half of the batch (a
 // frequent word, a pad token) takes as many workgroups as any other half.
 //
-//   launch 1  sorts runs of tokens, each in one workgroup's LDS, beside workgroups that write the
-//             zeros of tokens that are not there: a table of 131072 x 4096 bf16 is 1 GB of them,
-//             which hides the sort
-//   (merges   eight runs at a time, where there is more than one)
-//   launch 2  sums by chunk      launch 3  sums of tokens that cross chunks
+//   order   up to 16384 tokens: each one's place counted.  More: runs of 1024 sorted, each in one
+//           workgroup, and merged four at a time
+//   sums    by chunk
+//   join    of the sums of tokens that cross chunks
+//
+// The zeros of tokens that are not there are written by more workgroups of the first launch, which
+// they hide: a table of 131072 x 4096 bf16 is 1 GB of them.
 //
 // All sums are fp32 and each value of dtable is rounded once.
 #include <hip/hip_runtime.h>
@@ -31,62 +33,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int64_t kMaxCols = int64_t{1} << 24;
-
-// N values at the alignment of one.
-template <typename T, int N> struct Pack {
-  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-};
-template <typename T, int N> using PackT = typename Pack<T, N>::type;
-
-template <typename T, int N>
-__device__ __forceinline__ void load_cols(float (&v)[N], const T* __restrict__ p) {
-  const PackT<T, N> w = *reinterpret_cast<const PackT<T, N>*>(p);
-#pragma unroll
-  for (int e = 0; e < N; ++e) v[e] = static_cast<float>(w[e]);
-}
-
-// A lane's N columns of a row: columns j N .. j N + N - 1.  In rows that are not whole vectors
-// (WHOLE false) the last one is moved back to end with the row, and its first `skip` columns are
-// its neighbour's too; a row shorter than a vector is one vector cut at `n`.
-template <int N, bool WHOLE> struct Cols {
-  int c, skip, n;
-  bool any;
-  __device__ __forceinline__ Cols(int64_t j, int cols) {
-    const int64_t first = j * N;
-    any = first < cols;
-    c = static_cast<int>(first);
-    skip = 0;
-    n = N;
-    if constexpr (!WHOLE) {
-      if (first + N > cols) {
-        c = cols > N ? cols - N : 0;
-        skip = static_cast<int>(first) - c;
-        n = cols < N ? cols : N;
-      }
-    }
-  }
-  template <typename T> __device__ __forceinline__ void load(float (&v)[N], const T* row) const {
-    if (WHOLE || n == N) {
-      load_cols<T, N>(v, row + c);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = e < n ? static_cast<float>(row[c + e]) : 0.0f;
-    }
-  }
-  // Columns that are this lane's alone, so that each is written once.
-  template <typename T> __device__ __forceinline__ void store(T* row, const float (&v)[N]) const {
-    if (WHOLE || (skip == 0 && n == N)) {
-      PackT<T, N> w;
-#pragma unroll
-      for (int e = 0; e < N; ++e) w[e] = static_cast<T>(v[e]);
-      *reinterpret_cast<PackT<T, N>*>(row + c) = w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (e >= skip && e < n) row[c + e] = static_cast<T>(v[e]);
-    }
-  }
-};
 
 // ---------------------------------------------------------------------------
 // Lookup.  2^tpr_log2 lanes a row, U vectors of the table's type a lane.
@@ -127,59 +73,123 @@ __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Sorted tokens.  A run of 1024 J tokens is sorted by one workgroup: least significant digit
-// first, up to nine bits a pass.  A wave holds 64 J consecutive positions, 64 to a register, so
-// that "earlier" is a lower register, then a lower lane.  A lane's rank among equal digits of
-// its register comes from ballots; the wave's counters, one a digit, give what came before.
-// Tokens outside 0 .. vocab - 1 have the key `vocab`: they sort behind all others and are left
-// out.
+// Tokens in order: `keys` and the positions `ids` they come from.  Tokens outside 0 .. vocab - 1
+// have the key `vocab`: they come behind all others and are left out.
 // ---------------------------------------------------------------------------
-constexpr int kSortThreads = 1024;
-constexpr int kSortWaves = kSortThreads / kWave;
+constexpr int kRun = 1024;
+constexpr int kSortWaves = kRun / kWave;
+
+__device__ __forceinline__ int key_of(const int64_t* __restrict__ tokens, int64_t i, int vocab) {
+  const int64_t token = tokens[i];
+  return static_cast<int>(token >= 0 && token < vocab ? token : vocab);
+}
+
+typedef unsigned u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// Zeros in `bytes` (an even number) at p (2-byte aligned), by `blocks` workgroups.  Each has one
+// piece of them: strided through by all, 1 GB took 260 us, in pieces 165.  (Over two launches 200:
+// each has to drain its stores.)
+struct Zeros {
+  char* p;
+  int64_t bytes;
+  __device__ __forceinline__ void fill(int64_t block, int64_t blocks) const {
+    const int64_t vecs = bytes / 16, per = (vecs + blocks - 1) / blocks;
+    const int64_t end = (block + 1) * per < vecs ? (block + 1) * per : vecs;
+    for (int64_t i = block * per + threadIdx.x; i < end; i += kRun)
+      __builtin_nontemporal_store(u32x4_a2{0u, 0u, 0u, 0u},
+                                  reinterpret_cast<u32x4_a2*>(p + 16 * i));
+    if (block == 0 && static_cast<int64_t>(threadIdx.x) < bytes % 16 / 2)
+      *reinterpret_cast<uint16_t*>(p + 16 * vecs + 2 * threadIdx.x) = 0;
+  }
+};
+
+// Up to kCount tokens.  A token's place is how many are smaller, and how many equal ones are
+// before it: a workgroup has 64 tokens, a lane each, and its waves deal out all of the keys in
+// chunks of 64 (in LDS; a chunk is compared with before, behind or at the workgroup's own).
+// 16384^2 comparisons are two operations each, 14 us over all CUs; sorted by one workgroup the
+// same took 24, in runs of 1024 and two merges LATER.  Workgroups from `blocks` on write zeros.
+constexpr int kCount = 16384;
+
+__global__ __launch_bounds__(kRun) void embed_count_kernel(const int64_t* __restrict__ tokens,
+                                                          int* __restrict__ keys,
+                                                          int* __restrict__ ids, int n, int vocab,
+                                                          int blocks, Zeros zeros) {
+  __shared__ __attribute__((aligned(16))) int all[kCount];
+  __shared__ int counts[kSortWaves][kWave];
+  const int block = blockIdx.x;
+  if (block >= blocks) {
+    zeros.fill(block - blocks, gridDim.x - blocks);
+    return;
+  }
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int chunks = (n + kWave - 1) / kWave;
+  // (INT32_MAX is below nothing: keys go up to 2^31 - 2.)
+#pragma unroll 16
+  for (int i = threadIdx.x; i < chunks * kWave; i += kRun)
+    all[i] = i < n ? key_of(tokens, i, vocab) : INT32_MAX;
+  __syncthreads();
+  const int mine = block * kWave + lane, key = all[mine];
+  int count = 0;
+  for (int c = wave; c < chunks; c += kSortWaves) {
+    if (c == block) {
+#pragma unroll 1
+      for (int j = 0; j < kWave; ++j) {
+        const int k = all[c * kWave + j];
+        count += k < key || (k == key && j < lane) ? 1 : 0;
+      }
+    } else {
+      const int below = c < block ? key : key - 1;
+#pragma unroll 4
+      for (int j = 0; j < kWave; j += 4) {
+        const i32x4 k = *reinterpret_cast<const i32x4*>(all + c * kWave + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) count += k[e] <= below ? 1 : 0;
+      }
+    }
+  }
+  counts[wave][lane] = count;
+  __syncthreads();
+  if (wave > 0 || mine >= n) return;
+  for (int w = 1; w < kSortWaves; ++w) count += counts[w][lane];
+  keys[count] = key;
+  ids[count] = mine;
+}
+
+// More tokens.  A run of 1024 is sorted by one workgroup, a token to a lane: least significant
+// digit first, up to nine bits a pass.  A lane's rank among equal digits of its wave comes from
+// ballots, and the wave's counters, one a digit, give where its waves' tokens of each digit begin.
 constexpr int kMaxDigit = 9;
 
-template <int J>
 __device__ __forceinline__ void sort_run(const int64_t* __restrict__ tokens, int* __restrict__ keys,
                                          int* __restrict__ ids, int64_t n, int vocab,
                                          int64_t base) {
-  __shared__ uint32_t skey[kSortThreads * J];
-  __shared__ uint16_t sid[kSortThreads * J];
+  __shared__ uint32_t skey[kRun];
+  __shared__ uint16_t sid[kRun];
   __shared__ uint32_t count[kSortWaves << kMaxDigit];
   __shared__ uint32_t totals[kSortWaves];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int at0 = wave * (kWave * J) + lane;
-
-  uint32_t key[J], id[J], rank[J];
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    id[j] = at0 + j * kWave;
-    const int64_t i = base + id[j];
-    const int64_t token = i < n ? tokens[i] : -1;
-    key[j] = static_cast<uint32_t>(token >= 0 && token < vocab ? token : vocab);
-  }
+  uint32_t id = threadIdx.x;
+  const int64_t i = base + id;
+  uint32_t key = static_cast<uint32_t>(i < n ? key_of(tokens, i, vocab) : vocab);
   const int bits = 32 - __builtin_clz(static_cast<unsigned>(vocab));
   const int passes = (bits + kMaxDigit - 1) / kMaxDigit;
   const int width = (bits + passes - 1) / passes, digits = 1 << width;
   for (int shift = 0; shift < bits; shift += width) {
-    for (int c = threadIdx.x; c < kSortWaves * digits; c += kSortThreads) count[c] = 0;
+    for (int c = threadIdx.x; c < kSortWaves * digits; c += kRun) count[c] = 0;
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const uint32_t d = (key[j] >> shift) & (digits - 1);
-      uint64_t same = ~uint64_t{0};
-      for (int b = 0; b < width; ++b) {
-        const uint64_t set = __ballot((d >> b) & 1);
-        same &= (d >> b) & 1 ? set : ~set;
-      }
-      const int before = __popcll(same & ((uint64_t{1} << lane) - 1));
-      uint32_t old = 0;
-      if (before == 0) old = atomicAdd(&count[wave * digits + d], __popcll(same));
-      rank[j] = __shfl(old, __builtin_ctzll(same)) + before;
+    const uint32_t d = (key >> shift) & (digits - 1);
+    uint64_t same = ~uint64_t{0};
+    for (int b = 0; b < width; ++b) {
+      const uint64_t set = __ballot((d >> b) & 1);
+      same &= (d >> b) & 1 ? set : ~set;
     }
+    const uint32_t rank = __popcll(same & ((uint64_t{1} << lane) - 1));
+    if (rank == 0) count[wave * digits + d] = __popcll(same);
     __syncthreads();
     // The counters' sums before each, by digit and then by wave.
     const int entries = kSortWaves * digits;
-    const int per = (entries + kSortThreads - 1) / kSortThreads;
+    const int per = (entries + kRun - 1) / kRun;
     const int e0 = threadIdx.x * per;
     uint32_t sum = 0;
     for (int e = e0; e < e0 + per && e < entries; ++e)
@@ -193,7 +203,8 @@ __device__ __forceinline__ void sort_run(const int64_t* __restrict__ tokens, int
     if (lane == kWave - 1) totals[wave] = upto;
     __syncthreads();
     uint32_t start = upto - sum;
-    for (int w = 0; w < wave; ++w) start += totals[w];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) start += w < wave ? totals[w] : 0;
     for (int e = e0; e < e0 + per && e < entries; ++e) {
       uint32_t& c = count[(e % kSortWaves) * digits + e / kSortWaves];
       const uint32_t have = c;
@@ -201,78 +212,88 @@ __device__ __forceinline__ void sort_run(const int64_t* __restrict__ tokens, int
       start += have;
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const uint32_t to = count[wave * digits + ((key[j] >> shift) & (digits - 1))] + rank[j];
-      skey[to] = key[j];
-      sid[to] = static_cast<uint16_t>(id[j]);
-    }
+    const uint32_t to = count[wave * digits + d] + rank;
+    skey[to] = key;
+    sid[to] = static_cast<uint16_t>(id);
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      key[j] = skey[at0 + j * kWave];
-      id[j] = sid[at0 + j * kWave];
-    }
+    key = skey[threadIdx.x];
+    id = sid[threadIdx.x];
     __syncthreads();
   }
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    // What fills up the last run is behind all of the run's own tokens.
-    const int64_t i = base + at0 + j * kWave;
-    if (i < n) {
-      keys[i] = static_cast<int>(key[j]);
-      ids[i] = static_cast<int>(base + id[j]);
-    }
+  // What fills up the last run is behind all of the run's own tokens.
+  if (i < n) {
+    keys[i] = static_cast<int>(key);
+    ids[i] = static_cast<int>(base + id);
   }
 }
 
-typedef unsigned u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
-
-// Workgroups 0 .. runs - 1 sort a run each, the others fill `zeros` bytes (an even number) at
-// `fill` (2-byte aligned).
-template <int J>
-__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(
-    const int64_t* __restrict__ tokens, int* __restrict__ keys, int* __restrict__ ids, int64_t n,
-    int vocab, int runs, char* __restrict__ fill, int64_t zeros) {
-  if (static_cast<int>(blockIdx.x) < runs) {
-    sort_run<J>(tokens, keys, ids, n, vocab,
-                static_cast<int64_t>(blockIdx.x) * (kSortThreads * J));
-    return;
-  }
-  const int64_t step = static_cast<int64_t>(gridDim.x - runs) * kSortThreads;
-  int64_t i = static_cast<int64_t>(blockIdx.x - runs) * kSortThreads + threadIdx.x;
-  if (i < zeros % 16 / 2) *reinterpret_cast<uint16_t*>(fill + zeros / 16 * 16 + 2 * i) = 0;
-  for (; i < zeros / 16; i += step)
-    __builtin_nontemporal_store(u32x4_a2{0u, 0u, 0u, 0u},
-                                reinterpret_cast<u32x4_a2*>(fill + 16 * i));
+// Workgroups 0 .. runs - 1 sort a run each, the others write zeros.
+__global__ __launch_bounds__(kRun) void embed_sort_kernel(const int64_t* __restrict__ tokens,
+                                                         int* __restrict__ keys,
+                                                         int* __restrict__ ids, int n, int vocab,
+                                                         int runs, Zeros zeros) {
+  if (static_cast<int>(blockIdx.x) < runs)
+    sort_run(tokens, keys, ids, n, vocab, static_cast<int64_t>(blockIdx.x) * kRun);
+  else
+    zeros.fill(blockIdx.x - runs, gridDim.x - runs);
 }
 
-// Eight sorted runs of `len` become one: an element's place is its own in its run plus, for each
-// other run, how many there come before it (equal keys: those of earlier runs).
-constexpr int kMergeWays = 8;
+// Four sorted runs of `len` become one: an element's place is its own in its run plus, for each
+// other run, how many there come before it (equal keys: those of earlier runs).  The searches of
+// the runs go in step, in LDS: all of their keys where they are 1024 long, else every
+// len / 1024-th and the last few steps in memory.  (Sixteen runs at once: 15 searches an element
+// took 20 us for 16384 tokens, and 44 with all steps in memory.)
+constexpr int kMergeWays = 4, kSamples = kRun;
 
-__global__ __launch_bounds__(kThreads) void embed_merge_kernel(
-    const int* __restrict__ keys, const int* __restrict__ ids, int* __restrict__ keys_out,
-    int* __restrict__ ids_out, int64_t n, int64_t len) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= n) return;
-  const int key = keys[i];
-  const int64_t run = i / len, first = run / kMergeWays * kMergeWays;
-  int64_t to = first * len + (i - run * len);
-  for (int64_t other = first; other < first + kMergeWays && other * len < n; ++other) {
-    if (other == run) continue;
-    const int upto = other < run ? key : key - 1;    // keys are >= 0
-    const int64_t begin = other * len, end = begin + len < n ? begin + len : n;
-    int64_t lo = begin, hi = end;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (keys[mid] <= upto) lo = mid + 1;
-      else hi = mid;
-    }
-    to += lo - begin;
+__global__ __launch_bounds__(kThreads) void embed_merge_kernel(const int* __restrict__ keys,
+                                                              const int* __restrict__ ids,
+                                                              int* __restrict__ keys_out,
+                                                              int* __restrict__ ids_out, int n,
+                                                              int len) {
+  __shared__ int samples[kMergeWays * kSamples];
+  // Runs are whole workgroups long, so a workgroup's elements are one run's.
+  const unsigned i0 = blockIdx.x * kThreads, run = i0 / static_cast<unsigned>(len);
+  const int mine = run % kMergeWays, apart = len / kSamples;
+  const int64_t first = static_cast<int64_t>(run - mine) * len;
+#pragma unroll
+  for (int q = threadIdx.x; q < kMergeWays * kSamples; q += kThreads) {
+    const int64_t at = first + static_cast<int64_t>(q) * apart;
+    samples[q] = at < n ? keys[at] : INT32_MAX;
   }
+  const unsigned i = i0 + threadIdx.x;
+  const int key = i < static_cast<unsigned>(n) ? keys[i] : 0;
+  const int id = i < static_cast<unsigned>(n) ? ids[i] : 0;
+  __syncthreads();
+  if (i >= static_cast<unsigned>(n)) return;
+  // Of run w, the samples that come before this element: up to `key` in earlier runs, below it in
+  // later ones (keys are >= 0).
+  int below[kMergeWays] = {};
+#pragma unroll 1
+  for (int s = kSamples; s > 0; s /= 2) {
+#pragma unroll
+    for (int w = 0; w < kMergeWays; ++w) {
+      const int at = below[w] + s;
+      if (at <= kSamples && samples[w * kSamples + at - 1] <= key - (w > mine)) below[w] = at;
+    }
+  }
+  // Between the last of them and the next sample: `apart` - 1 elements.
+  int64_t lo[kMergeWays];
+#pragma unroll
+  for (int w = 0; w < kMergeWays; ++w)
+    lo[w] = below[w] > 0 ? int64_t{below[w] - 1} * apart + 1 : 0;
+#pragma unroll 1
+  for (int s = apart / 2; s > 0; s /= 2) {
+#pragma unroll
+    for (int w = 0; w < kMergeWays; ++w) {
+      const int64_t at = first + static_cast<int64_t>(w) * len + lo[w] + s - 1;
+      if (below[w] > 0 && w != mine && at < n && keys[at] <= key - (w > mine)) lo[w] += s;
+    }
+  }
+  int64_t to = first + (i - static_cast<int64_t>(run) * len);
+#pragma unroll
+  for (int w = 0; w < kMergeWays; ++w) to += w == mine ? 0 : lo[w];
   keys_out[to] = key;
-  ids_out[to] = ids[i];
+  ids_out[to] = id;
 }
 
 // ---------------------------------------------------------------------------
@@ -293,91 +314,181 @@ __device__ __forceinline__ void store_sum(T* __restrict__ row, const Cols<N, WHO
   at.store(row, v);
 }
 
-// Workgroup (chunk, columns): positions chunk * P .. of the sorted tokens.  A token that began
+// 2^tpr_log2 lanes walk a chunk: positions chunk * P .. of the sorted tokens.  A token that began
 // before the chunk leaves its sum at partials[2 chunk], one that goes on behind it at
 // partials[2 chunk + 1] (at [2 chunk] if it does both).
+// WAVES: a chunk is whole waves', and what it reads of the tokens is the same for all lanes.
 constexpr int kAhead = 8;       // rows whose loads are in flight
 
-template <typename T, typename O, bool WHOLE>
+template <typename T, typename O, bool WHOLE, bool WAVES>
 __global__ __launch_bounds__(kThreads) void embed_sums_kernel(
     const int* __restrict__ keys, const int* __restrict__ ids, const O* __restrict__ dout,
     T* __restrict__ dtable, float* __restrict__ partials, int64_t n, int vocab, int cols, int64_t P,
-    int tiles, float scale, bool accumulate) {
+    int tiles, int tpr_log2, float scale, bool accumulate) {
   constexpr int N = kVecElems<O>;
-  const int64_t chunk = blockIdx.x / tiles;
-  const Cols<N, WHOLE> at(static_cast<int64_t>(blockIdx.x % tiles) * kThreads + threadIdx.x, cols);
-  if (!at.any) return;
+  int group = threadIdx.x >> tpr_log2;
+  if constexpr (WAVES) group = __builtin_amdgcn_readfirstlane(group);
+  const int64_t chunk = static_cast<int64_t>(blockIdx.x / tiles) * (kThreads >> tpr_log2) + group;
+  const Cols<N, WHOLE> at((static_cast<int64_t>(blockIdx.x % tiles) << tpr_log2) +
+                              (threadIdx.x & ((1 << tpr_log2) - 1)), cols);
   const int64_t begin = chunk * P, end = begin + P < n ? begin + P : n;
+  // (All lanes of a wave take part in what its lanes tell each other.)
+  if (begin >= n || (WAVES ? __ballot(at.any) == 0 : !at.any)) return;
   int key = keys[begin];
   if (key == vocab) return;
   bool head = begin > 0 && keys[begin - 1] == key;
   float sum[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) sum[e] = 0.0f;
-  for (int64_t i0 = begin; i0 < end; i0 += kAhead) {
-    float v[kAhead][N];
-    int next[kAhead];
+  // Takes a row whose next token is `next`; true where the chunk's tokens end.
+  auto take = [&](const PackT<O, N>& v, int next, bool last) {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int64_t i = i0 + k < end ? i0 + k : end - 1;
-      next[k] = i + 1 < n ? keys[i + 1] : vocab;
-      at.load(v[k], dout + static_cast<int64_t>(ids[i]) * cols);
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (i0 + k >= end) break;
-#pragma unroll
-      for (int e = 0; e < N; ++e) sum[e] += v[k][e];
-      const bool last = i0 + k + 1 == end, goes_on = next[k] == key;
-      if (goes_on && !last) continue;
+    for (int e = 0; e < N; ++e) sum[e] += static_cast<float>(v[e]);
+    const bool goes_on = next == key;
+    if (goes_on && !last) return false;
+    if (at.any) {
       if (head || goes_on)
         at.store(partials + (2 * chunk + (head ? 0 : 1)) * cols, sum);
       else
         store_sum<T, N, WHOLE>(dtable + static_cast<int64_t>(key) * cols, at, sum, scale,
                                accumulate);
-      head = false;
-      key = next[k];
-      if (key == vocab) return;
+    }
+    head = false;
+    key = next;
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum[e] = 0.0f;
+    for (int e = 0; e < N; ++e) sum[e] = 0.0f;
+    return key == vocab;
+  };
+  if constexpr (WAVES) {
+    // 64 positions at a time, one to a lane; the rows that they name are loaded ahead of the
+    // additions, which wait for no other load.
+    const int lane = threadIdx.x % kWave;
+    for (int64_t s0 = begin; s0 < end; s0 += kWave) {
+      const int m = static_cast<int>(end - s0 < kWave ? end - s0 : kWave);
+      const int64_t i = s0 + (lane < m ? lane : m - 1);
+      const int id = ids[i], after = i + 1 < n ? keys[i + 1] : vocab;
+      auto load = [&](int k, PackT<O, N> (&v)[kAhead]) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int row = __builtin_amdgcn_readlane(id, k + u < m ? k + u : m - 1);
+          if (at.any) v[u] = at.load_raw(dout + static_cast<int64_t>(row) * cols);
+        }
+      };
+      PackT<O, N> v[kAhead] = {}, w[kAhead] = {};
+      load(0, v);
+      for (int k = 0; k < m; k += kAhead) {
+        if (k + kAhead < m) load(k + kAhead, w);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          if (k + u >= m) break;
+          if (take(v[u], __builtin_amdgcn_readlane(after, k + u), s0 + k + u + 1 == end)) return;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) v[u] = w[u];
+      }
+    }
+  } else {
+    for (int64_t i0 = begin; i0 < end; i0 += kAhead) {
+      PackT<O, N> v[kAhead];
+      int next[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int64_t i = i0 + k < end ? i0 + k : end - 1;
+        next[k] = i + 1 < n ? keys[i + 1] : vocab;
+        v[k] = at.load_raw(dout + static_cast<int64_t>(ids[i]) * cols);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (i0 + k >= end) break;
+        if (take(v[k], next[k], i0 + k + 1 == end)) return;
+      }
     }
   }
 }
 
-// A token that begins in this chunk and ends in a later one.
+// Tokens that begin in one chunk and end in a later one.  Each group of 2^tpr_log2 lanes looks
+// at a chunk, and adds up its token's sums if that ends within kNear chunks.  Tokens that go
+// further are added up by all groups, which deal out the later chunks; the groups' sums come
+// together in their order.
+constexpr int kNear = 16;
+
 template <typename T, int N, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void embed_join_kernel(
     const int* __restrict__ keys, T* __restrict__ dtable, const float* __restrict__ partials,
-    int64_t n, int vocab, int cols, int64_t P, int tiles, float scale, bool accumulate) {
-  const int64_t chunk = blockIdx.x / tiles, begin = chunk * P, end = begin + P;
-  if (end >= n) return;
-  const int key = keys[end - 1];
-  if (key == vocab || keys[end] != key || (begin > 0 && keys[begin - 1] == key)) return;
-  const Cols<N, WHOLE> at(static_cast<int64_t>(blockIdx.x % tiles) * kThreads + threadIdx.x, cols);
-  if (!at.any) return;
-  int64_t lo = end, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (keys[mid] <= key) lo = mid + 1;
-    else hi = mid;
-  }
-  const int64_t last = (lo - 1) / P;
+    int64_t n, int vocab, int cols, int64_t P, int chunks, int tiles, int tpr_log2, float scale,
+    bool accumulate) {
+  __shared__ float fold[kThreads * N];
+  __shared__ int far_key[32];                 // of each group's chunk, or -1
+  const int groups = kThreads >> tpr_log2, tpr = 1 << tpr_log2;
+  const int group = threadIdx.x >> tpr_log2, t = threadIdx.x & (tpr - 1);
+  const int c0 = blockIdx.x / tiles * groups;
+  const Cols<N, WHOLE> at((static_cast<int64_t>(blockIdx.x % tiles) << tpr_log2) + t, cols);
+  // Adds up the first sums of chunks c, c + step, .. up to `last`.
+  auto add = [&](float (&sum)[N], int c, int last, int step) {
+    constexpr int U = WHOLE ? 8 : 4;
+    for (; c <= last; c += U * step) {
+      float v[U][N];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        at.load(v[u], partials + 2 * static_cast<int64_t>(c + u * step <= last ? c + u * step : last) *
+                                     cols);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (c + u * step > last) break;
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += v[u][e];
+      }
+    }
+  };
   float sum[N];
-  at.load(sum, partials + (2 * chunk + 1) * cols);
-  constexpr int U = 8;
-  for (int64_t c0 = chunk + 1; c0 <= last; c0 += U) {
-    float v[U][N];
+  const int mine = c0 + group;
+  int far = -1;
+  if (mine + 1 < chunks) {
+    const int64_t begin = mine * P, end = begin + P;
+    const int key = keys[end - 1], before = begin > 0 ? keys[begin - 1] : -1;
+    int later = 0;                            // chunks that begin with the token
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      at.load(v[u], partials + 2 * (c0 + u <= last ? c0 + u : last) * cols);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (c0 + u > last) break;
-#pragma unroll
-      for (int e = 0; e < N; ++e) sum[e] += v[u][e];
+    for (int u = 0; u < kNear; ++u)
+      later += mine + 1 + u < chunks && keys[end + u * P] == key ? 1 : 0;
+    if (key != vocab && before != key && later > 0) {
+      if (later == kNear) {
+        far = key;
+      } else if (at.any) {
+        at.load(sum, partials + (2 * static_cast<int64_t>(mine) + 1) * cols);
+        add(sum, mine + 1, mine + later, 1);
+        store_sum<T, N, WHOLE>(dtable + static_cast<int64_t>(key) * cols, at, sum, scale,
+                               accumulate);
+      }
     }
   }
-  store_sum<T, N, WHOLE>(dtable + static_cast<int64_t>(key) * cols, at, sum, scale, accumulate);
+  if (t == 0) far_key[group] = far;
+  __syncthreads();
+  for (int g = 0; g < groups; ++g) {
+    const int key = far_key[g], chunk = c0 + g;
+    if (key < 0) continue;
+    int last = chunk;
+    for (int c = chunk + 1; c < chunks; c += kThreads) {
+      const int q = c + static_cast<int>(threadIdx.x);
+      const int have = __syncthreads_count(q < chunks && keys[q * P] == key);
+      last += have;
+      if (have < kThreads) break;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[e] = 0.0f;
+    if (at.any) add(sum, chunk + 1 + group, last, groups);
+#pragma unroll
+    for (int e = 0; e < N; ++e) fold[e * kThreads + threadIdx.x] = sum[e];
+    __syncthreads();
+    if (group == 0 && at.any) {
+      at.load(sum, partials + (2 * static_cast<int64_t>(chunk) + 1) * cols);
+      for (int k = 0; k < groups; ++k)
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += fold[e * kThreads + k * tpr + t];
+      store_sum<T, N, WHOLE>(dtable + static_cast<int64_t>(key) * cols, at, sum, scale,
+                             accumulate);
+    }
+    __syncthreads();      // fold is written again
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -385,15 +496,20 @@ __global__ __launch_bounds__(kThreads) void embed_join_kernel(
 // ---------------------------------------------------------------------------
 int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
 
-// Tokens a run: as few registers a lane as hold them in one run, else the most.
-int run_registers(int64_t rows) { return rows <= kSortThreads ? 1 : rows <= 4 * kSortThreads ? 4 : 16; }
-int64_t runs_of(int64_t rows) { return ceil_div(rows, kSortThreads * run_registers(rows)); }
 
-// Positions a chunk: up to 512 chunks, so that the join of a token that is all of the batch adds
-// up no more than that.
-int64_t chunk_of(int64_t rows) {
+// Lanes that a row takes, as 2^this: as many as cover it with vectors of N, 8 to a workgroup.
+int lanes_log2(int64_t cols, int n) {
+  int log2 = 3;
+  while (log2 < 8 && (int64_t{n} << log2) < cols) ++log2;
+  return log2;
+}
+
+// Positions a chunk: up to 512 workgroups of chunks.  (By vectors of 8: of rows and cols alone, so
+// that the workspace is sized without the types.)
+int64_t chunk_of(int64_t rows, int64_t cols) {
+  const int64_t chunks = int64_t{512} << (8 - lanes_log2(cols, 8));
   int64_t p = 4;
-  while (512 * p < rows) p *= 2;
+  while (chunks * p < rows) p *= 2;
   return p;
 }
 
@@ -402,8 +518,8 @@ struct Workspace {
   int lists;                    // 2, or 4 where runs are merged
   Workspace(int64_t rows, int64_t cols) {
     list = (4 * rows + 15) / 16 * 16;
-    lists = runs_of(rows) > 1 ? 4 : 2;
-    partials = 2 * ceil_div(rows, chunk_of(rows)) * cols * 4;
+    lists = rows > kCount ? 4 : 2;
+    partials = 2 * ceil_div(rows, chunk_of(rows, cols)) * cols * 4;
   }
   int64_t bytes() const { return list * lists + partials; }
 };
@@ -426,8 +542,7 @@ int launch_fwd(const int64_t* tokens, const void* table, void* out, int64_t rows
                int64_t cols, float scale, hipStream_t s) {
   constexpr int N = kVecElems<T>;
   const int64_t vecs = ceil_div(cols, N);
-  int tpr_log2 = 3;
-  while (tpr_log2 < 8 && (int64_t{1} << tpr_log2) < vecs) ++tpr_log2;
+  const int tpr_log2 = lanes_log2(cols, N);
   const int u = vecs > 256 ? 2 : 1;
   const int64_t y = ceil_div(vecs, int64_t{u} << tpr_log2);
   const int64_t groups = ceil_div(rows, kThreads >> tpr_log2);
@@ -453,33 +568,29 @@ struct BwdArgs {
   hipStream_t s;
 };
 
-template <int J> int launch_sort(const BwdArgs& a, int* keys, int* ids, int64_t zeros) {
-  const int runs = a.rows > 0 ? static_cast<int>(runs_of(a.rows)) : 0;
-  const int64_t fills = ceil_div(zeros, 16 * kSortThreads);
-  const unsigned grid = static_cast<unsigned>(runs + (fills < 1024 ? fills : 1024));
-  if (grid == 0) return ok();
-  embed_sort_kernel<J><<<grid, kSortThreads, 0, a.s>>>(a.tokens, keys, ids, a.rows,
-                                                       static_cast<int>(a.vocab), runs,
-                                                       static_cast<char*>(a.dtable), zeros);
-  MCKE_LAUNCH_CHECK("embed_sort_kernel");
-  return ok();
-}
-
 template <typename T, typename O, bool WHOLE>
 int launch_sums(const BwdArgs& a, const int* keys, const int* ids, float* partials) {
   constexpr int N = kVecElems<O>;
-  const int64_t P = chunk_of(a.rows), chunks = ceil_div(a.rows, P);
-  const int tiles = static_cast<int>(ceil_div(a.cols, int64_t{N} * kThreads));
+  const int64_t P = chunk_of(a.rows, a.cols), chunks = ceil_div(a.rows, P);
+  const int tpr_log2 = lanes_log2(a.cols, N), groups = kThreads >> tpr_log2;
+  const int tiles = static_cast<int>(ceil_div(a.cols, int64_t{N} << tpr_log2));
   const int vocab = static_cast<int>(a.vocab), cols = static_cast<int>(a.cols);
-  embed_sums_kernel<T, O, WHOLE><<<static_cast<unsigned>(chunks * tiles), kThreads, 0, a.s>>>(
-      keys, ids, static_cast<const O*>(a.dout), static_cast<T*>(a.dtable), partials, a.rows, vocab,
-      cols, P, tiles, a.scale, a.accumulate);
+  const unsigned grid = static_cast<unsigned>(ceil_div(chunks, groups) * tiles);
+  auto* fn = tpr_log2 >= 6 ? &embed_sums_kernel<T, O, WHOLE, true>
+                           : &embed_sums_kernel<T, O, WHOLE, false>;
+  fn<<<grid, kThreads, 0, a.s>>>(keys, ids, static_cast<const O*>(a.dout),
+                                 static_cast<T*>(a.dtable), partials, a.rows, vocab, cols, P, tiles,
+                                 tpr_log2, a.scale, a.accumulate);
   MCKE_LAUNCH_CHECK("embed_sums_kernel");
   if (chunks == 1) return ok();
-  embed_join_kernel<T, N, WHOLE>
-      <<<static_cast<unsigned>((chunks - 1) * tiles), kThreads, 0, a.s>>>(
-          keys, static_cast<T*>(a.dtable), partials, a.rows, vocab, cols, P, tiles, a.scale,
-          a.accumulate);
+  // The join has few sums to a lane: at most a wave a row, so that there are four groups or more.
+  const int join_log2 = tpr_log2 < 6 ? tpr_log2 : 6;
+  const int join_tiles = static_cast<int>(ceil_div(a.cols, int64_t{N} << join_log2));
+  const unsigned join_grid =
+      static_cast<unsigned>(ceil_div(chunks, kThreads >> join_log2) * join_tiles);
+  embed_join_kernel<T, N, WHOLE><<<join_grid, kThreads, 0, a.s>>>(
+      keys, static_cast<T*>(a.dtable), partials, a.rows, vocab, cols, P, static_cast<int>(chunks),
+      join_tiles, join_log2, a.scale, a.accumulate);
   MCKE_LAUNCH_CHECK("embed_join_kernel");
   return ok();
 }
@@ -488,19 +599,25 @@ template <typename T, typename O> int launch_bwd(const BwdArgs& a) {
   const Workspace w(a.rows, a.cols);
   int* keys = reinterpret_cast<int*>(a.ws);
   int* ids = reinterpret_cast<int*>(a.ws + w.list);
-  const int64_t zeros =
-      a.accumulate ? 0 : a.vocab * a.cols * static_cast<int64_t>(sizeof(T));
-  const int J = run_registers(a.rows);
-  if (int rc = J == 1   ? launch_sort<1>(a, keys, ids, zeros)
-               : J == 4 ? launch_sort<4>(a, keys, ids, zeros)
-                        : launch_sort<16>(a, keys, ids, zeros))
-    return rc;
+  // Zeros in pieces of 32 KB at least, 4096 at most (512 of them 3 us slower for 1 GB, 16384 25).
+  const Zeros zeros{static_cast<char*>(a.dtable),
+                    a.accumulate ? 0 : a.vocab * a.cols * static_cast<int64_t>(sizeof(T))};
+  const int64_t pieces = ceil_div(zeros.bytes, 32 * 1024), fill = pieces < 4096 ? pieces : 4096;
+  const bool count = a.rows <= kCount;
+  const int64_t blocks = ceil_div(a.rows, count ? kWave : kRun);
+  if (blocks + fill == 0) return ok();
+  auto* fn = count ? &embed_count_kernel : &embed_sort_kernel;
+  fn<<<static_cast<unsigned>(blocks + fill), kRun, 0, a.s>>>(
+      a.tokens, keys, ids, static_cast<int>(a.rows), static_cast<int>(a.vocab),
+      static_cast<int>(blocks), zeros);
+  MCKE_LAUNCH_CHECK("embed_count_kernel or embed_sort_kernel");
   if (a.rows == 0) return ok();
-  for (int64_t len = int64_t{kSortThreads} * J, turn = 0; len < a.rows; len *= kMergeWays, ++turn) {
+  int turn = 0;
+  for (int64_t len = kRun; !count && len < a.rows; len *= kMergeWays, ++turn) {
     int* to = reinterpret_cast<int*>(a.ws + (turn % 2 ? 0 : 2 * w.list));
     int* ids_to = reinterpret_cast<int*>(reinterpret_cast<char*>(to) + w.list);
     embed_merge_kernel<<<static_cast<unsigned>(ceil_div(a.rows, kThreads)), kThreads, 0, a.s>>>(
-        keys, ids, to, ids_to, a.rows, len);
+        keys, ids, to, ids_to, static_cast<int>(a.rows), static_cast<int>(len));
     MCKE_LAUNCH_CHECK("embed_merge_kernel");
     keys = to;
     ids = ids_to;

@@ -106,8 +106,9 @@ def test_embedding_workspace(mcke):
     assert f(0, 100, 64) == 0 and f(4, 0, 64) == 0 and f(4, 100, 0) == 0 and f(-1, 100, 64) == 0
     assert f(1 << 31, 100, 64) == 0 and f(4, 100, 1 << 25) == 0
     for rows in (1, 1000, 16384, 16385, 1 << 20):
-        # Positions and tokens, twice where runs are merged, and at most 1024 rows of sums.
-        assert 8 * rows <= f(rows, 100, 64) <= 16 * (rows + 16) + 1024 * 64 * 4
+        # Positions and tokens, twice where runs are merged, and sums of two rows a chunk: at most
+        # 1024 of 2048 columns, or as many narrow ones.
+        assert 8 * rows <= f(rows, 100, 64) <= 16 * (rows + 16) + 1024 * 2048 * 4
 
 
 # ---------------------------------------------------------------------------
@@ -176,7 +177,7 @@ def test_checkpoint8_workspace(mcke):
     for rows in (1, 5, 4096, 1 << 20):
         for cols in (1, 2048, 16384, 1 << 20):
             n = f(rows, cols)
-            assert n > 0 and n % (4 * cols) == 0 and n // (4 * cols) <= min(rows, 256)
+            assert n > 0 and n % (4 * cols) == 0 and n // (4 * cols) <= min(rows, 1024)
 
 
 # ---------------------------------------------------------------------------
