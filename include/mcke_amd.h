@@ -411,9 +411,10 @@ int mcke_launch_bias_act_checkpoint8_backward(const void* dy, const uint8_t* cod
  * No reference counterpart; the last product and its loss in one, where the logits would be the
  * largest tensor of a training step: they are never kept.  hidden (rows x dim, row-major) and
  * weight (vocab x dim, row-major: as a layer or a tied embedding holds it) are of dtype,
- * MCKE_DTYPE_BF16 or MCKE_DTYPE_F16; hidden at any alignment of its type, weight 16-byte aligned if dim is a
- * multiple of 64 (other widths are copied a piece at a time, and run slower).  rows and vocab up
- * to 2^24, dim up to 2^16; vocab and dim > 0.  scale > 0 multiplies the logits.  With
+ * MCKE_DTYPE_BF16 or MCKE_DTYPE_F16; hidden at any alignment of its type, weight 4-byte aligned if
+ * dim is even (odd widths are copied a piece at a time, and run slower) and finite (with
+ * a dim that is not a multiple of 64, an infinite one makes NaN of the row before it too).
+ * rows and vocab up to 2^24, dim up to 2^16; vocab and dim > 0.  scale > 0 multiplies the logits.  With
  * z = scale * hidden[r] . weight[j]:
  *   lse = log sum exp z, loss = lse - z[targets[r]]
  * Products are summed in fp32, and the same input gives the same bits on every run.

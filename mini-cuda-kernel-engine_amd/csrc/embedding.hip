@@ -256,7 +256,8 @@ __global__ __launch_bounds__(kThreads) void embed_merge_kernel(const int* __rest
   const int mine = run % kMergeWays, apart = len / kSamples;
   const int64_t first = static_cast<int64_t>(run - mine) * len;
 #pragma unroll
-  for (int q = threadIdx.x; q < kMergeWays * kSamples; q += kThreads) {
+  for (int k = 0; k < kMergeWays * kSamples / kThreads; ++k) {
+    const int q = k * kThreads + threadIdx.x;
     const int64_t at = first + static_cast<int64_t>(q) * apart;
     samples[q] = at < n ? keys[at] : INT32_MAX;
   }

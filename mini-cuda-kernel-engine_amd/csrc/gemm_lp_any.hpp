@@ -26,9 +26,10 @@
 // count of loads in flight the same in every step.
 //
 // K is a multiple of 64 here.  Rows past an operand's end along M and N repeat its last row and are
-// not to be stored.  Along K both operands have whole stages: kAlongK rows are as long, and of a
-// kAcrossK operand the last stage may lie elsewhere (`tail`), where rows of a matrix that ends inside
-// it are followed by zeros.
+// not to be stored.  16-byte loads may begin inside a row and end behind it, in the next one: what
+// lies there has to be multiplied by zeros of the other operand (along K), or not stored (along N).
+// Where that leaves the operand, or ends inside a stage of a kAcrossK operand, the caller has a copy of the
+// last rows with zeros behind them (`tail`).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -42,15 +43,14 @@ namespace mcke_amd {
 
 enum class Along { kAlongK, kAcrossK };
 
-// An operand's memory, 16-byte aligned, `row` elements between neighbouring rows.  `extent`: its
-// rows (kAlongK), or how many elements of a row may be read (kAcrossK; a multiple of 8, at least
-// 8).
+// An operand's memory, 4-byte aligned, `row` elements (an even number) between neighbouring rows.
+// `extent`: its rows (kAlongK), or how many elements a row has (kAcrossK).
 struct LpOperand {
   const uint16_t* p;
   int64_t row;
   int64_t extent;
   const uint16_t* tail = nullptr;
-  int64_t tail_stage = -1;     // the stage that is at `tail`
+  int64_t tail_stage = -1;     // the stage of a kAcrossK operand that is at `tail`
 };
 
 template <int B, Along L> struct LpAnyOperand {
@@ -106,7 +106,7 @@ template <int B, Along L> struct LpAnyOperand {
         const int rt = (64 / kLanes) * (wave * kDma + q) + lane / kLanes;
         const int64_t col = first + 8 * ((lane % kLanes) ^ swz(rt));
         src[q] = static_cast<uint32_t>(rt * o.row * 2) +
-                 static_cast<uint32_t>(2 * (col + 8 <= o.extent ? col : o.extent - 8)) + kBias -
+                 static_cast<uint32_t>(2 * (col < o.extent ? col : 0)) + kBias -
                  1024u * (q % 4);
       }
       // Lane r16 = 4 jq + qa of group g reads row 8 g + 4 t + jq at columns 4 qa of its block and

@@ -23,10 +23,14 @@
 // gradients' size with a power of two for m, 2.4e-4 like this; 2.1e-4 is the outputs' own rounding.)
 //
 // Rows without a target (target < 0) are not read.  The rows that have one are copied side by
-// side first, which skips the products of the others, ends them at whole stages of K with zeros,
-// and makes rows of any width and alignment whole 16-byte vectors.  (16384 x 4096: 0.3 ms of a
-// pass.)  How many there are is known on the device alone: the launches cover all rows, and
-// workgroups past the last one end.
+// side first, which skips the products of the others and ends rows and columns with zeros at
+// whole stages of the products.  (4096 x 4096: 25 us of 9 ms.)  How many there are is known on the
+// device alone: the launches cover all rows, and workgroups past the last one end.
+//
+// The weights are read as they are where dim is even: 16-byte loads that end behind a row meet the
+// zeros of the hidden states.  The last rows, whose loads would leave the matrix, are a copy.  Odd
+// rows are not at 4-byte addresses, as loads into LDS need them: they are copied a piece at a time
+// into rows of whole stages.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -129,17 +133,52 @@ __global__ __launch_bounds__(kPrepThreads) void lce_rows_kernel(
   if (threadIdx.x == 0) *out.meta = Meta{count, factor, unfactor, 0};
 }
 
+// A copy of the last values of a matrix, zeros behind them.
+struct Tail {
+  const uint16_t* from;
+  uint16_t* to;
+  int64_t values, all;         // copied; written (multiples of nothing)
+};
+
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8), aligned(2)));
+
+// `n` values from x (null: none) and zeros behind them, as eight.
+__device__ __forceinline__ u16x8 load8(const uint16_t* __restrict__ x, int64_t n) {
+  u16x8 v{};
+  if (x && n >= 8) {
+    v = *reinterpret_cast<const u16x8*>(x);
+  } else if (x && n > 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) v[e] = x[e];
+  }
+  return v;
+}
+
 // Packed rows: row k of `to` (`width` values, a multiple of 64) is row from[k] of x (`cols`
 // values) with zeros behind it, and behind the last row are rows of zeros up to the next multiple
 // of 64 (64 at least).  from null: the `given` rows as they are, and zeros up to `rows`.  A
-// workgroup a row.
-__global__ __launch_bounds__(kThreads) void lce_pack_kernel(const uint16_t* __restrict__ x,
-                                                            const int* __restrict__ from,
-                                                            const Meta* __restrict__ meta,
-                                                            uint16_t* __restrict__ to, int64_t given,
-                                                            int64_t rows, int cols, int width) {
-  typedef unsigned short u16x8 __attribute__((ext_vector_type(8), aligned(2)));
-  for (int64_t k = blockIdx.x; k < rows; k += gridDim.x) {
+// workgroup a row; those from `blocks` on copy the tail.
+__global__ __launch_bounds__(kThreads) void lce_pack_kernel(
+    const uint16_t* __restrict__ x, const int* __restrict__ from, const Meta* __restrict__ meta,
+    uint16_t* __restrict__ to, int64_t given, int64_t rows, int cols, int width, int blocks,
+    Tail tail) {
+  if (static_cast<int>(blockIdx.x) >= blocks) {
+    const int64_t step = 8 * static_cast<int64_t>(gridDim.x - blocks) * kThreads;
+    for (int64_t i = 8 * (static_cast<int64_t>(blockIdx.x - blocks) * kThreads + threadIdx.x);
+         i < tail.all; i += step) {
+      const u16x8 v = load8(tail.from + i, tail.values - i);
+      if (i + 8 <= tail.all) {
+        *reinterpret_cast<u16x8*>(tail.to + i) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i + e < tail.all) tail.to[i + e] = v[e];
+      }
+    }
+    return;
+  }
+  for (int64_t k = blockIdx.x; k < rows; k += blocks) {
     const uint16_t* row = nullptr;
     if (!from) {
       if (k < given) row = x + k * cols;
@@ -148,17 +187,8 @@ __global__ __launch_bounds__(kThreads) void lce_pack_kernel(const uint16_t* __re
       if (k >= up) return;
       if (k < n) row = x + static_cast<int64_t>(from[k]) * cols;
     }
-    for (int c = 8 * threadIdx.x; c < width; c += 8 * kThreads) {
-      u16x8 v{};
-      if (row && c + 8 <= cols) {
-        v = *reinterpret_cast<const u16x8*>(row + c);
-      } else if (row) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < cols) v[e] = row[c + e];
-      }
-      *reinterpret_cast<u16x8*>(to + k * width + c) = v;
-    }
+    for (int c = 8 * threadIdx.x; c < width; c += 8 * kThreads)
+      *reinterpret_cast<u16x8*>(to + k * width + c) = load8(row ? row + c : nullptr, cols - c);
   }
 }
 
@@ -183,12 +213,20 @@ __device__ __forceinline__ float across_groups_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
+// A piece of the weights: `rows` rows from `first` on, `row` values apart.  Rows from tail_first
+// on (a multiple of 256) are at `tail` too, as far apart, with zeros behind the last (null: none
+// are).
+struct Piece {
+  const uint16_t* p;
+  int64_t row, rows, first;
+  const uint16_t* tail;
+  int64_t tail_first;
+};
+
 struct Logits {
   const uint16_t* hidden;      // packed rows, `width` apart
-  const uint16_t* weight;      // the piece's rows, `width` apart
   int width;                   // a multiple of 64
-  int64_t piece;               // rows of the piece
-  int64_t first;               // its first row in the vocabulary
+  Piece w;
   float scale;
 };
 
@@ -196,7 +234,10 @@ template <int BM, int BN, typename T>
 __device__ __forceinline__ void logits_tile(f32x4 (&acc)[BM / 32][BN / 32], char* smem,
                                             const Logits& l, int n, int64_t m0, int64_t n0) {
   const LpOperand A{l.hidden, l.width, n > 0 ? n : 1};
-  const LpOperand B{l.weight, l.width, l.piece};
+  const uint16_t* w = l.w.tail && l.w.first + n0 >= l.w.tail_first
+                          ? l.w.tail - (l.w.tail_first - l.w.first) * l.w.row
+                          : l.w.p;
+  const LpOperand B{w, l.w.row, l.w.rows};
   lp_any_loop<T, BM, BN, Along::kAlongK, Along::kAlongK>(acc, smem, A, B, m0, n0, 0, l.width / 64);
 }
 
@@ -221,8 +262,8 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_stats_kernel(
   const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
   const float c = l.scale * kLog2e;
   // Columns of the wave that are in the vocabulary, less this lane's 4 g.
-  const bool cut = n0 + BN > l.piece;
-  const int left = static_cast<int>(cut ? l.piece - n0 - wn * WN - 4 * g : BN);
+  const bool cut = n0 + BN > l.w.rows;
+  const int left = static_cast<int>(cut ? l.w.rows - n0 - wn * WN - 4 * g : BN);
   const int64_t at = 2 * static_cast<int64_t>(tile0 + tn) + wn;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
@@ -259,7 +300,7 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_stats_kernel(
       sums[at * stride + row] = s;
     }
     // The target's column, where it is one of this wave's.
-    const int64_t t = (row < n ? target[row] : -1) - (l.first + n0 + wn * WN);
+    const int64_t t = (row < n ? target[row] : -1) - (l.w.first + n0 + wn * WN);
     if (__ballot(t >= 0 && t < WN)) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
@@ -271,21 +312,22 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_stats_kernel(
   }
 }
 
-// loss and lse of packed rows from their parts: 64 rows a workgroup (a row to a lane), the parts
-// dealt to its waves.
+// loss and lse of packed rows from their parts.  A workgroup has 2^rows_log2 rows, up to 16, and
+// its other lanes the parts in turn: few loads are behind each other in a lane.  (64 rows a
+// workgroup: 4 rows of 2048 parts 26 us, LATER like this.)
 constexpr int kJoinWaves = 16;
 
 __global__ __launch_bounds__(kJoinWaves * kWave) void lce_join_kernel(
     const float* __restrict__ largest, const float* __restrict__ sums,
     const float* __restrict__ at_target, const int* __restrict__ from,
     const int* __restrict__ target, const Meta* __restrict__ meta, float* __restrict__ loss,
-    float* __restrict__ lse_out, int64_t stride, int parts, float scale) {
-  __shared__ float lm[kJoinWaves][kWave], ls[kJoinWaves][kWave];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWave + lane;
+    float* __restrict__ lse_out, int64_t stride, int parts, int rows_log2, float scale) {
+  __shared__ float lm[kJoinWaves][16], ls[kJoinWaves][16];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, rows = 1 << rows_log2;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) << rows_log2) + lane % rows;
   const int n = meta->rows;
   const float c = scale * kLog2e;
-  if (static_cast<int64_t>(blockIdx.x) * kWave >= n) return;
+  if ((static_cast<int64_t>(blockIdx.x) << rows_log2) >= n) return;
   float m = -__builtin_inff(), s = 0.0f;
   auto add = [&](float m2, float s2) {
     // (An empty part has no largest logit; -inf against itself moves nothing.)
@@ -295,14 +337,23 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void lce_join_kernel(
     s = f * s + f2 * s2;
     m = to;
   };
+  const int step = kJoinWaves * kWave >> rows_log2;
   if (row < n) {
 #pragma unroll 8
-    for (int p = wave; p < parts; p += kJoinWaves) add(largest[p * stride + row], sums[p * stride + row]);
+    for (int p = threadIdx.x >> rows_log2; p < parts; p += step)
+      add(largest[p * stride + row], sums[p * stride + row]);
   }
-  lm[wave][lane] = m;
-  ls[wave][lane] = s;
+  // The lanes of a row, the lowest of which counts; then the waves in their order.
+  for (int d = kWave / 2; d >= rows; d /= 2) {
+    const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
+    add(m2, s2);
+  }
+  if (lane < rows) {
+    lm[wave][lane] = m;
+    ls[wave][lane] = s;
+  }
   __syncthreads();
-  if (wave > 0 || row >= n) return;
+  if (threadIdx.x >= static_cast<unsigned>(rows) || row >= n) return;
   for (int w = 1; w < kJoinWaves; ++w) add(lm[w][lane], ls[w][lane]);
   const float lse = __builtin_fmaf(kLn2, __builtin_amdgcn_logf(s), scale * m);
   if (lse_out) lse_out[from[row]] = lse;
@@ -328,8 +379,8 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows 
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
   const float c = l.scale * kLog2e;
-  const bool cut = n0 + BN > l.piece;
-  const int left = static_cast<int>(cut ? l.piece - n0 - wn * WN - 4 * g : BN);
+  const bool cut = n0 + BN > l.w.rows;
+  const int left = static_cast<int>(cut ? l.w.rows - n0 - wn * WN - 4 * g : BN);
   // Through LDS, so that the stores are whole rows: chunk q of tile row r at q ^ (r % kChunks).
   struct alignas(8) Quad { T v[4]; };
   constexpr int kRowBytes = BN * 2, kChunks = kRowBytes / 16, kSwz = kChunks < 32 ? kChunks : 32;
@@ -343,7 +394,7 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows 
     const bool have = row < n;
     const float lse2 = have ? rows.lse2[row] : 0.0f, cp = have ? rows.cp[row] : 0.0f;
     const float ct = have ? rows.ct[row] : 0.0f;
-    const int64_t t = (have ? rows.target[row] : -1) - (l.first + n0 + wn * WN) - 4 * g;
+    const int64_t t = (have ? rows.target[row] : -1) - (l.w.first + n0 + wn * WN) - 4 * g;
     // Columns from `past` on, and rows without a target, are zeros whatever their exponentials
     // are.
     int past = have ? left : 0;
@@ -380,12 +431,12 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows 
 }
 
 // dH's sums over part blockIdx.y of a piece: acc = dz W, written or added to the part's sums.
-// Where the piece ends inside a stage of 64 rows, `tail` is that stage with zeros behind it (dz has
-// zeros there, but what lies behind the weights is not the caller's to read).
+// The last stage of 64 rows of the weights' last piece is in the tail's copy: what lies behind the
+// weights is not the caller's to read (dz has zeros there).
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dh_kernel(
-    const uint16_t* __restrict__ dz, int64_t ld, const uint16_t* __restrict__ weight,
-    const uint16_t* __restrict__ tail, int width, int64_t piece, const Meta* __restrict__ meta, float* __restrict__ out, int64_t part_stride,
+    const uint16_t* __restrict__ dz, int64_t ld, Piece w, int width,
+    const Meta* __restrict__ meta, float* __restrict__ out, int64_t part_stride,
     int stages_per_part, bool add, int tiles_n) {
   using S = LpAnyShape<BM, BN, Along::kAlongK, Along::kAcrossK>;
   constexpr int MT = S::MT, NT = S::NT;
@@ -394,12 +445,15 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dh_kernel(
   int tm, tn;
   if (!tile_of_rows<BM>(n, tiles_n, tm, tn)) return;
   const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
-  const int all = static_cast<int>((piece + 63) / 64);
+  const int all = static_cast<int>((w.rows + 63) / 64);
   const int first = blockIdx.y * stages_per_part;
   const int stages = all - first < stages_per_part ? all - first : stages_per_part;
   if (stages <= 0) return;
   const LpOperand A{dz, ld, n > 0 ? n : 1};
-  const LpOperand B{weight, width, width, tail, piece % 64 ? all - 1 : -1};
+  const int64_t last = w.first + 64 * static_cast<int64_t>(all - 1);
+  const bool ends = w.tail && last >= w.tail_first;
+  const LpOperand B{w.p, w.row, w.row, ends ? w.tail + (last - w.tail_first) * w.row : nullptr,
+                    ends ? all - 1 : -1};
   f32x4 acc[MT][NT];
   lp_any_loop<T, BM, BN, Along::kAlongK, Along::kAcrossK>(acc, smem, A, B, m0, n0, first, stages);
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -548,7 +602,8 @@ struct Plan {
   int64_t rows, vocab, dim;
   int64_t width;             // dim, a multiple of 64
   int64_t up;                // rows, a multiple of 64
-  bool pad;                  // the weights need a padded copy
+  bool pad;                  // the weights need a padded copy, a piece at a time
+  int64_t tail_first, tail_values;   // or one of their last rows and zeros behind them (0: none)
   int64_t piece, pieces;     // rows of W at once
   Tile tile;                 // of the logits
   int64_t at;                // bytes of workspace so far
@@ -556,7 +611,13 @@ struct Plan {
   Plan(int64_t r, int64_t v, int64_t d, bool backward) : rows(r), vocab(v), dim(d), at(0) {
     width = round_up(d, 64);
     up = round_up(r, 64);
-    pad = d % 64 != 0;
+    pad = d % 2 != 0;
+    // Whole tiles before it read up to 63 values past their last row, which the matrix has to hold.
+    tail_first = (v - 1) / kPieceAlign * kPieceAlign;
+    if (tail_first > 0 && (v - tail_first) * d < 64) tail_first -= kPieceAlign;
+    tail_values = pad || (d % 64 == 0 && (!backward || v % 64 == 0))
+                      ? 0
+                      : (round_up(v, 64) - tail_first) * d + 64;
     int64_t most = round_up(v, kPieceAlign);
     auto limit = [&](int64_t per_row) {
       int64_t m = kPieceValues / per_row / kPieceAlign * kPieceAlign;
@@ -590,9 +651,7 @@ struct RowsAt {
       ct = p.take(4 * p.up);
     }
     hidden = p.take(2 * p.up * p.width);
-    // A padded piece of the weights, or the last stage of 64 of their rows.
-    weight = p.pad ? p.take(2 * p.piece * p.width)
-             : backward && p.vocab % 64 ? p.take(2 * 64 * p.width) : 0;
+    weight = p.take(p.pad ? 2 * p.piece * p.width : 2 * p.tail_values);
   }
   Rows rows(char* ws) const {
     return {reinterpret_cast<Meta*>(ws + meta),     reinterpret_cast<int*>(ws + from),
@@ -648,27 +707,42 @@ template <class F> int with_tile(Tile t, F f) {
 }
 
 int launch_pack(const void* x, const int* from, const Meta* meta, void* to, int64_t given,
-                int64_t rows, int64_t cols, int64_t width, hipStream_t s) {
-  const int64_t most = 65536;
-  lce_pack_kernel<<<static_cast<unsigned>(rows < most ? rows : most), kThreads, 0, s>>>(
-      static_cast<const uint16_t*>(x), from, meta, static_cast<uint16_t*>(to), given,
-      rows, static_cast<int>(cols), static_cast<int>(width));
+                int64_t rows, int64_t cols, int64_t width, const Tail& tail, hipStream_t s) {
+  const int blocks = static_cast<int>(rows < 65536 ? rows : 65536);
+  const int64_t more = ceil_div(tail.all, 8 * kThreads), extra = more < 1024 ? more : 1024;
+  lce_pack_kernel<<<static_cast<unsigned>(blocks + extra), kThreads, 0, s>>>(
+      static_cast<const uint16_t*>(x), from, meta, static_cast<uint16_t*>(to), given, rows,
+      static_cast<int>(cols), static_cast<int>(width), blocks, tail);
   MCKE_LAUNCH_CHECK("lce_pack_kernel");
   return ok();
 }
 
-// Calls f(piece's rows of W (`width` apart), its first row, how many) for each piece.
+// The hidden states' rows, and the tail of the weights.
+int pack_rows(const Plan& p, const RowsAt& r, const void* hidden, const void* weight, char* ws,
+              hipStream_t s) {
+  const Rows rows = r.rows(ws);
+  const uint16_t* last = static_cast<const uint16_t*>(weight) + p.tail_first * p.dim;
+  const Tail tail{last, reinterpret_cast<uint16_t*>(ws + r.weight),
+                  p.tail_values ? (p.vocab - p.tail_first) * p.dim : 0, p.tail_values};
+  return launch_pack(hidden, rows.from, rows.meta, ws + r.hidden, p.rows, p.up, p.dim, p.width,
+                     tail, s);
+}
+
+// Calls f(piece) for each piece of the weights.
 template <class F>
 int for_pieces(const Plan& p, const RowsAt& r, const void* weight, char* ws, hipStream_t s, F f) {
+  uint16_t* copy = reinterpret_cast<uint16_t*>(ws + r.weight);
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t first = i * p.piece, n = p.vocab - first < p.piece ? p.vocab - first : p.piece;
     const uint16_t* w = static_cast<const uint16_t*>(weight) + first * p.dim;
+    Piece piece{w, p.dim, n, first, p.tail_values ? copy : nullptr, p.tail_first};
     if (p.pad) {
-      if (int rc = launch_pack(w, nullptr, nullptr, ws + r.weight, n, round_up(n, 64),
-                               p.dim, p.width, s)) return rc;
-      w = reinterpret_cast<const uint16_t*>(ws + r.weight);
+      if (int rc = launch_pack(w, nullptr, nullptr, copy, n, round_up(n, 64), p.dim, p.width,
+                               Tail{nullptr, nullptr, 0, 0}, s))
+        return rc;
+      piece = Piece{copy, p.width, n, first, nullptr, 0};
     }
-    if (int rc = f(w, first, n)) return rc;
+    if (int rc = f(piece)) return rc;
   }
   return ok();
 }
@@ -681,28 +755,29 @@ int lce_forward(const void* hidden, const void* weight, const int64_t* targets, 
                                                     static_cast<int>(p.rows), p.vocab, scale, rows,
                                                     loss, lse);
   MCKE_LAUNCH_CHECK("lce_rows_kernel");
-  uint16_t* packed = reinterpret_cast<uint16_t*>(ws + p.r.hidden);
-  if (int rc = launch_pack(hidden, rows.from, rows.meta, packed, p.rows, p.up, p.dim, p.width,
-                           s)) return rc;
+  const uint16_t* packed = reinterpret_cast<const uint16_t*>(ws + p.r.hidden);
+  if (int rc = pack_rows(p, p.r, hidden, weight, ws, s)) return rc;
   float* largest = reinterpret_cast<float*>(ws + p.largest);
   float* sums = reinterpret_cast<float*>(ws + p.sums);
   float* at_target = reinterpret_cast<float*>(ws + p.at_target);
-  const int rc = for_pieces(p, p.r, weight, ws, s, [&](const uint16_t* w, int64_t first, int64_t n) {
+  const int rc = for_pieces(p, p.r, weight, ws, s, [&](const Piece& w) {
     return with_tile(p.tile, [&](auto bm, auto bn) {
       constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
-      const int64_t tiles_n = ceil_div(n, BN), tiles = ceil_div(p.rows, BM) * tiles_n;
+      const int64_t tiles_n = ceil_div(w.rows, BN), tiles = ceil_div(p.rows, BM) * tiles_n;
       lce_stats_kernel<T, BM, BN><<<static_cast<unsigned>(tiles), kMfmaThreads, 0, s>>>(
-          Logits{packed, w, static_cast<int>(p.width), n, first, scale}, rows.meta, rows.target,
-          largest, sums, at_target, p.stride, static_cast<int>(first / BN),
-          static_cast<int>(tiles_n));
+          Logits{packed, static_cast<int>(p.width), w, scale}, rows.meta, rows.target, largest,
+          sums, at_target, p.stride, static_cast<int>(w.first / BN), static_cast<int>(tiles_n));
       MCKE_LAUNCH_CHECK("lce_stats_kernel");
       return ok();
     });
   });
   if (rc) return rc;
-  lce_join_kernel<<<static_cast<unsigned>(ceil_div(p.rows, kWave)), kJoinWaves * kWave, 0, s>>>(
+  int rows_log2 = 0;
+  while (rows_log2 < 4 && (int64_t{1} << rows_log2) < p.rows) ++rows_log2;
+  lce_join_kernel<<<static_cast<unsigned>(ceil_div(p.rows, int64_t{1} << rows_log2)),
+                    kJoinWaves * kWave, 0, s>>>(
       largest, sums, at_target, rows.from, rows.target, rows.meta, loss, lse, p.stride,
-      static_cast<int>(p.parts), scale);
+      static_cast<int>(p.parts), rows_log2, scale);
   MCKE_LAUNCH_CHECK("lce_join_kernel");
   return ok();
 }
@@ -727,32 +802,18 @@ template <typename T> int lce_backward(const BwdArgs& a, const BwdPlan& p) {
                                                      static_cast<int>(p.rows), p.vocab, a.scale,
                                                      rows, nullptr, nullptr);
   MCKE_LAUNCH_CHECK("lce_rows_kernel");
-  uint16_t* packed = reinterpret_cast<uint16_t*>(a.ws + p.r.hidden);
-  if (int rc = launch_pack(a.hidden, rows.from, rows.meta, packed, p.rows, p.up, p.dim,
-                           p.width, a.s))
-    return rc;
-  // Where the vocabulary ends inside a stage: padded pieces have their zeros, else a copy.
-  uint16_t* tail = nullptr;
-  const int64_t tail_rows = p.vocab % 64, tail_at = p.vocab - tail_rows;
-  if (tail_rows > 0) {
-    tail = reinterpret_cast<uint16_t*>(a.ws + p.r.weight);
-    if (p.pad)
-      tail += (tail_at - (p.pieces - 1) * p.piece) * p.width;
-    else if (int rc = launch_pack(static_cast<const uint16_t*>(a.weight) + tail_at * p.dim, nullptr,
-                                  nullptr, tail, tail_rows, 64, p.dim, p.width, a.s))
-      return rc;
-  }
+  const uint16_t* packed = reinterpret_cast<const uint16_t*>(a.ws + p.r.hidden);
+  if (int rc = pack_rows(p, p.r, a.hidden, a.weight, a.ws, a.s)) return rc;
   uint16_t* dz = reinterpret_cast<uint16_t*>(a.ws + p.dz);
   float* dh = reinterpret_cast<float*>(a.ws + p.dh);
   const int width = static_cast<int>(p.width);
   const int rc =
-      for_pieces(p, p.r, a.weight, a.ws, a.s, [&](const uint16_t* w, int64_t first, int64_t n) {
+      for_pieces(p, p.r, a.weight, a.ws, a.s, [&](const Piece& w) {
         int rc = with_tile(p.tile, [&](auto bm, auto bn) {
           constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
-          const int64_t tiles_n = ceil_div(n, BN), tiles = ceil_div(p.rows, BM) * tiles_n;
+          const int64_t tiles_n = ceil_div(w.rows, BN), tiles = ceil_div(p.rows, BM) * tiles_n;
           lce_dz_kernel<T, BM, BN><<<static_cast<unsigned>(tiles), kMfmaThreads, 0, a.s>>>(
-              Logits{packed, w, width, n, first, a.scale}, rows, dz, p.ld,
-              static_cast<int>(tiles_n));
+              Logits{packed, width, w, a.scale}, rows, dz, p.ld, static_cast<int>(tiles_n));
           MCKE_LAUNCH_CHECK("lce_dz_kernel");
           return ok();
         });
@@ -763,8 +824,8 @@ template <typename T> int lce_backward(const BwdArgs& a, const BwdPlan& p) {
             const int64_t tiles_n = ceil_div(p.dim, BN), tiles = ceil_div(p.rows, BM) * tiles_n;
             lce_dh_kernel<T, BM, BN>
                 <<<dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(p.parts)),
-                   kMfmaThreads, 0, a.s>>>(dz, p.ld, w, tail, width, n, rows.meta, dh, p.part_stride,
-                                           static_cast<int>(p.stages_per_part), first > 0,
+                   kMfmaThreads, 0, a.s>>>(dz, p.ld, w, width, rows.meta, dh, p.part_stride,
+                                           static_cast<int>(p.stages_per_part), w.first > 0,
                                            static_cast<int>(tiles_n));
             MCKE_LAUNCH_CHECK("lce_dh_kernel");
             return ok();
@@ -774,9 +835,9 @@ template <typename T> int lce_backward(const BwdArgs& a, const BwdPlan& p) {
         if (!a.dweight) return ok();
         auto dw = [&](auto bt) {
           constexpr int B = decltype(bt)::value;
-          const int64_t tiles_m = ceil_div(n, B), tiles_n = ceil_div(p.dim, B);
+          const int64_t tiles_m = ceil_div(w.rows, B), tiles_n = ceil_div(p.dim, B);
           lce_dw_kernel<T, B, B><<<static_cast<unsigned>(tiles_m * tiles_n), kMfmaThreads, 0, a.s>>>(
-              dz, p.ld, packed, width, rows.meta, static_cast<T*>(a.dweight) + first * p.dim, n,
+              dz, p.ld, packed, width, rows.meta, static_cast<T*>(a.dweight) + w.first * p.dim, w.rows,
               static_cast<int>(p.dim), static_cast<int>(tiles_m), static_cast<int>(tiles_n));
           MCKE_LAUNCH_CHECK("lce_dw_kernel");
           return ok();
@@ -825,8 +886,8 @@ int check_workspace(const std::string& who, const void* ws, size_t bytes, size_t
 }
 
 int check_weight(const std::string& who, const void* weight, int64_t dim) {
-  if (dim % 64 == 0 && !aligned(weight, 16))
-    return invalid(who + ": weight must be 16-byte aligned where dim is a multiple of 64");
+  if (dim % 2 == 0 && !aligned(weight, 4))
+    return invalid(who + ": weight must be 4-byte aligned where dim is even");
   return ok();
 }
 

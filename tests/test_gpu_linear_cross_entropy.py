@@ -29,9 +29,11 @@ pytestmark = pytest.mark.gpu
 
 TYPES = [BF16, F16]
 # rows, vocab, dim: every tile (64 x 128 up to 64 rows, 128 x 128, 256 x 256 from 192 of them), one
-# token, one logit, widths that are not 64s (padded copies) down to one, vocabularies that end
-# inside a tile and inside a stage, rows that do, dH in parts and whole.
-SHAPES = [(1, 1, 64), (1, 1000, 128), (3, 130, 1), (5, 257, 33), (64, 128, 64), (17, 5003, 192),
+# token, one logit, widths that are not 64s down to one (odd: padded copies; even: rows that cross
+# 16-byte loads), vocabularies that end inside a tile and inside a stage, rows that do, dH in parts and
+# whole.
+SHAPES = [(1, 1, 64), (1, 1000, 128), (3, 130, 1), (5, 257, 33), (2, 256, 2), (70, 513, 6), (9, 514, 2),
+          (40, 128, 1000), (150, 1100, 222), (300, 25001, 190), (64, 128, 64), (17, 5003, 192),
           (65, 64, 320), (100, 1021, 100), (128, 300, 256), (200, 4100, 64), (300, 25000, 512),
           (700, 3001, 130), (1500, 8200, 64)]
 
@@ -102,7 +104,7 @@ def run_forward(m, h, w, t, dt, scale, shift=0, want=(True, True), stream=None):
     outs = [out(m, (rows,), torch.float32) if k else None for k in want]
     n = m.linear_cross_entropy_workspace_bytes(rows, vocab, dim)
     ws = workspace(m, n)
-    m.launch_linear_cross_entropy(Dev(m, h, shift), Dev(m, w, 0 if dim % 64 == 0 else shift),
+    m.launch_linear_cross_entropy(Dev(m, h, shift), Dev(m, w, shift if dim % 2 else 2 * shift),
                                   Dev(m, t), *outs, dt, rows, vocab, dim, scale, ws, n,
                                   stream).throw_if_error()
     m.device_synchronize()
@@ -117,7 +119,7 @@ def run_backward(m, h, w, t, lse, dloss, dlse, dt, scale, shift=0, want=(True, T
     ws = workspace(m, n)
     vec = [Dev(m, v) if v is not None else None for v in (lse, dloss, dlse)]
     m.launch_linear_cross_entropy_backward(
-        Dev(m, h, shift), Dev(m, w, 0 if dim % 64 == 0 else shift), Dev(m, t), *vec, *outs, dt, rows,
+        Dev(m, h, shift), Dev(m, w, shift if dim % 2 else 2 * shift), Dev(m, t), *vec, *outs, dt, rows,
         vocab, dim, scale, ws, n, stream).throw_if_error()
     m.device_synchronize()
     ws.get()
@@ -148,7 +150,7 @@ def test_loss_and_gradients(gpu, i, shape, dt):
     check("dweight", got[1], want[1], tol[1])
 
 
-@pytest.mark.parametrize("shape", [(12300, 7000, 64), (12300, 300, 1024), (5, 9000, 8190)], ids=str)
+@pytest.mark.parametrize("shape", [(12300, 7000, 64), (12300, 7001, 66), (12300, 300, 1024), (5, 9000, 8191)], ids=str)
 def test_pieces(gpu, shape):
     """Vocabularies in several pieces, of the weights as they are and of padded copies; dH at 256 x
     256 tiles."""

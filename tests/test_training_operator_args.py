@@ -208,7 +208,7 @@ def test_linear_cross_entropy_refusals(cpu_only):
     _refused(m, _lce(m, h=A + 1), "aligned")
     _refused(m, _lce(m, t=Cc + 4), "aligned")
     _refused(m, _lce(m, lse=E + 2), "aligned")
-    _refused(m, _lce(m, w=B + 2), "16-byte")
+    _refused(m, _lce(m, w=B + 2), "4-byte")
     need = m.linear_cross_entropy_workspace_bytes(4, 100, 64)
     _refused(m, _lce(m, ws=None), str(need))
     _refused(m, _lce(m, nbytes=need - 1), str(need))
@@ -235,7 +235,7 @@ def test_linear_cross_entropy_backward_refusals(cpu_only):
     _refused(m, _lceb(m, dt=0), "dtype")
     _refused(m, _lceb(m, scale=0.0), "scale")
     _refused(m, _lceb(m, dh=G + 1), "aligned")
-    _refused(m, _lceb(m, w=B + 8), "16-byte")
+    _refused(m, _lceb(m, w=B + 2), "4-byte")
     need = m.linear_cross_entropy_backward_workspace_bytes(4, 100, 64)
     _refused(m, _lceb(m, ws=None), str(need))
     _refused(m, _lceb(m, nbytes=need - 1), str(need))
