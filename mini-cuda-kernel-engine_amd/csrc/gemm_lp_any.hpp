@@ -14,14 +14,17 @@
 //             ds_read_b128;
 //   kAcrossK  64 rows (one k each) of 2 BM or 2 BN bytes, chunk c of row k at
 //             c ^ (4 (k % 4) + 2 ((k / 8) % 2)); a fragment is two ds_read_b64_tr_b16.
-// Neither read meets a bank twice.  A has three stage buffers and B two: 160 KB at 256 x 256.
+// Neither read meets a bank twice.  With D stages in flight A has D + 1 stage buffers and B has D:
+// 160 KB at 256 x 256 and D = 2.
 //
 // Stage p is two steps; a step computes on fragments read in the step before it:
-//   step 2 p      MFMAs of k half 0; reads of half 1; DMA of A stage p + 2
+//   step 2 p      MFMAs of k half 0; reads of half 1; DMA of A stage p + D
 //   step 2 p + 1  wait for A and B of stage p + 1, barrier; MFMAs of half 1; reads of
-//                 half 0 of stage p + 1; DMA of B stage p + 2 into the buffer of stage p
-// so a stage has two to three steps to land, and there is one barrier per 64 of K.  Each wave
-// waits for its own reads before that barrier, which makes every buffer of stage p free behind it.
+//                 half 0 of stage p + 1; DMA of B stage p + D into the buffer of stage p
+// so a stage has D to D + 1 steps or more to land, and there is one barrier per 64 of K.  Each
+// wave waits for its own reads before that barrier, which makes every buffer of stage p free
+// behind it.  D is 2 where two workgroups share a CU or one fills it; small tiles that are alone on
+// their CU take as many as fit, or every stage waits for memory.
 // Past the end the DMA repeats the last stage into buffers that nobody reads, which keeps the
 // count of loads in flight the same in every step.
 //
@@ -157,10 +160,11 @@ template <int B, Along L> struct LpAnyOperand {
   }
 };
 
-template <int BM, int BN, Along LA, Along LB> struct LpAnyShape {
+template <int BM, int BN, Along LA, Along LB, int D = 2> struct LpAnyShape {
   using OA = LpAnyOperand<BM, LA>;
   using OB = LpAnyOperand<BN, LB>;
-  static constexpr int kABufs = 3, kBBufs = 2;
+  static constexpr int kDepth = D, kABufs = D + 1, kBBufs = D;
+  static_assert(D >= 2 && D * (OA::kDma + OB::kDma) + OA::kDma <= 63, "vmcnt counts to 63");
   static constexpr int kBBase = kABufs * OA::kBuf;
   static constexpr int kLdsBytes = kBBase + kBBufs * OB::kBuf;
   static constexpr int MT = BM / 32, NT = BN / 32;
@@ -238,11 +242,11 @@ __device__ __forceinline__ void lp_any_slot(
 // acc, from zero.  `smem`: S::kLdsBytes, 1024-byte aligned; free behind the caller's next barrier.
 // Lane (g, r16), register e of block (i, j): row wm BM/2 + 16 i + r16, column
 // wn BN/2 + 16 j + 4 g + e of the tile.
-template <typename T, int BM, int BN, Along LA, Along LB>
+template <typename T, int BM, int BN, Along LA, Along LB, int D = 2>
 __device__ __forceinline__ void lp_any_loop(f32x4 (&acc)[BM / 32][BN / 32], char* smem,
                                             const LpOperand& A, const LpOperand& B, int64_t m0,
                                             int64_t n0, int64_t first, int stages) {
-  using S = LpAnyShape<BM, BN, LA, LB>;
+  using S = LpAnyShape<BM, BN, LA, LB, D>;
   constexpr int MT = S::MT, NT = S::NT;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave / 2, wn = wave % 2;
@@ -277,11 +281,13 @@ __device__ __forceinline__ void lp_any_loop(f32x4 (&acc)[BM / 32][BN / 32], char
       (ob.template dma<Q>(ob.source(stage(p)), buf, w), ...);
     }(std::make_integer_sequence<int, S::OB::kDma>{});
   };
-  dma_a(0, lds0);
-  dma_b(0, ldsb);
-  dma_a(1, lds0 + S::OA::kBuf);
-  dma_b(1, ldsb + S::OB::kBuf);
-  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(S::OA::kDma + S::OB::kDma) : "memory");
+#pragma unroll
+  for (int p = 0; p < D; ++p) {
+    dma_a(p, lds0 + p * S::OA::kBuf);
+    dma_b(p, ldsb + p * S::OB::kBuf);
+  }
+  // Stage 0 is there, the others may be on their way.
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"((D - 1) * (S::OA::kDma + S::OB::kDma)) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   typename S::OA::Frags fa[2];
@@ -293,28 +299,33 @@ __device__ __forceinline__ void lp_any_loop(f32x4 (&acc)[BM / 32][BN / 32], char
     (oa.template read<0, RR>(lds0, fa[0]), ...);
   }(std::make_integer_sequence<int, S::OA::kReads>{});
 
-  uint32_t abuf = 0;               // A buffer of stage p
+  // Buffers of stage p, and A's of stage p + D.
+  uint32_t abuf = 0, bbuf = 0, afill = D;
   for (int p = 0; p < stages; ++p) {
-    const uint32_t a1 = abuf == 2 ? 0 : abuf + 1, a2 = a1 == 2 ? 0 : a1 + 1;
-    const uint32_t bcur = ldsb + (p % 2) * S::OB::kBuf, bnext = ldsb + ((p + 1) % 2) * S::OB::kBuf;
-    const LpAnyStep even{lds0 + abuf * S::OA::kBuf, bcur, lds0 + a2 * S::OA::kBuf,
-                         oa.source(stage(p + 2))};
+    const uint32_t a1 = abuf == D ? 0 : abuf + 1, b1 = bbuf == D - 1 ? 0 : bbuf + 1;
+    const uint32_t bcur = ldsb + bbuf * S::OB::kBuf, bnext = ldsb + b1 * S::OB::kBuf;
+    const LpAnyStep even{lds0 + abuf * S::OA::kBuf, bcur, lds0 + afill * S::OA::kBuf,
+                         oa.source(stage(p + D))};
     [&]<int... I>(std::integer_sequence<int, I...>) {
       (lp_any_slot<T, S, 0, I>(acc, fa[0], fb[0], fa[1], fb[1], oa, ob, even, w),
        ...);
     }(std::make_integer_sequence<int, S::kMfmas>{});
-    // Of the loads in flight only A's of stage p + 2 may be outstanding, and none of this wave's
-    // reads.  A bare s_barrier: __syncthreads() would wait for all loads.
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(S::OA::kDma) : "memory");
+    // Of the loads in flight those of stages from p + 2 on may be outstanding, and none of this
+    // wave's reads.  A bare s_barrier: __syncthreads() would wait for all loads.
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((D - 2) * (S::OA::kDma + S::OB::kDma) +
+                                                       S::OA::kDma)
+                 : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    const LpAnyStep odd{lds0 + a1 * S::OA::kBuf, bnext, bcur, ob.source(stage(p + 2))};
+    const LpAnyStep odd{lds0 + a1 * S::OA::kBuf, bnext, bcur, ob.source(stage(p + D))};
     [&]<int... I>(std::integer_sequence<int, I...>) {
       (lp_any_slot<T, S, 1, I>(acc, fa[1], fb[1], fa[0], fb[0], oa, ob, odd, w),
        ...);
     }(std::make_integer_sequence<int, S::kMfmas>{});
+    afill = abuf;              // free behind the barrier
     abuf = a1;
+    bbuf = b1;
     pin();
   }
   // The last stage's reads of the next one go unused, but they land in these registers: named

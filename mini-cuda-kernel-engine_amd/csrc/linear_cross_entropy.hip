@@ -230,7 +230,7 @@ struct Logits {
   float scale;
 };
 
-template <int BM, int BN, typename T>
+template <int BM, int BN, int D, typename T>
 __device__ __forceinline__ void logits_tile(f32x4 (&acc)[BM / 32][BN / 32], char* smem,
                                             const Logits& l, int n, int64_t m0, int64_t n0) {
   const LpOperand A{l.hidden, l.width, n > 0 ? n : 1};
@@ -238,17 +238,18 @@ __device__ __forceinline__ void logits_tile(f32x4 (&acc)[BM / 32][BN / 32], char
                           ? l.w.tail - (l.w.tail_first - l.w.first) * l.w.row
                           : l.w.p;
   const LpOperand B{w, l.w.row, l.w.rows};
-  lp_any_loop<T, BM, BN, Along::kAlongK, Along::kAlongK>(acc, smem, A, B, m0, n0, 0, l.width / 64);
+  lp_any_loop<T, BM, BN, Along::kAlongK, Along::kAlongK, D>(acc, smem, A, B, m0, n0, 0,
+                                                            l.width / 64);
 }
 
 // (largest, sum) of each row's part in the tile: wave column wn of vocabulary tile `tile` is
 // entry 2 tile + wn, `stride` values apart.
-template <typename T, int BM, int BN>
+template <typename T, int BM, int BN, int D>
 __global__ __launch_bounds__(kMfmaThreads, 1) void lce_stats_kernel(
     Logits l, const Meta* __restrict__ meta, const int* __restrict__ target,
     float* __restrict__ largest, float* __restrict__ sums, float* __restrict__ at_target,
     int64_t stride, int tile0, int tiles_n) {
-  using S = LpAnyShape<BM, BN, Along::kAlongK, Along::kAlongK>;
+  using S = LpAnyShape<BM, BN, Along::kAlongK, Along::kAlongK, D>;
   constexpr int MT = S::MT, NT = S::NT, WN = BN / 2;
   __shared__ __attribute__((aligned(1024))) char smem[S::kLdsBytes];
   const int n = __builtin_amdgcn_readfirstlane(meta->rows);
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_stats_kernel(
   if (!tile_of_rows<BM>(n, tiles_n, tm, tn)) return;
   const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
   f32x4 acc[MT][NT];
-  logits_tile<BM, BN, T>(acc, smem, l, n, m0, n0);
+  logits_tile<BM, BN, D, T>(acc, smem, l, n, m0, n0);
 
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
@@ -361,11 +362,11 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void lce_join_kernel(
 }
 
 // dz of a tile, row-major (`ld` values a row), zeros in rows and columns that pad it.
-template <typename T, int BM, int BN>
+template <typename T, int BM, int BN, int D>
 __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows rows,
                                                                 uint16_t* __restrict__ dz,
                                                                 int64_t ld, int tiles_n) {
-  using S = LpAnyShape<BM, BN, Along::kAlongK, Along::kAlongK>;
+  using S = LpAnyShape<BM, BN, Along::kAlongK, Along::kAlongK, D>;
   using O = LpOut<T>;
   constexpr int MT = S::MT, NT = S::NT, WM = BM / 2, WN = BN / 2;
   __shared__ __attribute__((aligned(1024))) char smem[S::kLdsBytes];
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows 
   if (!tile_of_rows<BM>(n, tiles_n, tm, tn)) return;
   const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
   f32x4 acc[MT][NT];
-  logits_tile<BM, BN, T>(acc, smem, l, n, m0, n0);
+  logits_tile<BM, BN, D, T>(acc, smem, l, n, m0, n0);
 
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
@@ -478,35 +479,52 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dh_kernel(
   }
 }
 
-// dH from its parts' sums, the factor taken out; zeros for rows without a target.
+// dH from its parts' sums, the factor taken out; zeros for rows without a target.  2^lanes_log2
+// lanes have eight columns of a row each, and a workgroup's other lanes the parts in turn.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void lce_dh_store_kernel(
     const float* __restrict__ sums, int64_t part_stride, int parts, const int* __restrict__ rank,
-    const Meta* __restrict__ meta, T* __restrict__ dhidden, int rows, int cols, int width) {
+    const Meta* __restrict__ meta, T* __restrict__ dhidden, int rows, int cols, int width,
+    int lanes_log2) {
+  __shared__ float fold[kThreads * 8];
   const float unfactor = meta->unfactor;
+  const int lanes = 1 << lanes_log2, groups = kThreads >> lanes_log2;
+  const int t = threadIdx.x & (lanes - 1), group = threadIdx.x >> lanes_log2;
+  const int c = 8 * ((static_cast<int>(blockIdx.y) << lanes_log2) + t);
   for (int r = blockIdx.x; r < rows; r += gridDim.x) {
     const int k = rank[r];
-    for (int c = 8 * threadIdx.x; c < cols; c += 8 * kThreads) {
-      float v[8] = {};
-      if (k >= 0) {
-        const float* p = sums + static_cast<int64_t>(k) * width + c;
-        for (int s = 0; s < parts; ++s, p += part_stride) {
-          const f32x4 a = *reinterpret_cast<const f32x4*>(p);
-          const f32x4 b = *reinterpret_cast<const f32x4*>(p + 4);
+    float v[8] = {};
+    if (k >= 0 && c < width) {
+      const float* p = sums + static_cast<int64_t>(k) * width + c;
+#pragma unroll 4
+      for (int s = group; s < parts; s += groups) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p + s * part_stride);
+        const f32x4 b = *reinterpret_cast<const f32x4*>(p + s * part_stride + 4);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] += a[e];
-            v[4 + e] += b[e];
-          }
+        for (int e = 0; e < 4; ++e) {
+          v[e] += a[e];
+          v[4 + e] += b[e];
         }
       }
-      VecT16<T> o;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(v[e] * unfactor);
-      T* to = dhidden + static_cast<int64_t>(r) * cols + c;
-      if (c + 8 <= cols) *reinterpret_cast<VecT16<T>*>(to) = o;
-      else store_part<T>(to, o, cols - c);
     }
+    if (groups > 1) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) fold[e * kThreads + threadIdx.x] = v[e];
+      __syncthreads();
+      if (group == 0) {
+        for (int g = 1; g < groups; ++g)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += fold[e * kThreads + g * lanes + t];
+      }
+      __syncthreads();         // fold is written again
+    }
+    if (group > 0 || c >= cols) continue;
+    VecT16<T> o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = static_cast<T>(v[e] * unfactor);
+    T* to = dhidden + static_cast<int64_t>(r) * cols + c;
+    if (c + 8 <= cols) *reinterpret_cast<VecT16<T>*>(to) = o;
+    else store_part<T>(to, o, cols - c);
   }
 }
 
@@ -630,6 +648,10 @@ struct Plan {
     pieces = ceil_div(v, piece);
     tile = tile_of(r, backward ? (piece < v ? piece : v) : v);
   }
+  // Tiles of logits over `n` rows of the weights.
+  int64_t tiles(int64_t n) const {
+    return ceil_div(rows, tile_rows(tile)) * ceil_div(n, tile_cols(tile));
+  }
   int64_t take(int64_t bytes) {
     const int64_t from = at;
     at += round_up(bytes, 256);
@@ -681,22 +703,23 @@ struct BwdPlan : Plan {
     ld = piece;
     dz = take(2 * up * ld);
     dh_tile = tile_of(rows, dim);
-    // Few tiles of dH share a piece's stages: up to two workgroups a CU, at least 8 stages each.
+    // Few tiles of dH share a piece's stages: up to two workgroups a CU, at least 8 stages each, and
+    // up to 64 MB of sums.
     const int64_t tiles = ceil_div(rows, tile_rows(dh_tile)) * ceil_div(dim, tile_cols(dh_tile));
     const int64_t stages = ceil_div(piece < vocab ? piece : vocab, 64);
     parts = (dh_tile == Tile::k256 ? 256 : 512) / tiles;
-    if (parts > 16) parts = 16;
+    part_stride = up * width;
+    if (parts > (int64_t{1} << 24) / part_stride) parts = (int64_t{1} << 24) / part_stride;
     if (parts > ceil_div(stages, 8)) parts = ceil_div(stages, 8);
     if (parts < 1) parts = 1;
     stages_per_part = ceil_div(stages, parts);
     parts = ceil_div(stages, stages_per_part);
-    part_stride = up * width;
     dh = take(4 * parts * part_stride);
     dw_tile = rows > 128 && ceil_div(piece, 256) * ceil_div(dim, 256) >= 192 ? Tile::k256 : Tile::k128;
   }
 };
 
-// f(std::integral_constant<int, BM>, BN) for a tile.
+// f(BM, BN) as std::integral_constants, for a tile.
 template <class F> int with_tile(Tile t, F f) {
   using I64 = std::integral_constant<int, 64>;
   using I128 = std::integral_constant<int, 128>;
@@ -704,6 +727,17 @@ template <class F> int with_tile(Tile t, F f) {
   if (t == Tile::k64x128) return f(I64{}, I128{});
   if (t == Tile::k128) return f(I128{}, I128{});
   return f(I256{}, I256{});
+}
+
+// f(BM, BN, D) for tiles of logits: with as many stages in flight as LDS holds where each has a CU
+// for itself, with two elsewhere.
+template <class F> int with_logits_tile(Tile t, int64_t tiles, F f) {
+  return with_tile(t, [&](auto bm, auto bn) {
+    constexpr int BM = decltype(bm)::value;
+    constexpr int kDeep = BM == 64 ? 6 : BM == 128 ? 4 : 2;
+    if (tiles <= 256) return f(bm, bn, std::integral_constant<int, kDeep>{});
+    return f(bm, bn, std::integral_constant<int, 2>{});
+  });
 }
 
 int launch_pack(const void* x, const int* from, const Meta* meta, void* to, int64_t given,
@@ -761,10 +795,10 @@ int lce_forward(const void* hidden, const void* weight, const int64_t* targets, 
   float* sums = reinterpret_cast<float*>(ws + p.sums);
   float* at_target = reinterpret_cast<float*>(ws + p.at_target);
   const int rc = for_pieces(p, p.r, weight, ws, s, [&](const Piece& w) {
-    return with_tile(p.tile, [&](auto bm, auto bn) {
-      constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
-      const int64_t tiles_n = ceil_div(w.rows, BN), tiles = ceil_div(p.rows, BM) * tiles_n;
-      lce_stats_kernel<T, BM, BN><<<static_cast<unsigned>(tiles), kMfmaThreads, 0, s>>>(
+    return with_logits_tile(p.tile, p.tiles(w.rows), [&](auto bm, auto bn, auto d) {
+      constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, D = decltype(d)::value;
+      const int64_t tiles_n = ceil_div(w.rows, BN), tiles = p.tiles(w.rows);
+      lce_stats_kernel<T, BM, BN, D><<<static_cast<unsigned>(tiles), kMfmaThreads, 0, s>>>(
           Logits{packed, static_cast<int>(p.width), w, scale}, rows.meta, rows.target, largest,
           sums, at_target, p.stride, static_cast<int>(w.first / BN), static_cast<int>(tiles_n));
       MCKE_LAUNCH_CHECK("lce_stats_kernel");
@@ -809,10 +843,10 @@ template <typename T> int lce_backward(const BwdArgs& a, const BwdPlan& p) {
   const int width = static_cast<int>(p.width);
   const int rc =
       for_pieces(p, p.r, a.weight, a.ws, a.s, [&](const Piece& w) {
-        int rc = with_tile(p.tile, [&](auto bm, auto bn) {
-          constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
-          const int64_t tiles_n = ceil_div(w.rows, BN), tiles = ceil_div(p.rows, BM) * tiles_n;
-          lce_dz_kernel<T, BM, BN><<<static_cast<unsigned>(tiles), kMfmaThreads, 0, a.s>>>(
+        int rc = with_logits_tile(p.tile, p.tiles(w.rows), [&](auto bm, auto bn, auto d) {
+          constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, D = decltype(d)::value;
+          const int64_t tiles_n = ceil_div(w.rows, BN), tiles = p.tiles(w.rows);
+          lce_dz_kernel<T, BM, BN, D><<<static_cast<unsigned>(tiles), kMfmaThreads, 0, a.s>>>(
               Logits{packed, width, w, a.scale}, rows, dz, p.ld, static_cast<int>(tiles_n));
           MCKE_LAUNCH_CHECK("lce_dz_kernel");
           return ok();
@@ -847,10 +881,15 @@ template <typename T> int lce_backward(const BwdArgs& a, const BwdPlan& p) {
       });
   if (rc) return rc;
   if (!a.dhidden) return ok();
-  const int64_t blocks = p.rows < 65536 ? p.rows : 65536;
-  lce_dh_store_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, a.s>>>(
+  // A wave a row and four groups of parts where there are parts, else as many lanes as columns.
+  int lanes_log2 = 3;
+  while (lanes_log2 < (p.parts > 4 ? 6 : 8) && (int64_t{8} << lanes_log2) < p.width) ++lanes_log2;
+  const dim3 grid(static_cast<unsigned>(p.rows < 65536 ? p.rows : 65536),
+                  static_cast<unsigned>(ceil_div(p.width, int64_t{8} << lanes_log2)));
+  lce_dh_store_kernel<T><<<grid, kThreads, 0, a.s>>>(
       dh, p.part_stride, static_cast<int>(p.parts), rows.rank, rows.meta,
-      static_cast<T*>(a.dhidden), static_cast<int>(p.rows), static_cast<int>(p.dim), width);
+      static_cast<T*>(a.dhidden), static_cast<int>(p.rows), static_cast<int>(p.dim), width,
+      lanes_log2);
   MCKE_LAUNCH_CHECK("lce_dh_store_kernel");
   return ok();
 }
