@@ -108,7 +108,7 @@ struct Zeros {
 // before it: a workgroup has 64 tokens, a lane each, and its waves deal out all of the keys in
 // chunks of 64 (in LDS; a chunk is compared with before, behind or at the workgroup's own).
 // 16384^2 comparisons are two operations each, 14 us over all CUs; sorted by one workgroup the
-// same took 24, in runs of 1024 and two merges LATER.  Workgroups from `blocks` on write zeros.
+// same took 24, in runs of 1024 and two merges 26.  Workgroups from `blocks` on write zeros.
 constexpr int kCount = 16384;
 
 __global__ __launch_bounds__(kRun) void embed_count_kernel(const int64_t* __restrict__ tokens,

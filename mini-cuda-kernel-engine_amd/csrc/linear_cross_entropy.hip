@@ -315,7 +315,7 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_stats_kernel(
 
 // loss and lse of packed rows from their parts.  A workgroup has 2^rows_log2 rows, up to 16, and
 // its other lanes the parts in turn: few loads are behind each other in a lane.  (64 rows a
-// workgroup: 4 rows of 2048 parts 26 us, LATER like this.)
+// workgroup: 4 rows of 2048 parts 26 us, like this 5.)
 constexpr int kJoinWaves = 16;
 
 __global__ __launch_bounds__(kJoinWaves * kWave) void lce_join_kernel(
@@ -388,30 +388,44 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows 
   static_assert(BM * kRowBytes <= S::kLdsBytes, "the tile must fit the stage buffers");
   __syncthreads();
   __builtin_amdgcn_sched_barrier(0);
+  const bool whole = !cut && m0 + BM <= n;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int rt = wm * WM + 16 * i + r16;
     const int64_t row = m0 + rt;
     const bool have = row < n;
     const float lse2 = have ? rows.lse2[row] : 0.0f, cp = have ? rows.cp[row] : 0.0f;
-    const float ct = have ? rows.ct[row] : 0.0f;
-    const int64_t t = (have ? rows.target[row] : -1) - (l.w.first + n0 + wn * WN) - 4 * g;
-    // Columns from `past` on, and rows without a target, are zeros whatever their exponentials
-    // are.
-    int past = have ? left : 0;
-    asm("" : "+v"(past));          // (as in the statistics)
+    const int64_t t = (have ? rows.target[row] : -1) - (l.w.first + n0 + wn * WN);
+    float v[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[j][e] = cp * __builtin_amdgcn_exp2f(__builtin_fmaf(acc_get(acc[i][j][e]), c, -lse2));
+    // The target's column, where it is one of this wave's.
+    if (__ballot(t >= 0 && t < WN)) {
+      const float ct = have ? rows.ct[row] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (t == 16 * j + 4 * g + e) v[j][e] -= ct;
+    }
+    // Columns past the weights, and rows past the last, are zeros whatever their exponentials are.
+    if (!whole) {
+      int past = have ? left : 0;
+      asm("" : "+v"(past));        // (as in the statistics)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (16 * j + e >= past) v[j][e] = 0.0f;
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       Quad o;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p =
-            __builtin_amdgcn_exp2f(__builtin_fmaf(acc_get(acc[i][j][e]), c, -lse2));
-        float v = cp * p;
-        if (t == 16 * j + e) v -= ct;
-        if (16 * j + e >= past) v = 0.0f;
-        o.v[e] = O::from_f32(v);
-      }
+      for (int e = 0; e < 4; ++e) o.v[e] = O::from_f32(v[j][e]);
       const int col = wn * WN + 16 * j + 4 * g;
       *reinterpret_cast<Quad*>(smem + rt * kRowBytes + (((col / 8) ^ (rt % kSwz)) * 16) +
                                (col % 8) * 2) = o;
@@ -528,16 +542,21 @@ __global__ __launch_bounds__(kThreads) void lce_dh_store_kernel(
   }
 }
 
-// dW's rows of a piece: dz^T H, the factor taken out.
-template <typename T, int BM, int BN>
-__global__ __launch_bounds__(kMfmaThreads, 1) void lce_dw_kernel(
+// dW's rows of a piece: dz^T H, the factor taken out.  ONE: for up to 64 rows, a single stage.
+// `lines`: rows are whole 128-byte lines, and go past the caches, which the weights are read
+// through again (4 x 131072 x 4096: the next call's logits 247 -> 178 us).  Cut lines do not: 13 x
+// 27442 x 4918 took 124 us so, and 77 through the caches.
+template <typename T, int BM, int BN, bool ONE>
+__global__ __launch_bounds__(kMfmaThreads, ONE ? 4 : 1) void lce_dw_kernel(
     const uint16_t* __restrict__ dz, int64_t ld, const uint16_t* __restrict__ hidden, int width,
-    const Meta* __restrict__ meta, T* __restrict__ dweight, int64_t piece, int cols, int tiles_m,
-    int tiles_n) {
+    const Meta* __restrict__ meta, T* __restrict__ dweight, int64_t piece, int cols, bool lines,
+    int tiles_m, int tiles_n) {
   using S = LpAnyShape<BM, BN, Along::kAcrossK, Along::kAcrossK>;
   using O = LpOut<T>;
   constexpr int MT = S::MT, NT = S::NT, WM = BM / 2, WN = BN / 2;
-  __shared__ __attribute__((aligned(1024))) char smem[S::kLdsBytes];
+  constexpr int kLds = ONE ? kLdsOne<BM, BN> : S::kLdsBytes;
+  static_assert(BM * BN * 2 <= kLds, "the tile must fit the stage buffers");
+  __shared__ __attribute__((aligned(1024))) char smem[kLds];
   int tm, tn;
   mfma_tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
   const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
@@ -545,7 +564,10 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dw_kernel(
   const LpOperand A{dz, ld, ld};
   const LpOperand B{hidden, width, width};
   f32x4 acc[MT][NT];
-  lp_any_loop<T, BM, BN, Along::kAcrossK, Along::kAcrossK>(acc, smem, A, B, m0, n0, 0, stages);
+  if constexpr (ONE)
+    lp_any_one<T, BM, BN, Along::kAcrossK, Along::kAcrossK>(acc, smem, A, B, m0, n0);
+  else
+    lp_any_loop<T, BM, BN, Along::kAcrossK, Along::kAcrossK>(acc, smem, A, B, m0, n0, 0, stages);
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
   const float unfactor = meta->unfactor;
@@ -579,7 +601,8 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dw_kernel(
     if (m0 + rt >= piece) continue;
     T* to = dweight + (m0 + rt) * cols + col;
     if (col + 8 <= cols) {
-      *reinterpret_cast<u32x4_a2*>(to) = v;
+      if (lines) __builtin_nontemporal_store(static_cast<u32x4_a2>(v), reinterpret_cast<u32x4_a2*>(to));
+      else *reinterpret_cast<u32x4_a2*>(to) = v;
     } else {
       const VecT16<T> w = __builtin_bit_cast(VecT16<T>, v);
 #pragma unroll
@@ -649,7 +672,7 @@ struct Plan {
     tile = tile_of(r, backward ? (piece < v ? piece : v) : v);
   }
   // Tiles of logits over `n` rows of the weights.
-  int64_t tiles(int64_t n) const {
+  int64_t logits_tiles(int64_t n) const {
     return ceil_div(rows, tile_rows(tile)) * ceil_div(n, tile_cols(tile));
   }
   int64_t take(int64_t bytes) {
@@ -698,22 +721,30 @@ struct FwdPlan : Plan {
 struct BwdPlan : Plan {
   RowsAt r;
   Tile dh_tile, dw_tile;
-  int64_t dz, ld, parts, stages_per_part, dh, part_stride;
+  int64_t dz, ld, dh_tiles, parts, stages_per_part, dh, part_stride;   // (tiles and parts of dH)
   BwdPlan(int64_t rows, int64_t vocab, int64_t dim) : Plan(rows, vocab, dim, true), r(*this, true) {
     ld = piece;
     dz = take(2 * up * ld);
-    dh_tile = tile_of(rows, dim);
-    // Few tiles of dH share a piece's stages: up to two workgroups a CU, at least 8 stages each, and
-    // up to 64 MB of sums.
-    const int64_t tiles = ceil_div(rows, tile_rows(dh_tile)) * ceil_div(dim, tile_cols(dh_tile));
-    const int64_t stages = ceil_div(piece < vocab ? piece : vocab, 64);
-    parts = (dh_tile == Tile::k256 ? 256 : 512) / tiles;
+    // Few tiles of dH share a piece's stages: up to a workgroup a CU at 256 x 256 and two at smaller
+    // tiles, at least 8 stages each, and up to 80 MB of sums.  256 x 256 from 192 workgroups on
+    // (2047 x 32001 x 1024 fp16: 109 us with 8 parts, against 136 at 128 x 128 with 4).
     part_stride = up * width;
-    if (parts > (int64_t{1} << 24) / part_stride) parts = (int64_t{1} << 24) / part_stride;
-    if (parts > ceil_div(stages, 8)) parts = ceil_div(stages, 8);
-    if (parts < 1) parts = 1;
-    stages_per_part = ceil_div(stages, parts);
-    parts = ceil_div(stages, stages_per_part);
+    const int64_t stages = ceil_div(piece < vocab ? piece : vocab, 64);
+    auto share = [&](Tile t) {
+      dh_tiles = ceil_div(rows, tile_rows(t)) * ceil_div(dim, tile_cols(t));
+      parts = (t == Tile::k256 ? 256 : 512) / dh_tiles;
+      if (parts > 20 * (int64_t{1} << 20) / part_stride) parts = 20 * (int64_t{1} << 20) / part_stride;
+      if (parts > ceil_div(stages, 8)) parts = ceil_div(stages, 8);
+      if (parts < 1) parts = 1;
+      stages_per_part = ceil_div(stages, parts);
+      parts = ceil_div(stages, stages_per_part);
+    };
+    dh_tile = Tile::k256;
+    if (rows > 128 && dim > 128) share(dh_tile);
+    if (rows <= 128 || dim <= 128 || dh_tiles * parts < 192) {
+      dh_tile = rows <= 64 ? Tile::k64x128 : Tile::k128;
+      share(dh_tile);
+    }
     dh = take(4 * parts * part_stride);
     dw_tile = rows > 128 && ceil_div(piece, 256) * ceil_div(dim, 256) >= 192 ? Tile::k256 : Tile::k128;
   }
@@ -795,9 +826,9 @@ int lce_forward(const void* hidden, const void* weight, const int64_t* targets, 
   float* sums = reinterpret_cast<float*>(ws + p.sums);
   float* at_target = reinterpret_cast<float*>(ws + p.at_target);
   const int rc = for_pieces(p, p.r, weight, ws, s, [&](const Piece& w) {
-    return with_logits_tile(p.tile, p.tiles(w.rows), [&](auto bm, auto bn, auto d) {
+    return with_logits_tile(p.tile, p.logits_tiles(w.rows), [&](auto bm, auto bn, auto d) {
       constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, D = decltype(d)::value;
-      const int64_t tiles_n = ceil_div(w.rows, BN), tiles = p.tiles(w.rows);
+      const int64_t tiles_n = ceil_div(w.rows, BN), tiles = p.logits_tiles(w.rows);
       lce_stats_kernel<T, BM, BN, D><<<static_cast<unsigned>(tiles), kMfmaThreads, 0, s>>>(
           Logits{packed, static_cast<int>(p.width), w, scale}, rows.meta, rows.target, largest,
           sums, at_target, p.stride, static_cast<int>(w.first / BN), static_cast<int>(tiles_n));
@@ -838,14 +869,15 @@ template <typename T> int lce_backward(const BwdArgs& a, const BwdPlan& p) {
   MCKE_LAUNCH_CHECK("lce_rows_kernel");
   const uint16_t* packed = reinterpret_cast<const uint16_t*>(a.ws + p.r.hidden);
   if (int rc = pack_rows(p, p.r, a.hidden, a.weight, a.ws, a.s)) return rc;
+  const bool lines = p.dim % 64 == 0 && aligned(a.dweight, 128);
   uint16_t* dz = reinterpret_cast<uint16_t*>(a.ws + p.dz);
   float* dh = reinterpret_cast<float*>(a.ws + p.dh);
   const int width = static_cast<int>(p.width);
   const int rc =
       for_pieces(p, p.r, a.weight, a.ws, a.s, [&](const Piece& w) {
-        int rc = with_logits_tile(p.tile, p.tiles(w.rows), [&](auto bm, auto bn, auto d) {
+        int rc = with_logits_tile(p.tile, p.logits_tiles(w.rows), [&](auto bm, auto bn, auto d) {
           constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, D = decltype(d)::value;
-          const int64_t tiles_n = ceil_div(w.rows, BN), tiles = p.tiles(w.rows);
+          const int64_t tiles_n = ceil_div(w.rows, BN), tiles = p.logits_tiles(w.rows);
           lce_dz_kernel<T, BM, BN, D><<<static_cast<unsigned>(tiles), kMfmaThreads, 0, a.s>>>(
               Logits{packed, width, w, a.scale}, rows, dz, p.ld, static_cast<int>(tiles_n));
           MCKE_LAUNCH_CHECK("lce_dz_kernel");
@@ -867,17 +899,22 @@ template <typename T> int lce_backward(const BwdArgs& a, const BwdPlan& p) {
           if (rc) return rc;
         }
         if (!a.dweight) return ok();
-        auto dw = [&](auto bt) {
+        auto dw = [&](auto bt, auto one) {
           constexpr int B = decltype(bt)::value;
           const int64_t tiles_m = ceil_div(w.rows, B), tiles_n = ceil_div(p.dim, B);
-          lce_dw_kernel<T, B, B><<<static_cast<unsigned>(tiles_m * tiles_n), kMfmaThreads, 0, a.s>>>(
-              dz, p.ld, packed, width, rows.meta, static_cast<T*>(a.dweight) + w.first * p.dim, w.rows,
-              static_cast<int>(p.dim), static_cast<int>(tiles_m), static_cast<int>(tiles_n));
+          lce_dw_kernel<T, B, B, decltype(one)::value>
+              <<<static_cast<unsigned>(tiles_m * tiles_n), kMfmaThreads, 0, a.s>>>(
+                  dz, p.ld, packed, width, rows.meta, static_cast<T*>(a.dweight) + w.first * p.dim,
+                  w.rows, static_cast<int>(p.dim), lines, static_cast<int>(tiles_m),
+                  static_cast<int>(tiles_n));
           MCKE_LAUNCH_CHECK("lce_dw_kernel");
           return ok();
         };
-        return p.dw_tile == Tile::k256 ? dw(std::integral_constant<int, 256>{})
-                                       : dw(std::integral_constant<int, 128>{});
+        using I128 = std::integral_constant<int, 128>;
+        if (p.rows <= 64) return dw(I128{}, std::true_type{});
+        if (p.dw_tile == Tile::k256)
+          return dw(std::integral_constant<int, 256>{}, std::false_type{});
+        return dw(I128{}, std::false_type{});
       });
   if (rc) return rc;
   if (!a.dhidden) return ok();
