@@ -68,65 +68,91 @@ struct Rows {
   float* ct;
 };
 
+// What dz is stored times, and its inverse, for the largest gradient m of a row.
+__device__ __forceinline__ void factors(float m, float& factor, float& unfactor) {
+  factor = unfactor = 1.0f;
+  if (m > 0.0f) {
+    m = fmaxf(m, 0x1p-100f);       // (2^14 / m stays finite)
+    factor = 0x1p14f / m;
+    unfactor = m * 0x1p-14f;
+  }
+}
+
+struct RowsIn {
+  const int64_t* targets;
+  const float* lse;              // null forward
+  const float* dloss;
+  const float* dlse;
+  int rows;
+  int64_t vocab;
+  float scale;
+  // The largest gradient of row r, 0 where that is not finite or the row has no target.
+  __device__ __forceinline__ float size(int r) const {
+    if (targets[r] < 0) return 0.0f;
+    const float a = dloss ? scale * dloss[r] : 0.0f, b = dlse ? scale * dlse[r] : 0.0f;
+    const float big = __builtin_fabsf(a) + __builtin_fabsf(b);
+    return big < __builtin_inff() ? big : 0.0f;
+  }
+};
+
+// Row r, whose target is t >= 0, is packed row k.
+template <bool BACKWARD>
+__device__ __forceinline__ void put_row(const RowsIn& in, const Rows& out, int r, int64_t t, int k,
+                                        float factor) {
+  out.rank[r] = k;
+  out.from[k] = r;
+  out.target[k] = t < in.vocab ? static_cast<int>(t) : -2;
+  if constexpr (BACKWARD) {
+    const float a = in.dloss ? in.scale * in.dloss[r] * factor : 0.0f;
+    const float b = in.dlse ? in.scale * in.dlse[r] * factor : 0.0f;
+    out.lse2[k] = in.lse[r] * kLog2e;
+    out.cp[k] = t < in.vocab ? a + b : __builtin_nanf("");
+    out.ct[k] = a;
+  }
+}
+// Row r has no target.
+__device__ __forceinline__ void put_none(const Rows& out, int r, float* loss, float* lse) {
+  out.rank[r] = -1;
+  if (loss) loss[r] = 0.0f;
+  if (lse) lse[r] = 0.0f;
+}
+
 // ---------------------------------------------------------------------------
 // Rows that have a target, in order; one workgroup.
 // ---------------------------------------------------------------------------
 template <bool BACKWARD>
-__global__ __launch_bounds__(kPrepThreads) void lce_rows_kernel(
-    const int64_t* __restrict__ targets, const float* __restrict__ lse,
-    const float* __restrict__ dloss, const float* __restrict__ dlse, int rows, int64_t vocab,
-    float scale, Rows out, float* __restrict__ loss_out, float* __restrict__ lse_out) {
-  __shared__ int waves[kPrepThreads / kWave];
-  __shared__ float most[kPrepThreads / kWave];
+__global__ __launch_bounds__(kPrepThreads) void lce_rows_kernel(RowsIn in, Rows out,
+                                                               float* __restrict__ loss,
+                                                               float* __restrict__ lse) {
+  constexpr int W = kPrepThreads / kWave;
+  static_assert(W == 16, "a value of each wave to the lanes of a row of 16");
+  __shared__ int waves[W];
+  __shared__ float most[W];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   float factor = 1.0f, unfactor = 1.0f;
   if constexpr (BACKWARD) {
     float m = 0.0f;
-    for (int r = threadIdx.x; r < rows; r += kPrepThreads) {
-      if (targets[r] < 0) continue;
-      const float a = dloss ? scale * dloss[r] : 0.0f, b = dlse ? scale * dlse[r] : 0.0f;
-      const float big = __builtin_fabsf(a) + __builtin_fabsf(b);
-      m = fmaxf(m, big < __builtin_inff() ? big : 0.0f);
-    }
+    for (int r = threadIdx.x; r < in.rows; r += kPrepThreads) m = fmaxf(m, in.size(r));
     m = wave_max(m);
     if (lane == 0) most[wave] = m;
     __syncthreads();
-    m = wave_max<16>(most[threadIdx.x % 16]);
-    if (m > 0.0f) {
-      m = fmaxf(m, 0x1p-100f);     // (2^14 / m stays finite)
-      factor = 0x1p14f / m;
-      unfactor = m * 0x1p-14f;
-    }
-    static_assert(kPrepThreads / kWave == 16, "one value of each wave");
+    factors(wave_max<W>(most[threadIdx.x % W]), factor, unfactor);
   }
   int count = 0;
-  for (int r0 = 0; r0 < rows; r0 += kPrepThreads) {
+  for (int r0 = 0; r0 < in.rows; r0 += kPrepThreads) {
     const int r = r0 + threadIdx.x;
-    const int64_t t = r < rows ? targets[r] : -1;
+    const int64_t t = r < in.rows ? in.targets[r] : -1;
     const uint64_t set = __ballot(t >= 0);
     if (lane == 0) waves[wave] = __popcll(set);
     __syncthreads();
     int before = count + __popcll(set & ((uint64_t{1} << lane) - 1));
-    for (int w = 0; w < kPrepThreads / kWave; ++w) {
+    for (int w = 0; w < W; ++w) {
       if (w < wave) before += waves[w];
       count += waves[w];
     }
-    if (r < rows) {
-      out.rank[r] = t >= 0 ? before : -1;
-      if (t >= 0) {
-        out.from[before] = r;
-        out.target[before] = t < vocab ? static_cast<int>(t) : -2;
-        if constexpr (BACKWARD) {
-          const float a = dloss ? scale * dloss[r] * factor : 0.0f;
-          const float b = dlse ? scale * dlse[r] * factor : 0.0f;
-          out.lse2[before] = lse[r] * kLog2e;
-          out.cp[before] = t < vocab ? a + b : __builtin_nanf("");
-          out.ct[before] = a;
-        }
-      } else {
-        if (loss_out) loss_out[r] = 0.0f;
-        if (lse_out) lse_out[r] = 0.0f;
-      }
+    if (r < in.rows) {
+      if (t >= 0) put_row<BACKWARD>(in, out, r, t, before, factor);
+      else put_none(out, r, loss, lse);
     }
     __syncthreads();
   }
@@ -155,6 +181,30 @@ __device__ __forceinline__ u16x8 load8(const uint16_t* __restrict__ x, int64_t n
   return v;
 }
 
+// Workgroup `block` of `blocks` copies its part of the tail.
+__device__ __forceinline__ void copy_tail(const Tail& tail, int64_t block, int64_t blocks) {
+  for (int64_t i = 8 * (block * kThreads + threadIdx.x); i < tail.all; i += 8 * blocks * kThreads) {
+    const u16x8 v = load8(tail.from + i, tail.values - i);
+    if (i + 8 <= tail.all) {
+      *reinterpret_cast<u16x8*>(tail.to + i) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i + e < tail.all) tail.to[i + e] = v[e];
+    }
+  }
+}
+
+// A row of `cols` values (null: none) as one of `width`, zeros behind it.
+__device__ __forceinline__ void copy_row(const uint16_t* __restrict__ row, uint16_t* __restrict__ to,
+                                         int cols, int width) {
+  for (int c = 8 * threadIdx.x; c < width; c += 8 * kThreads)
+    *reinterpret_cast<u16x8*>(to + c) = load8(row ? row + c : nullptr, cols - c);
+}
+
+// Rows of zeros follow the packed ones up to here.
+__device__ __forceinline__ int rows_up(int n) { return n > 0 ? (n + 63) / 64 * 64 : 64; }
+
 // Packed rows: row k of `to` (`width` values, a multiple of 64) is row from[k] of x (`cols`
 // values) with zeros behind it, and behind the last row are rows of zeros up to the next multiple
 // of 64 (64 at least).  from null: the `given` rows as they are, and zeros up to `rows`.  A
@@ -164,18 +214,7 @@ __global__ __launch_bounds__(kThreads) void lce_pack_kernel(
     uint16_t* __restrict__ to, int64_t given, int64_t rows, int cols, int width, int blocks,
     Tail tail) {
   if (static_cast<int>(blockIdx.x) >= blocks) {
-    const int64_t step = 8 * static_cast<int64_t>(gridDim.x - blocks) * kThreads;
-    for (int64_t i = 8 * (static_cast<int64_t>(blockIdx.x - blocks) * kThreads + threadIdx.x);
-         i < tail.all; i += step) {
-      const u16x8 v = load8(tail.from + i, tail.values - i);
-      if (i + 8 <= tail.all) {
-        *reinterpret_cast<u16x8*>(tail.to + i) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (i + e < tail.all) tail.to[i + e] = v[e];
-      }
-    }
+    copy_tail(tail, blockIdx.x - blocks, gridDim.x - blocks);
     return;
   }
   for (int64_t k = blockIdx.x; k < rows; k += blocks) {
@@ -183,13 +222,69 @@ __global__ __launch_bounds__(kThreads) void lce_pack_kernel(
     if (!from) {
       if (k < given) row = x + k * cols;
     } else {
-      const int n = meta->rows, up = n > 0 ? (n + 63) / 64 * 64 : 64;
-      if (k >= up) return;
+      const int n = meta->rows;
+      if (k >= rows_up(n)) return;
       if (k < n) row = x + static_cast<int64_t>(from[k]) * cols;
     }
-    for (int c = 8 * threadIdx.x; c < width; c += 8 * kThreads)
-      *reinterpret_cast<u16x8*>(to + k * width + c) = load8(row ? row + c : nullptr, cols - c);
+    copy_row(row, to + k * width, cols, width);
   }
+}
+
+// Both for up to kFewRows rows: each workgroup has a row, counts the targets before it, and copies
+// its row there; those without a target make the zeros behind the packed rows.  (A launch less: 4
+// us of 16 for two tokens over a small vocabulary.)
+constexpr int kFewRows = 1024;
+
+template <bool BACKWARD>
+__global__ __launch_bounds__(kThreads) void lce_few_rows_kernel(
+    RowsIn in, Rows out, float* __restrict__ loss, float* __restrict__ lse,
+    const uint16_t* __restrict__ x, uint16_t* __restrict__ to, int cols, int width, int blocks,
+    Tail tail) {
+  constexpr int W = kThreads / kWave;
+  __shared__ int counts[2][W];
+  __shared__ float most[W];
+  if (static_cast<int>(blockIdx.x) >= blocks) {
+    copy_tail(tail, blockIdx.x - blocks, gridDim.x - blocks);
+    return;
+  }
+  const int mine = blockIdx.x, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  int before = 0, n = 0;
+  float m = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kFewRows / kThreads; ++k) {
+    const int r = k * kThreads + threadIdx.x;
+    const bool has = r < in.rows && in.targets[r] >= 0;
+    before += __popcll(__ballot(has && r < mine));
+    n += __popcll(__ballot(has));
+    if constexpr (BACKWARD)
+      if (has) m = fmaxf(m, in.size(r));
+  }
+  if constexpr (BACKWARD) m = wave_max(m);
+  if (lane == 0) {
+    counts[0][wave] = before;
+    counts[1][wave] = n;
+    most[wave] = m;
+  }
+  __syncthreads();
+  before = n = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    before += counts[0][w];
+    n += counts[1][w];
+    m = fmaxf(m, most[w]);
+  }
+  float factor, unfactor;
+  factors(m, factor, unfactor);
+  const int64_t t = mine < in.rows ? in.targets[mine] : -1;
+  if (threadIdx.x == 0) {
+    if (mine == 0) *out.meta = Meta{n, factor, unfactor, 0};
+    if (t >= 0) put_row<BACKWARD>(in, out, mine, t, before, factor);
+    else if (mine < in.rows) put_none(out, mine, loss, lse);
+  }
+  const int k = t >= 0 ? before : n + mine - before;
+  if (k < rows_up(n))
+    copy_row(t >= 0 ? x + static_cast<int64_t>(mine) * cols : nullptr,
+             to + static_cast<int64_t>(k) * width, cols, width);
 }
 
 // ---------------------------------------------------------------------------
@@ -435,7 +530,7 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows 
   __syncthreads();
   constexpr int kRowsPerPass = kMfmaThreads / kChunks;
   const int q = threadIdx.x % kChunks;
-  const int up = n > 0 ? (n + 63) / 64 * 64 : 64;
+  const int up = rows_up(n);
 #pragma unroll 4
   for (int r0 = 0; r0 < BM; r0 += kRowsPerPass) {
     const int rt = r0 + threadIdx.x / kChunks;
@@ -547,7 +642,7 @@ __global__ __launch_bounds__(kThreads) void lce_dh_store_kernel(
 // through again (4 x 131072 x 4096: the next call's logits 247 -> 178 us).  Cut lines do not: 13 x
 // 27442 x 4918 took 124 us so, and 77 through the caches.
 template <typename T, int BM, int BN, bool ONE>
-__global__ __launch_bounds__(kMfmaThreads, ONE ? 4 : 1) void lce_dw_kernel(
+__global__ __launch_bounds__(kMfmaThreads, ONE ? 3 : 1) void lce_dw_kernel(
     const uint16_t* __restrict__ dz, int64_t ld, const uint16_t* __restrict__ hidden, int width,
     const Meta* __restrict__ meta, T* __restrict__ dweight, int64_t piece, int cols, bool lines,
     int tiles_m, int tiles_n) {
@@ -771,24 +866,40 @@ template <class F> int with_logits_tile(Tile t, int64_t tiles, F f) {
   });
 }
 
+unsigned tail_blocks(const Tail& tail) {
+  const int64_t blocks = ceil_div(tail.all, 8 * kThreads);
+  return static_cast<unsigned>(blocks < 1024 ? blocks : 1024);
+}
+
 int launch_pack(const void* x, const int* from, const Meta* meta, void* to, int64_t given,
                 int64_t rows, int64_t cols, int64_t width, const Tail& tail, hipStream_t s) {
   const int blocks = static_cast<int>(rows < 65536 ? rows : 65536);
-  const int64_t more = ceil_div(tail.all, 8 * kThreads), extra = more < 1024 ? more : 1024;
-  lce_pack_kernel<<<static_cast<unsigned>(blocks + extra), kThreads, 0, s>>>(
+  lce_pack_kernel<<<static_cast<unsigned>(blocks) + tail_blocks(tail), kThreads, 0, s>>>(
       static_cast<const uint16_t*>(x), from, meta, static_cast<uint16_t*>(to), given, rows,
       static_cast<int>(cols), static_cast<int>(width), blocks, tail);
   MCKE_LAUNCH_CHECK("lce_pack_kernel");
   return ok();
 }
 
-// The hidden states' rows, and the tail of the weights.
-int pack_rows(const Plan& p, const RowsAt& r, const void* hidden, const void* weight, char* ws,
-              hipStream_t s) {
+// The rows that have a target, their hidden states, and the tail of the weights.
+template <bool BACKWARD>
+int pack_rows(const Plan& p, const RowsAt& r, const RowsIn& in, float* loss, float* lse,
+              const void* hidden, const void* weight, char* ws, hipStream_t s) {
   const Rows rows = r.rows(ws);
   const uint16_t* last = static_cast<const uint16_t*>(weight) + p.tail_first * p.dim;
   const Tail tail{last, reinterpret_cast<uint16_t*>(ws + r.weight),
                   p.tail_values ? (p.vocab - p.tail_first) * p.dim : 0, p.tail_values};
+  if (p.rows <= kFewRows) {
+    lce_few_rows_kernel<BACKWARD>
+        <<<static_cast<unsigned>(p.up) + tail_blocks(tail), kThreads, 0, s>>>(
+            in, rows, loss, lse, static_cast<const uint16_t*>(hidden),
+            reinterpret_cast<uint16_t*>(ws + r.hidden), static_cast<int>(p.dim),
+            static_cast<int>(p.width), static_cast<int>(p.up), tail);
+    MCKE_LAUNCH_CHECK("lce_few_rows_kernel");
+    return ok();
+  }
+  lce_rows_kernel<BACKWARD><<<1, kPrepThreads, 0, s>>>(in, rows, loss, lse);
+  MCKE_LAUNCH_CHECK("lce_rows_kernel");
   return launch_pack(hidden, rows.from, rows.meta, ws + r.hidden, p.rows, p.up, p.dim, p.width,
                      tail, s);
 }
@@ -816,12 +927,9 @@ template <typename T>
 int lce_forward(const void* hidden, const void* weight, const int64_t* targets, float* loss,
                 float* lse, const FwdPlan& p, float scale, char* ws, hipStream_t s) {
   const Rows rows = p.r.rows(ws);
-  lce_rows_kernel<false><<<1, kPrepThreads, 0, s>>>(targets, nullptr, nullptr, nullptr,
-                                                    static_cast<int>(p.rows), p.vocab, scale, rows,
-                                                    loss, lse);
-  MCKE_LAUNCH_CHECK("lce_rows_kernel");
+  const RowsIn in{targets, nullptr, nullptr, nullptr, static_cast<int>(p.rows), p.vocab, scale};
+  if (int rc = pack_rows<false>(p, p.r, in, loss, lse, hidden, weight, ws, s)) return rc;
   const uint16_t* packed = reinterpret_cast<const uint16_t*>(ws + p.r.hidden);
-  if (int rc = pack_rows(p, p.r, hidden, weight, ws, s)) return rc;
   float* largest = reinterpret_cast<float*>(ws + p.largest);
   float* sums = reinterpret_cast<float*>(ws + p.sums);
   float* at_target = reinterpret_cast<float*>(ws + p.at_target);
@@ -863,12 +971,10 @@ struct BwdArgs {
 
 template <typename T> int lce_backward(const BwdArgs& a, const BwdPlan& p) {
   const Rows rows = p.r.rows(a.ws);
-  lce_rows_kernel<true><<<1, kPrepThreads, 0, a.s>>>(a.targets, a.lse, a.dloss, a.dlse,
-                                                     static_cast<int>(p.rows), p.vocab, a.scale,
-                                                     rows, nullptr, nullptr);
-  MCKE_LAUNCH_CHECK("lce_rows_kernel");
+  const RowsIn in{a.targets, a.lse, a.dloss, a.dlse, static_cast<int>(p.rows), p.vocab, a.scale};
+  if (int rc = pack_rows<true>(p, p.r, in, nullptr, nullptr, a.hidden, a.weight, a.ws, a.s))
+    return rc;
   const uint16_t* packed = reinterpret_cast<const uint16_t*>(a.ws + p.r.hidden);
-  if (int rc = pack_rows(p, p.r, a.hidden, a.weight, a.ws, a.s)) return rc;
   const bool lines = p.dim % 64 == 0 && aligned(a.dweight, 128);
   uint16_t* dz = reinterpret_cast<uint16_t*>(a.ws + p.dz);
   float* dh = reinterpret_cast<float*>(a.ws + p.dh);

@@ -167,9 +167,11 @@ def test_pieces(gpu, shape):
 
 @pytest.mark.parametrize("dt", TYPES, ids=[ID[t] for t in TYPES])
 @pytest.mark.parametrize("keep", ["none", "one", "last 64", "all"])
-def test_rows_without_a_target(gpu, dt, keep):
-    """They are not read (NaN in their place changes no bit), give zeros and add nothing."""
-    rows, vocab, dim = 333, 700, 128
+@pytest.mark.parametrize("rows", [333, 1024, 1025])
+def test_rows_without_a_target(gpu, dt, keep, rows):
+    """They are not read (NaN in their place changes no bit), give zeros and add nothing; by either
+    way of packing the others (up to 1024 rows, and more)."""
+    vocab, dim = 700, 128
     h, w, t = _draw(rows, vocab, dim, dt, 5)
     t = t.abs() % vocab
     if keep != "all":
