@@ -439,8 +439,8 @@ int mcke_launch_linear_cross_entropy(const void* hidden, const void* weight, con
  *   dhidden = dz weight, dweight = dz^T hidden
  * dloss or dlse (rows values) may be null, not both; dhidden (as hidden) or dweight (as weight, at
  * any alignment of its type) may be null, not both; they are overwritten.  dz is rounded to dtype
- * once, relative to the largest gradient of a row in fp16.  rows == 0 gives a
- * dweight of zeros. */
+ * once, as a multiple of the largest |dloss| + |dlse| of a row, so that small ones keep their bits.
+ * rows == 0 gives a dweight of zeros. */
 int mcke_launch_linear_cross_entropy_backward(const void* hidden, const void* weight,
                                               const int64_t* targets, const float* lse,
                                               const float* dloss, const float* dlse, void* dhidden,

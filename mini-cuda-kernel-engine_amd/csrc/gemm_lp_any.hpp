@@ -79,7 +79,7 @@ template <int B, Along L> struct LpAnyOperand {
 
   // A DMA instruction's immediate offset (1 KB times its index, modulo four) moves its source too:
   // the offsets have it taken off, and are kept positive by 3 KB that the base gives back.
-  static constexpr uint32_t kBias = 3072;
+  static constexpr uint32_t kBias = 3 * 1024;
 
   // The workgroup's rows or columns begin at `first`, the wave's at `wave_first` of them.
   __device__ __forceinline__ void begin(const LpOperand& o, int64_t first, int wave_first,
