@@ -299,13 +299,31 @@ __device__ __forceinline__ bool tile_of_rows(int n, int tiles_n, int& tm, int& t
   return true;
 }
 
-__device__ __forceinline__ float across_groups_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+// Over the lanes 16 and 32 apart, each step a swap of half the lanes of two copies.
+template <class F> __device__ __forceinline__ float across_groups(float v, F f) {
+  auto both = [&](auto pair) {
+    const unsigned a = pair[0], b = pair[1];
+    v = f(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    return __builtin_bit_cast(unsigned, v);
+  };
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const unsigned w = both(__builtin_amdgcn_permlane16_swap(u, u, false, false));
+  both(__builtin_amdgcn_permlane32_swap(w, w, false, false));
+  return v;
 }
-__device__ __forceinline__ float across_groups_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+
+// x[row] of the rows row0, row0 + 16, .. that are below n, `none` for others.  Loaded before a
+// tile's products, behind which nothing waits for them: a wave has its SIMD to itself.  (4096 x
+// 65536 x 128 bf16: the forward pass takes 177 us with each row's loads where they are used, and
+// with __shfl_xor across the groups; 152 like this.)
+template <int MT, typename T>
+__device__ __forceinline__ void of_rows(T (&v)[MT], const T* x, int64_t row0, int n, T none) {
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t row = row0 + 16 * i;
+    v[i] = x[row < n ? row : 0];
+    v[i] = row < n ? v[i] : none;
+  }
 }
 
 // A piece of the weights: `rows` rows from `first` on, `row` values apart.  Rows from tail_first
@@ -351,11 +369,13 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_stats_kernel(
   int tm, tn;
   if (!tile_of_rows<BM>(n, tiles_n, tm, tn)) return;
   const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
+  int t[MT];
+  of_rows(t, target, m0 + wm * (BM / 2) + r16, n, -1);
   f32x4 acc[MT][NT];
   logits_tile<BM, BN, D, T>(acc, smem, l, n, m0, n0);
 
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
   const float c = l.scale * kLog2e;
   // Columns of the wave that are in the vocabulary, less this lane's 4 g.
   const bool cut = n0 + BN > l.w.rows;
@@ -383,26 +403,29 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_stats_kernel(
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) m = fmaxf(m, v[j][e]);
-    m = across_groups_max(m);
-    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    m = across_groups(m, [](float a, float b) { return fmaxf(a, b); });
+    // Exponentials of c v - fl(c m), one operation, and what fl() took off put back into their sum.
+    const float ref = m == -__builtin_inff() ? 0.0f : m, cref = c * ref;
     float s = 0.0f;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((v[j][e] - ref) * c);
-    s = across_groups_sum(s);
+      for (int e = 0; e < 4; ++e)
+        s += __builtin_amdgcn_exp2f(__builtin_fmaf(c, v[j][e], -cref));
+    s = across_groups(s, [](float a, float b) { return a + b; });
+    s *= __builtin_amdgcn_exp2f(-__builtin_fmaf(c, ref, -cref));
     if (g == 0 && row < n) {
       largest[at * stride + row] = m;
       sums[at * stride + row] = s;
     }
     // The target's column, where it is one of this wave's.
-    const int64_t t = (row < n ? target[row] : -1) - (l.w.first + n0 + wn * WN);
-    if (__ballot(t >= 0 && t < WN)) {
+    const int tc = t[i] - static_cast<int>(l.w.first + n0 + wn * WN);
+    if (__ballot(tc >= 0 && tc < WN)) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (t == 16 * j + 4 * g + e) at_target[row] = v[j][e];
+          if (tc == 16 * j + 4 * g + e) at_target[row] = v[j][e];
     }
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -427,33 +450,45 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void lce_join_kernel(
   float m = -__builtin_inff(), s = 0.0f;
   auto add = [&](float m2, float s2) {
     // (An empty part has no largest logit; -inf against itself moves nothing.)
-    const float to = fmaxf(m, m2);
-    const float f = m == to ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
-    const float f2 = m2 == to ? 1.0f : __builtin_amdgcn_exp2f((m2 - to) * c);
+    const float most = fmaxf(m, m2);
+    const float f = m == most ? 1.0f : __builtin_amdgcn_exp2f((m - most) * c);
+    const float f2 = m2 == most ? 1.0f : __builtin_amdgcn_exp2f((m2 - most) * c);
     s = f * s + f2 * s2;
-    m = to;
+    m = most;
   };
+  // What the result wants, on its way with the parts.
+  const bool out = threadIdx.x < static_cast<unsigned>(rows) && row < n;
+  const int to = out ? from[row] : 0, t = out ? target[row] : -1;
+  const float z = out ? at_target[row] : 0.0f;
   const int step = kJoinWaves * kWave >> rows_log2;
   if (row < n) {
 #pragma unroll 8
     for (int p = threadIdx.x >> rows_log2; p < parts; p += step)
       add(largest[p * stride + row], sums[p * stride + row]);
   }
-  // The lanes of a row, the lowest of which counts; then the waves in their order.
-  for (int d = kWave / 2; d >= rows; d /= 2) {
-    const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
-    add(m2, s2);
-  }
+  // The lanes of a row; then the waves, by the first one in the same way.
+  auto over_lanes = [&] {
+    for (int d = kWave / 2; d >= rows; d /= 2) {
+      const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
+      add(m2, s2);
+    }
+  };
+  over_lanes();
   if (lane < rows) {
     lm[wave][lane] = m;
     ls[wave][lane] = s;
   }
   __syncthreads();
-  if (threadIdx.x >= static_cast<unsigned>(rows) || row >= n) return;
-  for (int w = 1; w < kJoinWaves; ++w) add(lm[w][lane], ls[w][lane]);
+  if (wave > 0) return;
+  m = -__builtin_inff();
+  s = 0.0f;
+  for (int w = lane >> rows_log2; w < kJoinWaves; w += kWave >> rows_log2)
+    add(lm[w][lane % rows], ls[w][lane % rows]);
+  over_lanes();
+  if (!out) return;
   const float lse = __builtin_fmaf(kLn2, __builtin_amdgcn_logf(s), scale * m);
-  if (lse_out) lse_out[from[row]] = lse;
-  if (loss) loss[from[row]] = target[row] < 0 ? __builtin_nanf("") : lse - scale * at_target[row];
+  if (lse_out) lse_out[to] = lse;
+  if (loss) loss[to] = t < 0 ? __builtin_nanf("") : lse - scale * z;
 }
 
 // dz of a tile, row-major (`ld` values a row), zeros in rows and columns that pad it.
@@ -469,11 +504,17 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows 
   int tm, tn;
   if (!tile_of_rows<BM>(n, tiles_n, tm, tn)) return;
   const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * BN;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
+  const int64_t row0 = m0 + wm * WM + r16;
+  int target[MT];
+  float lse2[MT], cps[MT];
+  of_rows(target, rows.target, row0, n, -1);
+  of_rows(lse2, rows.lse2, row0, n, 0.0f);
+  of_rows(cps, rows.cp, row0, n, 0.0f);
   f32x4 acc[MT][NT];
   logits_tile<BM, BN, D, T>(acc, smem, l, n, m0, n0);
 
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
   const float c = l.scale * kLog2e;
   const bool cut = n0 + BN > l.w.rows;
   const int left = static_cast<int>(cut ? l.w.rows - n0 - wn * WN - 4 * g : BN);
@@ -489,14 +530,13 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows 
     const int rt = wm * WM + 16 * i + r16;
     const int64_t row = m0 + rt;
     const bool have = row < n;
-    const float lse2 = have ? rows.lse2[row] : 0.0f, cp = have ? rows.cp[row] : 0.0f;
-    const int64_t t = (have ? rows.target[row] : -1) - (l.w.first + n0 + wn * WN);
+    const int t = target[i] - static_cast<int>(l.w.first + n0 + wn * WN);
     float v[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        v[j][e] = cp * __builtin_amdgcn_exp2f(__builtin_fmaf(acc_get(acc[i][j][e]), c, -lse2));
+        v[j][e] = cps[i] * __builtin_amdgcn_exp2f(__builtin_fmaf(acc_get(acc[i][j][e]), c, -lse2[i]));
     // The target's column, where it is one of this wave's.
     if (__ballot(t >= 0 && t < WN)) {
       const float ct = have ? rows.ct[row] : 0.0f;
@@ -805,7 +845,7 @@ struct FwdPlan : Plan {
   RowsAt r;
   int64_t stride, parts, largest, sums, at_target;
   FwdPlan(int64_t rows, int64_t vocab, int64_t dim) : Plan(rows, vocab, dim, false), r(*this, false) {
-    stride = up;
+    stride = rows < 64 ? rows : up;      // (lines of 64 for 4 rows of 2048 parts: 8 us more)
     parts = 2 * ceil_div(vocab, tile_cols(tile));
     largest = take(4 * parts * stride);
     sums = take(4 * parts * stride);
