@@ -356,12 +356,13 @@ int mcke_launch_embedding(const int64_t* tokens, const void* table, void* out, i
                           int out_dtype, int64_t rows, int64_t vocab, int64_t cols, float scale,
                           void* stream);
 
-/* Bytes of workspace for the sorted tokens (0 for rows == 0); its contents on entry do not matter,
+/* Bytes of workspace (sorted tokens and sums of them; 0 for rows == 0); its contents on entry do not matter,
  * and two launches that may run at the same time need one each. */
 size_t mcke_embedding_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t cols);
 
 /* The gradient in the table:
  *   dtable[v] = scale * sum over r with tokens[r] == v, in the order of r, of dout[r]
+ * (the sums of consecutive parts of the rows are added up in their order);
  * zeros for tokens that are not there; accumulate != 0 adds to dtable instead, and touches the
  * rows of tokens that are there alone (tied weights: the loss's gradient is there already).
  * Tokens outside 0 .. vocab - 1 add nothing; their rows of dout are not read.  A 16-byte aligned
@@ -414,7 +415,8 @@ int mcke_launch_bias_act_checkpoint8_backward(const void* dy, const uint8_t* cod
  * MCKE_DTYPE_BF16 or MCKE_DTYPE_F16; hidden at any alignment of its type, weight 4-byte aligned if
  * dim is even (odd widths are copied a piece at a time, and run slower) and finite (with
  * a dim that is not a multiple of 64, an infinite one makes NaN of the row before it too).
- * rows and vocab up to 2^24, dim up to 2^16; vocab and dim > 0.  scale > 0 multiplies the logits.  With
+ * rows and vocab up to 2^24, dim up to 2^16; vocab and dim > 0.  scale > 0 multiplies the logits, which
+ * stay below 2^127 (a row that has a larger one gives NaN).  With
  * z = scale * hidden[r] . weight[j]:
  *   lse = log sum exp z, loss = lse - z[targets[r]]
  * Products are summed in fp32, and the same input gives the same bits on every run.

@@ -3,12 +3,14 @@
 //   out[r] = scale table[tokens[r]]
 //   dtable[v] = scale sum over r with tokens[r] = v of dout[r]      (or added to dtable[v])
 //
-// The gradient adds each token's rows up in the order of r, whatever the launch: the tokens are
-// sorted (stably), the sorted positions are cut into chunks of equal length, and a workgroup
-// walks a chunk and stores a token's sum where the token changes.  A token whose positions lie
-// in several chunks leaves a sum in the workspace for each, which the launch behind adds up in
-// order.  So no sum depends on the order of atomics, and a token that is half of the batch (a
-// frequent word, a pad token) takes as many workgroups as any other half.
+// The gradient adds each token's rows up in the order of r, whatever the launch (in parts of it,
+// which are then added up in order).  The sums of few tokens are each made by the workgroup of the
+// token's first position.  More tokens are sorted (stably), the sorted positions are cut into
+// chunks of equal length, and a workgroup walks a chunk and stores a token's sum where the token
+// changes.  A token whose positions lie in several chunks leaves a sum in the workspace for each,
+// which the launch behind adds up in order.  So no sum depends on the order of atomics, and a token
+// that is half of the batch (a frequent word, a pad token) takes as many workgroups as any other
+// half.
 //
 //   order   up to 16384 tokens: each one's place counted.  More: runs of 1024 sorted, each in one
 //           workgroup, and merged four at a time
@@ -492,6 +494,84 @@ __global__ __launch_bounds__(kThreads) void embed_join_kernel(
   }
 }
 
+// Few tokens: nothing is sorted.  A workgroup has a position, and goes on where that is its token's
+// first: the token's positions are listed in order, one or two waves have a tile of columns each and
+// the others the same tiles of later positions.  Up to 512 tokens and 2048 workgroups: 500 tokens
+// over 8000 x 512 bf16 take 8.3 us and 16.2 in order of tokens, 4096 columns of 1000 13.2 and 17.9,
+// 4096 columns of fp32 (4000 workgroups) 38.6 and 34.3.  (512 times the same token: 512 columns 15.0
+// and 24.6, 4096 32.7 and 29.4.)
+constexpr int kOnce = 512, kOnceWaves = kOnce / kWave, kOnceAhead = 16;
+constexpr int64_t kOnceMost = 2048;             // workgroups
+
+template <typename T, typename O, bool WHOLE>
+__global__ __launch_bounds__(kOnce) void embed_once_kernel(
+    const int64_t* __restrict__ tokens, const O* __restrict__ dout, T* __restrict__ dtable, int n,
+    int vocab, int cols, int tiles, int slots_log2, float scale, bool accumulate) {
+  constexpr int N = kVecElems<O>;
+  __shared__ int keys[kOnce];
+  __shared__ int ids[kOnce];
+  __shared__ float parts[kOnceWaves][N * kWave];
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int mine = blockIdx.x / tiles;
+  keys[threadIdx.x] =
+      static_cast<int>(threadIdx.x) < n ? key_of(tokens, threadIdx.x, vocab) : vocab;
+  __syncthreads();
+  const int key = keys[mine];
+  if (key == vocab) return;
+  int count = 0, before = 0;               // positions of the token; of them in earlier waves'
+  bool earlier = false;
+#pragma unroll
+  for (int w = 0; w < kOnceWaves; ++w) {
+    const uint64_t set = __ballot(keys[w * kWave + lane] == key);
+    const int at = mine - w * kWave;       // where this position is in the wave's
+    earlier |= (at >= kWave ? set : at > 0 ? set & ((uint64_t{1} << at) - 1) : 0) != 0;
+    if (w < wave) before += __popcll(set);
+    if (w == wave && (set >> lane & 1))
+      ids[before + __popcll(set & ((uint64_t{1} << lane) - 1))] = static_cast<int>(threadIdx.x);
+    count += __popcll(set);
+  }
+  if (earlier) return;
+  __syncthreads();
+  const int slots = 1 << slots_log2, splits = kOnceWaves >> slots_log2;
+  const int slot = wave % slots, split = wave / slots;
+  const Cols<N, WHOLE> at(
+      (static_cast<int64_t>(blockIdx.x % tiles) * slots + slot) * kWave + lane, cols);
+  // Positions a wave: one load's worth at least.
+  const int even = (count + splits - 1) / splits, per = even > kOnceAhead ? even : kOnceAhead;
+  const int begin = split * per, end = begin + per < count ? begin + per : count;
+  float sum[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) sum[e] = 0.0f;
+  auto add = [&]<int U>(int k) {
+    PackT<O, N> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      v[u] = at.load_raw(dout + static_cast<int64_t>(ids[k + u < end ? k + u : end - 1]) * cols);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u < end)
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += static_cast<float>(v[u][e]);
+  };
+  if (at.any) {
+    int k = begin;
+    for (; k + kOnceAhead <= end; k += kOnceAhead) add.template operator()<kOnceAhead>(k);
+    for (; k < end; k += 2) add.template operator()<2>(k);
+  }
+  if (per < count) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) parts[wave][e * kWave + lane] = sum[e];
+    __syncthreads();
+    if (split == 0)
+      for (int p = 1; p * per < count; ++p)
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += parts[p * slots + slot][e * kWave + lane];
+  }
+  if (split == 0 && at.any)
+    store_sum<T, N, WHOLE>(dtable + static_cast<int64_t>(key) * cols, at, sum, scale, accumulate);
+}
+
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
@@ -596,6 +676,22 @@ int launch_sums(const BwdArgs& a, const int* keys, const int* ids, float* partia
   return ok();
 }
 
+// Workgroups a position.
+template <typename O> int64_t once_tiles(int64_t cols) {
+  return ceil_div(cols, 2 * kVecElems<O> * kWave);
+}
+
+template <typename T, typename O, bool WHOLE> int launch_once(const BwdArgs& a) {
+  const int64_t tiles = once_tiles<O>(a.cols);
+  const int slots_log2 = a.cols > kVecElems<O> * kWave ? 1 : 0;
+  embed_once_kernel<T, O, WHOLE><<<static_cast<unsigned>(a.rows * tiles), kOnce, 0, a.s>>>(
+      a.tokens, static_cast<const O*>(a.dout), static_cast<T*>(a.dtable), static_cast<int>(a.rows),
+      static_cast<int>(a.vocab), static_cast<int>(a.cols), static_cast<int>(tiles), slots_log2,
+      a.scale, a.accumulate);
+  MCKE_LAUNCH_CHECK("embed_once_kernel");
+  return ok();
+}
+
 template <typename T, typename O> int launch_bwd(const BwdArgs& a) {
   const Workspace w(a.rows, a.cols);
   int* keys = reinterpret_cast<int*>(a.ws);
@@ -604,15 +700,19 @@ template <typename T, typename O> int launch_bwd(const BwdArgs& a) {
   const Zeros zeros{static_cast<char*>(a.dtable),
                     a.accumulate ? 0 : a.vocab * a.cols * static_cast<int64_t>(sizeof(T))};
   const int64_t pieces = ceil_div(zeros.bytes, 32 * 1024), fill = pieces < 4096 ? pieces : 4096;
+  const bool once = a.rows <= kOnce && a.rows * once_tiles<O>(a.cols) <= kOnceMost;
   const bool count = a.rows <= kCount;
-  const int64_t blocks = ceil_div(a.rows, count ? kWave : kRun);
-  if (blocks + fill == 0) return ok();
-  auto* fn = count ? &embed_count_kernel : &embed_sort_kernel;
-  fn<<<static_cast<unsigned>(blocks + fill), kRun, 0, a.s>>>(
-      a.tokens, keys, ids, static_cast<int>(a.rows), static_cast<int>(a.vocab),
-      static_cast<int>(blocks), zeros);
-  MCKE_LAUNCH_CHECK("embed_count_kernel or embed_sort_kernel");
+  const int64_t blocks = once ? 0 : ceil_div(a.rows, count ? kWave : kRun);
+  if (blocks + fill > 0) {
+    auto* fn = count ? &embed_count_kernel : &embed_sort_kernel;
+    fn<<<static_cast<unsigned>(blocks + fill), kRun, 0, a.s>>>(
+        a.tokens, keys, ids, static_cast<int>(a.rows), static_cast<int>(a.vocab),
+        static_cast<int>(blocks), zeros);
+    MCKE_LAUNCH_CHECK("embed_count_kernel or embed_sort_kernel");
+  }
   if (a.rows == 0) return ok();
+  if (once)
+    return a.cols % kVecElems<O> == 0 ? launch_once<T, O, true>(a) : launch_once<T, O, false>(a);
   int turn = 0;
   for (int64_t len = kRun; !count && len < a.rows; len *= kMergeWays, ++turn) {
     int* to = reinterpret_cast<int*>(a.ws + (turn % 2 ? 0 : 2 * w.list));

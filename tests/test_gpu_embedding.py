@@ -143,6 +143,22 @@ def test_backward_exact(gpu, rows, kind):
         assert torch.equal(got.double(), want), (vocab, kind)
 
 
+@pytest.mark.parametrize("tt,ot", [(BF16, BF16), (F16, F32), (F32, F32)], ids=["bf16", "f16-f32", "f32"])
+@pytest.mark.parametrize("kind", ["text", "one"])
+@pytest.mark.parametrize("rows,vocab,cols", [(512, 40, 64), (511, 600, 513), (513, 40, 64), (512, 5, 1030),
+                                             (300, 9, 4096), (200, 100, 8200), (65, 3, 2049)])
+def test_few_tokens(gpu, rows, vocab, cols, kind, tt, ot):
+    """Around the most tokens and columns whose sums each take one workgroup's way, most of them of
+    many rows."""
+    tokens = _tokens(rows, vocab, rows, kind)
+    dout = _draw((rows, cols), ot, rows)
+    old = _draw((vocab, cols), tt, 7)
+    for o in (None, old):
+        got = run_backward(gpu, tokens, dout, vocab, tt, ot, 1.5, old=o)
+        check("dtable", got, *backward_reference(tokens, dout, vocab, tt, 1.5, o))
+        assert same_bits(got, run_backward(gpu, tokens, dout, vocab, tt, ot, 1.5, old=o))
+
+
 def test_no_rows(gpu):
     """A table of zeros; with accumulate, the table as it was."""
     old = _draw((5, 9), BF16, 1)
@@ -234,13 +250,19 @@ def test_offsets_past_32_bits(gpu):
     for g, w in zip(got, (last[2], one, last[0], last[1], last[2], zero)):
         assert same_bits(g, w)
     dout = _draw((6, cols), BF16, 5, quarters=True)
-    n = m.embedding_backward_workspace_bytes(6, vocab, cols)
-    m.launch_embedding_backward(Dev(m, tokens), Dev(m, dout), big, BF16, BF16, 6, vocab, cols, 1.0,
-                                False, workspace(m, n), n).throw_if_error()
-    m.device_synchronize()
-    tail = np.empty((4, cols), np.int16)
-    m._check(L.mcke_rt_memcpy_async(tail.ctypes.data, big.ptr + at - 2 * cols, tail.nbytes, 1, None))
-    m.device_synchronize()
-    tail = torch.from_numpy(tail).view(torch.bfloat16)
-    for g, w in zip(tail, (zero, dout[2], dout[3], dout[0] + dout[4])):
-        assert same_bits(g, w)
+    for padding in (0, 600):             # few tokens, and more of them in order
+        rows = 6 + padding
+        t = torch.cat([tokens, torch.full((padding,), -1)])
+        d = torch.cat([dout, torch.full((padding, cols), torch.nan, dtype=torch.bfloat16)])
+        m._check(L.mcke_fill_u32_async(big.ptr, 0x3F803F80, vocab * cols // 2, None))
+        n = m.embedding_backward_workspace_bytes(rows, vocab, cols)
+        m.launch_embedding_backward(Dev(m, t), Dev(m, d), big, BF16, BF16, rows, vocab, cols, 1.0,
+                                    False, workspace(m, n), n).throw_if_error()
+        m.device_synchronize()
+        tail = np.empty((4, cols), np.int16)
+        m._check(L.mcke_rt_memcpy_async(tail.ctypes.data, big.ptr + at - 2 * cols, tail.nbytes, 1,
+                                        None))
+        m.device_synchronize()
+        tail = torch.from_numpy(tail).view(torch.bfloat16)
+        for g, w in zip(tail, (zero, dout[2], dout[3], dout[0] + dout[4])):
+            assert same_bits(g, w)
