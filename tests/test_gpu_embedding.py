@@ -192,9 +192,10 @@ def test_gradient_against_differences(gpu):
     assert abs(slope - (got * v).sum()) <= 2 * U * size + (tol * v.abs()).sum()
 
 
-def test_same_bits_capture_and_streams(gpu):
+@pytest.mark.parametrize("rows", [5003, 300])
+def test_same_bits_capture_and_streams(gpu, rows):
     m = gpu
-    rows, vocab, cols = 5003, 2000, 250
+    vocab, cols = 2000, 250
     tokens, dout = _tokens(rows, vocab, 11), _draw((rows, cols), BF16, 11)
     table = _draw((vocab, cols), BF16, 12)
     fwd = run_forward(m, tokens, table, BF16, BF16, 2.0)
