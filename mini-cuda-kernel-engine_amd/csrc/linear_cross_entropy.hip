@@ -765,10 +765,12 @@ constexpr int64_t kPieceValues = int64_t{1} << 26;     // of dz, and of a padded
 
 enum class Tile { k64x128, k128, k256 };
 
-// 256 x 256 where such tiles are most of the CUs' or more; 64 rows at 64 x 128.
-Tile tile_of(int64_t rows, int64_t cols) {
+// 256 x 256 where such tiles are most of the CUs' or more; 64 rows at 64 x 128.  Not for products of
+// up to 128 of K, most of which is the tile's epilogue: two workgroups a CU overlap theirs (gradients
+// of 7424 x 33536 x 64 573 -> 529 us, 4096 x 32768 x 128 284 -> 276, x 192 321 -> 325).
+Tile tile_of(int64_t rows, int64_t cols, int64_t dim) {
   if (rows <= 64) return Tile::k64x128;
-  if (rows > 128 && ceil_div(rows, 256) * ceil_div(cols, 256) >= 192) return Tile::k256;
+  if (rows > 128 && dim > 128 && ceil_div(rows, 256) * ceil_div(cols, 256) >= 192) return Tile::k256;
   return Tile::k128;
 }
 int tile_rows(Tile t) { return t == Tile::k64x128 ? 64 : t == Tile::k128 ? 128 : 256; }
@@ -804,7 +806,7 @@ struct Plan {
     if (pad) limit(width);
     piece = round_up(ceil_div(v, ceil_div(v, most)), kPieceAlign);
     pieces = ceil_div(v, piece);
-    tile = tile_of(r, backward ? (piece < v ? piece : v) : v);
+    tile = tile_of(r, backward ? (piece < v ? piece : v) : v, d);
   }
   // Tiles of logits over `n` rows of the weights.
   int64_t logits_tiles(int64_t n) const {
@@ -1094,7 +1096,7 @@ int check_args(const std::string& who, int dtype, int64_t rows, int64_t vocab, i
     return invalid(who + ": too large: rows and vocab up to 2^24, dim up to 2^16");
   if (!(scale > 0.0f) || !std::isfinite(scale) || !std::isfinite(scale * kLog2e))
     return invalid(who + ": scale must be finite and > 0");
-  const Tile t = tile_of(rows, vocab);
+  const Tile t = tile_of(rows, vocab, dim);
   if (ceil_div(rows, tile_rows(t)) * ceil_div(vocab, tile_cols(t)) > int64_t{INT32_MAX} / kThreads)
     return invalid(who + ": rows x vocab exceed the grid's 32-bit work size");
   return ok();

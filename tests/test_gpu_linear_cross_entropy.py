@@ -150,10 +150,11 @@ def test_loss_and_gradients(gpu, i, shape, dt):
     check("dweight", got[1], want[1], tol[1])
 
 
-@pytest.mark.parametrize("shape", [(12300, 7000, 64), (12300, 7001, 66), (12300, 300, 1024), (5, 9000, 8191)], ids=str)
+@pytest.mark.parametrize("shape", [(12300, 7000, 64), (12300, 7001, 66), (12300, 300, 1024), (5, 9000, 8191),
+                                   (12300, 7001, 130), (12300, 7040, 192)], ids=str)
 def test_pieces(gpu, shape):
-    """Vocabularies in several pieces, of the weights as they are and of padded copies; dH at 256 x
-    256 tiles."""
+    """Vocabularies in several pieces, of the weights as they are and of padded copies; logits
+    at 128 x 128 and 256 x 256 tiles, dH at 256 x 256."""
     h, w, t = _draw(*shape, BF16, 1)
     loss, lse = run_forward(gpu, h, w, t, BF16, 1.0)
     want, tol = forward_reference(h, w, t, 1.0)
