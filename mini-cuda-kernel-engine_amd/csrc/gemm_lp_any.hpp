@@ -31,8 +31,8 @@
 // K is a multiple of 64 here.  Rows past an operand's end along M and N repeat its last row and are
 // not to be stored.  16-byte loads may begin inside a row and end behind it, in the next one: what
 // lies there has to be multiplied by zeros of the other operand (along K), or not stored (along N).
-// Where that leaves the operand, or ends inside a stage of a kAcrossK operand, the caller has a copy of the
-// last rows with zeros behind them (`tail`).
+// Where that leaves the operand, or K ends inside a stage of a kAcrossK operand, the caller has a copy of
+// the last rows with zeros behind them (`tail`, or the operand itself).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -41,20 +41,11 @@
 #include <utility>
 
 #include "gemm_lp.hpp"
+#include "lp_operand.hpp"
 
 namespace mcke_amd {
 
 enum class Along { kAlongK, kAcrossK };
-
-// An operand's memory, 4-byte aligned, `row` elements (an even number) between neighbouring rows.
-// `extent`: its rows (kAlongK), or how many elements a row has (kAcrossK).
-struct LpOperand {
-  const uint16_t* p;
-  int64_t row;
-  int64_t extent;
-  const uint16_t* tail = nullptr;
-  int64_t tail_stage = -1;     // the stage of a kAcrossK operand that is at `tail`
-};
 
 template <int B, Along L> struct LpAnyOperand {
   static constexpr bool kAcross = L == Along::kAcrossK;
@@ -70,10 +61,8 @@ template <int B, Along L> struct LpAnyOperand {
   }
 
   // A lane's sources, relative to the stage's uniform base.
-  const char* base;
-  const char* tail;
-  int64_t tail_stage;
-  int64_t step;                                      // bytes between stages
+  const char* base;                                  // of stage 0
+  LpOperand operand;                                 // (kAcrossK)
   uint32_t src[kDma];
   uint32_t off[2];                                   // fragment addresses in a buffer
 
@@ -87,29 +76,24 @@ template <int B, Along L> struct LpAnyOperand {
     const int lane = threadIdx.x % kWave, g = lane / 16, r16 = lane % 16;
     if constexpr (!kAcross) {
       base = reinterpret_cast<const char*>(o.p + first * o.row) - kBias;
-      step = 128;
       const int64_t last = o.extent - 1 - first;
 #pragma unroll
       for (int q = 0; q < kDma; ++q) {
         const int rt = 8 * (wave * kDma + q) + lane / 8;
-        const int64_t r = rt < last ? rt : last;
-        src[q] = static_cast<uint32_t>(r * o.row * 2) + 16u * ((lane % 8) ^ swz(rt)) + kBias -
+        const int c = (lane % 8) ^ swz(rt);
+        src[q] = static_cast<uint32_t>(2 * lp_along_load(rt, c, o.row, last)) + kBias -
                  1024u * (q % 4);
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s)
         off[s] = (wave_first + r16) * kRow + 16 * ((4 * s + g) ^ (r16 % 8));
     } else {
-      base = reinterpret_cast<const char*>(o.p) - kBias;
-      tail = reinterpret_cast<const char*>(o.tail) - kBias;
-      tail_stage = o.tail_stage;
-      step = 64 * o.row * 2;
+      operand = o;
 #pragma unroll
       for (int q = 0; q < kDma; ++q) {
         const int rt = (64 / kLanes) * (wave * kDma + q) + lane / kLanes;
         const int64_t col = first + 8 * ((lane % kLanes) ^ swz(rt));
-        src[q] = static_cast<uint32_t>(rt * o.row * 2) +
-                 static_cast<uint32_t>(2 * (col < o.extent ? col : 0)) + kBias -
+        src[q] = static_cast<uint32_t>(2 * lp_across_load(rt, col, o.row, o.extent)) + kBias -
                  1024u * (q % 4);
       }
       // Lane r16 = 4 jq + qa of group g reads row 8 g + 4 t + jq at columns 4 qa of its block and
@@ -127,9 +111,8 @@ template <int B, Along L> struct LpAnyOperand {
     lds_dma16<(Q % 4) * 1024>(src[Q], from, buf + (wave * kDma + Q / 4 * 4) * 1024);
   }
   __device__ __forceinline__ const char* source(int64_t p) const {
-    if constexpr (kAcross)
-      if (p == tail_stage) return tail;
-    return base + p * step;
+    if constexpr (kAcross) return reinterpret_cast<const char*>(operand.stage(p)) - kBias;
+    else return base + p * (2 * kStageK);
   }
 
   struct Frags {

@@ -40,6 +40,7 @@
 #include "device_math.hpp"
 #include "elem.hpp"
 #include "gemm_lp_any.hpp"
+#include "linear_cross_entropy_plan.hpp"
 
 namespace mcke_amd {
 namespace {
@@ -326,16 +327,6 @@ __device__ __forceinline__ void of_rows(T (&v)[MT], const T* x, int64_t row0, in
   }
 }
 
-// A piece of the weights: `rows` rows from `first` on, `row` values apart.  Rows from tail_first
-// on (a multiple of 256) are at `tail` too, as far apart, with zeros behind the last (null: none
-// are).
-struct Piece {
-  const uint16_t* p;
-  int64_t row, rows, first;
-  const uint16_t* tail;
-  int64_t tail_first;
-};
-
 struct Logits {
   const uint16_t* hidden;      // packed rows, `width` apart
   int width;                   // a multiple of 64
@@ -347,12 +338,8 @@ template <int BM, int BN, int D, typename T>
 __device__ __forceinline__ void logits_tile(f32x4 (&acc)[BM / 32][BN / 32], char* smem,
                                             const Logits& l, int n, int64_t m0, int64_t n0) {
   const LpOperand A{l.hidden, l.width, n > 0 ? n : 1};
-  const uint16_t* w = l.w.tail && l.w.first + n0 >= l.w.tail_first
-                          ? l.w.tail - (l.w.tail_first - l.w.first) * l.w.row
-                          : l.w.p;
-  const LpOperand B{w, l.w.row, l.w.rows};
-  lp_any_loop<T, BM, BN, Along::kAlongK, Along::kAlongK, D>(acc, smem, A, B, m0, n0, 0,
-                                                            l.width / 64);
+  lp_any_loop<T, BM, BN, Along::kAlongK, Along::kAlongK, D>(acc, smem, A, l.w.of_logits(n0), m0, n0,
+                                                            0, l.width / kStageK);
 }
 
 // (largest, sum) of each row's part in the tile: wave column wn of vocabulary tile `tile` is
@@ -581,8 +568,6 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dz_kernel(Logits l, Rows 
 }
 
 // dH's sums over part blockIdx.y of a piece: acc = dz W, written or added to the part's sums.
-// The last stage of 64 rows of the weights' last piece is in the tail's copy: what lies behind the
-// weights is not the caller's to read (dz has zeros there).
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dh_kernel(
     const uint16_t* __restrict__ dz, int64_t ld, Piece w, int width,
@@ -600,12 +585,9 @@ __global__ __launch_bounds__(kMfmaThreads, 1) void lce_dh_kernel(
   const int stages = all - first < stages_per_part ? all - first : stages_per_part;
   if (stages <= 0) return;
   const LpOperand A{dz, ld, n > 0 ? n : 1};
-  const int64_t last = w.first + 64 * static_cast<int64_t>(all - 1);
-  const bool ends = w.tail && last >= w.tail_first;
-  const LpOperand B{w.p, w.row, w.row, ends ? w.tail + (last - w.tail_first) * w.row : nullptr,
-                    ends ? all - 1 : -1};
   f32x4 acc[MT][NT];
-  lp_any_loop<T, BM, BN, Along::kAlongK, Along::kAcrossK>(acc, smem, A, B, m0, n0, first, stages);
+  lp_any_loop<T, BM, BN, Along::kAlongK, Along::kAcrossK>(acc, smem, A, w.of_dh(), m0, n0, first,
+                                                          stages);
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int wm = wave / 2, wn = wave % 2, g = lane / 16, r16 = lane % 16;
   out += blockIdx.y * part_stride;
@@ -755,70 +737,8 @@ __global__ __launch_bounds__(kThreads) void lce_zero_kernel(uint16_t* __restrict
 }
 
 // ---------------------------------------------------------------------------
-// Plans: tiles, pieces and the workspace, by the extents alone
+// Plans of either pass
 // ---------------------------------------------------------------------------
-constexpr int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
-constexpr int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
-
-constexpr int64_t kPieceAlign = 256;
-constexpr int64_t kPieceValues = int64_t{1} << 26;     // of dz, and of a padded piece of W
-
-enum class Tile { k64x128, k128, k256 };
-
-// 256 x 256 where such tiles are most of the CUs' or more; 64 rows at 64 x 128.  Not for products of
-// up to 128 of K, most of which is the tile's epilogue: two workgroups a CU overlap theirs (gradients
-// of 7424 x 33536 x 64 573 -> 529 us, 4096 x 32768 x 128 284 -> 276, x 192 321 -> 325).
-Tile tile_of(int64_t rows, int64_t cols, int64_t dim) {
-  if (rows <= 64) return Tile::k64x128;
-  if (rows > 128 && dim > 128 && ceil_div(rows, 256) * ceil_div(cols, 256) >= 192) return Tile::k256;
-  return Tile::k128;
-}
-int tile_rows(Tile t) { return t == Tile::k64x128 ? 64 : t == Tile::k128 ? 128 : 256; }
-int tile_cols(Tile t) { return t == Tile::k256 ? 256 : 128; }
-
-struct Plan {
-  int64_t rows, vocab, dim;
-  int64_t width;             // dim, a multiple of 64
-  int64_t up;                // rows, a multiple of 64
-  bool pad;                  // the weights need a padded copy, a piece at a time
-  int64_t tail_first, tail_values;   // or one of their last rows and zeros behind them (0: none)
-  int64_t piece, pieces;     // rows of W at once
-  Tile tile;                 // of the logits
-  int64_t at;                // bytes of workspace so far
-
-  Plan(int64_t r, int64_t v, int64_t d, bool backward) : rows(r), vocab(v), dim(d), at(0) {
-    width = round_up(d, 64);
-    up = round_up(r, 64);
-    pad = d % 2 != 0;
-    // Whole tiles before it read up to 63 values past their last row, which the matrix has to hold.
-    tail_first = (v - 1) / kPieceAlign * kPieceAlign;
-    if (tail_first > 0 && (v - tail_first) * d < 64) tail_first -= kPieceAlign;
-    tail_values = pad || (d % 64 == 0 && (!backward || v % 64 == 0))
-                      ? 0
-                      : (round_up(v, 64) - tail_first) * d + 64;
-    int64_t most = round_up(v, kPieceAlign);
-    auto limit = [&](int64_t per_row) {
-      int64_t m = kPieceValues / per_row / kPieceAlign * kPieceAlign;
-      if (m < kPieceAlign) m = kPieceAlign;
-      if (m < most) most = m;
-    };
-    if (backward) limit(up);
-    if (pad) limit(width);
-    piece = round_up(ceil_div(v, ceil_div(v, most)), kPieceAlign);
-    pieces = ceil_div(v, piece);
-    tile = tile_of(r, backward ? (piece < v ? piece : v) : v, d);
-  }
-  // Tiles of logits over `n` rows of the weights.
-  int64_t logits_tiles(int64_t n) const {
-    return ceil_div(rows, tile_rows(tile)) * ceil_div(n, tile_cols(tile));
-  }
-  int64_t take(int64_t bytes) {
-    const int64_t from = at;
-    at += round_up(bytes, 256);
-    return from;
-  }
-};
-
 struct RowsAt {
   int64_t meta, from, rank, target, lse2, cp, ct, hidden, weight;
   RowsAt(Plan& p, bool backward) {
@@ -951,14 +871,12 @@ template <class F>
 int for_pieces(const Plan& p, const RowsAt& r, const void* weight, char* ws, hipStream_t s, F f) {
   uint16_t* copy = reinterpret_cast<uint16_t*>(ws + r.weight);
   for (int64_t i = 0; i < p.pieces; ++i) {
-    const int64_t first = i * p.piece, n = p.vocab - first < p.piece ? p.vocab - first : p.piece;
-    const uint16_t* w = static_cast<const uint16_t*>(weight) + first * p.dim;
-    Piece piece{w, p.dim, n, first, p.tail_values ? copy : nullptr, p.tail_first};
+    const Piece piece = p.piece_of(i, static_cast<const uint16_t*>(weight), copy);
     if (p.pad) {
-      if (int rc = launch_pack(w, nullptr, nullptr, copy, n, round_up(n, 64), p.dim, p.width,
-                               Tail{nullptr, nullptr, 0, 0}, s))
+      const uint16_t* w = static_cast<const uint16_t*>(weight) + piece.first * p.dim;
+      if (int rc = launch_pack(w, nullptr, nullptr, copy, piece.rows, round_up(piece.rows, 64),
+                               p.dim, p.width, Tail{nullptr, nullptr, 0, 0}, s))
         return rc;
-      piece = Piece{copy, p.width, n, first, nullptr, 0};
     }
     if (int rc = f(piece)) return rc;
   }
