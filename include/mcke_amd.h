@@ -381,9 +381,10 @@ int mcke_launch_embedding_backward(const int64_t* tokens, const void* dout, void
  *     ties to even)
  *   exponents (rows x ceil(cols / 32) bytes): E + 127 of each 32 columns of a row, the smallest
  *     E >= -126 with |u| <= 448 * 2^E for their finite values
- * so a value is restored within 2^-4 of itself, or 2^-10 * 2^E where that is more.  An infinite or
- * NaN u is kept as NaN.  Arithmetic is fp32, each output is rounded once, and the same input gives
- * the same bits on every run. */
+ * so a value is restored within 2^-4 of itself, or 2^-10 * 2^E where that is more (from 248 * 2^120 =
+ * 3.3e38 on it rounds to 2^128, which is infinite in fp32).  An infinite or NaN u is kept as NaN.
+ * Arithmetic is fp32, each output is rounded once, and the same input gives the same bits on every
+ * run. */
 
 /* y = act(u), codes and exponents of u.  bias null is none; y null saves alone.  activation is an
  * mcke_activation value, with the meaning it has in mcke_launch_bias_act_f32.  No output overlaps

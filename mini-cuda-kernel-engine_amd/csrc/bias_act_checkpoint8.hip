@@ -33,7 +33,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return a / b + (a % b != 0); }
 // ---------------------------------------------------------------------------
 // Activations with their slopes.  Beyond |v| = 10 both GELUs' slopes are 1, or less than 1e-20 from
 // 0, so the argument of what needs it is held there, where no power of it and no exponential
-// overflows; a NaN passes through.
+// overflows; a NaN passes through.  Far below 0 the value is 0, whatever v is (-infinity where a
+// code stands for -2^128): what is left of q or of the erfc is multiplied by a v that is held too.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float held10(float v) {
   return v > 10.0f ? 10.0f : v < -10.0f ? -10.0f : v;
@@ -53,7 +54,7 @@ template <int ACT> __device__ __forceinline__ void act_and_slope(float v, float&
     const float h = held10(v);
     const float pdf = 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * h * h);
     const float cdf = v >= 0.0f ? 1.0f - half : half;
-    y = v * cdf;
+    y = fmaxf(v, -30.0f) * cdf;               // (there cdf is 0, or NaN if v is)
     slope = __builtin_fmaf(h, pdf, cdf);
   } else {
     // q = 0.5 (1 + tanh z) = 1 / (1 + e), e = exp(-2 z), z = sqrt(2/pi) (v + 0.044715 v^3):
@@ -66,7 +67,7 @@ template <int ACT> __device__ __forceinline__ void act_and_slope(float v, float&
     const float h = held10(v), h2 = h * h;
     const float e = __builtin_amdgcn_exp2f(h * __builtin_fmaf(c2, h2, c1));
     const float q = __builtin_amdgcn_rcpf(1.0f + e);
-    y = v * q;
+    y = fmaxf(v, -10.0f) * q;                 // (there q is 2^-126, or NaN if v is)
     slope = __builtin_fmaf(h * __builtin_fmaf(d2, h2, d1), (e * q) * q, q);
   }
 }

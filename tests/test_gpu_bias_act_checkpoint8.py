@@ -353,3 +353,23 @@ def test_offsets_past_32_bits(gpu):
     got = torch.from_numpy(got).view(torch.bfloat16)
     assert (got[0] == 1).all()
     assert torch.equal(got[1].double(), saved(last.float())[0][0])
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=[ID[t] for t in DTYPES])
+@pytest.mark.parametrize("act", [ERF, TANH])
+def test_activation_is_zero_far_below(gpu, act, dt):
+    """y = act(u) once more, of every code whose value is below -20, down to -2^128 (what a u from
+    -248 2^120 on is rounded to): both GELUs are within 20 e^-200 of 0 there.  GELU_tanh's argument
+    is held at -10, where q is below 2^-125 and y below 10 times that; the erfc's exponential is 0.
+    (The forward pass gives -0 for all that are finite.)"""
+    ex = torch.arange(1, 248, dtype=torch.uint8)[:, None].repeat(1, 8)
+    code = torch.arange(256, dtype=torch.int32).to(torch.uint8)[None].repeat(247, 1)
+    code[:, 127], code[:, 255] = 0, 0
+    low = restored(code, ex) < -20
+    assert low.any(dim=1).sum() > 100
+    y = run_backward(gpu, None, code, ex, dt, dt, act, want=(False, True, False))[1]
+    assert (y[low].double().abs() <= 10 * 2.0**-125).all()
+    if dt != F16:                         # (their values are past fp16's)
+        u = restored(code, ex).to(TORCH[dt])
+        forward = run_forward(gpu, u, None, dt, dt, act)[0]
+        assert not forward[low & u.isfinite()].any()
