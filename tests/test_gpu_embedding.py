@@ -267,3 +267,32 @@ def test_offsets_past_32_bits(gpu):
         tail = torch.from_numpy(tail).view(torch.bfloat16)
         for g, w in zip(tail, (zero, dout[2], dout[3], dout[0] + dout[4])):
             assert same_bits(g, w)
+
+
+@pytest.mark.parametrize("tt,ot", [(BF16, BF16), (F16, F32), (F32, F32)], ids=["bf16", "f16-f32", "f32"])
+@pytest.mark.parametrize("rows,vocab,cols", [(700, 300, 509), (1500, 97, 1003), (9000, 700, 264),
+                                             (16500, 3000, 512), (20001, 500, 517), (140001, 1021, 260)])
+def test_wide_rows_of_many_tokens(gpu, rows, vocab, cols, tt, ot):
+    """Rows of whole waves whose tokens are put in order: cut and whole vectors, tokens counted and
+    merged, chunks of 4, 8, 16 and 128 positions (more than one round of loads in flight, and more
+    than a wave's 64)."""
+    tokens = _tokens(rows, vocab, rows)
+    dout = _draw((rows, cols), ot, rows)
+    old = _draw((vocab, cols), tt, 7)
+    for o in (None, old):
+        got = run_backward(gpu, tokens, dout, vocab, tt, ot, 1.5, old=o)
+        check("dtable", got, *backward_reference(tokens, dout, vocab, tt, 1.5, o))
+
+
+@pytest.mark.parametrize("kind", ["text", "one", "outside"])
+@pytest.mark.parametrize("rows,cols", [(700, 509), (16500, 512), (20001, 517), (140001, 260)])
+def test_wide_rows_exact(gpu, rows, cols, kind):
+    """Quarters: exact sums, a token that crosses every chunk among them."""
+    vocab = 37
+    tokens = _tokens(rows, vocab, rows, kind)
+    dout = _draw((rows, cols), BF16, rows, quarters=True)
+    got = run_backward(gpu, tokens, dout.float(), vocab, F32, F32, 2.0)
+    want, _ = backward_reference(tokens, dout, vocab, F32, 2.0)
+    assert torch.equal(got.double(), want)
+    got = run_backward(gpu, tokens, dout, vocab, BF16, BF16, 2.0)
+    assert same_bits(got, want.to(torch.bfloat16))
