@@ -387,3 +387,30 @@ def test_offsets_past_32_bits(gpu):
     want = dz.t() @ h.double()
     tol = tdz.t() @ h.double().abs()
     check("dweight", got, want, tol + HALF[BF16] * (want.abs() + tol) + TINY[BF16])
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=[ID[t] for t in TYPES])
+@pytest.mark.parametrize("shape", [(40, 1000, 192), (200, 4100, 64), (150, 300, 1024), (300, 25000, 512),
+                                   (700, 3001, 4096)], ids=str)
+def test_aligned_weight_gradient(gpu, shape, dt):
+    """dweight at whole 128-byte lines, as allocators give it, of one stage, 128 x 128 and 256 x 256
+    tiles: right, and the bits of one off the lines."""
+    m = gpu
+    rows, vocab, dim = shape
+    h, w, t = _draw(*shape, dt, 13)
+    _, lse = run_forward(m, h, w, t, dt, 1.0)
+    dloss, _ = _grads(rows, 13, dt)
+    ins = [Dev(m, x) for x in (h, w, t, lse, dloss)]
+    n = m.linear_cross_entropy_backward_workspace_bytes(rows, vocab, dim)
+    ws = workspace(m, n)
+    got = []
+    for shift in (32, 0):                       # values behind 64 bytes past a line of 256
+        dw = out(m, w.shape, w.dtype, shift)
+        assert (dw.ptr % 128 == 0) == (shift == 32)
+        m.launch_linear_cross_entropy_backward(*ins, None, None, dw, dt, rows, vocab, dim, 1.0, ws, n
+                                               ).throw_if_error()
+        m.device_synchronize()
+        got.append(dw.get())
+    want, tol = backward_reference(h, w, t, lse, dloss, None, 1.0, dt)
+    check("dweight", got[0], want[1], tol[1])
+    assert same_bits(*got)
