@@ -416,8 +416,9 @@ int mcke_launch_bias_act_checkpoint8_backward(const void* dy, const uint8_t* cod
  * MCKE_DTYPE_BF16 or MCKE_DTYPE_F16; hidden at any alignment of its type, weight 4-byte aligned if
  * dim is even (odd widths are copied a piece at a time, and run slower) and finite (with
  * a dim that is not a multiple of 64, an infinite one makes NaN of the row before it too).
- * rows and vocab up to 2^24, dim up to 2^16; vocab and dim > 0.  scale > 0 multiplies the logits, which
- * stay below 2^127 (a row that has a larger one gives NaN).  With
+ * rows and vocab up to 2^24, dim up to 2^16; vocab and dim > 0; the forward pass refuses 2^23 tiles of
+ * 256 x 256 logits and more (rows x vocab of 2^39).  scale > 0 multiplies the logits, which stay below
+ * 2^127 (a row that has a larger one gives NaN).  With
  * z = scale * hidden[r] . weight[j]:
  *   lse = log sum exp z, loss = lse - z[targets[r]]
  * Products are summed in fp32, and the same input gives the same bits on every run.

@@ -786,7 +786,7 @@ struct BwdPlan : Plan {
     // tiles, at least 8 stages each, and up to 80 MB of sums.  256 x 256 from 192 workgroups on
     // (2047 x 32001 x 1024 fp16: 109 us with 8 parts, against 136 at 128 x 128 with 4).
     part_stride = up * width;
-    const int64_t stages = ceil_div(piece < vocab ? piece : vocab, 64);
+    const int64_t stages = ceil_div(at_once(), 64);
     auto share = [&](Tile t) {
       dh_tiles = ceil_div(rows, tile_rows(t)) * ceil_div(dim, tile_cols(t));
       parts = (t == Tile::k256 ? 256 : 512) / dh_tiles;
@@ -1014,9 +1014,6 @@ int check_args(const std::string& who, int dtype, int64_t rows, int64_t vocab, i
     return invalid(who + ": too large: rows and vocab up to 2^24, dim up to 2^16");
   if (!(scale > 0.0f) || !std::isfinite(scale) || !std::isfinite(scale * kLog2e))
     return invalid(who + ": scale must be finite and > 0");
-  const Tile t = tile_of(rows, vocab, dim);
-  if (ceil_div(rows, tile_rows(t)) * ceil_div(vocab, tile_cols(t)) > int64_t{INT32_MAX} / kThreads)
-    return invalid(who + ": rows x vocab exceed the grid's 32-bit work size");
   return ok();
 }
 
@@ -1066,6 +1063,8 @@ int mcke_launch_linear_cross_entropy(const void* hidden, const void* weight, con
     return invalid(who + ": a pointer is not aligned to its type");
   if (int rc = check_weight(who, weight, dim)) return rc;
   const FwdPlan p(rows, vocab, dim);
+  if (!p.fits())
+    return invalid(who + ": rows x vocab exceed the grid's 32-bit work size");
   const size_t need = static_cast<size_t>(p.at);
   if (int rc = check_workspace(who, workspace, workspace_bytes, need)) return rc;
   const uint64_t n = rows, h = 2 * n * dim, w = 2 * static_cast<uint64_t>(vocab) * dim;

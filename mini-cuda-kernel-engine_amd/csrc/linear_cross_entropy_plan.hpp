@@ -28,6 +28,9 @@ constexpr Tile tile_of(int64_t rows, int64_t cols, int64_t dim) {
 constexpr int tile_rows(Tile t) { return t == Tile::k64x128 ? 64 : t == Tile::k128 ? 128 : 256; }
 constexpr int tile_cols(Tile t) { return t == Tile::k256 ? 256 : 128; }
 
+// Workgroups of a launch: 256 lanes each of the grid's 32-bit work size.
+constexpr int64_t kMostTiles = INT32_MAX / 256;
+
 // A piece of the weights: `rows` rows from `first` on, `row` values apart.  Rows from tail_first
 // on (a multiple of 256) are at `tail` too, as far apart, with zeros behind the last up to a
 // multiple of 64 rows and 64 values more (null: none are).
@@ -79,8 +82,12 @@ struct Plan {
     if (pad) limit(width);
     piece = round_up(ceil_div(v, ceil_div(v, most)), kPieceAlign);
     pieces = ceil_div(v, piece);
-    tile = tile_of(r, backward ? (piece < v ? piece : v) : v, d);
+    // Tiles that are too many for a launch are larger instead (the backward pass's pieces never are).
+    tile = tile_of(r, backward ? at_once() : v, d);
+    if (!fits()) tile = Tile::k256;
   }
+  int64_t at_once() const { return piece < vocab ? piece : vocab; }
+  bool fits() const { return logits_tiles(at_once()) <= kMostTiles; }
   // Piece i of `weight`, with `copy` where the tail's copy or the piece's padded one is.
   Piece piece_of(int64_t i, const uint16_t* weight, const uint16_t* copy) const {
     const int64_t first = i * piece, n = vocab - first < piece ? vocab - first : piece;

@@ -414,3 +414,46 @@ def test_aligned_weight_gradient(gpu, shape, dt):
     want, tol = backward_reference(h, w, t, lse, dloss, None, 1.0, dt)
     check("dweight", got[0], want[1], tol[1])
     assert same_bits(*got)
+
+
+def test_more_logits_than_small_tiles(gpu):
+    """2^19 rows x 2^18 logits, one 128 x 128 tile too many for a launch: some rows of both passes."""
+    m = gpu
+    rows, vocab, dim = 1 << 19, 1 << 18, 128
+    h, w, t = _draw(rows, vocab, dim, BF16, 14)
+    t = torch.where(t < 0, t, (t * 7919 + 5) % vocab)
+    some = torch.tensor([0, 1, 255, 131072, 300001, rows - 129, rows - 2, rows - 1])
+    t[some] = torch.tensor([vocab - 1, 0, 128, 131071, 77777, 200000, 1, vocab - 2])
+    ins = [Dev(m, x) for x in (h, w, t)]
+    loss, lse = (out(m, (rows,), torch.float32) for _ in range(2))
+    n = m.linear_cross_entropy_workspace_bytes(rows, vocab, dim)
+    ws = m.DeviceBuffer(n)
+    m.launch_linear_cross_entropy(*ins, loss, lse, BF16, rows, vocab, dim, 1.0, ws, n).throw_if_error()
+    m.device_synchronize()
+    got = [x.get() for x in (loss, lse)]
+    want, tol = forward_reference(h[some], w, t[some], 1.0)
+    check("loss", got[0][some], want[0], tol[0])
+    check("lse", got[1][some], want[1], tol[1])
+    dloss = torch.full((rows,), 1.0 / rows)
+    dh, dw = out(m, h.shape, h.dtype), out(m, w.shape, w.dtype)
+    n = m.linear_cross_entropy_backward_workspace_bytes(rows, vocab, dim)
+    ws = m.DeviceBuffer(n)
+    m.launch_linear_cross_entropy_backward(*ins, lse, Dev(m, dloss), None, dh, dw, BF16, rows, vocab, dim,
+                                           1.0, ws, n).throw_if_error()
+    m.device_synchronize()
+    dh, dw = dh.get(), dw.get()
+    want, tol = backward_reference(h[some], w, t[some], got[1][some], dloss[some], None, 1.0, BF16)
+    check("dhidden", dh[some], want[0], tol[0])
+    # Some rows of dweight, over all rows of the batch: dz in 64 bits for those columns alone.
+    cols = torch.tensor([0, 255, 256, 131072, vocab - 1])
+    z, tz = _logits(h, w[cols], 1.0)
+    have = (t >= 0)[:, None]
+    p = torch.where(have, torch.exp(z - got[1].double()[:, None]), 0.0)
+    dz = (p - (t[:, None] == cols).double()) * (have.double() / rows)
+    tdz = p * (tz + 4 * U * (z.abs() + got[1].double().abs()[:, None]) + 2 * U) / rows
+    tdz = tdz + 4 * U * dz.abs()
+    tdz = torch.where(have, tdz + HALF[BF16] * (dz.abs() + tdz), 0.0)
+    hd = h.double()
+    want = dz.t() @ hd
+    tol = tdz.t() @ hd.abs() + rows * U * (dz.abs().t() @ hd.abs())
+    check("dweight", dw[cols], want, tol + HALF[BF16] * (want.abs() + tol) + TINY[BF16])

@@ -253,3 +253,21 @@ def test_linear_cross_entropy_workspace(mcke):
     # A training batch: far below its logits (2 GiB in 16 bits), its copy of the rows included.
     assert mcke.linear_cross_entropy_workspace_bytes(8192, 131072, 4096) < 192 << 20
     assert mcke.linear_cross_entropy_backward_workspace_bytes(8192, 131072, 4096) < 384 << 20
+
+
+def test_linear_cross_entropy_of_many_logits(cpu_only):
+    """More logits than one launch has 128 x 128 tiles for are not refused (what is missing here is
+    the workspace): the forward pass takes 256 x 256 ones, up to 2^23 of them, and the backward pass
+    goes by pieces of the vocabulary."""
+    m = cpu_only
+    for dim in (64, 65, 128, 4096):
+        for rows, vocab in ((1 << 19, 1 << 18), (1 << 24, (1 << 15) - 256), (1 << 15, 1 << 24)):
+            rows -= 256 if rows == 1 << 15 else 0
+            need = m.linear_cross_entropy_workspace_bytes(rows, vocab, dim)
+            _refused(m, _lce(m, 1 << 50, 1 << 51, 1 << 52, 1 << 53, 1 << 54, rows=rows, vocab=vocab,
+                             dim=dim, ws=None), str(need))
+        for rows, vocab in ((1 << 19, 1 << 18), (1 << 24, 1 << 24)):
+            need = m.linear_cross_entropy_backward_workspace_bytes(rows, vocab, dim)
+            _refused(m, _lceb(m, 1 << 50, 1 << 51, 1 << 52, 1 << 53, 1 << 54, 1 << 55, 1 << 56, 1 << 57,
+                              rows=rows, vocab=vocab, dim=dim, ws=None), str(need))
+    _refused(m, _lce(m, rows=1 << 24, vocab=1 << 15, ws=None), "32-bit work size")
