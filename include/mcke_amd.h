@@ -361,9 +361,9 @@ int mcke_launch_embedding(const int64_t* tokens, const void* table, void* out, i
 size_t mcke_embedding_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t cols);
 
 /* The gradient in the table:
- *   dtable[v] = scale * sum over r with tokens[r] == v, in the order of r, of dout[r]
- * (the sums of consecutive parts of the rows are added up in their order);
- * zeros for tokens that are not there; accumulate != 0 adds to dtable instead, and touches the
+ *   dtable[v] = scale * sum over r with tokens[r] == v of dout[r]
+ * (in an order that the tokens and the extents fix: parts of the rows in the order of r, then the
+ * parts); zeros for tokens that are not there; accumulate != 0 adds to dtable instead, and touches the
  * rows of tokens that are there alone (tied weights: the loss's gradient is there already).
  * Tokens outside 0 .. vocab - 1 add nothing; their rows of dout are not read.  A 16-byte aligned
  * workspace is needed (see above).  vocab == 0 or cols == 0 is a no-op. */
@@ -414,8 +414,9 @@ int mcke_launch_bias_act_checkpoint8_backward(const void* dy, const uint8_t* cod
  * largest tensor of a training step: they are never kept.  hidden (rows x dim, row-major) and
  * weight (vocab x dim, row-major: as a layer or a tied embedding holds it) are of dtype,
  * MCKE_DTYPE_BF16 or MCKE_DTYPE_F16; hidden at any alignment of its type, weight 4-byte aligned if
- * dim is even (odd widths are copied a piece at a time, and run slower) and finite (with
- * a dim that is not a multiple of 64, an infinite one makes NaN of the row before it too).
+ * dim is even (odd widths are copied a piece at a time, and run slower) and finite (with an even
+ * dim that is not a multiple of 64, an infinite one makes NaN of rows before it too: of one, or for
+ * narrow ones of as many as make up 64 values).
  * rows and vocab up to 2^24, dim up to 2^16; vocab and dim > 0; the forward pass refuses 2^23 tiles of
  * 256 x 256 logits and more (rows x vocab of 2^39).  scale > 0 multiplies the logits, which stay below
  * 2^127 (a row that has a larger one gives NaN).  With
@@ -443,7 +444,8 @@ int mcke_launch_linear_cross_entropy(const void* hidden, const void* weight, con
  *   dhidden = dz weight, dweight = dz^T hidden
  * dloss or dlse (rows values) may be null, not both; dhidden (as hidden) or dweight (as weight, at
  * any alignment of its type) may be null, not both; they are overwritten.  dz is rounded to dtype
- * once, as a multiple of the largest |dloss| + |dlse| of a row, so that small ones keep their bits.
+ * once, as a multiple of the largest |dloss| + |dlse| of a row, so that small ones keep their bits;
+ * all else is fp32 up to the outputs' rounding.
  * rows == 0 gives a dweight of zeros. */
 int mcke_launch_linear_cross_entropy_backward(const void* hidden, const void* weight,
                                               const int64_t* targets, const float* lse,

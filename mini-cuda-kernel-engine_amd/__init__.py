@@ -696,7 +696,7 @@ def embedding_backward_workspace_bytes(rows: int, vocab: int, cols: int) -> int:
 def launch_embedding_backward(tokens, dout, dtable, dout_dtype, table_dtype, rows: int, vocab: int,
                               cols: int, scale: float = 1.0, accumulate: bool = False,
                               workspace=None, workspace_bytes: int = 0, stream=None) -> Status:
-    """The table's gradient, each token's rows of dout added up in their order; accumulate adds
+    """The table's gradient, each token's rows of dout added up in a fixed order; accumulate adds
     to dtable, else all of it is written."""
     return _st(lib().mcke_launch_embedding_backward(
         _ptr(tokens), _ptr(dout), _ptr(dtable), dout_dtype, table_dtype, rows, vocab, cols, scale,

@@ -3,12 +3,12 @@
 //   out[r] = scale table[tokens[r]]
 //   dtable[v] = scale sum over r with tokens[r] = v of dout[r]      (or added to dtable[v])
 //
-// The gradient adds each token's rows up in the order of r, whatever the launch (in parts of it,
-// which are then added up in order).  The sums of few tokens are each made by the workgroup of the
-// token's first position.  More tokens are sorted (stably), the sorted positions are cut into
+// The gradient adds each token's rows up in an order that the tokens and the extents fix: parts of
+// them in the order of r, and then the parts.  The sums of few tokens are each made by the workgroup
+// of the token's first position.  More tokens are sorted (stably), the sorted positions are cut into
 // chunks of equal length, and a workgroup walks a chunk and stores a token's sum where the token
 // changes.  A token whose positions lie in several chunks leaves a sum in the workspace for each,
-// which the launch behind adds up in order.  So no sum depends on the order of atomics, and a token
+// which the launch behind adds up.  So no sum depends on the order of atomics, and a token
 // that is half of the batch (a frequent word, a pad token) takes as many workgroups as any other
 // half.
 //
@@ -110,7 +110,11 @@ struct Zeros {
 // before it: a workgroup has 64 tokens, a lane each, and its waves deal out all of the keys in
 // chunks of 64 (in LDS; a chunk is compared with before, behind or at the workgroup's own).
 // 16384^2 comparisons are two operations each, 14 us over all CUs; sorted by one workgroup the
-// same took 24, in runs of 1024 and two merges 26.  Workgroups from `blocks` on write zeros.
+// same took 24, in runs of 1024 and two merges 26.  Counting takes the square of the tokens, merges a
+// launch for each four times as many: gradients over 8000 x 1024 bf16 take 39 us counted and 44 merged
+// at 10000 tokens, 52 and 50 at 16384 (226 and 245 over 131072 x 4096, whose zeros hide the count),
+// 69 and 58 at 16385, 85 and 61 at 20000, 125 and 66 at 32768.  Workgroups from `blocks` on write
+// zeros.
 constexpr int kCount = 16384;
 
 __global__ __launch_bounds__(kRun) void embed_count_kernel(const int64_t* __restrict__ tokens,
@@ -411,8 +415,8 @@ __global__ __launch_bounds__(kThreads) void embed_sums_kernel(
 
 // Tokens that begin in one chunk and end in a later one.  Each group of 2^tpr_log2 lanes looks
 // at a chunk, and adds up its token's sums if that ends within kNear chunks.  Tokens that go
-// further are added up by all groups, which deal out the later chunks; the groups' sums come
-// together in their order.
+// further are added up by all groups, which deal out the later chunks (of G groups each every
+// G-th); then the groups' sums are added up.
 constexpr int kNear = 16;
 
 template <typename T, int N, bool WHOLE>

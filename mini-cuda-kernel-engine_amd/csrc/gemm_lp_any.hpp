@@ -4,8 +4,8 @@
 //
 // each operand with its k contiguous (kAlongK: rows of A[m][k], of B[n][k], as a layer's weights
 // [out][in] and activations are) or with its other index contiguous (kAcrossK: A[k][m],
-// B[k][n]).  A layer's three products, y = x W^T, dx = dy W and dW = dy^T x, are one of these
-// each, with no transposed copy.
+// B[k][n]).  The products of a layer and its gradients, y = x W^T, dx = dy W and dW = dy^T x, are one of
+// these each, with no transposed copy: those of the cross entropy of hidden states are made so.
 //
 // A workgroup of four waves (2 x 2) owns BM x BN, a wave MT x NT blocks of 16 x 16
 // (v_mfma_f32_16x16x32).  K goes in stages of 64 (two steps of 32), each operand's stage straight

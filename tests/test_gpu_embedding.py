@@ -20,8 +20,8 @@ pytestmark = pytest.mark.gpu
 PAIRS = [(BF16, BF16), (F16, F16), (F32, F32), (BF16, F32), (F16, F32)]     # table, out
 PAIR_IDS = [f"{ID[t]}-{ID[o]}" for t, o in PAIRS]
 # rows, vocab, cols: one of each, rows shorter than a 16-byte vector, odd widths, more than one
-# round of lanes; more tokens than one sort takes in one register a lane (1024), in four (4096)
-# and in one workgroup (16384), and than eight of those (one more merge).
+# round of lanes; more tokens than are added up without an order (512), than a run of the sort has
+# (1024), and than are counted (16384: runs and three merges, four above 65536).
 SHAPES = [(1, 1, 1), (3, 5, 3), (7, 2, 8), (64, 1000, 127), (5, 300, 2050), (1024, 513, 40),
           (1025, 70, 64), (4097, 1000, 9), (2000, 131072, 16), (300, 77, 4099), (20001, 4001, 24),
           (140001, 1021, 8)]
