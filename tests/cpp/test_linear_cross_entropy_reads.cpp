@@ -72,6 +72,9 @@ int main() {
   for (int64_t dim : {1, 2, 4, 6, 63, 66, 192, 1026})
     for (int64_t vocab : {5376, 5377, 7001, 10752, 10753, 10754, 10817, 10818})
       for (bool backward : {false, true}) scan(12300, vocab, dim, backward);
+  // Pieces of 256, the last one of so few rows that the copy begins a piece before it.
+  for (int64_t dim : {2, 4, 6, 8, 30, 62, 130})
+    for (int64_t vocab = 510; vocab <= 580; ++vocab) scan(131100, vocab, dim, true);
   std::printf("%ld loads, %ld failures\n", g_loads, g_failures);
   return g_failures ? 1 : 0;
 }

@@ -457,3 +457,20 @@ def test_more_logits_than_small_tiles(gpu):
     want = dz.t() @ hd
     tol = tdz.t() @ hd.abs() + rows * U * (dz.abs().t() @ hd.abs())
     check("dweight", dw[cols], want, tol + HALF[BF16] * (want.abs() + tol) + TINY[BF16])
+
+
+@pytest.mark.parametrize("shape", [(5, 65, 2), (7, 66, 2), (3, 129, 4), (70, 321, 2), (9, 322, 2), (5, 449, 6),
+                                   (131100, 513, 2), (131100, 514, 4)], ids=str)
+def test_narrow_rows_at_the_end(gpu, shape):
+    """Vocabularies that end one or two narrow rows into a stage, whose loads in the stage before it
+    reach past them; with pieces of 256 rows, the copy of the last ones begins a piece earlier."""
+    h, w, t = _draw(*shape, BF16, 15)
+    loss, lse = run_forward(gpu, h, w, t, BF16, 1.25)
+    want, tol = forward_reference(h, w, t, 1.25)
+    check("loss", loss, want[0], tol[0])
+    check("lse", lse, want[1], tol[1])
+    dloss, dlse = _grads(shape[0], 15, BF16)
+    got = run_backward(gpu, h, w, t, lse, dloss, dlse, BF16, 1.25)
+    want, tol = backward_reference(h, w, t, lse, dloss, dlse, 1.25, BF16)
+    check("dhidden", got[0], want[0], tol[0])
+    check("dweight", got[1], want[1], tol[1])
